@@ -324,6 +324,22 @@ int vdn_window_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
                          int64_t g_st, int64_t g_sh, void* out, int64_t o_st, int64_t o_sh,
                          float* lse, int64_t l_st, int64_t l_sh, void* stream);
 
+/*
+ * Causal softmax attention of packed sequences (dtype 0: bf16, 1: fp16; head_dim 64, 128 or
+ * 256): query head h = u group + j reads K/V head u; a token sees its sequence up to itself.
+ * The tokens x group rows of a sequence and a K/V head are counted token major and cut into
+ * blocks of block_rows (128 or 256): blocks int32 [nblocks, 4] = (first packed row of the
+ * sequence, its tokens, first row of the block, unused). q, k, v, out addressed by (token, head)
+ * strides (multiples of 8 elements, unit channel stride, 16-byte aligned); K/V token strides up
+ * to 2^22. lse (nullable): fp32 natural-log sum-exp of the scaled scores. Only the rows of
+ * the blocks are written.
+ */
+int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                         int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                         const int* blocks, int nblocks, int block_rows, int kv_heads, int group,
+                         int head_dim, int dtype, float scale, void* out, int64_t o_st,
+                         int64_t o_sh, float* lse, int64_t l_st, int64_t l_sh, void* stream);
+
 /* vdn_window_attention with the output quantized in the epilogue instead of stored as bf16:
  * query row q, head h -> MXFP8 codes[q, 128 (chunk0 + h) .. +128) of a [rows, kp] code
  * matrix and the four E8M0 scales of that chunk in its SWIZZLE_32_4_4 scale array; the same

@@ -1,0 +1,119 @@
+"""Causal attention over packed prompts: grouped heads, sequences of different lengths.
+
+The companion of window.paper_window_attention for token sequences (a prompt in front of the
+block, a causal decoder's prefill): each token sees itself and the tokens before it in its own
+sequence. Device work runs in libvdnmi.so; the host prepares a plan of row blocks once per
+batch of lengths. What a prompt leaves for later steps goes into the 8-bit cache (kvcache.py).
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+MAX_ROWS = 2 ** 31 - 512   # rows (tokens x query heads of a K/V head) of one sequence
+
+
+@dataclass(frozen=True)
+class CausalPlan:
+    """Blocks of the packed sequences: `blocks` int32 [nblocks, 4] on the device = (first packed
+    row of the sequence, its tokens, first row of the block among the sequence's tokens x
+    heads / kv_heads rows, 0), the blocks with most keys first. `rows` counts the packed
+    rows; `block_rows` is the kernel variant."""
+    lengths: tuple
+    heads: int
+    kv_heads: int
+    rows: int
+    block_rows: int
+    blocks: torch.Tensor
+
+    @property
+    def device(self):
+        return self.blocks.device
+
+
+def _blocks(lengths, group, block_rows):
+    """[nblocks, 4] of all sequences, by falling number of keys."""
+    n = torch.tensor(lengths, dtype=torch.int64)
+    first = n.cumsum(0) - n
+    count = (n * group + block_rows - 1) // block_rows
+    seq = torch.repeat_interleave(torch.arange(len(lengths)), count)
+    r0 = (torch.arange(seq.numel()) - (count.cumsum(0) - count)[seq]) * block_rows
+    keys = torch.minimum(r0 + block_rows, n[seq] * group)
+    order = torch.argsort(keys, descending=True, stable=True)
+    blocks = torch.stack((first[seq], n[seq], r0, torch.zeros_like(r0)), 1)
+    return blocks[order].to(torch.int32)
+
+
+def prepare_causal_plan(lengths, heads, kv_heads=None, *, device="cpu"):
+    """Plan of sequences of `lengths` tokens (ints >= 0), packed in that order from row 0, for
+    `heads` query heads that share `kv_heads` K/V heads (all of their own by default)."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    lengths = tuple(lengths)
+    if any(type(n) is not int or n < 0 for n in lengths):
+        raise ValueError("lengths must be non-negative integers")
+    if any(type(h) is not int or h <= 0 for h in (heads, kv_heads)) or heads % kv_heads:
+        raise ValueError("heads must be a positive multiple of kv_heads")
+    group = heads // kv_heads
+    if sum(lengths) * group > MAX_ROWS:
+        raise ValueError("too many rows for one plan")
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return CausalPlan(lengths, heads, kv_heads, sum(lengths), 256,
+                      _blocks(lengths, group, 256).to(device))
+
+
+def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_lse=False,
+                     out=None):
+    """softmax(scale Q Kᵀ) V over each token's own sequence up to itself.
+
+    query [rows, H, D], key and value [rows, Hkv, D] (BF16 or FP16, D 64, 128 or 256, unit
+    channel stride, rows >= plan.rows; any token and head strides that keep 16-byte alignment);
+    query head h reads K/V head h // (H / Hkv). Returns [rows, H, D] of the same dtype, scores
+    and sums in fp32, probabilities rounded to the activation dtype before the product with V;
+    with return_lse also the natural-log sum of exp of the scaled scores, fp32 [rows, H].
+    Rows behind the plan's last sequence are zero (LSE -inf); in a caller's `out` they are left
+    as they were. Values of tokens that a row does not see never reach it, nonfinite ones
+    included."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("causal attention is inference-only; use no_grad/inference_mode")
+    if not isinstance(plan, CausalPlan):
+        raise TypeError("plan must be prepared with prepare_causal_plan")
+    if any(x.ndim != 3 for x in (query, key, value)):
+        raise ValueError("Q/K/V must be [rows, heads, D]")
+    rows, heads, d = query.shape
+    if (heads != plan.heads or key.shape != (rows, plan.kv_heads, d) or value.shape != key.shape
+            or rows < plan.rows or d not in (64, 128, 256)):
+        raise ValueError("Q/K/V do not match the plan's heads and rows, or D is not 64, 128 or 256")
+    if query.dtype not in (torch.bfloat16, torch.float16) or \
+            any(x.dtype != query.dtype or x.stride(-1) != 1 for x in (query, key, value)):
+        raise ValueError("Q/K/V must share BF16 or FP16 and have unit innermost stride")
+    if not query.is_cuda or any(x.device != query.device for x in (key, value)) \
+            or query.device != plan.device:
+        raise ValueError("Q/K/V and prepared plan must be on the same CUDA device")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("scale must be finite and positive")
+    if out is None:
+        out = torch.empty((rows, heads, d), dtype=query.dtype, device=query.device)
+        out[plan.rows:].zero_()
+    elif (out.shape != (rows, heads, d) or out.dtype != query.dtype or out.device != query.device
+          or out.stride(-1) != 1):
+        raise ValueError("out must be a [rows, H, D] view like the queries, unit channel stride")
+    lse = None
+    if return_lse:
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=query.device)
+        lse[plan.rows:].fill_(-math.inf)
+    with torch.cuda.device(query.device):
+        _lib.call("vdn_causal_attention", query.data_ptr(), query.stride(0), query.stride(1),
+                  key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
+                  value.stride(0), value.stride(1), plan.blocks.data_ptr(),
+                  plan.blocks.shape[0], plan.block_rows, plan.kv_heads, heads // plan.kv_heads,
+                  d, int(query.dtype == torch.float16), scale, out.data_ptr(), out.stride(0),
+                  out.stride(1), _lib.ptr(lse), 0 if lse is None else lse.stride(0),
+                  0 if lse is None else lse.stride(1), _lib.stream(query.device))
+    return (out, lse) if return_lse else out

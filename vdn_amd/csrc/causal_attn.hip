@@ -1,0 +1,386 @@
+// Causal attention over packed prompts for gfx950 (bf16 or fp16; head_dim 64, 128, 256).
+//
+//   out[i, h] = sum_{j <= i} softmax_j(scale q[i, h] . k[j, u]) v[j, u],   u = h / G
+//
+// for the tokens i, j of one sequence; G query heads share the K/V head u. A sequence's n
+// tokens and the G heads of u make n G rows, token major (row r: token r / G, head u G + r % G),
+// and a workgroup takes a block of 32 kWaves of them: each K/V tile serves all G heads, and a
+// block spans few tokens, so few of its tiles cross the diagonal.
+//
+// Per tile of kBN keys, as the frame-window kernel: Sᵀ = K Qᵀ on 32x32x16 MFMAs with Q in
+// registers, online softmax in the exp2 domain (fp32 maximum and sum per row), and Oᵀ += Vᵀ Pᵀ,
+// where Pᵀ is the Sᵀ accumulator itself and Vᵀ comes from the token-major V tile by transpose
+// reads. Tiles stream global -> LDS, double-buffered.
+//
+// A nonfinite V value of a token that a row does not see must not reach that row, and 0 inf is
+// NaN in an MFMA. Only tiles on the diagonal hold such tokens: there every wave looks its share
+// of the V tile over as it lands, replaces nonfinite values by zeros and notes, per channel, the
+// first token with a positive and with a negative one. What a row sees is a prefix, so the row
+// holds that value exactly if the token is not behind its own: it is added after the product.
+#include "attn_tiles.h"
+
+#include <math.h>
+
+#include <type_traits>
+
+namespace vdn {
+namespace {
+
+struct CausalIn {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // token / head strides (elements)
+};
+
+struct CausalOut {
+  uint16_t* out;
+  float* lse;
+  int64_t o_st, o_sh, l_st, l_sh;
+};
+
+// blocks: int32 [nblocks, 4] = (first token row, tokens n of the sequence, first row r0 of the
+// block among the sequence's n G, unused), most keys first.
+template <int kD, int kWaves, int kBN, bool kF16>
+__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, int nblocks,
+                   int kv_heads, int group, float scale_log2) {
+  constexpr int kKT = kBN / 32;           // 32-key score accumulators per tile
+  constexpr int kDB = kD / 32;            // 32-channel output accumulators
+  constexpr int kSteps = kD / 16;         // channel steps of Sᵀ
+  constexpr int kChunks = kD / 8;         // 16-byte chunks per tile row
+  constexpr int kSegRows = 64 / kChunks;  // rows per 1 KB DMA segment (one wave instruction)
+  constexpr int kBM = 32 * kWaves;
+  constexpr int kThreads = 64 * kWaves;
+  constexpr int kSegs = kBN / kSegRows / kWaves;  // 1 KB segments per tensor per wave
+  static_assert(kSegs * kWaves * kSegRows == kBN, "segment mapping");
+  static_assert(kBM <= 4 * kBN, "the epilogue stages the block in the tile buffers");
+  typedef Elem<kF16> E;
+  typedef typename E::x8 x8;
+  // one array per buffer: the compiler then tells a prefetch into one from reads of the other
+  __shared__ __attribute__((aligned(1024))) uint16_t sK0[kBN * kD];
+  __shared__ __attribute__((aligned(1024))) uint16_t sK1[kBN * kD];
+  __shared__ __attribute__((aligned(1024))) uint16_t sV0[kBN * kD];
+  __shared__ __attribute__((aligned(1024))) uint16_t sV1[kBN * kD];
+  __shared__ int sPos[kD], sNeg[kD], sDirty;
+
+  // With a multiple of 8 K/V heads each XCD keeps its own heads, so that a head's tiles are
+  // shared in one L2; otherwise consecutive ids go round the XCDs. Either way an XCD starts
+  // with its longest blocks.
+  int u, blk;
+  {
+    const int pid = blockIdx.x;
+    if (kv_heads % 8 == 0) {
+      const int xcd = pid & 7, local = pid >> 3;
+      u = xcd + 8 * (local / nblocks);
+      blk = local % nblocks;
+    } else {
+      u = pid % kv_heads;
+      blk = pid / kv_heads;
+    }
+  }
+  const int64_t row0 = __builtin_amdgcn_readfirstlane(blocks[4 * blk]);
+  const int n = __builtin_amdgcn_readfirstlane(blocks[4 * blk + 1]);
+  const int r0 = __builtin_amdgcn_readfirstlane(blocks[4 * blk + 2]);
+  const int rows = n * group;
+  const int i_first = r0 / group;                               // the block's tokens
+  const int nkeys = min(r0 + kBM - 1, rows - 1) / group + 1;    // keys that its last row sees
+  const int ntiles = (nkeys + kBN - 1) / kBN;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, col = lane & 31;
+  for (int d = tid; d < kD; d += kThreads) sPos[d] = sNeg[d] = 0x7fffffff;
+  if (tid == 0) sDirty = 0;
+
+  const int w0 = r0 + wave * 32;                 // the wave's rows
+  const bool wave_live = w0 < rows;
+  const int w_first = w0 / group;
+  const int w_last = min(w0 + 31, rows - 1) / group;
+  const int my_r = w0 + col;
+  const bool live = my_r < rows;
+  const int my_i = live ? my_r / group : i_first;
+  const int my_h = u * group + (live ? my_r - my_i * group : 0);
+
+  // ---- Q fragments: row my_r, channels 16 ks + 8 g .. +8 ----
+  x8 qf[kSteps];
+  {
+    const uint16_t* src = in.q + (row0 + my_i) * in.q_st + my_h * in.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(src + 16 * ks + 8 * g);
+      qf[ks] = __builtin_bit_cast(x8, w);
+    }
+  }
+
+  // lane's share of a tile load: kSegs segments of kSegRows rows per tensor, at fixed byte
+  // offsets from the tile's first row
+  const int seg_row = lane / kChunks, phys = lane % kChunks;
+  uint32_t koff[kSegs], voff[kSegs];
+#pragma unroll
+  for (int j = 0; j < kSegs; ++j) {
+    const int row = (j * kWaves + wave) * kSegRows + seg_row;
+    koff[j] = static_cast<uint32_t>(row * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row)));
+    voff[j] = static_cast<uint32_t>(row * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)));
+  }
+  const char* k_head = reinterpret_cast<const char*>(in.k + row0 * in.k_st + u * in.k_sh);
+  const char* v_head = reinterpret_cast<const char*>(in.v + row0 * in.v_st + u * in.v_sh);
+  auto issue_tile = [&](int a, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t k_rsrc = tile_rsrc(k_head + static_cast<int64_t>(a) * in.k_st * 2);
+    const __amdgpu_buffer_rsrc_t v_rsrc = tile_rsrc(v_head + static_cast<int64_t>(a) * in.v_st * 2);
+    const int last = nkeys - 1 - a;  // rows behind the last key repeat it
+#pragma unroll
+    for (int j = 0; j < kSegs; ++j) {
+      const int seg = j * kWaves + wave;
+      uint32_t ko = koff[j], vo = voff[j];
+      if (last < kBN - 1) {
+        const int row = seg * kSegRows + seg_row, r = min(row, last);
+        ko = static_cast<uint32_t>(r * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row)));
+        vo = static_cast<uint32_t>(r * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)));
+      }
+      load_to_lds16(k_rsrc, ko, 0, dk + seg * kSegRows * kD);
+      load_to_lds16(v_rsrc, vo, 0, dv + seg * kSegRows * kD);
+    }
+  };
+
+  f32x16 o[kDB];
+#pragma unroll
+  for (int db = 0; db < kDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
+  float m = -INFINITY, l = 0.f;
+
+  // transpose-read coordinates (16-lane group G = lane / 16)
+  const int G = lane >> 4, L = lane & 15;
+  const int tr_row = 4 * (G >> 1) + (L >> 2);
+  const int tr_col = 16 * (G & 1) + 4 * (L & 3);
+
+  // Running maximum m in scaled (exp2) units; it may lag the true one by up to kLazy, so that
+  // most tiles need no rescale (p <= 2^kLazy).
+  constexpr float kLazy = 8.f;
+  auto process = [&](int t, auto buf_tag) __attribute__((always_inline)) {
+    constexpr int kBuf = decltype(buf_tag)::value;
+    const uint16_t* tk = kBuf == 0 ? sK0 : sK1;
+    uint16_t* tv = kBuf == 0 ? sV0 : sV1;
+    const int a = t * kBN;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile t is there
+    const bool diagonal = a + kBN - 1 > i_first;      // some row does not see the whole tile
+    if (diagonal) {
+      constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+      for (int j = 0; j < kSegs; ++j) {
+        const int seg = j * kWaves + wave;
+        uint16_t* p = tv + seg * kSegRows * kD + lane * 8;
+        u32x4 w = *reinterpret_cast<const u32x4*>(p);
+        u16x2 mag = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          mag = __builtin_elementwise_max(mag, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+        if (mag[0] < kInf && mag[1] < kInf) continue;
+        const int row = seg * kSegRows + seg_row;
+        const int ch = 8 * (phys ^ swz_v<kD>(row));
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t b = p[i];
+          if ((b & 0x7fffu) < kInf) continue;
+          const bool nan = (b & 0x7fffu) > kInf;
+          if (nan || b < 0x8000u) atomicMin(&sPos[ch + i], a + row);
+          if (nan || b >= 0x8000u) atomicMin(&sNeg[ch + i], a + row);
+          p[i] = 0;
+        }
+        sDirty = 1;
+      }
+    }
+    __syncthreads();  // tile t is resident and every wave is done with the other buffer
+    const bool sees = wave_live && a <= w_last;
+    if (t + 1 < ntiles)
+      issue_tile(a + kBN, kBuf == 0 ? sK1 : sK0, kBuf == 0 ? sV1 : sV0);
+    if (!sees) return;
+
+    // ---- Sᵀ = K Qᵀ (kKT 32-key accumulators), the fragments of step ks + 1 read before the
+    // MFMAs of step ks ----
+    f32x16 s[kKT];
+#pragma unroll
+    for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s[kt][v] = 0.f;
+    x8 kf[2][kKT];
+    auto kload = [&](int ks, x8 (&dst)[kKT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int kt = 0; kt < kKT; ++kt) {
+        const int row = kt * 32 + col;
+        const int chunk = (2 * ks + g) ^ swz_k<kD>(row);
+        dst[kt] = *reinterpret_cast<const x8*>(tk + row * kD + chunk * 8);
+      }
+    };
+    kload(0, kf[0]);
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      if (ks + 1 < kSteps) kload(ks + 1, kf[(ks + 1) & 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kt = 0; kt < kKT; ++kt) s[kt] = E::mfma(kf[ks & 1][kt], qf[ks], s[kt]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // ---- online softmax ----
+    if (a + kBN - 1 > w_first) {  // keys behind the row's token
+#pragma unroll
+      for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int key = a + kt * 32 + (v >> 2) * 8 + g * 4 + (v & 3);
+          if (key > my_i) s[kt][v] = -INFINITY;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kt][v]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale_log2;
+    const bool grow = mx > m + kLazy;
+    if (__any(grow)) {
+      const float m_new = grow ? mx : m;
+      const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
+      l *= corr;
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[db][v] *= corr;
+      m = m_new;
+    }
+    float rs = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][v], scale_log2, -m));
+        s[kt][v] = p;
+        rs += p;
+      }
+    rs += __shfl_xor(rs, 32);
+    l += rs;
+
+    // ---- Oᵀ += Vᵀ Pᵀ, 16 keys per MFMA; the V fragments of MFMA i + kVA are read before
+    // MFMA i ----
+    constexpr int kItems = (kBN / 16) * kDB;
+    constexpr int kVA = 2;
+    x8 vf[kVA + 1];
+    auto vload = [&](int i, x8& dst) __attribute__((always_inline)) {
+      const int c = i / kDB, db = i % kDB;
+      const int e = 32 * db + tr_col;
+      const int lo_row = 16 * c + tr_row, hi_row = lo_row + 8;
+      const typename E::x4 lo = E::read_tr(tv + lo_row * kD + ((e >> 3) ^ swz_v<kD>(lo_row)) * 8 + (e & 7));
+      const typename E::x4 hi = E::read_tr(tv + hi_row * kD + ((e >> 3) ^ swz_v<kD>(hi_row)) * 8 + (e & 7));
+      dst = x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+#pragma unroll
+    for (int i = 0; i < kVA; ++i) vload(i, vf[i]);
+    x8 pb;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      if (i + kVA < kItems) vload(i + kVA, vf[(i + kVA) % (kVA + 1)]);
+      __builtin_amdgcn_sched_barrier(0x406);
+      const int c = i / kDB, db = i % kDB;
+      if (db == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pb[j] = static_cast<typename E::type>(s[c >> 1][(c & 1) * 8 + j]);
+      }
+      o[db] = E::mfma(vf[i % (kVA + 1)], pb, o[db]);
+      __builtin_amdgcn_sched_barrier(0x406);
+    }
+    if (diagonal && sDirty != 0) {
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int d = 32 * db + (v >> 2) * 8 + g * 4 + (v & 3);
+          if (sPos[d] <= my_i) o[db][v] += INFINITY;
+          if (sNeg[d] <= my_i) o[db][v] -= INFINITY;
+        }
+    }
+  };
+  __syncthreads();  // sPos, sNeg, sDirty
+  issue_tile(0, sK0, sV0);
+  for (int t = 0; t < ntiles; t += 2) {
+    process(t, std::integral_constant<int, 0>{});
+    if (t + 1 < ntiles) process(t + 1, std::integral_constant<int, 1>{});
+  }
+  const float inv_l = 1.0f / l;   // every row sees its own token: l > 0
+  __syncthreads();                // the epilogue reuses the tile buffers
+
+  // ---- epilogue: O / l through LDS to rows, kBN rows per buffer ----
+  auto stage_rows = [&](int r) -> uint16_t* {
+    const int which = r / kBN;
+    return which == 0 ? sK0 : which == 1 ? sK1 : which == 2 ? sV0 : sV1;
+  };
+  const int qr = wave * 32 + col;
+  uint16_t* sO = stage_rows(qr);
+#pragma unroll
+  for (int db = 0; db < kDB; ++db)
+#pragma unroll
+    for (int v = 0; v < 16; ++v)
+      sO[(qr % kBN) * kD + 32 * db + (v >> 2) * 8 + g * 4 + (v & 3)] = E::bits(o[db][v] * inv_l);
+  if (to.lse != nullptr && live && g == 0)
+    to.lse[(row0 + my_i) * to.l_st + my_h * to.l_sh] = (m + log2f(l)) * kLn2;
+  __syncthreads();
+  for (int r = tid / kChunks; r < kBM; r += kThreads / kChunks) {
+    if (r0 + r >= rows) continue;
+    const int i = (r0 + r) / group, h = u * group + (r0 + r) - i * group;
+    const int c8 = (tid % kChunks) * 8;
+    const u32x4 row8 = *reinterpret_cast<const u32x4*>(&stage_rows(r)[(r % kBN) * kD + c8]);
+    *reinterpret_cast<u32x4*>(to.out + (row0 + i) * to.o_st + h * to.o_sh + c8) = row8;
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+}  // namespace vdn
+
+using namespace vdn;
+
+VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k,
+                                 int64_t k_st, int64_t k_sh, const void* v, int64_t v_st,
+                                 int64_t v_sh, const int* blocks, int nblocks, int block_rows,
+                                 int kv_heads, int group, int head_dim, int dtype, float scale,
+                                 void* out, int64_t o_st, int64_t o_sh, float* lse, int64_t l_st,
+                                 int64_t l_sh, void* stream) {
+  const char* name = "vdn_causal_attention";
+  if (nblocks < 0 || kv_heads <= 0 || group <= 0)
+    return set_error(kInvalidArgument, "%s: bad geometry", name);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return set_error(kInvalidArgument, "%s: head_dim must be 64, 128 or 256", name);
+  if (dtype != 0 && dtype != 1)
+    return set_error(kInvalidArgument, "%s: dtype must be 0 (bf16) or 1 (fp16)", name);
+  if (block_rows != 128 && block_rows != 256)
+    return set_error(kInvalidArgument, "%s: block_rows must be 128 or 256", name);
+  if (!(scale > 0.f) || !isfinite(scale)) return set_error(kInvalidArgument, "%s: bad scale", name);
+  if (nblocks == 0) return kOk;
+  if (q == nullptr || k == nullptr || v == nullptr || blocks == nullptr || out == nullptr)
+    return set_error(kInvalidArgument, "%s: null pointer", name);
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || q_st % 8 || q_sh % 8 ||
+      k_st % 8 || k_sh % 8 || v_st % 8 || v_sh % 8 || o_st % 8 || o_sh % 8)
+    return set_error(kInvalidArgument, "%s: rows need 16-byte alignment", name);
+  // a lane's offset inside a tile of at most 128 keys is a 32-bit byte count
+  if (k_st < 0 || v_st < 0 || k_st > (1 << 22) || v_st > (1 << 22))
+    return set_error(kUnsupported, "%s: K/V token strides must be in [0, 2^22] elements", name);
+  const int64_t total = static_cast<int64_t>(nblocks) * kv_heads;
+  if (total > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many blocks", name);
+  const CausalIn in{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                    static_cast<const uint16_t*>(v), q_st, q_sh, k_st, k_sh, v_st, v_sh};
+  const CausalOut to{static_cast<uint16_t*>(out), lse, o_st, o_sh, l_st, l_sh};
+  const auto launch = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(total)), dim3(threads), 0,
+                       static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, group,
+                       scale * kLog2e);
+  };
+#define VDN_CAUSAL(D, F16)                                              \
+  (block_rows == 256 ? launch(causal_attn_kernel<D, 8, D == 256 ? 64 : 128, F16>, 512) \
+                     : launch(causal_attn_kernel<D, 4, D == 256 ? 32 : 64, F16>, 256))
+  if (dtype == 0)
+    head_dim == 64 ? VDN_CAUSAL(64, false) : head_dim == 128 ? VDN_CAUSAL(128, false) : VDN_CAUSAL(256, false);
+  else
+    head_dim == 64 ? VDN_CAUSAL(64, true) : head_dim == 128 ? VDN_CAUSAL(128, true) : VDN_CAUSAL(256, true);
+#undef VDN_CAUSAL
+  return check_launch(name);
+}
