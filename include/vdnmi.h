@@ -340,6 +340,50 @@ int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
                          int head_dim, int dtype, float scale, void* out, int64_t o_st,
                          int64_t o_sh, float* lse, int64_t l_st, int64_t l_sh, void* stream);
 
+/*
+ * The 8-bit key/value cache: k_codes uint8 [pages, kv_heads, page, head_dim], v_codes uint8 [pages,
+ * kv_heads, head_dim, page] (E4M3, 16-byte aligned), k_scales and v_scales uint8 [pages, kv_heads]
+ * (E8M0: exponent + 127, at least 27), contiguous; page a power of two in 16..256, head_dim 64,
+ * 128 or 256. table int32 [batch, width] (row stride table_st): the pages of each sequence in
+ * order. A page id outside [0, pages), a negative or too large length and offsets outside the rows
+ * are not followed; *faults (device int32) becomes 1.
+ *
+ * vdn_cache_write: rows offsets[i] .. offsets[i + 1] - 1 (int32 [batch + 1]; null: one row each)
+ * of key and value [rows, kv_heads, head_dim] (dtype 0 bf16, 1 fp16; (token, head) strides,
+ * multiples of 8) become tokens starts[i] .. of sequence i. A touched page's scale is the
+ * least 2^e >= 2^-100 with max |x| <= 448 * 2^e over its new finite values, or the page's own if that
+ * is larger and it holds earlier tokens (position 0 is in front of starts[i]); held codes are
+ * rounded again when the scale grows. Nonfinite values become NaN codes.
+ * vdn_cache_read: the reverse (NaN rows for a page that is not there, zeros from offsets[batch] on).
+ */
+int vdn_cache_write(void* k_codes, void* k_scales, void* v_codes, void* v_scales, int* faults,
+                    int pages, int kv_heads, int page, int head_dim, const int* table,
+                    int64_t table_st, int batch, int width, const int* starts, const int* offsets,
+                    const void* key, int64_t k_st, int64_t k_sh, const void* value, int64_t v_st,
+                    int64_t v_sh, int rows, int dtype, void* stream);
+int vdn_cache_read(const void* k_codes, const void* k_scales, const void* v_codes,
+                   const void* v_scales, int* faults, int pages, int kv_heads, int page,
+                   int head_dim, const int* table, int64_t table_st, int batch, int width,
+                   const int* starts, const int* offsets, void* key, int64_t k_st, int64_t k_sh,
+                   void* value, int64_t v_st, int64_t v_sh, int rows, int dtype, void* stream);
+
+/*
+ * Softmax attention of the `tokens` newest tokens of each sequence, whose K/V are in the cache
+ * already, over its lengths[b] cached tokens: query i sees tokens j < lengths[b] - tokens + 1
+ * + i; a row that sees none is zero, its lse -inf; rows of a sequence with a fault are NaN. q, out:
+ * [batch, tokens, kv_heads * group, head_dim] by (sequence, token, head) strides, multiples of 8,
+ * dtype 0 bf16 or 1 fp16; lse (nullable): fp32 [batch, tokens, heads] contiguous. workspace:
+ * 16-byte aligned, vdn_cache_attention_workspace's byte count; its contents need no preparation.
+ */
+int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                        const void* k_codes, const void* k_scales, const void* v_codes,
+                        const void* v_scales, int* faults, int pages, int kv_heads, int page,
+                        int head_dim, const int* table, int64_t table_st, int batch, int width,
+                        const int* lengths, int tokens, int group, int dtype, float scale,
+                        void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int vdn_cache_attention_workspace(int tokens, int group, int head_dim, int64_t* bytes);
+
 /* vdn_window_attention with the output quantized in the epilogue instead of stored as bf16:
  * query row q, head h -> MXFP8 codes[q, 128 (chunk0 + h) .. +128) of a [rows, kp] code
  * matrix and the four E8M0 scales of that chunk in its SWIZZLE_32_4_4 scale array; the same

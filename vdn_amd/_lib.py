@@ -66,6 +66,14 @@ SIGNATURES = {
     "vdn_causal_attention": [_ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i32,
                              _i32, _i32, _i32, _i32, _i32, _f32, _ptr, _i64, _i64, _ptr, _i64,
                              _i64, _ptr],
+    "vdn_cache_write": [_ptr, _ptr, _ptr, _ptr, _ptr, _i32, _i32, _i32, _i32, _ptr, _i64, _i32,
+                        _i32, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _i32, _ptr],
+    "vdn_cache_read": [_ptr, _ptr, _ptr, _ptr, _ptr, _i32, _i32, _i32, _i32, _ptr, _i64, _i32,
+                       _i32, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _i32, _ptr],
+    "vdn_cache_attention": [_ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i32, _i32,
+                            _i32, _i32, _ptr, _i64, _i32, _i32, _ptr, _i32, _i32, _i32, _f32,
+                            _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr],
+    "vdn_cache_attention_workspace": [_i32, _i32, _i32, _ptr],
     "vdn_vda_readout_mxfp8": [_ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _i32, _f32, _ptr, _i64,
                               _i64, _i64, _ptr, _ptr, _i64, _i32, _i32, _i32, _i32, _ptr],
     "vdn_vda_readout_gated": [_ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _i32, _f32, _ptr, _i64,

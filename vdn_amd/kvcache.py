@@ -1,0 +1,226 @@
+"""The 8-bit key/value cache: pages of E4M3 codes with one E8M0 scale per page, head and side.
+
+The block format is that of the MXFP8 operands (mxfp8.py) with another block: a page of one
+sequence's tokens and one K/V head shares a power-of-two scale 2^e, the least e >= -100 with
+max |x| <= 448 * 2^e over the page's finite values. K codes are [pages, kv_heads, page, D]; V
+codes [pages, kv_heads, D, page], the order in which the attention reads them.
+
+The caller owns the pool's bookkeeping: an int32 table [batch, width] names each sequence's pages
+in order, an int32 tensor the tokens that it holds. Both stay on the device, so that a decode step
+can be captured into a graph and replayed as they change. A page id outside the pool, a
+length that the table cannot hold, offsets that do not fit the rows: kernels follow none of
+them; they raise the cache's `faults` word, and KVCache.check() reports it.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+PAGES = (16, 32, 64, 128, 256)
+HEAD_DIMS = (64, 128, 256)
+_DTYPES = (torch.bfloat16, torch.float16)
+
+
+@dataclass(frozen=True)
+class KVCache:
+    """k_codes uint8 [pages, kv_heads, page, D], k_scales uint8 [pages, kv_heads] (e + 127), v_codes
+    uint8 [pages, kv_heads, D, page], v_scales like k_scales, faults int32 [1]; all contiguous."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+    faults: torch.Tensor
+
+    def __post_init__(self):
+        k, v = self.k_codes, self.v_codes
+        if k.ndim != 4 or k.shape[0] <= 0 or k.shape[1] <= 0 or k.shape[2] not in PAGES \
+                or k.shape[3] not in HEAD_DIMS:
+            raise ValueError(f"K codes must be [pages, kv_heads, page in {PAGES}, D in {HEAD_DIMS}]")
+        if v.shape != (*k.shape[:2], k.shape[3], k.shape[2]) or \
+                any(s.shape != k.shape[:2] for s in (self.k_scales, self.v_scales)) or \
+                self.faults.shape != (1,):
+            raise ValueError("V codes, scales and faults do not match the K codes")
+        if any(t.dtype != torch.uint8 for t in (k, v, self.k_scales, self.v_scales)) or \
+                self.faults.dtype != torch.int32:
+            raise ValueError("codes and scales must be uint8, faults int32")
+        if any(t.device != k.device or not t.is_contiguous()
+               for t in (k, v, self.k_scales, self.v_scales, self.faults)):
+            raise ValueError("the cache's tensors must be contiguous and on one device")
+
+    @property
+    def pages(self):
+        return self.k_codes.shape[0]
+
+    @property
+    def kv_heads(self):
+        return self.k_codes.shape[1]
+
+    @property
+    def page(self):
+        return self.k_codes.shape[2]
+
+    @property
+    def head_dim(self):
+        return self.k_codes.shape[3]
+
+    @property
+    def device(self):
+        return self.k_codes.device
+
+    def check(self):
+        """Reads the fault word on the host (waits for the device) and raises if it is set."""
+        if int(self.faults.item()):
+            self.faults.zero_()
+            raise RuntimeError("a table, length or offset named what the cache does not have")
+
+
+def empty_cache(pages, kv_heads, head_dim, page=64, *, device):
+    """A pool of `pages` pages of `page` tokens (16 .. 256, a power of two)."""
+    if any(type(x) is not int or x <= 0 for x in (pages, kv_heads)):
+        raise ValueError("pages and kv_heads must be positive integers")
+    if page not in PAGES or head_dim not in HEAD_DIMS:
+        raise ValueError(f"page must be in {PAGES} and head_dim in {HEAD_DIMS}")
+
+    def codes(*shape):
+        return torch.empty((pages, kv_heads, *shape), dtype=torch.uint8, device=device)
+
+    return KVCache(codes(page, head_dim), codes(), codes(head_dim, page), codes(),
+                   torch.zeros(1, dtype=torch.int32, device=device))
+
+
+def _check_cache(cache, what):
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is inference-only; use no_grad/inference_mode")
+    if not isinstance(cache, KVCache):
+        raise TypeError("cache must be a KVCache")
+    if cache.device.type != "cuda":
+        raise ValueError("the cache must be on a CUDA (HIP) device")
+
+
+def _check_indices(cache, table, vectors):
+    """`table` int32 [batch, width], vectors [(name, tensor, length)] int32."""
+    if table.ndim != 2 or table.dtype != torch.int32 or table.device != cache.device \
+            or table.stride(1) != 1 and table.shape[1] > 1:
+        raise ValueError("table must be int32 [batch, width] on the cache's device, unit inner stride")
+    for name, t, n in vectors:
+        if t.shape != (n,) or t.dtype != torch.int32 or t.device != cache.device \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
+
+
+def _cache_args(cache):
+    return (cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
+            cache.v_scales.data_ptr(), cache.faults.data_ptr(), cache.pages, cache.kv_heads,
+            cache.page, cache.head_dim)
+
+
+def _move(name, cache, key, value, table, starts, offsets):
+    rows = key.shape[0]
+    batch = table.shape[0]
+    _check_indices(cache, table, [("starts", starts, batch)]
+                   + ([] if offsets is None else [("offsets", offsets, batch + 1)]))
+    if offsets is None and rows != batch:
+        raise ValueError("without offsets there is one row for each sequence")
+    if rows > 2 ** 31 - 1:
+        raise ValueError("too many rows")
+    with torch.cuda.device(cache.device):
+        _lib.call(name, *_cache_args(cache), table.data_ptr(), table.stride(0), batch,
+                  table.shape[1], starts.data_ptr(), _lib.ptr(offsets), key.data_ptr(),
+                  key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+                  value.stride(1), rows, int(key.dtype == torch.float16),
+                  _lib.stream(cache.device))
+
+
+def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
+    """Appends packed rows to their sequences.
+
+    key, value [rows, kv_heads, D] (BF16 or FP16, unit channel stride); rows offsets[i] ..
+    offsets[i + 1] - 1 (int32 [batch + 1], rising from 0; one row each without it) become
+    the tokens starts[i], starts[i] + 1, ... of sequence i, in the pages that table[i] names.
+    Rows from offsets[batch] on are not written.
+
+    A page that holds earlier tokens of the sequence (the first one, if starts[i] is not a multiple
+    of the page) keeps the larger of its scale and the new tokens' one; if that is the new
+    tokens', the held codes are rounded once more. A nonfinite value becomes the NaN code and
+    leaves the scale alone. Two sequences must not bring rows for one page in the same call."""
+    _check_cache(cache, "write_cache")
+    if key.ndim != 3 or key.shape[1:] != (cache.kv_heads, cache.head_dim) or value.shape != key.shape:
+        raise ValueError("key and value must be [rows, kv_heads, D] of the cache")
+    if key.dtype not in _DTYPES or value.dtype != key.dtype or \
+            any(x.stride(-1) != 1 or x.device != cache.device for x in (key, value)):
+        raise ValueError("key and value must share BF16 or FP16, unit innermost stride and the "
+                         "cache's device")
+    _move("vdn_cache_write", cache, key, value, table, starts, offsets)
+
+
+def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bfloat16):
+    """The values of cached tokens, packed: rows offsets[i] .. offsets[i + 1] - 1 of the two
+    fresh [rows, kv_heads, D] tensors (keys, values) are the tokens starts[i], ... of sequence i
+    (arguments as write_cache). Exact in BF16; FP16 rounds what is under its normal range and
+    saturates at 65504. Rows of a page that is not there are NaN, rows from offsets[batch] on
+    zero."""
+    _check_cache(cache, "read_cache")
+    if type(rows) is not int or rows < 0:
+        raise ValueError("rows must be a non-negative integer")
+    if dtype not in _DTYPES:
+        raise ValueError("dtype must be BF16 or FP16")
+    key, value = (torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=dtype,
+                              device=cache.device) for _ in range(2))
+    _move("vdn_cache_read", cache, key, value, table, starts, offsets)
+    return key, value
+
+
+def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return_lse=False,
+                    out=None):
+    """Softmax attention of each sequence's newest tokens over all its cached ones.
+
+    query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16, H a multiple of the cache's
+    kv_heads (query head h reads K/V head h // (H / kv_heads)); lengths int32 [batch] counts
+    the tokens that the cache holds, the Q queries' own among them: query i sees the tokens j <
+    lengths - Q + 1 + i. A row that sees none is zero (LSE -inf). Returns a tensor like the query,
+    with return_lse also the natural-log sum of exp of the scaled scores, fp32 [batch, Q, H]
+    (or [batch, H]). Scores, sums and the output are accumulated in fp32; probabilities are
+    rounded to the query's dtype before the product with V, the codes' values are exact.
+
+    A sequence with a bad page id or length gets NaN (see KVCache.check). For FP16 queries
+    the cached values must be within FP16's range."""
+    _check_cache(cache, "cache_attention")
+    if query.ndim not in (3, 4):
+        raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
+    q = query.unsqueeze(1) if query.ndim == 3 else query
+    batch, tokens, heads, d = q.shape
+    if d != cache.head_dim or heads <= 0 or heads % cache.kv_heads or tokens <= 0:
+        raise ValueError("query heads must be a multiple of the cache's, D the same, Q positive")
+    if q.dtype not in _DTYPES or q.stride(-1) != 1 or q.device != cache.device:
+        raise ValueError("query must be BF16 or FP16 with unit innermost stride, on the cache's device")
+    _check_indices(cache, table, [("lengths", lengths, batch)])
+    if table.shape != (batch, table.shape[1]) or table.shape[1] <= 0:
+        raise ValueError("table must name at least one page for each sequence of the query")
+    if table.shape[1] * cache.page > 2 ** 31 - 1024:
+        raise ValueError("the table is too wide")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValueError("scale must be finite and positive")
+    if out is None:
+        out = torch.empty(query.shape, dtype=q.dtype, device=q.device)
+    elif (out.shape != query.shape or out.dtype != q.dtype or out.device != q.device
+          or out.stride(-1) != 1):
+        raise ValueError("out must be a view like the query, unit channel stride")
+    o = out.unsqueeze(1) if out.ndim == 3 else out
+    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
+    group = heads // cache.kv_heads
+    with torch.cuda.device(q.device):
+        nbytes = ctypes.c_int64(0)
+        _lib.call("vdn_cache_attention_workspace", tokens, group, d, ctypes.addressof(nbytes))
+        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
+        _lib.call("vdn_cache_attention", q.data_ptr(), *q.stride()[:3], *_cache_args(cache),
+                  table.data_ptr(), table.stride(0), batch, table.shape[1], lengths.data_ptr(),
+                  tokens, group, int(q.dtype == torch.float16), scale, o.data_ptr(),
+                  *o.stride()[:3], _lib.ptr(lse), workspace.data_ptr(), nbytes.value,
+                  _lib.stream(q.device))
+    return (out, lse) if return_lse else out
