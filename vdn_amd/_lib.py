@@ -144,7 +144,7 @@ _TIMERS: list[LaunchTimer] = []
 
 def call(name: str, *args) -> None:
     lib = load()
-    timers = [t for t in _TIMERS if name in t.names]
+    timers = [t for t in _TIMERS if name in t.names] if _TIMERS else None
     if timers:
         start = torch.cuda.Event(enable_timing=True)
         start.record()
@@ -165,7 +165,19 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream(device: torch.device) -> int:
     """The caller's current HIP stream on `device` (launches never go to a private stream)."""
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None
+                                              else index)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() with `device` as the current one: a launch goes to the current device, whatever
+    its stream's is."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

@@ -83,37 +83,40 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
         raise RuntimeError("causal attention is inference-only; use no_grad/inference_mode")
     if not isinstance(plan, CausalPlan):
         raise TypeError("plan must be prepared with prepare_causal_plan")
-    if any(x.ndim != 3 for x in (query, key, value)):
+    if query.ndim != 3:
         raise ValueError("Q/K/V must be [rows, heads, D]")
     rows, heads, d = query.shape
-    if (heads != plan.heads or key.shape != (rows, plan.kv_heads, d) or value.shape != key.shape
+    kv_heads, dtype, device = plan.kv_heads, query.dtype, query.device
+    if (heads != plan.heads or key.shape != (rows, kv_heads, d) or value.shape != key.shape
             or rows < plan.rows or d not in (64, 128, 256)):
         raise ValueError("Q/K/V do not match the plan's heads and rows, or D is not 64, 128 or 256")
-    if query.dtype not in (torch.bfloat16, torch.float16) or \
-            any(x.dtype != query.dtype or x.stride(-1) != 1 for x in (query, key, value)):
+    q_st, q_sh, q_sd = query.stride()
+    k_st, k_sh, k_sd = key.stride()
+    v_st, v_sh, v_sd = value.stride()
+    if dtype not in (torch.bfloat16, torch.float16) or key.dtype != dtype or value.dtype != dtype \
+            or q_sd != 1 or k_sd != 1 or v_sd != 1:
         raise ValueError("Q/K/V must share BF16 or FP16 and have unit innermost stride")
-    if not query.is_cuda or any(x.device != query.device for x in (key, value)) \
-            or query.device != plan.device:
+    if device.type != "cuda" or key.device != device or value.device != device \
+            or plan.blocks.device != device:
         raise ValueError("Q/K/V and prepared plan must be on the same CUDA device")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = torch.empty((rows, heads, d), dtype=query.dtype, device=query.device)
-        out[plan.rows:].zero_()
-    elif (out.shape != (rows, heads, d) or out.dtype != query.dtype or out.device != query.device
-          or out.stride(-1) != 1):
+        out = torch.empty((rows, heads, d), dtype=dtype, device=device)
+        if rows > plan.rows:
+            out[plan.rows:].zero_()
+    elif (out.shape != query.shape or out.dtype != dtype or out.device != device
+          or out.stride(2) != 1):
         raise ValueError("out must be a [rows, H, D] view like the queries, unit channel stride")
     lse = None
     if return_lse:
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=query.device)
-        lse[plan.rows:].fill_(-math.inf)
-    with torch.cuda.device(query.device):
-        _lib.call("vdn_causal_attention", query.data_ptr(), query.stride(0), query.stride(1),
-                  key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(),
-                  value.stride(0), value.stride(1), plan.blocks.data_ptr(),
-                  plan.blocks.shape[0], plan.block_rows, plan.kv_heads, heads // plan.kv_heads,
-                  d, int(query.dtype == torch.float16), scale, out.data_ptr(), out.stride(0),
-                  out.stride(1), _lib.ptr(lse), 0 if lse is None else lse.stride(0),
-                  0 if lse is None else lse.stride(1), _lib.stream(query.device))
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=device)
+        if rows > plan.rows:
+            lse[plan.rows:].fill_(-math.inf)
+    _lib.call_on(device, "vdn_causal_attention", query.data_ptr(), q_st, q_sh, key.data_ptr(),
+                 k_st, k_sh, value.data_ptr(), v_st, v_sh, plan.blocks.data_ptr(),
+                 plan.blocks.shape[0], plan.block_rows, kv_heads, heads // kv_heads, d,
+                 int(dtype == torch.float16), scale, out.data_ptr(), out.stride(0), out.stride(1),
+                 _lib.ptr(lse), heads, 1, _lib.stream(device))
     return (out, lse) if return_lse else out

@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -98,42 +99,44 @@ def _check_cache(cache, what):
         raise RuntimeError(f"{what} is inference-only; use no_grad/inference_mode")
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
-    if cache.device.type != "cuda":
+    if cache.k_codes.device.type != "cuda":
         raise ValueError("the cache must be on a CUDA (HIP) device")
 
 
-def _check_indices(cache, table, vectors):
-    """`table` int32 [batch, width], vectors [(name, tensor, length)] int32."""
-    if table.ndim != 2 or table.dtype != torch.int32 or table.device != cache.device \
+def _check_table(table, device):
+    if table.ndim != 2 or table.dtype != torch.int32 or table.device != device \
             or table.stride(1) != 1 and table.shape[1] > 1:
         raise ValueError("table must be int32 [batch, width] on the cache's device, unit inner stride")
-    for name, t, n in vectors:
-        if t.shape != (n,) or t.dtype != torch.int32 or t.device != cache.device \
-                or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
+
+
+def _check_vector(name, t, n, device):
+    if t.shape != (n,) or t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
 
 
 def _cache_args(cache):
-    return (cache.k_codes.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
-            cache.v_scales.data_ptr(), cache.faults.data_ptr(), cache.pages, cache.kv_heads,
-            cache.page, cache.head_dim)
+    k = cache.k_codes
+    return (k.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
+            cache.v_scales.data_ptr(), cache.faults.data_ptr(), *k.shape)
 
 
 def _move(name, cache, key, value, table, starts, offsets):
-    rows = key.shape[0]
-    batch = table.shape[0]
-    _check_indices(cache, table, [("starts", starts, batch)]
-                   + ([] if offsets is None else [("offsets", offsets, batch + 1)]))
-    if offsets is None and rows != batch:
+    rows, device = key.shape[0], cache.k_codes.device
+    _check_table(table, device)
+    batch, width = table.shape
+    _check_vector("starts", starts, batch, device)
+    if offsets is not None:
+        _check_vector("offsets", offsets, batch + 1, device)
+    elif rows != batch:
         raise ValueError("without offsets there is one row for each sequence")
     if rows > 2 ** 31 - 1:
         raise ValueError("too many rows")
-    with torch.cuda.device(cache.device):
-        _lib.call(name, *_cache_args(cache), table.data_ptr(), table.stride(0), batch,
-                  table.shape[1], starts.data_ptr(), _lib.ptr(offsets), key.data_ptr(),
-                  key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-                  value.stride(1), rows, int(key.dtype == torch.float16),
-                  _lib.stream(cache.device))
+    k_st, k_sh, _ = key.stride()
+    v_st, v_sh, _ = value.stride()
+    _lib.call_on(device, name, *_cache_args(cache), table.data_ptr(), table.stride(0), batch, width,
+                 starts.data_ptr(), _lib.ptr(offsets), key.data_ptr(), k_st, k_sh,
+                 value.data_ptr(), v_st, v_sh, rows, int(key.dtype == torch.float16),
+                 _lib.stream(device))
 
 
 def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
@@ -149,10 +152,12 @@ def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
     tokens', the held codes are rounded once more. A nonfinite value becomes the NaN code and
     leaves the scale alone. Two sequences must not bring rows for one page in the same call."""
     _check_cache(cache, "write_cache")
-    if key.ndim != 3 or key.shape[1:] != (cache.kv_heads, cache.head_dim) or value.shape != key.shape:
+    k = cache.k_codes
+    if key.ndim != 3 or key.shape[1] != k.shape[1] or key.shape[2] != k.shape[3] \
+            or value.shape != key.shape:
         raise ValueError("key and value must be [rows, kv_heads, D] of the cache")
-    if key.dtype not in _DTYPES or value.dtype != key.dtype or \
-            any(x.stride(-1) != 1 or x.device != cache.device for x in (key, value)):
+    if key.dtype not in _DTYPES or value.dtype != key.dtype or key.stride(2) != 1 \
+            or value.stride(2) != 1 or key.device != k.device or value.device != k.device:
         raise ValueError("key and value must share BF16 or FP16, unit innermost stride and the "
                          "cache's device")
     _move("vdn_cache_write", cache, key, value, table, starts, offsets)
@@ -169,8 +174,9 @@ def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bflo
         raise ValueError("rows must be a non-negative integer")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be BF16 or FP16")
-    key, value = (torch.empty((rows, cache.kv_heads, cache.head_dim), dtype=dtype,
-                              device=cache.device) for _ in range(2))
+    _, heads, _, d = cache.k_codes.shape
+    key = torch.empty((rows, heads, d), dtype=dtype, device=cache.k_codes.device)
+    value = torch.empty_like(key)
     _move("vdn_cache_read", cache, key, value, table, starts, offsets)
     return key, value
 
@@ -192,35 +198,50 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     _check_cache(cache, "cache_attention")
     if query.ndim not in (3, 4):
         raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
-    q = query.unsqueeze(1) if query.ndim == 3 else query
-    batch, tokens, heads, d = q.shape
-    if d != cache.head_dim or heads <= 0 or heads % cache.kv_heads or tokens <= 0:
+    k, dtype, device = cache.k_codes, query.dtype, query.device
+    _, kv_heads, page, dim = k.shape
+    if query.ndim == 4:
+        batch, tokens, heads, d = query.shape
+        q_sb, q_st, q_sh, q_sd = query.stride()
+    else:
+        batch, heads, d = query.shape
+        q_sb, q_sh, q_sd = query.stride()
+        tokens, q_st = 1, 0
+    if d != dim or heads <= 0 or heads % kv_heads or tokens <= 0:
         raise ValueError("query heads must be a multiple of the cache's, D the same, Q positive")
-    if q.dtype not in _DTYPES or q.stride(-1) != 1 or q.device != cache.device:
+    if dtype not in _DTYPES or q_sd != 1 or device != k.device:
         raise ValueError("query must be BF16 or FP16 with unit innermost stride, on the cache's device")
-    _check_indices(cache, table, [("lengths", lengths, batch)])
-    if table.shape != (batch, table.shape[1]) or table.shape[1] <= 0:
+    _check_table(table, device)
+    _check_vector("lengths", lengths, batch, device)
+    if table.shape[0] != batch or table.shape[1] <= 0:
         raise ValueError("table must name at least one page for each sequence of the query")
-    if table.shape[1] * cache.page > 2 ** 31 - 1024:
+    if table.shape[1] * page > 2 ** 31 - 1024:
         raise ValueError("the table is too wide")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = torch.empty(query.shape, dtype=q.dtype, device=q.device)
-    elif (out.shape != query.shape or out.dtype != q.dtype or out.device != q.device
+        out = torch.empty(query.shape, dtype=dtype, device=device)
+    elif (out.shape != query.shape or out.dtype != dtype or out.device != device
           or out.stride(-1) != 1):
         raise ValueError("out must be a view like the query, unit channel stride")
-    o = out.unsqueeze(1) if out.ndim == 3 else out
-    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=q.device) if return_lse else None
-    group = heads // cache.kv_heads
-    with torch.cuda.device(q.device):
-        nbytes = ctypes.c_int64(0)
-        _lib.call("vdn_cache_attention_workspace", tokens, group, d, ctypes.addressof(nbytes))
-        workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=q.device)
-        _lib.call("vdn_cache_attention", q.data_ptr(), *q.stride()[:3], *_cache_args(cache),
-                  table.data_ptr(), table.stride(0), batch, table.shape[1], lengths.data_ptr(),
-                  tokens, group, int(q.dtype == torch.float16), scale, o.data_ptr(),
-                  *o.stride()[:3], _lib.ptr(lse), workspace.data_ptr(), nbytes.value,
-                  _lib.stream(q.device))
+    o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
+    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=device) if return_lse else None
+    group = heads // kv_heads
+    nbytes = _workspace_bytes(device.index, tokens, group, d)
+    # from the allocator in stream order: calls on other streams and captured graphs have their own
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _lib.call_on(device, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
+                 *_cache_args(cache), table.data_ptr(), table.stride(0), batch, table.shape[1],
+                 lengths.data_ptr(), tokens, group, int(dtype == torch.float16), scale,
+                 out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), workspace.data_ptr(), nbytes,
+                 _lib.stream(device))
     return (out, lse) if return_lse else out
+
+
+@lru_cache(maxsize=None)
+def _workspace_bytes(device_index, tokens, group, head_dim):
+    nbytes = ctypes.c_int64(0)
+    _lib.call_on(torch.device("cuda", device_index), "vdn_cache_attention_workspace", tokens, group,
+                 head_dim, ctypes.addressof(nbytes))
+    return nbytes.value
