@@ -59,7 +59,7 @@ def test_entry_points_validate_before_launching():
                              (dict(c=cache(codes=None)), b"null"), (dict(key=None), b"null"),
                              (dict(starts=None), b"null"), (dict(table=None), b"null"),
                              (dict(k_st=132), b"16-byte"), (dict(key=p + 2), b"16-byte"),
-                             (dict(c=cache(heads=1 << 17)), b"too many")):
+                             (dict(c=cache(heads=1 << 30)), b"too many")):
             assert move(fn, **change) != 0, change
             assert word in lib.vdn_last_error(), change
         assert move(fn, rows=0, key=None) == 0

@@ -1,8 +1,10 @@
 // Writing rows into the 8-bit key/value cache, and reading them back (kv_cache.h).
 //
 // Both move memory only: a write reads 2 bytes and writes 1 per value, a read the reverse. A
-// workgroup takes one page of one sequence, one K/V head and one side. Rows are 16-bit and token
-// major; V goes through LDS to change to the cache's channel-major order and back.
+// workgroup takes one page of one sequence, one K/V head and one side; a wave tile is 2048 values,
+// four 16-byte pieces of 8 values a lane. K's order is that of the rows. V's codes are channel
+// major: a lane takes the same 8 channels of 4 consecutive positions and transposes its 4 x 8
+// codes in registers, so that it moves 4 bytes of each channel, 16 lanes the 64 of a page row.
 //
 // Which page a workgroup takes: sequence i brings rows [offsets[i], offsets[i + 1]) and can touch
 // at most (rows >> log_page) + 2 pages, so with base_i = (offsets[i] >> log_page) + 2 i the
@@ -15,7 +17,7 @@
 namespace vdn {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kTileValues = 2048;
 
 struct Rows {
   uint16_t* k;
@@ -39,6 +41,18 @@ struct Piece {
   int64_t row;
 };
 
+// A workgroup's slot, K/V head and side. The heads of a page's rows lie next to each other in
+// memory, so they go to neighbouring workgroups.
+struct Item {
+  int slot, u;
+  bool v;
+};
+
+__device__ __forceinline__ Item item_of(const KvCache& c) {
+  const int w = blockIdx.x, page = w / (2 * c.kv_heads), rest = w - page * 2 * c.kv_heads;
+  return Item{page, rest % c.kv_heads, rest >= c.kv_heads};
+}
+
 __device__ __forceinline__ int seq_base(const Seqs& s, int i, int log_page) {
   return (s.offsets[i] >> log_page) + 2 * i;
 }
@@ -47,28 +61,42 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
   const int log_page = c.log_page;
   Piece p{0, 0, 0, 0, 0};
   int64_t first, end;
-  int j = 0;
+  int j = 0, start;
   if (s.offsets == nullptr) {
-    p.seq = slot;
+    p.seq = min(slot, s.batch);
     first = min(slot, rows);
     end = min(slot + 1, rows);
-    if (slot >= s.batch) return p.seq = s.batch, p.row = first, p.n = static_cast<int>(end - first), p;
+    if (p.seq == s.batch) {
+      p.row = first;
+      p.n = static_cast<int>(end - first);
+      return p;
+    }
+    start = s.starts[p.seq];
   } else {
     // the last i in [0, batch] with base_i <= slot
     const int lane = threadIdx.x & 63;
     int lo = 0, step = 1;
     while (static_cast<int64_t>(step) * 64 < s.batch + 1) step *= 64;
-    for (; step >= 1; step /= 64) {
+    for (; step > 1; step /= 64) {
       const int64_t i = lo + static_cast<int64_t>(lane) * step;
       const bool le = i <= s.batch && seq_base(s, static_cast<int>(i), log_page) <= slot;
       const int found = __popcll(__ballot(le));
       if (found == 0) return p;
-      lo += (found - 1) * step;
+      lo = min(lo + (found - 1) * step, s.batch);
     }
-    p.seq = min(lo, s.batch);
-    j = slot - seq_base(s, p.seq, log_page);
+    // the last round has loaded what the sequence needs: one memory latency less
+    const int i = min(lo + lane, s.batch);
+    const int off = s.offsets[i], next = s.offsets[min(i + 1, s.batch)];
+    const int from = s.batch > 0 ? s.starts[min(i, s.batch - 1)] : 0;
+    const int base = (off >> log_page) + 2 * i;
+    const int found = __popcll(__ballot(lo + lane <= s.batch && base <= slot));
+    if (found == 0) return p;
+    p.seq = lo + found - 1;
+    j = slot - __builtin_amdgcn_readlane(base, found - 1);
     if (j < 0) return p;
-    const int o0 = s.offsets[p.seq], o1 = p.seq == s.batch ? rows : s.offsets[p.seq + 1];
+    start = __builtin_amdgcn_readlane(from, found - 1);
+    const int o0 = __builtin_amdgcn_readlane(off, found - 1);
+    const int o1 = p.seq == s.batch ? rows : __builtin_amdgcn_readlane(next, found - 1);
     if (o0 < 0 || o1 < o0 || o1 > rows) *c.faults = 1;
     first = min(max(o0, 0), rows);
     end = min(max(o1, 0), rows);
@@ -78,13 +106,13 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
       return p;
     }
   }
-  const int64_t start = max(s.starts[p.seq], 0), stop = start + end - first;
-  const int64_t index = (start >> log_page) + j;
-  const int64_t lo = max(start, index << log_page), hi = min(stop, (index + 1) << log_page);
-  p.index = s.starts[p.seq] < 0 ? -1 : static_cast<int>(index);   // -1: a fault, no page
+  const int64_t from = max(start, 0), stop = from + end - first;
+  const int64_t index = (from >> log_page) + j;
+  const int64_t lo = max(from, index << log_page), hi = min(stop, (index + 1) << log_page);
+  p.index = start < 0 ? -1 : static_cast<int>(index);   // -1: a fault, no page
   p.lo = static_cast<int>(lo - (index << log_page));
   p.n = end > first ? static_cast<int>(max(hi - lo, static_cast<int64_t>(-1))) : 0;
-  p.row = first + lo - start;
+  p.row = first + lo - from;
   return p;
 }
 
@@ -119,100 +147,146 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t codes, float up) {
   return e4m3x4_scaled(lo[0], lo[1], hi[0], hi[1], up);
 }
 
-template <int kD, bool kF16>
-__global__ void __launch_bounds__(kThreads)
-cache_write_kernel(KvCache c, Rows rows, Seqs s) {
-  constexpr int kChunks = kD / 8;             // 8-value pieces of a row
-  constexpr int kStep = kThreads / kChunks;   // rows of a pass
-  const int page = 1 << c.log_page, pitch = page + 4;
-  extern __shared__ uint8_t tile[];           // V: [kD][pitch]
-  __shared__ uint32_t s_mag[kThreads / 64];
-  const Piece p = find_piece(c, s, rows.count, blockIdx.x);
-  if (p.n <= 0 || p.seq >= s.batch) return;
-  const int u = blockIdx.y, tid = threadIdx.x;
-  const bool is_v = blockIdx.z != 0;
+// Piece j (0..3) of tile `t` of a page for this lane: its position in the page and its first
+// channel. V: positions 4 a + j of up to 64 positions x 32 channels (the page's own 16 or 32
+// positions x 128 or 64).
+struct Spot {
+  int pos, ch;
+};
+
+template <int kD, bool kV>
+__device__ __forceinline__ Spot spot(int t, int j, int lane, int log_page) {
+  if (!kV) {
+    const int piece = t * 256 + j * 64 + lane;
+    return Spot{piece / (kD / 8), piece % (kD / 8) * 8};
+  }
+  const int log_a = min(log_page - 2, 4);             // runs of 4 positions: 2^log_a a tile
+  const int groups = 64 >> log_a;                     // 8-channel groups a tile
+  const int across = max(kD / 8 / groups, 1);         // tiles side by side
+  const int a = lane & ((1 << log_a) - 1), cg = lane >> log_a;
+  return Spot{((t / across) << (log_a + 2)) + 4 * a + j, (t % across * groups + cg) * 8};
+}
+
+// kTiles wave tiles per wave; the workgroup's waves hold the whole page. (A page of 16 positions
+// and 64 channels is half a tile: the lanes behind it have a position or channel outside.)
+template <int kD, int kTiles, bool kF16, bool kV>
+__device__ __forceinline__ void write_page(const KvCache& c, const Rows& rows, const Seqs& s,
+                                           const Piece& p, int u) {
+  __shared__ uint32_t s_mag[16];
+  const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = threads >> 6;
+  const int page = 1 << c.log_page;
+  const int64_t st = kV ? rows.v_st : rows.k_st;
+  const uint16_t* src = (kV ? rows.v + u * rows.v_sh : rows.k + u * rows.k_sh) + p.row * st;
+  const int end = p.lo + p.n;
+
+  // ---- the new rows (on their way before the page is looked up), and their largest finite
+  // magnitude (16-bit ones order as integers) ----
+  u32x4 w[kTiles][4];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Spot at = spot<kD, kV>(t * waves + wave, j, lane, c.log_page);
+      w[t][j] = u32x4{0, 0, 0, 0};
+      if (at.pos >= p.lo && at.pos < end && at.ch < kD)
+        w[t][j] = *reinterpret_cast<const u32x4*>(src + (at.pos - p.lo) * st + at.ch);
+    }
   const int id = cache_page(c, s.table + p.seq * s.t_st, p.index, s.width);
   if (id < 0) return;
   const int64_t block = static_cast<int64_t>(id) * c.kv_heads + u;
-  uint8_t* codes = (is_v ? c.v : c.k) + block * page * kD;
-  uint8_t* scale = (is_v ? c.vs : c.ks) + block;
-  const int64_t st = is_v ? rows.v_st : rows.k_st;
-  const uint16_t* src = (is_v ? rows.v + u * rows.v_sh : rows.k + u * rows.k_sh) + p.row * st;
-  const int ch = tid % kChunks, r0 = tid / kChunks;
-
-  // ---- largest finite magnitude of the new rows (16-bit magnitudes order as integers) ----
+  uint8_t* codes = (kV ? c.v : c.k) + block * page * kD;
+  uint8_t* scale = (kV ? c.vs : c.ks) + block;
+  const uint32_t held = p.lo > 0 ? max(static_cast<uint32_t>(*scale), kLeastScaleByte) : 0u;
   constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
   uint32_t mag = 0;
-  for (int r = r0; r < p.n; r += kStep) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(src + r * st + 8 * ch);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = w[i] & 0x7fffu, hi = (w[i] >> 16) & 0x7fffu;
-      if (lo < kInf) mag = max(mag, lo);
-      if (hi < kInf) mag = max(mag, hi);
-    }
-  }
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = w[t][j][i] & 0x7fffu, hi = (w[t][j][i] >> 16) & 0x7fffu;
+        mag = max(mag, lo < kInf ? lo : 0u);
+        mag = max(mag, hi < kInf ? hi : 0u);
+      }
 #pragma unroll
   for (int d = 32; d; d >>= 1) mag = max(mag, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mag), d)));
-  if ((tid & 63) == 0) s_mag[tid >> 6] = mag;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) mag = max(mag, s_mag[i]);
+  if (waves > 1) {
+    if (lane == 0) s_mag[wave] = mag;
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) mag = max(mag, s_mag[i]);
+  }
   uint32_t byte = cache_scale_byte(widen<kF16>(mag));
 
   // ---- a page that holds tokens keeps the larger scale ----
   if (p.lo > 0) {
-    const uint32_t held = max(static_cast<uint32_t>(*scale), kLeastScaleByte);
     if (byte > held) {
       // every 16-byte run with a held token; positions from lo on are overwritten or unused
       const float up = __uint_as_float(min(byte - held + 127u, 254u) << 23);
-      const int runs = is_v ? kD * (page / 16) : p.lo * (kD / 16);
-      for (int i = tid; i < runs; i += kThreads) {
-        if (is_v && (i % (page / 16)) * 16 >= p.lo) continue;
+      const int runs = kV ? kD * (page / 16) : p.lo * (kD / 16);
+      for (int i = tid; i < runs; i += threads) {
+        if (kV && (i % (page / 16)) * 16 >= p.lo) continue;
         u32x4* at = reinterpret_cast<u32x4*>(codes) + i;
-        u32x4 w = *at;
+        u32x4 x = *at;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = rescale4(w[j], up);
-        *at = w;
+        for (int j = 0; j < 4; ++j) x[j] = rescale4(x[j], up);
+        *at = x;
       }
+      __syncthreads();  // the new codes may lie in the same runs
     } else {
       byte = held;
     }
   }
-  __syncthreads();  // held codes are rewritten, and every thread has read the held scale
+  if (waves > 1) __syncthreads();  // every wave has read the held scale
   if (tid == 0) *scale = static_cast<uint8_t>(byte);
   const float sf = e8m0_scale(byte);
 
   // ---- codes of the new rows ----
-  for (int r = r0; r < p.n; r += kStep) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(src + r * st + 8 * ch);
-    u32x2 out;
-    out[0] = codes2<kF16>(w[0], sf) | codes2<kF16>(w[1], sf) << 16;
-    out[1] = codes2<kF16>(w[2], sf) | codes2<kF16>(w[3], sf) << 16;
-    if (!is_v) {
-      *reinterpret_cast<u32x2*>(codes + (p.lo + r) * kD + 8 * ch) = out;
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        tile[(8 * ch + i) * pitch + p.lo + r] = static_cast<uint8_t>(out[i >> 2] >> (8 * (i & 3)));
+  for (int t = 0; t < kTiles; ++t) {
+    u32x2 out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      out[j][0] = codes2<kF16>(w[t][j][0], sf) | codes2<kF16>(w[t][j][1], sf) << 16;
+      out[j][1] = codes2<kF16>(w[t][j][2], sf) | codes2<kF16>(w[t][j][3], sf) << 16;
+    }
+    const Spot at = spot<kD, kV>(t * waves + wave, 0, lane, c.log_page);
+    if (!kV) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Spot to = spot<kD, kV>(t * waves + wave, j, lane, c.log_page);
+        if (to.pos >= p.lo && to.pos < end) *reinterpret_cast<u32x2*>(codes + to.pos * kD + to.ch) = out[j];
+      }
+    } else if (at.ch < kD && at.pos + 4 > p.lo && at.pos < end) {
+      const bool whole = at.pos >= p.lo && at.pos + 4 <= end;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t word = 0;   // channel at.ch + i, 4 positions
+#pragma unroll
+        for (int j = 0; j < 4; ++j) word |= (out[j][i >> 2] >> (8 * (i & 3)) & 0xffu) << (8 * j);
+        uint8_t* to = codes + (at.ch + i) * page + at.pos;
+        if (whole) {
+          *reinterpret_cast<uint32_t*>(to) = word;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (at.pos + j >= p.lo && at.pos + j < end) to[j] = static_cast<uint8_t>(word >> (8 * j));
+        }
+      }
     }
   }
-  if (!is_v) return;
-  __syncthreads();
-  // rows of 4 positions; a run that holds other positions too goes byte by byte
-  const int words = page / 4;
-  for (int i = tid; i < kD * words; i += kThreads) {
-    const int d = i / words, at = (i % words) * 4;
-    if (at + 4 <= p.lo || at >= p.lo + p.n) continue;
-    const uint8_t* from = tile + d * pitch + at;
-    uint8_t* to = codes + d * page + at;
-    if (at >= p.lo && at + 4 <= p.lo + p.n) {
-      *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
-    } else {
-      for (int b = 0; b < 4; ++b)
-        if (at + b >= p.lo && at + b < p.lo + p.n) to[b] = from[b];
-    }
-  }
+}
+
+template <int kD, int kTiles, bool kF16>
+__global__ void __launch_bounds__(1024) cache_write_kernel(KvCache c, Rows rows, Seqs s) {
+  const Item item = item_of(c);
+  const Piece p = find_piece(c, s, rows.count, item.slot);
+  if (p.n <= 0 || p.seq >= s.batch) return;
+  if (item.v)
+    write_page<kD, kTiles, kF16, true>(c, rows, s, p, item.u);
+  else
+    write_page<kD, kTiles, kF16, false>(c, rows, s, p, item.u);
 }
 
 // Two values of the codes in the low two bytes, as packed 16-bit numbers. fp16 saturates at its
@@ -227,56 +301,77 @@ __device__ __forceinline__ uint32_t values2(uint32_t codes, float scale) {
   return f32_to_f16_bits(a) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16;
 }
 
-template <int kD, bool kF16>
-__global__ void __launch_bounds__(kThreads)
-cache_read_kernel(KvCache c, Rows rows, Seqs s) {
-  constexpr int kChunks = kD / 8;
-  constexpr int kStep = kThreads / kChunks;
-  const int page = 1 << c.log_page, pitch = page + 4;
-  extern __shared__ uint8_t tile[];
-  const Piece p = find_piece(c, s, rows.count, blockIdx.x);
-  if (p.n <= 0) return;
-  const int u = blockIdx.y, tid = threadIdx.x;
-  const bool is_v = blockIdx.z != 0;
-  const int64_t st = is_v ? rows.v_st : rows.k_st;
-  uint16_t* dst = (is_v ? rows.v + u * rows.v_sh : rows.k + u * rows.k_sh) + p.row * st;
-  const int ch = tid % kChunks, r0 = tid / kChunks;
-  const bool behind = p.seq >= s.batch;
-  const int id = behind ? -1 : cache_page(c, s.table + p.seq * s.t_st, p.index, s.width);
-  if (id < 0) {  // no such page: NaN; rows behind the last sequence: zeros
-    const uint32_t fill = behind ? 0u : kF16 ? 0x7e007e00u : 0x7fc07fc0u;
-    for (int r = r0; r < p.n; r += kStep)
-      *reinterpret_cast<u32x4*>(dst + r * st + 8 * ch) = u32x4{fill, fill, fill, fill};
-    return;
-  }
-  const int64_t block = static_cast<int64_t>(id) * c.kv_heads + u;
-  const uint8_t* codes = (is_v ? c.v : c.k) + block * page * kD;
-  const float sf = e8m0_scale(max(static_cast<uint32_t>((is_v ? c.vs : c.ks)[block]), kLeastScaleByte));
-  if (is_v) {
-    const int runs = page / 16;
-    for (int i = tid; i < kD * runs; i += kThreads) {
-      const int d = i / runs, at = (i % runs) * 16;
-      if (at + 16 <= p.lo || at >= p.lo + p.n) continue;
-      const u32x4 w = *reinterpret_cast<const u32x4*>(codes + d * page + at);
+template <int kD, int kTiles, bool kF16, bool kV>
+__device__ __forceinline__ void read_page(const KvCache& c, const Rows& rows, const Piece& p, int id,
+                                          int u, uint32_t fill) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int page = 1 << c.log_page;
+  const int64_t block = static_cast<int64_t>(max(id, 0)) * c.kv_heads + u;
+  const uint8_t* codes = (kV ? c.v : c.k) + block * page * kD;
+  const float sf = e8m0_scale(max(static_cast<uint32_t>((kV ? c.vs : c.ks)[block]), kLeastScaleByte));
+  const int64_t st = kV ? rows.v_st : rows.k_st;
+  uint16_t* dst = (kV ? rows.v + u * rows.v_sh : rows.k + u * rows.k_sh) + p.row * st;
+  const int end = p.lo + p.n;
+  // all codes first: V as [channel] words of 4 positions, K as rows
+  uint32_t w[kTiles][8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t*>(tile + d * pitch + at + 4 * j) = w[j];
-    }
-    __syncthreads();
-  }
-  for (int r = r0; r < p.n; r += kStep) {
-    u32x2 w;
-    if (!is_v) {
-      w = *reinterpret_cast<const u32x2*>(codes + (p.lo + r) * kD + 8 * ch);
-    } else {
-      w = u32x2{0, 0};
+  for (int t = 0; t < kTiles; ++t) {
+    if (kV) {
+      const Spot at = spot<kD, kV>(t * waves + wave, 0, lane, c.log_page);
+      const bool any = at.ch < kD && at.pos + 4 > p.lo && at.pos < end;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        w[i >> 2] |= static_cast<uint32_t>(tile[(8 * ch + i) * pitch + p.lo + r]) << (8 * (i & 3));
+        w[t][i] = any ? *reinterpret_cast<const uint32_t*>(codes + (at.ch + i) * page + at.pos) : 0u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Spot at = spot<kD, kV>(t * waves + wave, j, lane, c.log_page);
+        u32x2 x = {0, 0};
+        if (at.pos >= p.lo && at.pos < end) x = *reinterpret_cast<const u32x2*>(codes + at.pos * kD + at.ch);
+        w[t][2 * j] = x[0];
+        w[t][2 * j + 1] = x[1];
+      }
     }
-    const u32x4 out{values2<kF16>(w[0], sf), values2<kF16>(w[0] >> 16, sf),
-                    values2<kF16>(w[1], sf), values2<kF16>(w[1] >> 16, sf)};
-    *reinterpret_cast<u32x4*>(dst + r * st + 8 * ch) = out;
   }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Spot at = spot<kD, kV>(t * waves + wave, j, lane, c.log_page);
+      if (at.pos < p.lo || at.pos >= end || at.ch >= kD) continue;
+      uint32_t x[2];
+      if (kV) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x[h] = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[h] |= (w[t][4 * h + i] >> (8 * j) & 0xffu) << (8 * i);
+        }
+      } else {
+        x[0] = w[t][2 * j];
+        x[1] = w[t][2 * j + 1];
+      }
+      u32x4 out{values2<kF16>(x[0], sf), values2<kF16>(x[0] >> 16, sf), values2<kF16>(x[1], sf),
+                values2<kF16>(x[1] >> 16, sf)};
+      if (id < 0) out = u32x4{fill, fill, fill, fill};
+      *reinterpret_cast<u32x4*>(dst + (at.pos - p.lo) * st + at.ch) = out;
+    }
+}
+
+template <int kD, int kTiles, bool kF16>
+__global__ void __launch_bounds__(1024) cache_read_kernel(KvCache c, Rows rows, Seqs s) {
+  const Item item = item_of(c);
+  const Piece p = find_piece(c, s, rows.count, item.slot);
+  if (p.n <= 0) return;
+  const bool behind = p.seq >= s.batch;
+  const int id = behind ? -1 : cache_page(c, s.table + p.seq * s.t_st, p.index, s.width);
+  // no such page: NaN; rows behind the last sequence: zeros
+  const uint32_t fill = behind ? 0u : kF16 ? 0x7e007e00u : 0x7fc07fc0u;
+  if (item.v)
+    read_page<kD, kTiles, kF16, true>(c, rows, p, id, item.u, fill);
+  else
+    read_page<kD, kTiles, kF16, false>(c, rows, p, id, item.u, fill);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -302,15 +397,18 @@ int move_rows(const char* name, const KvCache& c, int page, Rows rows, Seqs s, i
   const int64_t slots = s.offsets == nullptr
                             ? (kWrite ? s.batch : static_cast<int64_t>(max(s.batch, rows.count)))
                             : (rows.count >> c.log_page) + 2 * static_cast<int64_t>(s.batch) + (kWrite ? 0 : 1);
-  if (slots > (1ll << 31) - 1 || c.kv_heads > 65535)
-    return set_error(kUnsupported, "%s: too many pages or heads", name);
-  const dim3 grid(static_cast<unsigned>(slots), static_cast<unsigned>(c.kv_heads), 2);
-  const size_t lds = static_cast<size_t>(head_dim) * (page + 4);
+  const int64_t workgroups = slots * 2 * c.kv_heads;
+  if (workgroups > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many pages or heads", name);
+  const dim3 grid(static_cast<unsigned>(workgroups));
+  // waves that hold a page: one tile each, two where that would take over 16 waves
+  const int tiles = (page * head_dim + kTileValues - 1) / kTileValues;
+  const int waves = tiles > 16 ? 16 : tiles;
   const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, static_cast<hipStream_t>(stream), c, rows, s);
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, static_cast<hipStream_t>(stream), c, rows, s);
   };
-#define VDN_MOVE(D, F16) \
-  (kWrite ? launch(cache_write_kernel<D, F16>) : launch(cache_read_kernel<D, F16>))
+#define VDN_MOVE(D, F16)                                                                            \
+  (kWrite ? (tiles > 16 ? launch(cache_write_kernel<D, 2, F16>) : launch(cache_write_kernel<D, 1, F16>)) \
+          : (tiles > 16 ? launch(cache_read_kernel<D, 2, F16>) : launch(cache_read_kernel<D, 1, F16>)))
   if (dtype == 0)
     head_dim == 64 ? VDN_MOVE(64, false) : head_dim == 128 ? VDN_MOVE(128, false) : VDN_MOVE(256, false);
   else
