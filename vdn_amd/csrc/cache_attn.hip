@@ -37,6 +37,9 @@ constexpr int kWaves = 4;
 constexpr int kTile = 64;              // tokens of a wave's step
 constexpr int kQuad = kTile * kWaves;  // tokens of a workgroup's step
 
+// Workgroups that share a CU: two (256 registers a lane); one where a tile's codes, Q and O need more.
+constexpr int workgroups_per_cu(int head_dim, int rows) { return head_dim * rows > 128 * 16 ? 1 : 2; }
+
 struct Queries {
   const uint16_t* q;
   uint16_t* out;
@@ -66,55 +69,52 @@ __device__ __forceinline__ int seq_tokens(const KvCache& c, const Lengths& s, in
 
 __device__ __forceinline__ int quads_of(int tokens) { return max((tokens + kQuad - 1) / kQuad, 1); }
 
-// Prefix over the sequences' quads by the whole workgroup: the total, and the sequence that holds
-// quad `at` of the flattened order (quads of sequence b: units * quads_of(len_b)) with the quads
-// in front of it. Each thread takes a strip of consecutive sequences.
+// Where quad `at` of the flattened order lies (sequence b's quads: units * quads_of(len_b)), from a
+// prefix over the lengths. Every wave does it for itself, 64 strips of sequences at a time: no
+// barrier, and for up to 64 sequences one load.
 struct Place {
-  int64_t total, before;
+  int64_t total;    // quads of all units
+  int64_t per;      // quads of a workgroup
+  int64_t before;   // quads in front of sequence seq
   int seq;
 };
 
-__device__ Place find_quad(const KvCache& c, const Lengths& s, int units, int workgroups, int wg,
-                           int64_t* per_out) {
-  __shared__ int64_t s_sum[kThreads / 64];
-  __shared__ int64_t s_before;
-  __shared__ int s_seq;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int strip = (s.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * strip, s.batch), b1 = min(b0 + strip, s.batch);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += quads_of(seq_tokens(c, s, b));
-  int64_t incl = mine;
+__device__ __forceinline__ int wave_prefix(int x, int lane) {   // inclusive
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t other = __shfl_up(incl, d);
-    if (lane >= d) incl += other;
+    const int other = __shfl_up(x, d);
+    x += lane >= d ? other : 0;
   }
-  if (lane == 63) s_sum[tid >> 6] = incl;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kThreads / 64; ++w) {
-    if (w < (tid >> 6)) incl += s_sum[w];
-    total += s_sum[w];
-  }
-  total *= units;
-  const int64_t per = max((total + workgroups - 1) / workgroups, static_cast<int64_t>(1));
-  const int64_t at = per * wg;
-  int64_t before = (incl - mine) * units;
-  if (at >= before && at < incl * units) {
-    for (int b = b0; b < b1; ++b) {
-      const int64_t n = static_cast<int64_t>(quads_of(seq_tokens(c, s, b))) * units;
-      if (at < before + n) {
-        s_before = before;
-        s_seq = b;
-        break;
-      }
+  return x;
+}
+
+__device__ Place find_quad(const KvCache& c, const Lengths& s, int units, int workgroups, int wg) {
+  const int lane = threadIdx.x & 63;
+  const int strip = (s.batch + 63) / 64;
+  const int b0 = min(lane * strip, s.batch), b1 = min(b0 + strip, s.batch);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += quads_of(seq_tokens(c, s, b));
+  const int incl = wave_prefix(mine, lane);
+  Place p;
+  p.total = static_cast<int64_t>(__builtin_amdgcn_readlane(incl, 63)) * units;
+  p.per = max((p.total + workgroups - 1) / workgroups, static_cast<int64_t>(1));
+  const int64_t at = p.per * wg;
+  // the strip, then the sequence inside it
+  const int front = __popcll(__ballot(static_cast<int64_t>(incl) * units <= at));
+  const int owner = min(front, 63);
+  int before = __builtin_amdgcn_readlane(incl - mine, owner);
+  int seq = __builtin_amdgcn_readlane(b0, owner);
+  if (strip > 1) {
+    const int last = min(seq + strip, s.batch) - 1;
+    for (; seq < last; ++seq) {
+      const int n = quads_of(seq_tokens(c, s, seq));
+      if (at < static_cast<int64_t>(before + n) * units) break;
       before += n;
     }
   }
-  __syncthreads();
-  *per_out = per;
-  return Place{total, s_before, s_seq};
+  p.before = static_cast<int64_t>(before) * units;
+  p.seq = seq;
+  return p;
 }
 
 template <bool kF16>
@@ -170,7 +170,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 }
 
 template <int kD, int kNR, bool kF16>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, workgroups_per_cu(kD, 16 * kNR))
 cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2) {
   constexpr int kRows = 16 * kNR;     // query rows of a unit
   constexpr int kKL = kD / 64;        // 16-byte K loads per key row and lane
@@ -184,11 +184,10 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   const int row16 = lane & 15, g = lane >> 4;
   const int page = 1 << c.log_page;
   const int units = row_blocks * c.kv_heads;
-  int64_t per;
   const int wg = blockIdx.x;
-  const Place place = find_quad(c, s, units, sp.workgroups, wg, &per);
-  int64_t at = per * wg;
-  const int64_t end = min(at + per, place.total);
+  const Place place = find_quad(c, s, units, sp.workgroups, wg);
+  int64_t at = place.per * wg;
+  const int64_t end = min(at + place.per, place.total);
   if (at >= end) return;
   const int64_t range0 = at;
   int b = __builtin_amdgcn_readfirstlane(place.seq);
@@ -238,10 +237,19 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     // Pages of a tile's 16-token groups: lane's K rows lie in group row16 / 4, its V run and
     // scores in group g. Groups behind the last token repeat the last one.
     const int last_group = max(len - 1, 0) & ~15;
-    auto page_of = [&](int pos, bool& ok) __attribute__((always_inline)) {
-      const int id = table[min(pos, last_group) >> c.log_page];
-      ok = id >= 0 && id < c.pages;
-      return ok ? id : 0;
+    struct Ids {
+      int k, v;   // page of the lane's K rows, of its V run
+      bool ok;
+    };
+    auto ids_of = [&](int tile0) __attribute__((always_inline)) {
+      const int ik = table[min(tile0 + 16 * (row16 >> 2), last_group) >> c.log_page];
+      const int iv = table[min(tile0 + 16 * g, last_group) >> c.log_page];
+      const bool ok = iv >= 0 && iv < c.pages;
+      return Ids{ik >= 0 && ik < c.pages ? ik : 0, ok ? iv : 0, ok};
+    };
+    auto scale_of = [&](const uint8_t* scales, int id) __attribute__((always_inline)) {
+      return max(static_cast<uint32_t>(scales[static_cast<int64_t>(id) * c.kv_heads + u]),
+                 kLeastScaleByte);
     };
     u32x4 kr[4][kKL], vr[kDB];
     auto load_k = [&](int id, int tile0) __attribute__((always_inline)) {
@@ -262,24 +270,20 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
       for (int db = 0; db < kDB; ++db) vr[db] = *reinterpret_cast<const u32x4*>(p + 16 * db * page);
     };
 
+    // The codes of a tile are loaded one step ahead, K's as soon as the scores have used the
+    // last ones and V's after the product; their page ids one step before that, the scales with K.
     int tile0 = (qa * kWaves + wave) * kTile;
     const int tile_end = min(qb * kQuad, len);
     if (tile0 < tile_end) {
-      bool ok_k, ok_v;
-      int id_k = page_of(tile0 + 16 * (row16 >> 2), ok_k), id_v = page_of(tile0 + 16 * g, ok_v);
-      load_k(id_k, tile0);
-      load_v(id_v, tile0);
+      Ids now = ids_of(tile0), next = ids_of(tile0 + kQuad);
+      uint32_t ks = scale_of(c.ks, now.v), vs = scale_of(c.vs, now.v);
+      load_k(now.k, tile0);
+      load_v(now.v, tile0);
       for (; tile0 < tile_end; tile0 += kQuad) {
-        bad |= !ok_v;                                    // the g groups are all of the tile's
-        const int64_t sc = static_cast<int64_t>(id_v) * c.kv_heads + u;
-        const uint32_t ks = max(static_cast<uint32_t>(c.ks[sc]), kLeastScaleByte);
-        const uint32_t vs = max(static_cast<uint32_t>(c.vs[sc]), kLeastScaleByte);
+        bad |= !now.ok;                                  // the g groups are all of the tile's
         const int next0 = tile0 + kQuad;
         const bool more = next0 < tile_end;
-        if (more) {
-          id_k = page_of(next0 + 16 * (row16 >> 2), ok_k);
-          id_v = page_of(next0 + 16 * g, ok_v);
-        }
+        const Ids after = ids_of(next0 + kQuad);
         // ---- Sᵀ ----
         f32x4 sc_t[kNR][4];
 #pragma unroll
@@ -297,10 +301,16 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
             }
           }
         }
-        if (more) load_k(id_k, next0);
+        const float k_scale = e8m0_scale(ks) * scale_log2;
+        float v_scale = e8m0_scale(vs);
+        uint32_t top = vs;
+        if (more) {
+          load_k(next.k, next0);
+          ks = scale_of(c.ks, next.v);
+          vs = scale_of(c.vs, next.v);
+        }
 
         // ---- softmax: scores times K's scale, running maximum in exp2 units ----
-        const float k_scale = e8m0_scale(ks) * scale_log2;
         const bool masked = tile0 + kTile > seen0;
         u32x4 pb[kNR][2];
 #pragma unroll
@@ -343,9 +353,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
         }
 
         // ---- V: tail bytes to zero, scale ----
-        float v_scale = e8m0_scale(vs);
         if (kF16) {
-          uint32_t top = vs;
           top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
           top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
           // within what fp16 values ask for (2^-32 .. 2^16), so that no rescaling overflows
@@ -419,7 +427,9 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
 #pragma unroll
             for (int nr = 0; nr < kNR; ++nr) o[nr][db] = E::mfma(a, pb[nr][h], o[nr][db]);
           }
-        if (more) load_v(id_v, next0);
+        if (more) load_v(next.v, next0);
+        now = next;
+        next = after;
       }
     }
 
@@ -499,79 +509,87 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   }
 }
 
-// Joins the slots of every unit that more than one workgroup worked on. One workgroup per row of
-// a unit: kD / 4 lanes for the channels, the others take slots in turn.
-template <int kD, int kNR, bool kF16>
-__global__ void __launch_bounds__(kThreads)
+// Joins the slots of every unit that more than one workgroup worked on: a workgroup per row of a
+// unit, kD / 4 lanes for the channels, the others take slots in turn. One wave where rows are many
+// (units then have few slots), four where they are few (and have many).
+template <int kD, int kNR, bool kF16, int kJoinWaves>
+__global__ void __launch_bounds__(64 * kJoinWaves)
 cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
   constexpr int kRows = 16 * kNR;
-  constexpr int kVec = kD / 4, kLanes = kThreads / kVec;   // lanes of a row: kLanes slots at a time
-  __shared__ int64_t s_sum[kThreads / 64], s_front[kThreads / 64];
+  constexpr int kVec = kD / 4, kLanes = 64 * kJoinWaves / kVec;   // slots at a time
   __shared__ float s_part[kLanes][kD], s_pm[kLanes], s_pl[kLanes];
   const int units = row_blocks * c.kv_heads;
   const int rows = io.tokens * io.group;
   const int b = blockIdx.x / (rows * c.kv_heads);
   const int row = blockIdx.x / c.kv_heads % rows, u = blockIdx.x % c.kv_heads;
-  const int tid = threadIdx.x;
-  int64_t all = 0, front = 0;
-  for (int i = tid; i < s.batch; i += kThreads) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  int all = 0, front = 0, own = 0;
+  for (int i = lane; i < s.batch; i += 64) {
     const int n = quads_of(seq_tokens(c, s, i));
     all += n;
     if (i < b) front += n;
+    if (i == b) own = n;
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     all += __shfl_xor(all, d);
     front += __shfl_xor(front, d);
+    own += __shfl_xor(own, d);
   }
-  if ((tid & 63) == 0) {
-    s_sum[tid >> 6] = all;
-    s_front[tid >> 6] = front;
-  }
-  __syncthreads();
-  all = front = 0;
-  for (int w = 0; w < kThreads / 64; ++w) {
-    all += s_sum[w];
-    front += s_front[w];
-  }
-  const int64_t per = max((all * units + sp.workgroups - 1) / sp.workgroups, static_cast<int64_t>(1));
-  const int nq = quads_of(seq_tokens(c, s, b));
-  const int64_t start = front * units + static_cast<int64_t>((row / kRows) * c.kv_heads + u) * nq;
-  const int64_t w0 = start / per, w1 = (start + nq - 1) / per;
+  const int64_t per = max((static_cast<int64_t>(all) * units + sp.workgroups - 1) / sp.workgroups,
+                          static_cast<int64_t>(1));
+  const int64_t start = static_cast<int64_t>(front) * units +
+                        static_cast<int64_t>((row / kRows) * c.kv_heads + u) * own;
+  const int64_t w0 = start / per, w1 = (start + own - 1) / per;
   if (w0 == w1) return;   // written by its one workgroup
   const int d = (tid % kVec) * 4, part = tid / kVec;
   float top = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t w = w0 + part; w <= w1; w += kLanes) {
-    const int64_t slot = 2 * w + (w == w0 && start != w0 * per ? 1 : 0);
-    const float* src = sp.slots + (slot * kRows + row % kRows) * (kD + 4);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(src + d);
-    const float m = src[kD], l = src[kD + 1];
-    const float m_new = fmaxf(top, m);
-    const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - m_new);
-    const float f1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-    sum = sum * f0 + l * f1;
+  constexpr int kAhead = 4;   // slots in flight
+  for (int64_t w = w0 + part; w <= w1; w += kLanes * kAhead) {
+    f32x4 x[kAhead];
+    float m[kAhead], l[kAhead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = (f0 == 0.f ? 0.f : acc[i] * f0) + (f1 == 0.f ? 0.f : x[i] * f1);
-    top = m_new;
-  }
-  *reinterpret_cast<f32x4*>(&s_part[part][d]) = acc;
-  if (d == 0) {
-    s_pm[part] = top;
-    s_pl[part] = sum;
-  }
-  __syncthreads();
-  if (part != 0) return;
-  top = -INFINITY;
-  for (int i = 0; i < kLanes; ++i) top = fmaxf(top, s_pm[i]);
-  sum = 0.f;
-  acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < kLanes; ++i) {
-    const float f = s_pm[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_pm[i] - top);
-    sum += s_pl[i] * f;
-    const f32x4 x = *reinterpret_cast<const f32x4*>(&s_part[i][d]);
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t wa = min(w + a * kLanes, w1);
+      const int64_t slot = 2 * wa + (wa == w0 && start != w0 * per ? 1 : 0);
+      const float* src = sp.slots + (slot * kRows + row % kRows) * (kD + 4);
+      x[a] = *reinterpret_cast<const f32x4*>(src + d);
+      m[a] = src[kD];
+      l[a] = src[kD + 1];
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] += f == 0.f ? 0.f : x[j] * f;
+    for (int a = 0; a < kAhead; ++a) {
+      if (w + a * kLanes > w1) break;
+      const float m_new = fmaxf(top, m[a]);
+      const float f0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - m_new);
+      const float f1 = m[a] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[a] - m_new);
+      sum = sum * f0 + l[a] * f1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[i] = (f0 == 0.f ? 0.f : acc[i] * f0) + (f1 == 0.f ? 0.f : x[a][i] * f1);
+      top = m_new;
+    }
+  }
+  if (kLanes > 1) {
+    *reinterpret_cast<f32x4*>(&s_part[part][d]) = acc;
+    if (d == 0) {
+      s_pm[part] = top;
+      s_pl[part] = sum;
+    }
+    __syncthreads();
+    if (part != 0) return;
+    top = -INFINITY;
+    for (int i = 0; i < kLanes; ++i) top = fmaxf(top, s_pm[i]);
+    sum = 0.f;
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < kLanes; ++i) {
+      const float f = s_pm[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_pm[i] - top);
+      sum += s_pl[i] * f;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(&s_part[i][d]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += f == 0.f ? 0.f : x[j] * f;
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int i = row / io.group, h = u * io.group + row - i * io.group;
@@ -594,13 +612,15 @@ using namespace vdn;
 namespace vdn {
 namespace {
 
-// Row blocks of 32 for more than 16 rows: every code is widened once for both halves. Wide heads
-// stay at 16 (32 rows of 256 channels and the codes in flight exceed the registers).
+// Row blocks of 32 for more than 16 rows: every code is loaded and widened once for both halves.
+// With 256 channels 32 rows spill (50.1 us against 50.4 in blocks of 16: 16 sequences of 4096
+// tokens, 4 K/V heads, 32 rows), so those stay at 16.
 int rows_of_block(int rows, int head_dim) { return rows > 16 && head_dim <= 128 ? 32 : 16; }
 
-// Two workgroups fit a CU; fewer if there are not so many quads at all.
-int64_t workgroups_of(int64_t most_quads) {
-  return std::max<int64_t>(1, std::min<int64_t>(2 * cu_count(), most_quads));
+// As many workgroups as run at once, fewer if there are not so many quads at all.
+int64_t workgroups_of(int64_t most_quads, int head_dim, int block) {
+  const int64_t fit = static_cast<int64_t>(workgroups_per_cu(head_dim, block)) * cu_count();
+  return std::max<int64_t>(1, std::min(fit, most_quads));
 }
 
 }  // namespace
@@ -610,7 +630,7 @@ VDN_API int vdn_cache_attention_workspace(int tokens, int group, int head_dim, i
   if (bytes == nullptr || tokens <= 0 || group <= 0)
     return set_error(kInvalidArgument, "vdn_cache_attention_workspace: invalid argument");
   const int64_t rows = static_cast<int64_t>(tokens) * group;
-  const int block = rows_of_block(static_cast<int>(std::min<int64_t>(rows, 1 << 20)), head_dim);
+  const int block = rows_of_block(static_cast<int>(std::min<int64_t>(rows, 32)), head_dim);
   *bytes = 4ll * 2 * 2 * cu_count() * block * (head_dim + 4);
   return kOk;
 }
@@ -645,11 +665,11 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
   const int64_t rows = static_cast<int64_t>(tokens) * group;
   if (rows * kv_heads * batch > (1ll << 31) - 1)
     return set_error(kUnsupported, "%s: too many query rows", name);
-  const int block = rows_of_block(static_cast<int>(rows), head_dim);
+  const int block = rows_of_block(static_cast<int>(std::min<int64_t>(rows, 32)), head_dim);
   const int row_blocks = static_cast<int>((rows + block - 1) / block);
   const int64_t unit_quads = ((static_cast<int64_t>(width) << c.log_page) + kQuad - 1) / kQuad;
   const int64_t units = static_cast<int64_t>(row_blocks) * kv_heads * batch;
-  const int workgroups = static_cast<int>(workgroups_of(units * unit_quads));
+  const int workgroups = static_cast<int>(workgroups_of(units * unit_quads, head_dim, block));
   const Split sp{static_cast<float*>(workspace), workgroups};
   if (unit_quads > 1) {
     if (workspace == nullptr || !aligned16(workspace) ||
@@ -659,15 +679,22 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
   const Queries io{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lse, q_sb, q_st, q_sh,
                    o_sb, o_st, o_sh, tokens, group};
   const Lengths s{table, lengths, table_st, batch, width};
-  const auto launch = [&](auto main, auto join) {
+  if (batch * unit_quads > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many tokens", name);
+  const int64_t join_rows = rows * kv_heads * batch;
+  const auto launch = [&](auto main, auto join1, auto join4) {
     const auto st = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(main, dim3(static_cast<unsigned>(workgroups)), dim3(kThreads), 0, st, c, io, s, sp,
                        row_blocks, scale * kLog2e);
-    if (unit_quads > 1)   // a unit may have been shared
-      hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(rows * kv_heads * batch)), dim3(kThreads), 0, st,
-                         c, io, s, sp, row_blocks);
+    if (unit_quads <= 1) return;   // no unit is shared
+    const dim3 grid(static_cast<unsigned>(join_rows));
+    if (join_rows > 4 * cu_count())
+      hipLaunchKernelGGL(join1, grid, dim3(64), 0, st, c, io, s, sp, row_blocks);
+    else
+      hipLaunchKernelGGL(join4, grid, dim3(256), 0, st, c, io, s, sp, row_blocks);
   };
-#define VDN_CACHE(D, NR, F16) launch(cache_attn_kernel<D, NR, F16>, cache_join_kernel<D, NR, F16>)
+#define VDN_CACHE(D, NR, F16)                                               \
+  launch(cache_attn_kernel<D, NR, F16>, cache_join_kernel<D, NR, F16, 1>, \
+         cache_join_kernel<D, NR, F16, 4>)
 #define VDN_CACHE_D(F16)                                                            \
   head_dim == 64 ? (block == 16 ? VDN_CACHE(64, 1, F16) : VDN_CACHE(64, 2, F16))    \
   : head_dim == 128 ? (block == 16 ? VDN_CACHE(128, 1, F16) : VDN_CACHE(128, 2, F16)) \
