@@ -328,7 +328,7 @@ int vdn_window_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * Causal softmax attention of packed sequences (dtype 0: bf16, 1: fp16; head_dim 64, 128 or
  * 256): query head h = u group + j reads K/V head u; a token sees its sequence up to itself.
  * The tokens x group rows of a sequence and a K/V head are counted token major and cut into
- * blocks of block_rows (128 or 256): blocks int32 [nblocks, 4] = (first packed row of the
+ * blocks of block_rows (128, or 256 with head_dim 128): blocks int32 [nblocks, 4] = (first packed row of the
  * sequence, its tokens, first row of the block, unused). q, k, v, out addressed by (token, head)
  * strides (multiples of 8 elements, unit channel stride, 16-byte aligned); K/V token strides up
  * to 2^22. lse (nullable): fp32 natural-log sum-exp of the scaled scores. Only the rows of

@@ -59,6 +59,39 @@ def test_long(device, dim, dtype, n, heads, kv_heads):
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("lengths,heads,kv_heads", [([130, 1, 0, 700], 6, 2), ([513], 1, 1)])
+@torch.no_grad()
+def test_wide_blocks(device, dtype, lengths, heads, kv_heads):
+    """The 256-row blocks, which the plan takes for long prompts, on small ones: within the bounds, and
+    nonfinite values of later tokens stay away from a row there too."""
+    q, k, v = make(lengths, heads, kv_heads, 128, dtype, seed=9)
+    wide = vc._blocks(tuple(lengths), heads // kv_heads, 256).to(device)
+    plan = vc.CausalPlan(tuple(lengths), heads, kv_heads, sum(lengths), wide, wide)
+    got, lse = vc.causal_attention(q, k, v, plan, return_lse=True)
+    check(q, k, v, lengths, got, lse)
+    bad, last = v.clone(), sum(lengths) - 1
+    bad[last] = math.inf
+    same = vc.causal_attention(q, k, bad, plan)
+    assert torch.equal(same[:last], got[:last]) and (same[last] == math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@torch.no_grad()
+def test_long_prompt_takes_the_wide_blocks(device, dtype):
+    """4200 tokens, 32 heads: the first and last rows, against the oracle of those rows."""
+    n = 4200
+    q, k, v = make([n], 32, 8, 128, dtype, seed=13)
+    plan = vc.prepare_causal_plan([n], 32, 8, device=device)
+    assert plan.wide_blocks is not None
+    got, lse = vc.causal_attention(q, k, v, plan, return_lse=True)
+    for a, b in ((0, 70), (2000, 2040), (n - 40, n)):
+        out, el, mass, size = oc.attention(q[a:b].cpu(), k[:b].cpu(), v[:b].cpu(), a, 128 ** -0.5)
+        tol, ltol = oc.bounds(out, mass, size, v[:b].cpu(), dtype, 128, b)
+        assert bool(((got[a:b].cpu().double() - out).abs() <= tol).all())
+        assert bool(((lse[a:b].cpu().double() - el).abs() <= ltol).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
 @torch.no_grad()
 def test_scores_that_grow_and_another_scale(device, dtype):
     """Key magnitudes that ramp up: the running maximum is raised from tile to tile."""

@@ -9,21 +9,31 @@ from vdn_amd import _lib
 from vdn_amd import causal as vc
 
 
+@pytest.mark.parametrize("block_rows", [128, 256])
 @pytest.mark.parametrize("lengths,heads,kv_heads", [([5, 0, 700, 1], 6, 2), ([1], 1, 1), ([300] * 3, 7, 1),
                                                     ([], 2, 1), ([0], 2, 2)])
-def test_blocks_cover_every_row_once(lengths, heads, kv_heads):
+def test_blocks_cover_every_row_once(lengths, heads, kv_heads, block_rows):
     plan = vc.prepare_causal_plan(lengths, heads, kv_heads)
     group, seen = heads // kv_heads, set()
+    blocks = vc._blocks(tuple(lengths), group, block_rows)
+    assert block_rows == 256 or torch.equal(blocks, plan.blocks)
     first = {sum(lengths[:i]): n for i, n in enumerate(lengths) if n}
     keys = []
-    for row0, n, r0, _ in plan.blocks.tolist():
-        assert first[row0] == n and r0 % plan.block_rows == 0 and 0 <= r0 < n * group
-        for r in range(r0, min(r0 + plan.block_rows, n * group)):
+    for row0, n, r0, _ in blocks.tolist():
+        assert first[row0] == n and r0 % block_rows == 0 and 0 <= r0 < n * group
+        for r in range(r0, min(r0 + block_rows, n * group)):
             assert (row0, r) not in seen
             seen.add((row0, r))
-        keys.append((min(r0 + plan.block_rows, n * group) - 1) // group)
+        keys.append((min(r0 + block_rows, n * group) - 1) // group)
     assert len(seen) == sum(lengths) * group == plan.rows * group
     assert keys == sorted(keys, reverse=True)
+
+
+def test_wide_blocks_where_rows_see_many_keys():
+    assert vc.prepare_causal_plan([4096], 32, 8).wide_blocks.shape == (64, 4)
+    assert vc.prepare_causal_plan([4094], 32, 8).wide_blocks is None     # 2047.5 keys
+    assert vc.prepare_causal_plan([8192], 8, 1).wide_blocks is None      # 256 blocks
+    assert vc.prepare_causal_plan([2048] * 4, 32, 8).wide_blocks is None
 
 
 def test_plan_refusals():
@@ -56,7 +66,8 @@ def test_entry_point_validates_before_launching():
         return lib.vdn_causal_attention(q, 256, 128, fake, k_st, 128, fake, 256, 128, blocks, nblocks,
                                         rows, 2, 1, dim, dtype, scale, out, 256, 128, None, 0, 0, None)
     for change, word in ((dict(q=None), b"null"), (dict(out=None), b"null"), (dict(nblocks=-1), b"geometry"),
-                         (dict(rows=64), b"block_rows"), (dict(dim=96), b"head_dim"),
+                         (dict(rows=64), b"block_rows"), (dict(rows=256, dim=64), b"block_rows"),
+                         (dict(dim=96), b"head_dim"),
                          (dict(dtype=2), b"dtype"), (dict(scale=0.0), b"scale"),
                          (dict(q=fake + 8), b"16-byte"), (dict(k_st=252), b"16-byte"),
                          (dict(k_st=1 << 23), b"strides")):

@@ -19,20 +19,30 @@ MAX_ROWS = 2 ** 31 - 512   # rows (tokens x query heads of a K/V head) of one se
 
 @dataclass(frozen=True)
 class CausalPlan:
-    """Blocks of the packed sequences: `blocks` int32 [nblocks, 4] on the device = (first packed
-    row of the sequence, its tokens, first row of the block among the sequence's tokens x
-    heads / kv_heads rows, 0), the blocks with most keys first. `rows` counts the packed
-    rows; `block_rows` is the kernel variant."""
+    """Blocks of the packed sequences: `blocks` int32 [n, 4] on the device = (first packed row of
+    the sequence, its tokens, first row of the block among the sequence's tokens x heads /
+    kv_heads rows, 0), 128 rows each, the blocks with most keys first; `wide_blocks` the same of
+    256 rows, or None where they would be slower. `rows` counts the packed rows."""
     lengths: tuple
     heads: int
     kv_heads: int
     rows: int
-    block_rows: int
     blocks: torch.Tensor
+    wide_blocks: torch.Tensor | None
 
     @property
     def device(self):
         return self.blocks.device
+
+
+# When head dim 128 takes 256-row blocks (8 waves, one workgroup a CU) instead of 128-row ones (two
+# of 4 waves): a K/V tile then serves twice the rows, which pays where rows see many keys, and a
+# block takes the CU to itself, so that there have to be enough of them. Microseconds of 256 and
+# 128 rows: 32768 tokens 8000, 8600; 8192: 534, 565; 4096: 162, 172; 4 x 2048: 188, 178; 24 prompts
+# of 77 - 1200: 174, 140 (the mean row sees 2048 keys of 4096); 8192 tokens of 8 heads that share
+# one K/V head, 256 blocks: 214, 195; 16384 of them, 512 blocks: 525, 612.
+WIDE_MEAN_KEYS = 2048
+WIDE_LEAST_BLOCKS = 512    # two for each of 256 CUs
 
 
 def _blocks(lengths, group, block_rows):
@@ -63,8 +73,14 @@ def prepare_causal_plan(lengths, heads, kv_heads=None, *, device="cpu"):
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    return CausalPlan(lengths, heads, kv_heads, sum(lengths), 256,
-                      _blocks(lengths, group, 256).to(device))
+    rows = sum(lengths)
+    blocks = _blocks(lengths, group, 128)
+    wide = _blocks(lengths, group, 256)
+    if sum(n * (n + 1) // 2 for n in lengths) < WIDE_MEAN_KEYS * rows or \
+            wide.shape[0] * kv_heads < WIDE_LEAST_BLOCKS:
+        return CausalPlan(lengths, heads, kv_heads, rows, blocks.to(device), None)
+    both = torch.cat((blocks, wide)).to(device)     # one transfer
+    return CausalPlan(lengths, heads, kv_heads, rows, both[:blocks.shape[0]], both[blocks.shape[0]:])
 
 
 def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_lse=False,
@@ -114,9 +130,12 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
         lse = torch.empty((rows, heads), dtype=torch.float32, device=device)
         if rows > plan.rows:
             lse[plan.rows:].fill_(-math.inf)
+    blocks, block_rows = plan.blocks, 128
+    if d == 128 and plan.wide_blocks is not None:
+        blocks, block_rows = plan.wide_blocks, 256
     _lib.call_on(device, "vdn_causal_attention", query.data_ptr(), q_st, q_sh, key.data_ptr(),
-                 k_st, k_sh, value.data_ptr(), v_st, v_sh, plan.blocks.data_ptr(),
-                 plan.blocks.shape[0], plan.block_rows, kv_heads, heads // kv_heads, d,
+                 k_st, k_sh, value.data_ptr(), v_st, v_sh, blocks.data_ptr(), blocks.shape[0],
+                 block_rows, kv_heads, heads // kv_heads, d,
                  int(dtype == torch.float16), scale, out.data_ptr(), out.stride(0), out.stride(1),
                  _lib.ptr(lse), heads, 1, _lib.stream(device))
     return (out, lse) if return_lse else out

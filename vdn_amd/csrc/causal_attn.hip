@@ -41,8 +41,11 @@ struct CausalOut {
 
 // blocks: int32 [nblocks, 4] = (first token row, tokens n of the sequence, first row r0 of the
 // block among the sequence's n G, unused), most keys first.
-template <int kD, int kWaves, int kBN, bool kF16>
-__global__ void __launch_bounds__(kWaves * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+// kWaves waves of 32 rows, tiles of kBN keys, kPerSimd waves on a SIMD (of one workgroup or of
+// several); kSpread sends the next tile's loads out along Sᵀ instead of all at once.
+template <int kD, int kWaves, int kBN, int kPerSimd, bool kSpread, bool kF16>
+__global__ void __launch_bounds__(kWaves * 64)
+    __attribute__((amdgpu_waves_per_eu(kPerSimd, kPerSimd)))
 causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, int nblocks,
                    int kv_heads, int group, float scale_log2) {
   constexpr int kKT = kBN / 32;           // 32-key score accumulators per tile
@@ -116,31 +119,49 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   // lane's share of a tile load: kSegs segments of kSegRows rows per tensor, at fixed byte
   // offsets from the tile's first row
   const int seg_row = lane / kChunks, phys = lane % kChunks;
-  uint32_t koff[kSegs], voff[kSegs];
+  // Segments a multiple of 16 rows apart share the lane's swizzle: one offset per lane, the
+  // segments' distance as the scalar one.
+  constexpr int kApart = kWaves * kSegRows;
+  constexpr int kOffs = kApart % 16 == 0 ? 1 : kSegs;
+  uint32_t koff[kOffs], voff[kOffs];
 #pragma unroll
-  for (int j = 0; j < kSegs; ++j) {
+  for (int j = 0; j < kOffs; ++j) {
     const int row = (j * kWaves + wave) * kSegRows + seg_row;
     koff[j] = static_cast<uint32_t>(row * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row)));
     voff[j] = static_cast<uint32_t>(row * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)));
   }
   const char* k_head = reinterpret_cast<const char*>(in.k + row0 * in.k_st + u * in.k_sh);
   const char* v_head = reinterpret_cast<const char*>(in.v + row0 * in.v_st + u * in.v_sh);
-  auto issue_tile = [&](int a, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t k_rsrc = tile_rsrc(k_head + static_cast<int64_t>(a) * in.k_st * 2);
-    const __amdgpu_buffer_rsrc_t v_rsrc = tile_rsrc(v_head + static_cast<int64_t>(a) * in.v_st * 2);
-    const int last = nkeys - 1 - a;  // rows behind the last key repeat it
+  struct Source {
+    __amdgpu_buffer_rsrc_t k, v;
+    int last;   // the tile's last row with a key; rows behind it repeat that
+  };
+  auto source = [&](int a) __attribute__((always_inline)) {
+    return Source{tile_rsrc(k_head + static_cast<int64_t>(a) * in.k_st * 2),
+                  tile_rsrc(v_head + static_cast<int64_t>(a) * in.v_st * 2), min(nkeys - 1 - a, kBN - 1)};
+  };
+  // segment j of 2 kSegs: K's, then V's
+  auto issue_full = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
+    const bool is_v = j >= kSegs;
+    const int js = is_v ? j - kSegs : j, seg = js * kWaves + wave;
+    const uint32_t apart = kOffs > 1 ? 0 : static_cast<uint32_t>(js * kApart * (is_v ? in.v_st : in.k_st) * 2);
+    load_to_lds16(is_v ? src.v : src.k, is_v ? voff[js % kOffs] : koff[js % kOffs], apart,
+                  (is_v ? dv : dk) + seg * kSegRows * kD);
+  };
+  auto issue = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
+    if (src.last == kBN - 1) return issue_full(src, j, dk, dv);
+    const bool is_v = j >= kSegs;
+    const int seg = (is_v ? j - kSegs : j) * kWaves + wave, row = seg * kSegRows + seg_row;
+    const int r = min(row, src.last);
+    load_to_lds16(is_v ? src.v : src.k,
+                  is_v ? static_cast<uint32_t>(r * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)))
+                       : static_cast<uint32_t>(r * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row))),
+                  0, (is_v ? dv : dk) + seg * kSegRows * kD);
+  };
+  auto issue_all = [&](int a, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
+    const Source src = source(a);
 #pragma unroll
-    for (int j = 0; j < kSegs; ++j) {
-      const int seg = j * kWaves + wave;
-      uint32_t ko = koff[j], vo = voff[j];
-      if (last < kBN - 1) {
-        const int row = seg * kSegRows + seg_row, r = min(row, last);
-        ko = static_cast<uint32_t>(r * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row)));
-        vo = static_cast<uint32_t>(r * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)));
-      }
-      load_to_lds16(k_rsrc, ko, 0, dk + seg * kSegRows * kD);
-      load_to_lds16(v_rsrc, vo, 0, dv + seg * kSegRows * kD);
-    }
+    for (int j = 0; j < 2 * kSegs; ++j) issue(src, j, dk, dv);
   };
 
   f32x16 o[kDB];
@@ -167,7 +188,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     const bool diagonal = a + kBN - 1 > i_first;      // some row does not see the whole tile
     if (diagonal) {
       constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
-#pragma unroll
+#pragma unroll 1
       for (int j = 0; j < kSegs; ++j) {
         const int seg = j * kWaves + wave;
         uint16_t* p = tv + seg * kSegRows * kD + lane * 8;
@@ -179,6 +200,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
         if (mag[0] < kInf && mag[1] < kInf) continue;
         const int row = seg * kSegRows + seg_row;
         const int ch = 8 * (phys ^ swz_v<kD>(row));
+#pragma unroll 1
         for (int i = 0; i < 8; ++i) {
           const uint32_t b = p[i];
           if ((b & 0x7fffu) < kInf) continue;
@@ -191,10 +213,18 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
       }
     }
     __syncthreads();  // tile t is resident and every wave is done with the other buffer
+    // The memory pipe takes 16 cycles for a segment, so a wave that issues its 2 kSegs at once is
+    // held up; spread over the channel steps of Sᵀ they go out in the shadow of its MFMAs (two
+    // workgroups of 4 waves a CU: 3% faster over 32768 tokens). With 8 waves of 128 channels the
+    // scalars and offsets that stay alive for it spill, which costs 2%. A tile with a tail, and a
+    // wave that sees nothing of this tile, issue theirs here.
+    uint16_t* ndk = kBuf == 0 ? sK1 : sK0;
+    uint16_t* ndv = kBuf == 0 ? sV1 : sV0;
     const bool sees = wave_live && a <= w_last;
-    if (t + 1 < ntiles)
-      issue_tile(a + kBN, kBuf == 0 ? sK1 : sK0, kBuf == 0 ? sV1 : sV0);
+    const bool spread = kSpread && sees && nkeys - a >= 2 * kBN;
+    if (t + 1 < ntiles && !spread) issue_all(a + kBN, ndk, ndv);
     if (!sees) return;
+    const Source next = source(a + kBN);
 
     // ---- Sᵀ = K Qᵀ (kKT 32-key accumulators), the fragments of step ks + 1 read before the
     // MFMAs of step ks ----
@@ -220,16 +250,21 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
 #pragma unroll
       for (int kt = 0; kt < kKT; ++kt) s[kt] = E::mfma(kf[ks & 1][kt], qf[ks], s[kt]);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kSpread) {
+        constexpr int kEvery = kSteps / (2 * kSegs);
+        static_assert(kEvery * 2 * kSegs == kSteps, "a segment every kEvery steps");
+        if (spread && ks % kEvery == 0) issue_full(next, ks / kEvery, ndk, ndv);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     // ---- online softmax ----
     if (a + kBN - 1 > w_first) {  // keys behind the row's token
+      const int last = my_i - a - 4 * g;
 #pragma unroll
       for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int key = a + kt * 32 + (v >> 2) * 8 + g * 4 + (v & 3);
-          if (key > my_i) s[kt][v] = -INFINITY;
-        }
+        for (int v = 0; v < 16; ++v)
+          if (kt * 32 + (v >> 2) * 8 + (v & 3) > last) s[kt][v] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -300,7 +335,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     }
   };
   __syncthreads();  // sPos, sNeg, sDirty
-  issue_tile(0, sK0, sV0);
+  issue_all(0, sK0, sV0);
   for (int t = 0; t < ntiles; t += 2) {
     process(t, std::integral_constant<int, 0>{});
     if (t + 1 < ntiles) process(t + 1, std::integral_constant<int, 1>{});
@@ -352,8 +387,8 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
     return set_error(kInvalidArgument, "%s: head_dim must be 64, 128 or 256", name);
   if (dtype != 0 && dtype != 1)
     return set_error(kInvalidArgument, "%s: dtype must be 0 (bf16) or 1 (fp16)", name);
-  if (block_rows != 128 && block_rows != 256)
-    return set_error(kInvalidArgument, "%s: block_rows must be 128 or 256", name);
+  if (block_rows != 128 && (block_rows != 256 || head_dim != 128))
+    return set_error(kInvalidArgument, "%s: block_rows must be 128, or 256 with head_dim 128", name);
   if (!(scale > 0.f) || !isfinite(scale)) return set_error(kInvalidArgument, "%s: bad scale", name);
   if (nblocks == 0) return kOk;
   if (q == nullptr || k == nullptr || v == nullptr || blocks == nullptr || out == nullptr)
@@ -374,13 +409,19 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
                        static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, group,
                        scale * kLog2e);
   };
-#define VDN_CAUSAL(D, F16)                                              \
-  (block_rows == 256 ? launch(causal_attn_kernel<D, 8, D == 256 ? 64 : 128, F16>, 512) \
-                     : launch(causal_attn_kernel<D, 4, D == 256 ? 32 : 64, F16>, 256))
+  // 64 and 256 channels have one variant each. 64: three workgroups a CU (128-row blocks with two:
+  // 370 us, 256-row ones 373, so 343 us over 4 x 4096 tokens, 32 heads). 256: Q and O alone take 192
+  // registers, so one wave per SIMD with twice the registers (203 us against 420 with two, which
+  // spill, over 4097 tokens, 16 heads).
+#define VDN_CAUSAL(F16)                                                                          \
+  head_dim == 64 ? launch(causal_attn_kernel<64, 4, 64, 3, true, F16>, 256)                      \
+  : head_dim == 256 ? launch(causal_attn_kernel<256, 4, 64, 1, true, F16>, 256)                  \
+  : block_rows == 256 ? launch(causal_attn_kernel<128, 8, 128, 2, false, F16>, 512)              \
+                      : launch(causal_attn_kernel<128, 4, 64, 2, true, F16>, 256)
   if (dtype == 0)
-    head_dim == 64 ? VDN_CAUSAL(64, false) : head_dim == 128 ? VDN_CAUSAL(128, false) : VDN_CAUSAL(256, false);
+    VDN_CAUSAL(false);
   else
-    head_dim == 64 ? VDN_CAUSAL(64, true) : head_dim == 128 ? VDN_CAUSAL(128, true) : VDN_CAUSAL(256, true);
+    VDN_CAUSAL(true);
 #undef VDN_CAUSAL
   return check_launch(name);
 }
