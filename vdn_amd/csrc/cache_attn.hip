@@ -237,24 +237,23 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     // Pages of a tile's 16-token groups: lane's K rows lie in group row16 / 4, its V run and
     // scores in group g. Groups behind the last token repeat the last one.
     const int last_group = max(len - 1, 0) & ~15;
+    // Ids and scales stay as loaded until they are used: a check here would wait for every load
+    // that was issued before.
     struct Ids {
       int k, v;   // page of the lane's K rows, of its V run
-      bool ok;
     };
     auto ids_of = [&](int tile0) __attribute__((always_inline)) {
-      const int ik = table[min(tile0 + 16 * (row16 >> 2), last_group) >> c.log_page];
-      const int iv = table[min(tile0 + 16 * g, last_group) >> c.log_page];
-      const bool ok = iv >= 0 && iv < c.pages;
-      return Ids{ik >= 0 && ik < c.pages ? ik : 0, ok ? iv : 0, ok};
+      return Ids{table[min(tile0 + 16 * (row16 >> 2), last_group) >> c.log_page],
+                 table[min(tile0 + 16 * g, last_group) >> c.log_page]};
     };
+    auto in_pool = [&](int id) __attribute__((always_inline)) { return id >= 0 && id < c.pages; };
     auto scale_of = [&](const uint8_t* scales, int id) __attribute__((always_inline)) {
-      return max(static_cast<uint32_t>(scales[static_cast<int64_t>(id) * c.kv_heads + u]),
-                 kLeastScaleByte);
+      return static_cast<uint32_t>(scales[static_cast<int64_t>(in_pool(id) ? id : 0) * c.kv_heads + u]);
     };
     u32x4 kr[4][kKL], vr[kDB];
     auto load_k = [&](int id, int tile0) __attribute__((always_inline)) {
       const int pos = min(tile0 + 16 * (row16 >> 2), last_group) & (page - 1);
-      const uint8_t* p = c.k + (static_cast<int64_t>(id) * c.kv_heads + u) * page * kD +
+      const uint8_t* p = c.k + (static_cast<int64_t>(in_pool(id) ? id : 0) * c.kv_heads + u) * page * kD +
                          (pos + (row16 & 3)) * kD + 16 * g;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -264,7 +263,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     };
     auto load_v = [&](int id, int tile0) __attribute__((always_inline)) {
       const int pos = min(tile0 + 16 * g, last_group) & (page - 1);
-      const uint8_t* p = c.v + (static_cast<int64_t>(id) * c.kv_heads + u) * page * kD +
+      const uint8_t* p = c.v + (static_cast<int64_t>(in_pool(id) ? id : 0) * c.kv_heads + u) * page * kD +
                          row16 * page + pos;
 #pragma unroll
       for (int db = 0; db < kDB; ++db) vr[db] = *reinterpret_cast<const u32x4*>(p + 16 * db * page);
@@ -276,11 +275,11 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     const int tile_end = min(qb * kQuad, len);
     if (tile0 < tile_end) {
       Ids now = ids_of(tile0), next = ids_of(tile0 + kQuad);
-      uint32_t ks = scale_of(c.ks, now.v), vs = scale_of(c.vs, now.v);
       load_k(now.k, tile0);
+      uint32_t ks = scale_of(c.ks, now.v), vs = scale_of(c.vs, now.v);
       load_v(now.v, tile0);
       for (; tile0 < tile_end; tile0 += kQuad) {
-        bad |= !now.ok;                                  // the g groups are all of the tile's
+        bad |= !in_pool(now.v);                          // the g groups are all of the tile's
         const int next0 = tile0 + kQuad;
         const bool more = next0 < tile_end;
         const Ids after = ids_of(next0 + kQuad);
@@ -301,9 +300,9 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
             }
           }
         }
-        const float k_scale = e8m0_scale(ks) * scale_log2;
-        float v_scale = e8m0_scale(vs);
-        uint32_t top = vs;
+        const float k_scale = e8m0_scale(max(ks, kLeastScaleByte)) * scale_log2;
+        uint32_t top = max(vs, kLeastScaleByte);
+        float v_scale = e8m0_scale(top);
         if (more) {
           load_k(next.k, next0);
           ks = scale_of(c.ks, next.v);
@@ -545,7 +544,7 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
   const int d = (tid % kVec) * 4, part = tid / kVec;
   float top = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kAhead = 4;   // slots in flight
+  constexpr int kAhead = 8;   // slots in flight
   for (int64_t w = w0 + part; w <= w1; w += kLanes * kAhead) {
     f32x4 x[kAhead];
     float m[kAhead], l[kAhead];

@@ -25,6 +25,7 @@ from . import _lib
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 _DTYPES = (torch.bfloat16, torch.float16)
+WHOLE_TOKENS = 256   # tokens of a sequence that are never split: no workspace for shorter tables
 
 
 @dataclass(frozen=True)
@@ -228,13 +229,15 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
     lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=device) if return_lse else None
     group = heads // kv_heads
-    nbytes = _workspace_bytes(device.index, tokens, group, d)
-    # from the allocator in stream order: calls on other streams and captured graphs have their own
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    workspace, nbytes = None, 0
+    if table.shape[1] * page > WHOLE_TOKENS:
+        # from the allocator in stream order: calls on other streams and captured graphs have their own
+        nbytes = _workspace_bytes(device.index, tokens, group, d)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _lib.call_on(device, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
                  *_cache_args(cache), table.data_ptr(), table.stride(0), batch, table.shape[1],
                  lengths.data_ptr(), tokens, group, int(dtype == torch.float16), scale,
-                 out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), workspace.data_ptr(), nbytes,
+                 out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), _lib.ptr(workspace), nbytes,
                  _lib.stream(device))
     return (out, lse) if return_lse else out
 
