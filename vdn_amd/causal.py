@@ -119,7 +119,7 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = torch.empty((rows, heads, d), dtype=dtype, device=device)
+        out = query.new_empty(query.shape)
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != query.shape or out.dtype != dtype or out.device != device

@@ -53,6 +53,11 @@ class KVCache:
         if any(t.device != k.device or not t.is_contiguous()
                for t in (k, v, self.k_scales, self.v_scales, self.faults)):
             raise ValueError("the cache's tensors must be contiguous and on one device")
+        # the entry points' arguments, and what every call asks for
+        object.__setattr__(self, "_args", (k.data_ptr(), self.k_scales.data_ptr(), v.data_ptr(),
+                                           self.v_scales.data_ptr(), self.faults.data_ptr(),
+                                           *k.shape))
+        object.__setattr__(self, "_device", k.device)
 
     @property
     def pages(self):
@@ -100,29 +105,24 @@ def _check_cache(cache, what):
         raise RuntimeError(f"{what} is inference-only; use no_grad/inference_mode")
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
-    if cache.k_codes.device.type != "cuda":
+    if cache._device.type != "cuda":
         raise ValueError("the cache must be on a CUDA (HIP) device")
 
 
 def _check_table(table, device):
-    if table.ndim != 2 or table.dtype != torch.int32 or table.device != device \
+    if table.ndim != 2 or table.dtype is not torch.int32 or table.device != device \
             or table.stride(1) != 1 and table.shape[1] > 1:
         raise ValueError("table must be int32 [batch, width] on the cache's device, unit inner stride")
 
 
 def _check_vector(name, t, n, device):
-    if t.shape != (n,) or t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+    if t.shape != (n,) or t.dtype is not torch.int32 or t.device != device \
+            or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
 
 
-def _cache_args(cache):
-    k = cache.k_codes
-    return (k.data_ptr(), cache.k_scales.data_ptr(), cache.v_codes.data_ptr(),
-            cache.v_scales.data_ptr(), cache.faults.data_ptr(), *k.shape)
-
-
 def _move(name, cache, key, value, table, starts, offsets):
-    rows, device = key.shape[0], cache.k_codes.device
+    rows, device = key.shape[0], cache._device
     _check_table(table, device)
     batch, width = table.shape
     _check_vector("starts", starts, batch, device)
@@ -134,7 +134,7 @@ def _move(name, cache, key, value, table, starts, offsets):
         raise ValueError("too many rows")
     k_st, k_sh, _ = key.stride()
     v_st, v_sh, _ = value.stride()
-    _lib.call_on(device, name, *_cache_args(cache), table.data_ptr(), table.stride(0), batch, width,
+    _lib.call_on(device, name, *cache._args, table.data_ptr(), table.stride(0), batch, width,
                  starts.data_ptr(), _lib.ptr(offsets), key.data_ptr(), k_st, k_sh,
                  value.data_ptr(), v_st, v_sh, rows, int(key.dtype == torch.float16),
                  _lib.stream(device))
@@ -153,12 +153,12 @@ def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
     tokens', the held codes are rounded once more. A nonfinite value becomes the NaN code and
     leaves the scale alone. Two sequences must not bring rows for one page in the same call."""
     _check_cache(cache, "write_cache")
-    k = cache.k_codes
-    if key.ndim != 3 or key.shape[1] != k.shape[1] or key.shape[2] != k.shape[3] \
-            or value.shape != key.shape:
+    _, heads, _, d = cache._args[5:]
+    if key.shape[1:] != (heads, d) or key.ndim != 3 or value.shape != key.shape:
         raise ValueError("key and value must be [rows, kv_heads, D] of the cache")
-    if key.dtype not in _DTYPES or value.dtype != key.dtype or key.stride(2) != 1 \
-            or value.stride(2) != 1 or key.device != k.device or value.device != k.device:
+    device = cache._device
+    if key.dtype not in _DTYPES or value.dtype is not key.dtype or key.stride(2) != 1 \
+            or value.stride(2) != 1 or key.device != device or value.device != device:
         raise ValueError("key and value must share BF16 or FP16, unit innermost stride and the "
                          "cache's device")
     _move("vdn_cache_write", cache, key, value, table, starts, offsets)
@@ -175,8 +175,8 @@ def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bflo
         raise ValueError("rows must be a non-negative integer")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be BF16 or FP16")
-    _, heads, _, d = cache.k_codes.shape
-    key = torch.empty((rows, heads, d), dtype=dtype, device=cache.k_codes.device)
+    _, heads, _, d = cache._args[5:]
+    key = torch.empty((rows, heads, d), dtype=dtype, device=cache._device)
     value = torch.empty_like(key)
     _move("vdn_cache_read", cache, key, value, table, starts, offsets)
     return key, value
@@ -199,8 +199,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     _check_cache(cache, "cache_attention")
     if query.ndim not in (3, 4):
         raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
-    k, dtype, device = cache.k_codes, query.dtype, query.device
-    _, kv_heads, page, dim = k.shape
+    dtype, device = query.dtype, query.device
+    _, kv_heads, page, dim = cache._args[5:]
     if query.ndim == 4:
         batch, tokens, heads, d = query.shape
         q_sb, q_st, q_sh, q_sd = query.stride()
@@ -210,19 +210,20 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
         tokens, q_st = 1, 0
     if d != dim or heads <= 0 or heads % kv_heads or tokens <= 0:
         raise ValueError("query heads must be a multiple of the cache's, D the same, Q positive")
-    if dtype not in _DTYPES or q_sd != 1 or device != k.device:
+    if dtype not in _DTYPES or q_sd != 1 or device != cache._device:
         raise ValueError("query must be BF16 or FP16 with unit innermost stride, on the cache's device")
     _check_table(table, device)
     _check_vector("lengths", lengths, batch, device)
-    if table.shape[0] != batch or table.shape[1] <= 0:
+    table_batch, width = table.shape
+    if table_batch != batch or width <= 0:
         raise ValueError("table must name at least one page for each sequence of the query")
-    if table.shape[1] * page > 2 ** 31 - 1024:
+    if width * page > 2 ** 31 - 1024:
         raise ValueError("the table is too wide")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = torch.empty(query.shape, dtype=dtype, device=device)
+        out = query.new_empty(query.shape)
     elif (out.shape != query.shape or out.dtype != dtype or out.device != device
           or out.stride(-1) != 1):
         raise ValueError("out must be a view like the query, unit channel stride")
@@ -230,12 +231,12 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=device) if return_lse else None
     group = heads // kv_heads
     workspace, nbytes = None, 0
-    if table.shape[1] * page > WHOLE_TOKENS:
+    if width * page > WHOLE_TOKENS:
         # from the allocator in stream order: calls on other streams and captured graphs have their own
         nbytes = _workspace_bytes(device.index, tokens, group, d)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
     _lib.call_on(device, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
-                 *_cache_args(cache), table.data_ptr(), table.stride(0), batch, table.shape[1],
+                 *cache._args, table.data_ptr(), table.stride(0), batch, width,
                  lengths.data_ptr(), tokens, group, int(dtype == torch.float16), scale,
                  out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), _lib.ptr(workspace), nbytes,
                  _lib.stream(device))
