@@ -221,6 +221,8 @@ def test_refusals(device):
             vc.causal_attention(q, k, v, plan, scale)
     with pytest.raises(ValueError, match="out"):
         vc.causal_attention(q, k, v, plan, out=torch.empty_like(q, dtype=FP16))
+    with pytest.raises(ValueError, match="out"):
+        vc.causal_attention(q, k, v, plan, out=torch.empty(40, 1, 128, dtype=BF16, device=device).expand(40, 4, 128))
     with pytest.raises(RuntimeError, match="16-byte"):
         odd = torch.zeros(40, 4, 132, dtype=BF16, device=device)[..., 4:]
         vc.causal_attention(odd, k, v, plan)

@@ -204,7 +204,7 @@ def test_faults_are_reported_and_not_followed(device):
     keep[p] = False
     for t, old in zip((cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales), codes):
         assert torch.equal(t[keep.cuda()], old[keep.cuda()])
-    for offsets in ((0, 12, 12, 12), (-4, 2, 2, 2), (0, 5, 3, 3)):
+    for offsets in ((0, 12, 12, 12), (-4, 2, 2, 2), (0, 5, 3, 3), (2, 3, 5, 9), (40, 50, 60, 70)):
         kv.read_cache(cache, table.cuda(), ints(0, 0, 0), ints(*offsets), 9)
         with pytest.raises(RuntimeError):
             cache.check()
@@ -463,7 +463,8 @@ def test_refusals(device):
                 dict(table=table.long()), dict(table=table[0]), dict(table=table[:, :0]),
                 dict(table=table.t().contiguous().t()), dict(table=table.cpu()), dict(lengths=one.long()),
                 dict(lengths=one[:1]), dict(lengths=one.cpu()), dict(scale=-1.0), dict(scale=math.inf),
-                dict(out=q.float()), dict(out=q[:1])):
+                dict(out=q.float()), dict(out=q[:1]),
+                dict(out=q[:, :1].expand(2, 4, 64))):
         args = dict(query=q, cache=cache, table=table, lengths=one) | bad
         with pytest.raises(ValueError):
             kv.cache_attention(**args)

@@ -17,7 +17,7 @@ from . import _lib
 MAX_ROWS = 2 ** 31 - 512   # rows (tokens x query heads of a K/V head) of one sequence
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class CausalPlan:
     """Blocks of the packed sequences: `blocks` int32 [n, 4] on the device = (first packed row of
     the sequence, its tokens, first row of the block among the sequence's tokens x heads /
@@ -123,8 +123,9 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != query.shape or out.dtype != dtype or out.device != device
-          or out.stride(2) != 1):
-        raise ValueError("out must be a [rows, H, D] view like the queries, unit channel stride")
+          or out.stride(2) != 1 or 0 in out.stride()):
+        raise ValueError("out must be a [rows, H, D] view like the queries, unit channel stride, "
+                         "no broadcast")
     lse = None
     if return_lse:
         lse = torch.empty((rows, heads), dtype=torch.float32, device=device)

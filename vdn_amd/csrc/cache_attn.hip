@@ -662,7 +662,7 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
       q_sh % 8 || o_sb % 8 || o_st % 8 || o_sh % 8)
     return set_error(kInvalidArgument, "%s: codes and rows need 16-byte alignment", name);
   const int64_t rows = static_cast<int64_t>(tokens) * group;
-  if (rows * kv_heads * batch > (1ll << 31) - 1)
+  if (rows * kv_heads * batch * kThreads >= (1ll << 32))
     return set_error(kUnsupported, "%s: too many query rows", name);
   const int block = rows_of_block(static_cast<int>(std::min<int64_t>(rows, 32)), head_dim);
   const int row_blocks = static_cast<int>((rows + block - 1) / block);

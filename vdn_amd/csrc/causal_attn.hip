@@ -400,7 +400,7 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   if (k_st < 0 || v_st < 0 || k_st > (1 << 22) || v_st > (1 << 22))
     return set_error(kUnsupported, "%s: K/V token strides must be in [0, 2^22] elements", name);
   const int64_t total = static_cast<int64_t>(nblocks) * kv_heads;
-  if (total > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many blocks", name);
+  if (total * 512 >= (1ll << 32)) return set_error(kUnsupported, "%s: too many blocks", name);
   const CausalIn in{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                     static_cast<const uint16_t*>(v), q_st, q_sh, k_st, k_sh, v_st, v_sh};
   const CausalOut to{static_cast<uint16_t*>(out), lse, o_st, o_sh, l_st, l_sh};

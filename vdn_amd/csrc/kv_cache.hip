@@ -81,7 +81,10 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
       const int64_t i = lo + static_cast<int64_t>(lane) * step;
       const bool le = i <= s.batch && seq_base(s, static_cast<int>(i), log_page) <= slot;
       const int found = __popcll(__ballot(le));
-      if (found == 0) return p;
+      if (found == 0) {
+        *c.faults = 1;
+        return p;
+      }
       lo = min(lo + (found - 1) * step, s.batch);
     }
     // the last round has loaded what the sequence needs: one memory latency less
@@ -90,14 +93,17 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
     const int from = s.batch > 0 ? s.starts[min(i, s.batch - 1)] : 0;
     const int base = (off >> log_page) + 2 * i;
     const int found = __popcll(__ballot(lo + lane <= s.batch && base <= slot));
-    if (found == 0) return p;
+    if (found == 0) {
+      *c.faults = 1;   // rows in front of the first sequence
+      return p;
+    }
     p.seq = lo + found - 1;
     j = slot - __builtin_amdgcn_readlane(base, found - 1);
     if (j < 0) return p;
     start = __builtin_amdgcn_readlane(from, found - 1);
     const int o0 = __builtin_amdgcn_readlane(off, found - 1);
     const int o1 = p.seq == s.batch ? rows : __builtin_amdgcn_readlane(next, found - 1);
-    if (o0 < 0 || o1 < o0 || o1 > rows) *c.faults = 1;
+    if (o0 < 0 || o1 < o0 || o1 > rows || (p.seq == 0 && o0 > 0)) *c.faults = 1;
     first = min(max(o0, 0), rows);
     end = min(max(o1, 0), rows);
     if (p.seq == s.batch) {
@@ -397,12 +403,13 @@ int move_rows(const char* name, const KvCache& c, int page, Rows rows, Seqs s, i
   const int64_t slots = s.offsets == nullptr
                             ? (kWrite ? s.batch : static_cast<int64_t>(max(s.batch, rows.count)))
                             : (rows.count >> c.log_page) + 2 * static_cast<int64_t>(s.batch) + (kWrite ? 0 : 1);
-  const int64_t workgroups = slots * 2 * c.kv_heads;
-  if (workgroups > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many pages or heads", name);
-  const dim3 grid(static_cast<unsigned>(workgroups));
   // waves that hold a page: one tile each, two where that would take over 16 waves
   const int tiles = (page * head_dim + kTileValues - 1) / kTileValues;
   const int waves = tiles > 16 ? 16 : tiles;
+  const int64_t workgroups = slots * 2 * c.kv_heads;
+  if (workgroups * 64 * waves >= (1ll << 32))
+    return set_error(kUnsupported, "%s: too many pages or heads", name);
+  const dim3 grid(static_cast<unsigned>(workgroups));
   const auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, static_cast<hipStream_t>(stream), c, rows, s);
   };

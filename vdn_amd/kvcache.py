@@ -28,7 +28,7 @@ _DTYPES = (torch.bfloat16, torch.float16)
 WHOLE_TOKENS = 256   # tokens of a sequence that are never split: no workspace for shorter tables
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class KVCache:
     """k_codes uint8 [pages, kv_heads, page, D], k_scales uint8 [pages, kv_heads] (e + 127), v_codes
     uint8 [pages, kv_heads, D, page], v_scales like k_scales, faults int32 [1]; all contiguous."""
@@ -225,8 +225,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     if out is None:
         out = query.new_empty(query.shape)
     elif (out.shape != query.shape or out.dtype != dtype or out.device != device
-          or out.stride(-1) != 1):
-        raise ValueError("out must be a view like the query, unit channel stride")
+          or out.stride(-1) != 1 or 0 in out.stride()):
+        raise ValueError("out must be a view like the query, unit channel stride, no broadcast")
     o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
     lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=device) if return_lse else None
     group = heads // kv_heads
