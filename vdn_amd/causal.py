@@ -10,6 +10,7 @@ from __future__ import annotations
 import math
 from dataclasses import dataclass
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -46,16 +47,18 @@ WIDE_LEAST_BLOCKS = 512    # two for each of 256 CUs
 
 
 def _blocks(lengths, group, block_rows):
-    """[nblocks, 4] of all sequences, by falling number of keys."""
-    n = torch.tensor(lengths, dtype=torch.int64)
-    first = n.cumsum(0) - n
+    """[nblocks, 4] of all sequences, by falling number of keys (a host tensor)."""
+    n = np.array(lengths, dtype=np.int64)
+    first = n.cumsum() - n
     count = (n * group + block_rows - 1) // block_rows
-    seq = torch.repeat_interleave(torch.arange(len(lengths)), count)
-    r0 = (torch.arange(seq.numel()) - (count.cumsum(0) - count)[seq]) * block_rows
-    keys = torch.minimum(r0 + block_rows, n[seq] * group)
-    order = torch.argsort(keys, descending=True, stable=True)
-    blocks = torch.stack((first[seq], n[seq], r0, torch.zeros_like(r0)), 1)
-    return blocks[order].to(torch.int32)
+    seq = np.repeat(np.arange(len(lengths)), count)
+    r0 = (np.arange(seq.size) - (count.cumsum() - count)[seq]) * block_rows
+    keys = np.minimum(r0 + block_rows, n[seq] * group)
+    blocks = np.zeros((seq.size, 4), dtype=np.int32)
+    order = np.argsort(-keys, kind="stable")
+    for column, values in enumerate((first[seq], n[seq], r0)):
+        blocks[:, column] = values[order]
+    return torch.from_numpy(blocks)
 
 
 def prepare_causal_plan(lengths, heads, kv_heads=None, *, device="cpu"):
@@ -75,12 +78,13 @@ def prepare_causal_plan(lengths, heads, kv_heads=None, *, device="cpu"):
         device = torch.device("cuda", torch.cuda.current_device())
     rows = sum(lengths)
     blocks = _blocks(lengths, group, 128)
-    wide = _blocks(lengths, group, 256)
-    if sum(n * (n + 1) // 2 for n in lengths) < WIDE_MEAN_KEYS * rows or \
-            wide.shape[0] * kv_heads < WIDE_LEAST_BLOCKS:
-        return CausalPlan(lengths, heads, kv_heads, rows, blocks.to(device), None)
-    both = torch.cat((blocks, wide)).to(device)     # one transfer
-    return CausalPlan(lengths, heads, kv_heads, rows, both[:blocks.shape[0]], both[blocks.shape[0]:])
+    if sum(n * (n + 1) // 2 for n in lengths) >= WIDE_MEAN_KEYS * rows > 0:
+        wide = _blocks(lengths, group, 256)
+        if wide.shape[0] * kv_heads >= WIDE_LEAST_BLOCKS:
+            both = torch.cat((blocks, wide)).to(device)     # one transfer
+            return CausalPlan(lengths, heads, kv_heads, rows, both[:blocks.shape[0]],
+                              both[blocks.shape[0]:])
+    return CausalPlan(lengths, heads, kv_heads, rows, blocks.to(device), None)
 
 
 def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_lse=False,

@@ -26,6 +26,16 @@
 namespace vdn {
 namespace {
 
+// Maximum and sum over lanes l and l ^ 32 (the two halves of a row's keys), without LDS.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+
 struct CausalIn {
   const uint16_t* q;
   const uint16_t* k;
@@ -57,7 +67,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   constexpr int kThreads = 64 * kWaves;
   constexpr int kSegs = kBN / kSegRows / kWaves;  // 1 KB segments per tensor per wave
   static_assert(kSegs * kWaves * kSegRows == kBN, "segment mapping");
-  static_assert(kBM <= 4 * kBN, "the epilogue stages the block in the tile buffers");
+  static_assert(kBM <= 4 * kBN && kBN % 32 == 0, "the epilogue stages the block in the tile buffers");
   typedef Elem<kF16> E;
   typedef typename E::x8 x8;
   // one array per buffer: the compiler then tells a prefetch into one from reads of the other
@@ -93,8 +103,6 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, col = lane & 31;
-  for (int d = tid; d < kD; d += kThreads) sPos[d] = sNeg[d] = 0x7fffffff;
-  if (tid == 0) sDirty = 0;
 
   const int w0 = r0 + wave * 32;                 // the wave's rows
   const bool wave_live = w0 < rows;
@@ -104,17 +112,6 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   const bool live = my_r < rows;
   const int my_i = live ? my_r / group : i_first;
   const int my_h = u * group + (live ? my_r - my_i * group : 0);
-
-  // ---- Q fragments: row my_r, channels 16 ks + 8 g .. +8 ----
-  x8 qf[kSteps];
-  {
-    const uint16_t* src = in.q + (row0 + my_i) * in.q_st + my_h * in.q_sh;
-#pragma unroll
-    for (int ks = 0; ks < kSteps; ++ks) {
-      const u32x4 w = *reinterpret_cast<const u32x4*>(src + 16 * ks + 8 * g);
-      qf[ks] = __builtin_bit_cast(x8, w);
-    }
-  }
 
   // lane's share of a tile load: kSegs segments of kSegRows rows per tensor, at fixed byte
   // offsets from the tile's first row
@@ -164,12 +161,36 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     for (int j = 0; j < 2 * kSegs; ++j) issue(src, j, dk, dv);
   };
 
+  for (int d = tid; d < kD; d += kThreads) sPos[d] = sNeg[d] = 0x7fffffff;
+  if (tid == 0) sDirty = 0;
+  issue_all(0, sK0, sV0);
+
+  // ---- Q fragments: row my_r, channels 16 ks + 8 g .. +8 ----
+  x8 qf[kSteps];
+  {
+    const uint16_t* src = in.q + (row0 + my_i) * in.q_st + my_h * in.q_sh;
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(src + 16 * ks + 8 * g);
+      qf[ks] = __builtin_bit_cast(x8, w);
+    }
+  }
+
   f32x16 o[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m = -INFINITY, l = 0.f;
+  // With one wave per SIMD half of the registers are accumulation registers, and O stays in them
+  // if the rare branches that compute on it hand it back there; otherwise the compiler moves all
+  // of O to the other half and back in every tile.
+  auto keep = [&]() __attribute__((always_inline)) {
+    if constexpr (kPerSimd == 1) {
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) asm volatile("" : "+a"(o[db]));
+    }
+  };
 
   // transpose-read coordinates (16-lane group G = lane / 16)
   const int G = lane >> 4, L = lane & 15;
@@ -271,16 +292,18 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kt][v]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale_log2;
+    mx = max_halves(mx) * scale_log2;
     const bool grow = mx > m + kLazy;
     if (__any(grow)) {
       const float m_new = grow ? mx : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
       l *= corr;
+      keep();
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[db][v] *= corr;
+      keep();
       m = m_new;
     }
     float rs = 0.f;
@@ -292,8 +315,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
         s[kt][v] = p;
         rs += p;
       }
-    rs += __shfl_xor(rs, 32);
-    l += rs;
+    l += rs;   // of this lane's keys; the halves are joined at the end
 
     // ---- Oᵀ += Vᵀ Pᵀ, 16 keys per MFMA; the V fragments of MFMA i + kVA are read before
     // MFMA i ----
@@ -324,6 +346,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
       __builtin_amdgcn_sched_barrier(0x406);
     }
     if (diagonal && sDirty != 0) {
+      keep();
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -332,38 +355,43 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
           if (sPos[d] <= my_i) o[db][v] += INFINITY;
           if (sNeg[d] <= my_i) o[db][v] -= INFINITY;
         }
+      keep();
     }
   };
   __syncthreads();  // sPos, sNeg, sDirty
-  issue_all(0, sK0, sV0);
   for (int t = 0; t < ntiles; t += 2) {
     process(t, std::integral_constant<int, 0>{});
     if (t + 1 < ntiles) process(t + 1, std::integral_constant<int, 1>{});
   }
+  keep();
+  l = sum_halves(l);
   const float inv_l = 1.0f / l;   // every row sees its own token: l > 0
   __syncthreads();                // the epilogue reuses the tile buffers
 
-  // ---- epilogue: O / l through LDS to rows, kBN rows per buffer ----
-  auto stage_rows = [&](int r) -> uint16_t* {
-    const int which = r / kBN;
-    return which == 0 ? sK0 : which == 1 ? sK1 : which == 2 ? sV0 : sV1;
-  };
-  const int qr = wave * 32 + col;
-  uint16_t* sO = stage_rows(qr);
+  // ---- epilogue: O / l through LDS to rows. Each wave stages its own 32 (no further barrier), four
+  // channels a write; chunk c of row r lies at c ^ swz_k(r), so that the 32 rows of a write and the
+  // rows of a read spread over the banks. ----
+  const int first = wave * 32;
+  uint16_t* sO = (first / kBN == 0 ? sK0 : first / kBN == 1 ? sK1 : first / kBN == 2 ? sV0 : sV1) +
+                 first % kBN * kD;
 #pragma unroll
   for (int db = 0; db < kDB; ++db)
 #pragma unroll
-    for (int v = 0; v < 16; ++v)
-      sO[(qr % kBN) * kD + 32 * db + (v >> 2) * 8 + g * 4 + (v & 3)] = E::bits(o[db][v] * inv_l);
+    for (int j = 0; j < 4; ++j) {
+      typename E::x4 y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = static_cast<typename E::type>(o[db][4 * j + i] * inv_l);
+      *reinterpret_cast<typename E::x4*>(sO + col * kD + ((4 * db + j) ^ swz_k<kD>(col)) * 8 + 4 * g) = y;
+    }
   if (to.lse != nullptr && live && g == 0)
     to.lse[(row0 + my_i) * to.l_st + my_h * to.l_sh] = (m + log2f(l)) * kLn2;
-  __syncthreads();
-  for (int r = tid / kChunks; r < kBM; r += kThreads / kChunks) {
-    if (r0 + r >= rows) continue;
-    const int i = (r0 + r) / group, h = u * group + (r0 + r) - i * group;
-    const int c8 = (tid % kChunks) * 8;
-    const u32x4 row8 = *reinterpret_cast<const u32x4*>(&stage_rows(r)[(r % kBN) * kD + c8]);
-    *reinterpret_cast<u32x4*>(to.out + (row0 + i) * to.o_st + h * to.o_sh + c8) = row8;
+#pragma unroll
+  for (int k = 0; k < 32; k += kSegRows) {
+    const int r = k + seg_row;   // kChunks lanes a row
+    const u32x4 row8 = *reinterpret_cast<const u32x4*>(sO + r * kD + (phys ^ swz_k<kD>(r)) * 8);
+    const int i = __shfl(my_i, r), h = __shfl(my_h, r);
+    if (w0 + r < rows)
+      *reinterpret_cast<u32x4*>(to.out + (row0 + i) * to.o_st + h * to.o_sh + phys * 8) = row8;
   }
 }
 
