@@ -170,14 +170,23 @@ def stream(device: torch.device) -> int:
                                               else index)
 
 
-def call_on(device: torch.device, name: str, *args) -> None:
-    """call() with `device` as the current one: a launch goes to the current device, whatever
-    its stream's is."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args)
-    else:
-        with torch.cuda.device(device):
-            call(name, *args)
+def call_on(device_index: int, name: str, *args) -> None:
+    """call() with device `device_index` as the current one: a launch goes to the current device,
+    whatever its stream's is."""
+    if device_index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device_index):
+            return call(name, *args)
+    if _TIMERS:
+        return call(name, *args)
+    lib = _LIB or load()
+    status = getattr(lib, name)(*args)
+    if status != 0:
+        raise RuntimeError(f"{name} failed ({status}): {lib.vdn_last_error().decode()}")
+
+
+def raw_stream(device_index: int) -> int:
+    """stream() by device index."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 
+_DTYPES = (torch.bfloat16, torch.float16)
 MAX_ROWS = 2 ** 31 - 512   # rows (tokens x query heads of a K/V head) of one sequence
 
 
@@ -106,18 +107,19 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
     if query.ndim != 3:
         raise ValueError("Q/K/V must be [rows, heads, D]")
     rows, heads, d = query.shape
-    kv_heads, dtype, device = plan.kv_heads, query.dtype, query.device
+    kv_heads, dtype = plan.kv_heads, query.dtype
     if (heads != plan.heads or key.shape != (rows, kv_heads, d) or value.shape != key.shape
             or rows < plan.rows or d not in (64, 128, 256)):
         raise ValueError("Q/K/V do not match the plan's heads and rows, or D is not 64, 128 or 256")
     q_st, q_sh, q_sd = query.stride()
     k_st, k_sh, k_sd = key.stride()
     v_st, v_sh, v_sd = value.stride()
-    if dtype not in (torch.bfloat16, torch.float16) or key.dtype != dtype or value.dtype != dtype \
+    if dtype not in _DTYPES or key.dtype is not dtype or value.dtype is not dtype \
             or q_sd != 1 or k_sd != 1 or v_sd != 1:
         raise ValueError("Q/K/V must share BF16 or FP16 and have unit innermost stride")
-    if device.type != "cuda" or key.device != device or value.device != device \
-            or plan.blocks.device != device:
+    index = query.get_device()
+    if not query.is_cuda or key.get_device() != index or value.get_device() != index \
+            or plan.blocks.get_device() != index:
         raise ValueError("Q/K/V and prepared plan must be on the same CUDA device")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
@@ -126,21 +128,21 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
         out = query.new_empty(query.shape)
         if rows > plan.rows:
             out[plan.rows:].zero_()
-    elif (out.shape != query.shape or out.dtype != dtype or out.device != device
+    elif (out.shape != query.shape or out.dtype is not dtype or out.device != query.device
           or out.stride(2) != 1 or 0 in out.stride()):
         raise ValueError("out must be a [rows, H, D] view like the queries, unit channel stride, "
                          "no broadcast")
     lse = None
     if return_lse:
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=device)
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=query.device)
         if rows > plan.rows:
             lse[plan.rows:].fill_(-math.inf)
     blocks, block_rows = plan.blocks, 128
     if d == 128 and plan.wide_blocks is not None:
         blocks, block_rows = plan.wide_blocks, 256
-    _lib.call_on(device, "vdn_causal_attention", query.data_ptr(), q_st, q_sh, key.data_ptr(),
+    _lib.call_on(index, "vdn_causal_attention", query.data_ptr(), q_st, q_sh, key.data_ptr(),
                  k_st, k_sh, value.data_ptr(), v_st, v_sh, blocks.data_ptr(), blocks.shape[0],
                  block_rows, kv_heads, heads // kv_heads, d,
-                 int(dtype == torch.float16), scale, out.data_ptr(), out.stride(0), out.stride(1),
-                 _lib.ptr(lse), heads, 1, _lib.stream(device))
+                 int(dtype is torch.float16), scale, out.data_ptr(), out.stride(0), out.stride(1),
+                 _lib.ptr(lse), heads, 1, _lib.raw_stream(index))
     return (out, lse) if return_lse else out

@@ -57,7 +57,7 @@ class KVCache:
         object.__setattr__(self, "_args", (k.data_ptr(), self.k_scales.data_ptr(), v.data_ptr(),
                                            self.v_scales.data_ptr(), self.faults.data_ptr(),
                                            *k.shape))
-        object.__setattr__(self, "_device", k.device)
+        object.__setattr__(self, "_index", k.get_device())   # -1 off the GPU
 
     @property
     def pages(self):
@@ -105,39 +105,39 @@ def _check_cache(cache, what):
         raise RuntimeError(f"{what} is inference-only; use no_grad/inference_mode")
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
-    if cache._device.type != "cuda":
+    if cache._index < 0:
         raise ValueError("the cache must be on a CUDA (HIP) device")
 
 
-def _check_table(table, device):
-    if table.ndim != 2 or table.dtype is not torch.int32 or table.device != device \
+def _check_table(table, index):
+    if table.ndim != 2 or table.dtype is not torch.int32 or table.get_device() != index \
             or table.stride(1) != 1 and table.shape[1] > 1:
         raise ValueError("table must be int32 [batch, width] on the cache's device, unit inner stride")
 
 
-def _check_vector(name, t, n, device):
-    if t.shape != (n,) or t.dtype is not torch.int32 or t.device != device \
+def _check_vector(name, t, n, index):
+    if t.shape != (n,) or t.dtype is not torch.int32 or t.get_device() != index \
             or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
 
 
 def _move(name, cache, key, value, table, starts, offsets):
-    rows, device = key.shape[0], cache._device
-    _check_table(table, device)
+    rows, index = key.shape[0], cache._index
+    _check_table(table, index)
     batch, width = table.shape
-    _check_vector("starts", starts, batch, device)
+    _check_vector("starts", starts, batch, index)
     if offsets is not None:
-        _check_vector("offsets", offsets, batch + 1, device)
+        _check_vector("offsets", offsets, batch + 1, index)
     elif rows != batch:
         raise ValueError("without offsets there is one row for each sequence")
     if rows > 2 ** 31 - 1:
         raise ValueError("too many rows")
     k_st, k_sh, _ = key.stride()
     v_st, v_sh, _ = value.stride()
-    _lib.call_on(device, name, *cache._args, table.data_ptr(), table.stride(0), batch, width,
+    _lib.call_on(index, name, *cache._args, table.data_ptr(), table.stride(0), batch, width,
                  starts.data_ptr(), _lib.ptr(offsets), key.data_ptr(), k_st, k_sh,
-                 value.data_ptr(), v_st, v_sh, rows, int(key.dtype == torch.float16),
-                 _lib.stream(device))
+                 value.data_ptr(), v_st, v_sh, rows, int(key.dtype is torch.float16),
+                 _lib.raw_stream(index))
 
 
 def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
@@ -154,11 +154,11 @@ def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
     leaves the scale alone. Two sequences must not bring rows for one page in the same call."""
     _check_cache(cache, "write_cache")
     _, heads, _, d = cache._args[5:]
-    if key.shape[1:] != (heads, d) or key.ndim != 3 or value.shape != key.shape:
+    if key.ndim != 3 or key.shape != (key.shape[0], heads, d) or value.shape != key.shape:
         raise ValueError("key and value must be [rows, kv_heads, D] of the cache")
-    device = cache._device
     if key.dtype not in _DTYPES or value.dtype is not key.dtype or key.stride(2) != 1 \
-            or value.stride(2) != 1 or key.device != device or value.device != device:
+            or value.stride(2) != 1 or key.get_device() != cache._index \
+            or value.get_device() != cache._index:
         raise ValueError("key and value must share BF16 or FP16, unit innermost stride and the "
                          "cache's device")
     _move("vdn_cache_write", cache, key, value, table, starts, offsets)
@@ -176,7 +176,7 @@ def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bflo
     if dtype not in _DTYPES:
         raise ValueError("dtype must be BF16 or FP16")
     _, heads, _, d = cache._args[5:]
-    key = torch.empty((rows, heads, d), dtype=dtype, device=cache._device)
+    key = torch.empty((rows, heads, d), dtype=dtype, device=cache.k_codes.device)
     value = torch.empty_like(key)
     _move("vdn_cache_read", cache, key, value, table, starts, offsets)
     return key, value
@@ -199,7 +199,7 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     _check_cache(cache, "cache_attention")
     if query.ndim not in (3, 4):
         raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
-    dtype, device = query.dtype, query.device
+    dtype, index = query.dtype, cache._index
     _, kv_heads, page, dim = cache._args[5:]
     if query.ndim == 4:
         batch, tokens, heads, d = query.shape
@@ -210,10 +210,10 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
         tokens, q_st = 1, 0
     if d != dim or heads <= 0 or heads % kv_heads or tokens <= 0:
         raise ValueError("query heads must be a multiple of the cache's, D the same, Q positive")
-    if dtype not in _DTYPES or q_sd != 1 or device != cache._device:
+    if dtype not in _DTYPES or q_sd != 1 or query.get_device() != index:
         raise ValueError("query must be BF16 or FP16 with unit innermost stride, on the cache's device")
-    _check_table(table, device)
-    _check_vector("lengths", lengths, batch, device)
+    _check_table(table, index)
+    _check_vector("lengths", lengths, batch, index)
     table_batch, width = table.shape
     if table_batch != batch or width <= 0:
         raise ValueError("table must name at least one page for each sequence of the query")
@@ -224,28 +224,28 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
         raise ValueError("scale must be finite and positive")
     if out is None:
         out = query.new_empty(query.shape)
-    elif (out.shape != query.shape or out.dtype != dtype or out.device != device
+    elif (out.shape != query.shape or out.dtype is not dtype or out.get_device() != index
           or out.stride(-1) != 1 or 0 in out.stride()):
         raise ValueError("out must be a view like the query, unit channel stride, no broadcast")
     o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
-    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=device) if return_lse else None
+    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=query.device) if return_lse else None
     group = heads // kv_heads
     workspace, nbytes = None, 0
     if width * page > WHOLE_TOKENS:
         # from the allocator in stream order: calls on other streams and captured graphs have their own
-        nbytes = _workspace_bytes(device.index, tokens, group, d)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _lib.call_on(device, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
+        nbytes = _workspace_bytes(index, tokens, group, d)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+    _lib.call_on(index, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
                  *cache._args, table.data_ptr(), table.stride(0), batch, width,
-                 lengths.data_ptr(), tokens, group, int(dtype == torch.float16), scale,
+                 lengths.data_ptr(), tokens, group, int(dtype is torch.float16), scale,
                  out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), _lib.ptr(workspace), nbytes,
-                 _lib.stream(device))
+                 _lib.raw_stream(index))
     return (out, lse) if return_lse else out
 
 
 @lru_cache(maxsize=None)
 def _workspace_bytes(device_index, tokens, group, head_dim):
     nbytes = ctypes.c_int64(0)
-    _lib.call_on(torch.device("cuda", device_index), "vdn_cache_attention_workspace", tokens, group,
+    _lib.call_on(device_index, "vdn_cache_attention_workspace", tokens, group,
                  head_dim, ctypes.addressof(nbytes))
     return nbytes.value
