@@ -127,23 +127,47 @@ __device__ __forceinline__ float widen(uint32_t bits) {
   return kF16 ? f16_bits_to_f32(static_cast<uint16_t>(bits)) : __uint_as_float(bits << 16);
 }
 
-// Codes of two 16-bit values (low half first) in the low two bytes. A nonfinite value gives
-// the NaN code; bf16 values over 1.875 * 2^127 count as that, so that their code (at most 240 at
-// the largest scale 2^120) stands for a finite number.
+// Codes of eight finite 16-bit values (low half first) for the scale s = 2^e.
 template <bool kF16>
-__device__ __forceinline__ uint32_t codes2(uint32_t w, float scale) {
-  constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
-  float x[2];
+__device__ __forceinline__ u32x2 codes8(const u32x4& w, float s) {
+  if constexpr (!kF16) {
+    return e4m3x8_bf16(w, s);
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    u32x2 out;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t b = i ? w >> 16 : w & 0xffffu;
-    x[i] = widen<kF16>(b);
-    if (!kF16) x[i] = fminf(fmaxf(x[i], -0x1.ep127f), 0x1.ep127f);
-    if ((b & 0x7fffu) >= kInf) x[i] = __uint_as_float(0x7fc00000u);
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = w[2 * h], hi = w[2 * h + 1];
+      s16x2_t r = {0, 0};
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, lo), s, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(f16x2, hi), s, true);
+      out[h] = __builtin_bit_cast(uint32_t, r);
+    }
+    return out;
   }
-  s16x2_t r = {0, 0};
-  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[0], x[1], scale, false);
-  return static_cast<uint32_t>(__builtin_bit_cast(uint32_t, r)) & 0xffffu;
+}
+
+// The same for any values. A nonfinite one gives the NaN code; bf16 values over 1.875 * 2^127 count
+// as that, so that their code (at most 240 at the largest scale 2^120) stands for a finite number.
+template <bool kF16>
+__device__ u32x2 codes8_any(const u32x4& w, float s) {
+  constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
+  u32x2 out = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t b = j ? w[i] >> 16 : w[i] & 0xffffu;
+      x[j] = widen<kF16>(b);
+      if (!kF16) x[j] = fminf(fmaxf(x[j], -0x1.ep127f), 0x1.ep127f);
+      if ((b & 0x7fffu) >= kInf) x[j] = __uint_as_float(0x7fc00000u);
+    }
+    s16x2_t r = {0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, x[0], x[1], s, false);
+    out[i >> 1] |= (static_cast<uint32_t>(__builtin_bit_cast(uint32_t, r)) & 0xffffu) << (16 * (i & 1));
+  }
+  return out;
 }
 
 // Four held codes for a scale 2^up larger: rounded once more.
@@ -178,7 +202,7 @@ __device__ __forceinline__ Spot spot(int t, int j, int lane, int log_page) {
 template <int kD, int kTiles, bool kF16, bool kV>
 __device__ __forceinline__ void write_page(const KvCache& c, const Rows& rows, const Seqs& s,
                                            const Piece& p, int u) {
-  __shared__ uint32_t s_mag[16];
+  __shared__ uint32_t s_mag[2][16];
   const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = threads >> 6;
   const int page = 1 << c.log_page;
@@ -205,23 +229,37 @@ __device__ __forceinline__ void write_page(const KvCache& c, const Rows& rows, c
   uint8_t* scale = (kV ? c.vs : c.ks) + block;
   const uint32_t held = p.lo > 0 ? max(static_cast<uint32_t>(*scale), kLeastScaleByte) : 0u;
   constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
-  uint32_t mag = 0;
+  u16x2 pair = {0, 0};
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) pair = __builtin_elementwise_max(pair, mag8_bf16(w[t][j]));
+  auto page_max = [&](uint32_t x, uint32_t* shared) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t lo = w[t][j][i] & 0x7fffu, hi = (w[t][j][i] >> 16) & 0x7fffu;
-        mag = max(mag, lo < kInf ? lo : 0u);
-        mag = max(mag, hi < kInf ? hi : 0u);
-      }
+    for (int d = 32; d; d >>= 1) x = max(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), d)));
+    if (waves > 1) {
+      if (lane == 0) shared[wave] = x;
+      __syncthreads();
+      for (int i = 0; i < waves; ++i) x = max(x, shared[i]);
+    }
+    return x;
+  };
+  uint32_t mag = page_max(max(pair[0], pair[1]), s_mag[0]);
+  // a nonfinite value, or one that is clamped, sends the page to the careful conversion
+  const bool plain = mag < (kF16 ? kInf : 0x7f70u);
+  if (mag >= kInf) {
+    mag = 0;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) mag = max(mag, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mag), d)));
-  if (waves > 1) {
-    if (lane == 0) s_mag[wave] = mag;
-    __syncthreads();
-    for (int i = 0; i < waves; ++i) mag = max(mag, s_mag[i]);
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t lo = w[t][j][i] & 0x7fffu, hi = (w[t][j][i] >> 16) & 0x7fffu;
+          mag = max(mag, lo < kInf ? lo : 0u);
+          mag = max(mag, hi < kInf ? hi : 0u);
+        }
+    mag = page_max(mag, s_mag[1]);
   }
   uint32_t byte = cache_scale_byte(widen<kF16>(mag));
 
@@ -252,10 +290,12 @@ __device__ __forceinline__ void write_page(const KvCache& c, const Rows& rows, c
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
     u32x2 out[4];
+    if (plain) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      out[j][0] = codes2<kF16>(w[t][j][0], sf) | codes2<kF16>(w[t][j][1], sf) << 16;
-      out[j][1] = codes2<kF16>(w[t][j][2], sf) | codes2<kF16>(w[t][j][3], sf) << 16;
+      for (int j = 0; j < 4; ++j) out[j] = codes8<kF16>(w[t][j], sf);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = codes8_any<kF16>(w[t][j], sf);
     }
     const Spot at = spot<kD, kV>(t * waves + wave, 0, lane, c.log_page);
     if (!kV) {
@@ -299,9 +339,9 @@ __global__ void __launch_bounds__(1024) cache_write_kernel(KvCache c, Rows rows,
 // largest value (a value next to it may have been rounded up to 65536); NaN stays NaN.
 template <bool kF16>
 __device__ __forceinline__ uint32_t values2(uint32_t codes, float scale) {
+  if (!kF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
   const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(codes, false);
   float a = f[0] * scale, b = f[1] * scale;
-  if (!kF16) return pack_bf16x2(a, b);
   if (fabsf(a) > 65504.f) a = copysignf(65504.f, a);
   if (fabsf(b) > 65504.f) b = copysignf(65504.f, b);
   return f32_to_f16_bits(a) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16;
