@@ -40,9 +40,10 @@ class CausalPlan:
 # When head dim 128 takes 256-row blocks (8 waves, one workgroup a CU) instead of 128-row ones (two
 # of 4 waves): a K/V tile then serves twice the rows, which pays where rows see many keys, and a
 # block takes the CU to itself, so that there have to be enough of them. Microseconds of 256 and
-# 128 rows: 32768 tokens 8000, 8600; 8192: 534, 565; 4096: 162, 172; 4 x 2048: 188, 178; 24 prompts
-# of 77 - 1200: 174, 140 (the mean row sees 2048 keys of 4096); 8192 tokens of 8 heads that share
-# one K/V head, 256 blocks: 214, 195; 16384 of them, 512 blocks: 525, 612.
+# 128 rows, 32 heads and 8 K/V heads: 32768 tokens 7810, 8410; 8192: 518, 551; 4096: 150, 158 (the
+# mean row sees 2048 keys); 4 x 2048: 174, 169; 2048: 61, 55; 24 prompts of 77 - 1200 with 56 heads
+# 159, 127. 8 heads that share one K/V head: 16384 tokens, 512 blocks: 507, 581; 8192, 256 blocks:
+# 204, 193.
 WIDE_MEAN_KEYS = 2048
 WIDE_LEAST_BLOCKS = 512    # two for each of 256 CUs
 

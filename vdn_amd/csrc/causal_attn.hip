@@ -65,8 +65,9 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   constexpr int kSegRows = 64 / kChunks;  // rows per 1 KB DMA segment (one wave instruction)
   constexpr int kBM = 32 * kWaves;
   constexpr int kThreads = 64 * kWaves;
-  constexpr int kSegs = kBN / kSegRows / kWaves;  // 1 KB segments per tensor per wave
-  static_assert(kSegs * kWaves * kSegRows == kBN, "segment mapping");
+  constexpr int kLoaders = kSpread ? kWaves : kWaves / 2;  // the waves that load tiles (below)
+  constexpr int kSegs = kBN / kSegRows / kLoaders;  // 1 KB segments per tensor per loading wave
+  static_assert(kSegs * kLoaders * kSegRows == kBN, "segment mapping");
   static_assert(kBM <= 4 * kBN && kBN % 32 == 0, "the epilogue stages the block in the tile buffers");
   typedef Elem<kF16> E;
   typedef typename E::x8 x8;
@@ -118,12 +119,12 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   const int seg_row = lane / kChunks, phys = lane % kChunks;
   // Segments a multiple of 16 rows apart share the lane's swizzle: one offset per lane, the
   // segments' distance as the scalar one.
-  constexpr int kApart = kWaves * kSegRows;
+  constexpr int kApart = kLoaders * kSegRows;
   constexpr int kOffs = kApart % 16 == 0 ? 1 : kSegs;
   uint32_t koff[kOffs], voff[kOffs];
 #pragma unroll
   for (int j = 0; j < kOffs; ++j) {
-    const int row = (j * kWaves + wave) * kSegRows + seg_row;
+    const int row = (j * kLoaders + wave) * kSegRows + seg_row;
     koff[j] = static_cast<uint32_t>(row * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row)));
     voff[j] = static_cast<uint32_t>(row * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)));
   }
@@ -140,7 +141,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   // segment j of 2 kSegs: K's, then V's
   auto issue_full = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
     const bool is_v = j >= kSegs;
-    const int js = is_v ? j - kSegs : j, seg = js * kWaves + wave;
+    const int js = is_v ? j - kSegs : j, seg = js * kLoaders + wave;
     const uint32_t apart = kOffs > 1 ? 0 : static_cast<uint32_t>(js * kApart * (is_v ? in.v_st : in.k_st) * 2);
     load_to_lds16(is_v ? src.v : src.k, is_v ? voff[js % kOffs] : koff[js % kOffs], apart,
                   (is_v ? dv : dk) + seg * kSegRows * kD);
@@ -148,7 +149,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   auto issue = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
     if (src.last == kBN - 1) return issue_full(src, j, dk, dv);
     const bool is_v = j >= kSegs;
-    const int seg = (is_v ? j - kSegs : j) * kWaves + wave, row = seg * kSegRows + seg_row;
+    const int seg = (is_v ? j - kSegs : j) * kLoaders + wave, row = seg * kSegRows + seg_row;
     const int r = min(row, src.last);
     load_to_lds16(is_v ? src.v : src.k,
                   is_v ? static_cast<uint32_t>(r * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)))
@@ -163,7 +164,8 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
 
   for (int d = tid; d < kD; d += kThreads) sPos[d] = sNeg[d] = 0x7fffffff;
   if (tid == 0) sDirty = 0;
-  issue_all(0, sK0, sV0);
+  const bool loads = wave < kLoaders;
+  if (loads) issue_all(0, sK0, sV0);
 
   // ---- Q fragments: row my_r, channels 16 ks + 8 g .. +8 ----
   x8 qf[kSteps];
@@ -207,11 +209,11 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     const int a = t * kBN;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of tile t is there
     const bool diagonal = a + kBN - 1 > i_first;      // some row does not see the whole tile
-    if (diagonal) {
+    if (diagonal && loads) {
       constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
 #pragma unroll 1
       for (int j = 0; j < kSegs; ++j) {
-        const int seg = j * kWaves + wave;
+        const int seg = j * kLoaders + wave;
         uint16_t* p = tv + seg * kSegRows * kD + lane * 8;
         u32x4 w = *reinterpret_cast<const u32x4*>(p);
         u16x2 mag = {0, 0};
@@ -234,16 +236,19 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
       }
     }
     __syncthreads();  // tile t is resident and every wave is done with the other buffer
-    // The memory pipe takes 16 cycles for a segment, so a wave that issues its 2 kSegs at once is
-    // held up; spread over the channel steps of Sᵀ they go out in the shadow of its MFMAs (two
-    // workgroups of 4 waves a CU: 3% faster over 32768 tokens). With 8 waves of 128 channels the
-    // scalars and offsets that stay alive for it spill, which costs 2%. A tile with a tail, and a
-    // wave that sees nothing of this tile, issue theirs here.
+    // The memory pipe takes 16 cycles for a segment, so a wave that issues many at once is held up
+    // (about 70 cycles each). Two workgroups of 4 waves a CU: every wave loads its share, spread over
+    // the channel steps of Sᵀ, in the shadow of its MFMAs (3% faster over 32768 tokens; V's along P V
+    // instead came too late for the next tile). One workgroup of 8: waves 0 - 3, the older ones of
+    // their SIMDs, come first through a tile and load for all behind their P V, where they would
+    // wait for the others (3%; spread loads spill there). A tile with a tail, and a wave that sees
+    // nothing of this tile, issue theirs here.
     uint16_t* ndk = kBuf == 0 ? sK1 : sK0;
     uint16_t* ndv = kBuf == 0 ? sV1 : sV0;
     const bool sees = wave_live && a <= w_last;
     const bool spread = kSpread && sees && nkeys - a >= 2 * kBN;
-    if (t + 1 < ntiles && !spread) issue_all(a + kBN, ndk, ndv);
+    const bool behind = !kSpread && sees;
+    if (t + 1 < ntiles && !spread && !behind && loads) issue_all(a + kBN, ndk, ndv);
     if (!sees) return;
     const Source next = source(a + kBN);
 
@@ -345,6 +350,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
       o[db] = E::mfma(vf[i % (kVA + 1)], pb, o[db]);
       __builtin_amdgcn_sched_barrier(0x406);
     }
+    if (behind && loads && t + 1 < ntiles) issue_all(a + kBN, ndk, ndv);
     if (diagonal && sDirty != 0) {
       keep();
 #pragma unroll
@@ -437,10 +443,10 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
                        static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, group,
                        scale * kLog2e);
   };
-  // 64 and 256 channels have one variant each. 64: three workgroups a CU (128-row blocks with two:
-  // 370 us, 256-row ones 373, so 343 us over 4 x 4096 tokens, 32 heads). 256: Q and O alone take 192
-  // registers, so one wave per SIMD with twice the registers (203 us against 420 with two, which
-  // spill, over 4097 tokens, 16 heads).
+  // 64 and 256 channels have one variant each. 64: three workgroups a CU (7% faster than two over 4 x
+  // 4096 tokens of 32 heads, 18% over 64 prompts of 1 - 400; four spill). 256: Q and O alone take 192
+  // registers, so one wave per SIMD with twice the registers (1.10 ms over 2 x 8192 tokens of 16
+  // heads, 1000 TFLOP/s; two waves per SIMD spill and take 2.1).
 #define VDN_CAUSAL(F16)                                                                          \
   head_dim == 64 ? launch(causal_attn_kernel<64, 4, 64, 3, true, F16>, 256)                      \
   : head_dim == 256 ? launch(causal_attn_kernel<256, 4, 64, 1, true, F16>, 256)                  \
