@@ -228,3 +228,22 @@ def test_refusals(device):
         vc.causal_attention(odd, k, v, plan)
     with torch.enable_grad(), pytest.raises(RuntimeError, match="inference-only"):
         vc.causal_attention(q, k, v, plan)
+
+
+@pytest.mark.parametrize("dim,dtype,block_rows", [(64, FP16, 128), (128, BF16, 128), (128, BF16, 256),
+                                                  (256, BF16, 128)])
+@torch.no_grad()
+def test_keys_that_score_minus_infinity(device, dim, dtype, block_rows):
+    """The first keys score -inf against every query, whole tiles of them: they get weight 0, and
+    rows that see no others are NaN with LSE -inf."""
+    n, shut = 451, 200
+    q, k, v = (x.clone() for x in make([n], 4, 2, dim, dtype, seed=13))
+    q[..., 5] = 1.0
+    k[:shut, :, 5] = -math.inf
+    plan = vc.prepare_causal_plan([n], 4, 2, device=device)
+    if block_rows == 256:
+        wide = vc._blocks((n,), 2, 256).cuda()
+        plan = vc.CausalPlan(plan.lengths, 4, 2, n, plan.blocks, wide)
+    got, lse = vc.causal_attention(q, k, v, plan, return_lse=True)
+    assert got[:shut].isnan().all() and (lse[:shut] == -math.inf).all()
+    check(q[shut:], k[shut:], v[shut:], [n - shut], got[shut:], lse[shut:])

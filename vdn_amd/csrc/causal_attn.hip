@@ -19,6 +19,7 @@
 // holds that value exactly if the token is not behind its own: it is added after the product.
 #include "attn_tiles.h"
 
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -183,7 +184,8 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   for (int db = 0; db < kDB; ++db)
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  // m starts finite: a tile whose scores are all -inf then adds nothing instead of inf - inf
+  float m = -FLT_MAX, l = 0.f;
   // With one wave per SIMD half of the registers are accumulation registers, and O stays in them
   // if the rare branches that compute on it hand it back there; otherwise the compiler moves all
   // of O to the other half and back in every tile.
@@ -371,7 +373,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   }
   keep();
   l = sum_halves(l);
-  const float inv_l = 1.0f / l;   // every row sees its own token: l > 0
+  const float inv_l = 1.0f / l;   // l = 0 only if all scores are -inf: NaN, LSE -inf
   __syncthreads();                // the epilogue reuses the tile buffers
 
   // ---- epilogue: O / l through LDS to rows. Each wave stages its own 32 (no further barrier), four
