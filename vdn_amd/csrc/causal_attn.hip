@@ -44,6 +44,16 @@ struct CausalIn {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // token / head strides (elements)
 };
 
+// r / group for 0 <= r < 2^31, without a division: with s = ceil(log2 group) and mul = ceil(2^(31 + s) /
+// group), r mul is r 2^(31 + s) / group and less than r <= 2^31 too much: the quotient stays.
+struct GroupOf {
+  uint32_t mul;
+  int shift;   // 31 + s
+  __device__ __forceinline__ int operator()(int r) const {
+    return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(r)) * mul >> shift);
+  }
+};
+
 struct CausalOut {
   uint16_t* out;
   float* lse;
@@ -58,7 +68,7 @@ template <int kD, int kWaves, int kBN, int kPerSimd, bool kSpread, bool kF16>
 __global__ void __launch_bounds__(kWaves * 64)
     __attribute__((amdgpu_waves_per_eu(kPerSimd, kPerSimd)))
 causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, int nblocks,
-                   int kv_heads, int group, float scale_log2) {
+                   int kv_heads, int group, GroupOf token_of, float scale_log2) {
   constexpr int kKT = kBN / 32;           // 32-key score accumulators per tile
   constexpr int kDB = kD / 32;            // 32-channel output accumulators
   constexpr int kSteps = kD / 16;         // channel steps of Sᵀ
@@ -98,8 +108,8 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   const int n = __builtin_amdgcn_readfirstlane(blocks[4 * blk + 1]);
   const int r0 = __builtin_amdgcn_readfirstlane(blocks[4 * blk + 2]);
   const int rows = n * group;
-  const int i_first = r0 / group;                               // the block's tokens
-  const int nkeys = min(r0 + kBM - 1, rows - 1) / group + 1;    // keys that its last row sees
+  const int i_first = token_of(r0);                             // the block's tokens
+  const int nkeys = token_of(min(r0 + kBM - 1, rows - 1)) + 1;   // keys that its last row sees
   const int ntiles = (nkeys + kBN - 1) / kBN;
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -108,11 +118,11 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
 
   const int w0 = r0 + wave * 32;                 // the wave's rows
   const bool wave_live = w0 < rows;
-  const int w_first = w0 / group;
-  const int w_last = min(w0 + 31, rows - 1) / group;
+  const int w_first = token_of(w0);
+  const int w_last = token_of(min(w0 + 31, rows - 1));
   const int my_r = w0 + col;
   const bool live = my_r < rows;
-  const int my_i = live ? my_r / group : i_first;
+  const int my_i = live ? token_of(my_r) : i_first;
   const int my_h = u * group + (live ? my_r - my_i * group : 0);
 
   // lane's share of a tile load: kSegs segments of kSegRows rows per tensor, at fixed byte
@@ -393,13 +403,14 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     }
   if (to.lse != nullptr && live && g == 0)
     to.lse[(row0 + my_i) * to.l_st + my_h * to.l_sh] = (m + log2f(l)) * kLn2;
+  const int64_t my_out = (row0 + my_i) * to.o_st + my_h * to.o_sh;
+  const int out_lo = static_cast<int>(my_out), out_hi = static_cast<int>(my_out >> 32);
 #pragma unroll
   for (int k = 0; k < 32; k += kSegRows) {
     const int r = k + seg_row;   // kChunks lanes a row
     const u32x4 row8 = *reinterpret_cast<const u32x4*>(sO + r * kD + (phys ^ swz_k<kD>(r)) * 8);
-    const int i = __shfl(my_i, r), h = __shfl(my_h, r);
-    if (w0 + r < rows)
-      *reinterpret_cast<u32x4*>(to.out + (row0 + i) * to.o_st + h * to.o_sh + phys * 8) = row8;
+    const int64_t at = static_cast<int64_t>(__shfl(out_hi, r)) << 32 | static_cast<uint32_t>(__shfl(out_lo, r));
+    if (w0 + r < rows) *reinterpret_cast<u32x4*>(to.out + at + phys * 8) = row8;
   }
 }
 
@@ -440,9 +451,11 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   const CausalIn in{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                     static_cast<const uint16_t*>(v), q_st, q_sh, k_st, k_sh, v_st, v_sh};
   const CausalOut to{static_cast<uint16_t*>(out), lse, o_st, o_sh, l_st, l_sh};
+  const int ceil_log2 = group > 1 ? 32 - __builtin_clz(static_cast<unsigned>(group - 1)) : 0;
+  const GroupOf token_of{static_cast<uint32_t>(((1ull << (31 + ceil_log2)) + group - 1) / group), 31 + ceil_log2};
   const auto launch = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(total)), dim3(threads), 0,
-                       static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, group,
+                       static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, group, token_of,
                        scale * kLog2e);
   };
   // 64 and 256 channels have one variant each. 64: three workgroups a CU (7% faster than two over 4 x
