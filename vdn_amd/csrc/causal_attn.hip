@@ -61,14 +61,14 @@ struct CausalOut {
 };
 
 // blocks: int32 [nblocks, 4] = (first token row, tokens n of the sequence, first row r0 of the
-// block among the sequence's n G, unused), most keys first.
+// block among the sequence's n G, unused), in the order of the launch.
 // kWaves waves of 32 rows, tiles of kBN keys, kPerSimd waves on a SIMD (of one workgroup or of
 // several); kSpread sends the next tile's loads out along Sᵀ instead of all at once.
 template <int kD, int kWaves, int kBN, int kPerSimd, bool kSpread, bool kF16>
 __global__ void __launch_bounds__(kWaves * 64)
     __attribute__((amdgpu_waves_per_eu(kPerSimd, kPerSimd)))
 causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, int nblocks,
-                   int kv_heads, int group, GroupOf token_of, float scale_log2) {
+                   int kv_heads, int together, int group, GroupOf token_of, float scale_log2) {
   constexpr int kKT = kBN / 32;           // 32-key score accumulators per tile
   constexpr int kDB = kD / 32;            // 32-channel output accumulators
   constexpr int kSteps = kD / 16;         // channel steps of Sᵀ
@@ -89,16 +89,17 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   __shared__ __attribute__((aligned(1024))) uint16_t sV1[kBN * kD];
   __shared__ int sPos[kD], sNeg[kD], sDirty;
 
-  // With a multiple of 8 K/V heads each XCD keeps its own heads, so that a head's tiles are
-  // shared in one L2; otherwise consecutive ids go round the XCDs. Either way an XCD starts
-  // with its longest blocks.
+  // With a multiple of 8 K/V heads each XCD keeps its own heads, so that a head's tiles are shared
+  // in one L2; `together` of them go through the plan's blocks at a time. Otherwise consecutive ids
+  // go round the XCDs.
   int u, blk;
   {
     const int pid = blockIdx.x;
     if (kv_heads % 8 == 0) {
-      const int xcd = pid & 7, local = pid >> 3;
-      u = xcd + 8 * (local / nblocks);
-      blk = local % nblocks;
+      const int xcd = pid & 7, local = pid >> 3, turn = local / (together * nblocks);
+      const int rest = local - turn * together * nblocks;
+      blk = rest / together;
+      u = xcd + 8 * (turn * together + rest - blk * together);
     } else {
       u = pid % kv_heads;
       blk = pid / kv_heads;
@@ -451,12 +452,19 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   const CausalIn in{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                     static_cast<const uint16_t*>(v), q_st, q_sh, k_st, k_sh, v_st, v_sh};
   const CausalOut to{static_cast<uint16_t*>(out), lse, o_st, o_sh, l_st, l_sh};
+  // An XCD's heads all at once finish evenly, but their K/V no longer fits the L2: that pays as long
+  // as all K/V fits the 256 MB cache behind it. At once against one after the other, tokens x heads
+  // of their own x 128, us: 2048 x 32 55, 68; 4096 x 32 145, 190; 4096 x 56 253, 283; 8192 x 56 943,
+  // 1029; 16384 x 32 (256 MB) 2000, 2070; 4 x 4096 x 56 1200, 1055; 32768 x 32 8390, 7850. Of many
+  // short prompts 24 x 77 - 1200 x 16 47.6, 48.7, but 16 x 512 x 32 74.6, 69.5.
+  const int64_t kv_bytes = static_cast<int64_t>(nblocks) * block_rows / group * head_dim * 4 * kv_heads;
+  const int together = kv_heads % 8 == 0 && kv_bytes <= (256ll << 20) ? kv_heads / 8 : 1;
   const int ceil_log2 = group > 1 ? 32 - __builtin_clz(static_cast<unsigned>(group - 1)) : 0;
   const GroupOf token_of{static_cast<uint32_t>(((1ull << (31 + ceil_log2)) + group - 1) / group), 31 + ceil_log2};
   const auto launch = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(total)), dim3(threads), 0,
-                       static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, group, token_of,
-                       scale * kLog2e);
+                       static_cast<hipStream_t>(stream), in, to, blocks, nblocks, kv_heads, together, group,
+                       token_of, scale * kLog2e);
   };
   // 64 and 256 channels have one variant each. 64: three workgroups a CU (7% faster than two over 4 x
   // 4096 tokens of 32 heads, 18% over 64 prompts of 1 - 400; four spill). 256: Q and O alone take 192
