@@ -126,7 +126,7 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = query.new_empty(query.shape)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != query.shape or out.dtype is not dtype or out.device != query.device

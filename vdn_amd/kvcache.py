@@ -223,7 +223,7 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = query.new_empty(query.shape)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif (out.shape != query.shape or out.dtype is not dtype or out.get_device() != index
           or out.stride(-1) != 1 or 0 in out.stride()):
         raise ValueError("out must be a view like the query, unit channel stride, no broadcast")
