@@ -4,7 +4,9 @@
 //
 // for the Q newest tokens of sequence b (their K/V are in the cache already), u = h / G. Every
 // K/V head has Q G query rows against all its cached tokens: a few rows, so reading the codes
-// bounds it, 2 D bytes per token and K/V head.
+// bounds it, 2 D bytes per token and K/V head. One token against 131072, 56 heads on 8 x 128: 268 MB in
+// 45 us (6 TB/s, as a large read), 64 sequences of 512 - 8192, 40 heads: 368 MB in 72 (5.1: units that
+// start and end inside a workgroup's range), and 5 - 6 us of the join.
 //
 // A wave takes 64 tokens at a time, straight from memory into registers (no LDS, no barrier):
 //   Sᵀ[key][row] = K Qᵀ on 16x16x32 MFMAs of 16-bit values. A lane's 16-byte load holds 16

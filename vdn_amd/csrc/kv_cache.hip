@@ -1,6 +1,8 @@
 // Writing rows into the 8-bit key/value cache, and reading them back (kv_cache.h).
 //
-// Both move memory only: a write reads 2 bytes and writes 1 per value, a read the reverse. A
+// Both move memory only: a write reads 2 bytes and writes 1 per value, a read the reverse. Prompts of
+// 40600 tokens x 8 heads x 128: write 59 us (4.2 TB/s), read 54 with cold codes (4.6); a large copy
+// reaches 4.9. One token for each of 64 sequences: write 10 us, latency and V's D cache lines a head. A
 // workgroup takes one page of one sequence, one K/V head and one side; a wave tile is 2048 values,
 // four 16-byte pieces of 8 values a lane. K's order is that of the rows. V's codes are channel
 // major: a lane takes the same 8 channels of 4 consecutive positions and transposes its 4 x 8
