@@ -37,6 +37,11 @@ def test_calls_need_a_device():
                 call()
 
 
+def test_no_stream_of_a_host_device():
+    with pytest.raises(ValueError, match="device"):
+        _lib.stream(torch.device("cpu"))
+
+
 def test_entry_points_validate_before_launching():
     lib, p = _lib.load(), 1 << 20
 

@@ -165,6 +165,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream(device: torch.device) -> int:
     """The caller's current HIP stream on `device` (launches never go to a private stream)."""
+    if device.type != "cuda":
+        raise ValueError(f"expected a CUDA (HIP) device, but got {device}")
     index = device.index
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None
                                               else index)
