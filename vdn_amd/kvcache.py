@@ -80,7 +80,7 @@ class KVCache:
         return self.k_codes.device
 
     def check(self):
-        """Reads the fault word on the host (waits for the device) and raises if it is set."""
+        """Reads the fault word on the host (waits for the current stream) and raises if it is set."""
         if int(self.faults.item()):
             self.faults.zero_()
             raise RuntimeError("a table, length or offset named what the cache does not have")
@@ -151,7 +151,8 @@ def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
     A page that holds earlier tokens of the sequence (the first one, if starts[i] is not a multiple
     of the page) keeps the larger of its scale and the new tokens' one; if that is the new
     tokens', the held codes are rounded once more. A nonfinite value becomes the NaN code and
-    leaves the scale alone. Two sequences must not bring rows for one page in the same call."""
+    leaves the scale alone. No page may be written twice in one call, by two sequences or by a table
+    that names it twice."""
     _check_cache(cache, "write_cache")
     _, heads, _, d = cache._args[5:]
     if key.ndim != 3 or key.shape != (key.shape[0], heads, d) or value.shape != key.shape:
