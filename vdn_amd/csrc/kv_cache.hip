@@ -75,36 +75,50 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
     }
     start = s.starts[p.seq];
   } else {
-    // the last i in [0, batch] with base_i <= slot
+    // the last i in [0, batch) with base_i <= slot, or the rows behind the last sequence
     const int lane = threadIdx.x & 63;
+    const int behind = s.offsets[s.batch];
     int lo = 0, step = 1;
-    while (static_cast<int64_t>(step) * 64 < s.batch + 1) step *= 64;
+    while (static_cast<int64_t>(step) * 64 < s.batch) step *= 64;
     for (; step > 1; step /= 64) {
       const int64_t i = lo + static_cast<int64_t>(lane) * step;
-      const bool le = i <= s.batch && seq_base(s, static_cast<int>(i), log_page) <= slot;
+      const bool le = i < s.batch && seq_base(s, static_cast<int>(i), log_page) <= slot;
       const int found = __popcll(__ballot(le));
       if (found == 0) {
         *c.faults = 1;
         return p;
       }
-      lo = min(lo + (found - 1) * step, s.batch);
+      lo += (found - 1) * step;
     }
-    // the last round has loaded what the sequence needs: one memory latency less
-    const int i = min(lo + lane, s.batch);
-    const int off = s.offsets[i], next = s.offsets[min(i + 1, s.batch)];
-    const int from = s.batch > 0 ? s.starts[min(i, s.batch - 1)] : 0;
-    const int base = (off >> log_page) + 2 * i;
-    const int found = __popcll(__ballot(lo + lane <= s.batch && base <= slot));
-    if (found == 0) {
+    // the last round loads what the sequence needs with its base: one memory latency less
+    const int i = lo + lane;
+    int off = 0, next = 0, from = 0, base = 0;
+    if (i < s.batch) {
+      off = s.offsets[i];
+      next = s.offsets[i + 1];
+      from = s.starts[i];
+      base = (off >> log_page) + 2 * i;
+    }
+    const int found = __popcll(__ballot(i < s.batch && base <= slot));
+    const int base_end = (behind >> log_page) + 2 * s.batch;
+    int o0, o1;
+    if (base_end <= slot) {
+      p.seq = s.batch;
+      j = slot - base_end;
+      start = 0;
+      o0 = behind;
+      o1 = rows;
+    } else if (found > 0) {
+      p.seq = lo + found - 1;
+      j = slot - __builtin_amdgcn_readlane(base, found - 1);
+      if (j < 0) return p;
+      start = __builtin_amdgcn_readlane(from, found - 1);
+      o0 = __builtin_amdgcn_readlane(off, found - 1);
+      o1 = __builtin_amdgcn_readlane(next, found - 1);
+    } else {
       *c.faults = 1;   // rows in front of the first sequence
       return p;
     }
-    p.seq = lo + found - 1;
-    j = slot - __builtin_amdgcn_readlane(base, found - 1);
-    if (j < 0) return p;
-    start = __builtin_amdgcn_readlane(from, found - 1);
-    const int o0 = __builtin_amdgcn_readlane(off, found - 1);
-    const int o1 = p.seq == s.batch ? rows : __builtin_amdgcn_readlane(next, found - 1);
     if (o0 < 0 || o1 < o0 || o1 > rows || (p.seq == 0 && o0 > 0)) *c.faults = 1;
     first = min(max(o0, 0), rows);
     end = min(max(o1, 0), rows);
