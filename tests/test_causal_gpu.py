@@ -247,3 +247,19 @@ def test_keys_that_score_minus_infinity(device, dim, dtype, block_rows):
     got, lse = vc.causal_attention(q, k, v, plan, return_lse=True)
     assert got[:shut].isnan().all() and (lse[:shut] == -math.inf).all()
     check(q[shut:], k[shut:], v[shut:], [n - shut], got[shut:], lse[shut:])
+
+
+@torch.no_grad()
+def test_rows_behind_two_to_the_31_elements(device):
+    """Rows of a wide buffer: the last sequence and the end of the first lie behind 2^31 elements."""
+    lengths, wide = [33000, 70], 66000
+    rows = sum(lengths)
+    base = torch.empty(rows, wide, dtype=BF16, device=device)
+    q, k, v = make(lengths, 2, 1, 64, BF16, seed=17)
+    far = [base[:, 128 * i:128 * i + x.shape[1] * 64].unflatten(1, (-1, 64)) for i, x in enumerate((q, k, v, q))]
+    for x, y in zip(far, (q, k, v)):
+        x.copy_(y)
+    plan = vc.prepare_causal_plan(lengths, 2, 1, device=device)
+    got = vc.causal_attention(*far[:3], plan, out=far[3])
+    assert got is far[3] and torch.equal(got, vc.causal_attention(q, k, v, plan))
+    check(q[lengths[0]:], k[lengths[0]:], v[lengths[0]:], lengths[1:], got[lengths[0]:])

@@ -506,3 +506,26 @@ def test_nothing_to_do(device):
                                   return_lse=True)
     assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
     cache.check()
+
+
+@torch.no_grad()
+def test_rows_behind_two_to_the_31_elements(device):
+    """Written rows of a wide buffer, the last ones behind 2^31 elements."""
+    rows, wide, page = 33070, 66000, 256
+    base = torch.empty(rows, wide, dtype=BF16, device=device)
+    near = torch.randn(2, rows, 1, 64, generator=torch.Generator().manual_seed(3)).to(BF16).cuda()
+    far = [base[:, 64 * i:64 * i + 64].unflatten(1, (1, 64)) for i in range(2)]
+    for x, y in zip(far, near):
+        x.copy_(y)
+    pages = -(-rows // page)
+    table = torch.arange(pages, dtype=torch.int32, device=device)[None]
+    starts = torch.zeros(1, dtype=torch.int32, device=device)
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=device)
+    got = []
+    for key, value in (far, near):
+        cache = kv.empty_cache(pages, 1, 64, page, device=device)
+        kv.write_cache(cache, key, value, table, starts, offsets)
+        cache.check()
+        got.append(kv.read_cache(cache, table, starts, offsets, rows))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert (got[0][0].float() - near[0].float()).abs().max() <= 2.0 ** -4 * near[0].abs().max()
