@@ -374,7 +374,7 @@ int vdn_cache_read(const void* k_codes, const void* k_scales, const void* v_code
  * [batch, tokens, kv_heads * group, head_dim] by (sequence, token, head) strides, multiples of 8,
  * dtype 0 bf16 or 1 fp16; lse (nullable): fp32 [batch, tokens, heads] contiguous. workspace:
  * 16-byte aligned, vdn_cache_attention_workspace's byte count, its contents need no preparation; not
- * needed where the table holds at most 256 tokens (width * page).
+ * needed where the table holds at most 512 tokens (width * page).
  */
 int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                         const void* k_codes, const void* k_scales, const void* v_codes,

@@ -20,7 +20,8 @@
 //
 // Work: a quad is 256 tokens (one tile for each of a workgroup's 4 waves) of one (sequence, row
 // block, K/V head) unit. The quads of all units in order are shared out evenly over the
-// workgroups, which find their range from the lengths on the device. A workgroup that holds a
+// workgroups, which find their range from the lengths on the device (with tables of up to kWholeQuads a
+// unit stays whole, for the workgroup in whose range it starts). A workgroup that holds a
 // unit's every quad writes its output; else it leaves maximum, sum and O in a slot, and a second
 // kernel joins a unit's slots in order (no atomics: the same call gives the same bits).
 #include "kv_cache.h"
@@ -38,6 +39,11 @@ constexpr int kThreads = 256;
 constexpr int kWaves = 4;
 constexpr int kTile = 64;              // tokens of a wave's step
 constexpr int kQuad = kTile * kWaves;  // tokens of a workgroup's step
+
+// Units of tables of up to so many quads are not split: the second step costs less than the join.
+// 128 sequences of 100 - 300 tokens, 32 heads on 8: 22.5 us against 25.6; one of 500, 56 heads: 8.7,
+// 10.3. With four quads 64 of 100 - 1000 tokens take 26.9 against 25.0, one of 1000 12.4 against 10.5.
+constexpr int kWholeQuads = 2;
 
 // Workgroups that share a CU, by the registers that a tile's codes, Q and O take: one for wide heads
 // or 32 rows, three for 64 channels (128 sequences of 100 - 300 tokens, 8 K/V heads: 17.4 us
@@ -64,7 +70,7 @@ struct Lengths {
 // Workspace slots: two per workgroup (its first and its last unfinished unit), each kRows rows
 // of D + 2 floats (O, m, l).
 struct Split {
-  float* slots;
+  float* slots;   // null: units are not split
   int workgroups;
 };
 
@@ -207,7 +213,18 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     const int unit = static_cast<int>((at - seq0) / nq);
     const int64_t unit0 = seq0 + static_cast<int64_t>(unit) * nq;
     const int qa = static_cast<int>(at - unit0);
-    const int qb = static_cast<int>(min(end - unit0, static_cast<int64_t>(nq)));
+    int qb = static_cast<int>(min(end - unit0, static_cast<int64_t>(nq)));
+    if (sp.slots == nullptr) {
+      if (qa > 0) {   // another workgroup's
+        at = unit0 + nq;
+        if (at - seq0 >= static_cast<int64_t>(nq) * units) {
+          seq0 = at;
+          ++b;
+        }
+        continue;
+      }
+      qb = nq;
+    }
     const int u = unit % c.kv_heads, r_block = (unit / c.kv_heads) * kRows;
     const int* table = s.table + b * s.t_st;
     const int seen0 = len - io.tokens + 1;   // keys that the first of the Q tokens sees
@@ -675,8 +692,9 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
   const int64_t unit_quads = ((static_cast<int64_t>(width) << c.log_page) + kQuad - 1) / kQuad;
   const int64_t units = static_cast<int64_t>(row_blocks) * kv_heads * batch;
   const int workgroups = static_cast<int>(workgroups_of(units * unit_quads, head_dim, block));
-  const Split sp{static_cast<float*>(workspace), workgroups};
-  if (unit_quads > 1) {
+  const bool split = unit_quads > kWholeQuads;
+  const Split sp{split ? static_cast<float*>(workspace) : nullptr, workgroups};
+  if (split) {
     if (workspace == nullptr || !aligned16(workspace) ||
         workspace_bytes < 4ll * 2 * workgroups * block * (head_dim + 4))
       return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);
@@ -690,7 +708,7 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
     const auto st = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(main, dim3(static_cast<unsigned>(workgroups)), dim3(kThreads), 0, st, c, io, s, sp,
                        row_blocks, scale * kLog2e);
-    if (unit_quads <= 1) return;   // no unit is shared
+    if (!split) return;
     const dim3 grid(static_cast<unsigned>(join_rows));
     if (join_rows > 4 * cu_count())
       hipLaunchKernelGGL(join1, grid, dim3(64), 0, st, c, io, s, sp, row_blocks);

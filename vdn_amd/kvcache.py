@@ -25,7 +25,7 @@ from . import _lib
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128, 256)
 _DTYPES = (torch.bfloat16, torch.float16)
-WHOLE_TOKENS = 256   # tokens of a sequence that are never split: no workspace for shorter tables
+WHOLE_TOKENS = 512   # tokens of a sequence that are never split: no workspace for shorter tables
 
 
 @dataclass(frozen=True, eq=False)
