@@ -161,8 +161,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     load_to_lds16(is_v ? src.v : src.k, is_v ? voff[js % kOffs] : koff[js % kOffs], apart,
                   (is_v ? dv : dk) + seg * kSegRows * kD);
   };
-  auto issue = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
-    if (src.last == kBN - 1) return issue_full(src, j, dk, dv);
+  auto issue_tail = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
     const bool is_v = j >= kSegs;
     const int seg = (is_v ? j - kSegs : j) * kLoaders + wave, row = seg * kSegRows + seg_row;
     const int r = min(row, src.last);
@@ -173,8 +172,13 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   };
   auto issue_all = [&](int a, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
     const Source src = source(a);
+    if (src.last == kBN - 1) {
 #pragma unroll
-    for (int j = 0; j < 2 * kSegs; ++j) issue(src, j, dk, dv);
+      for (int j = 0; j < 2 * kSegs; ++j) issue_full(src, j, dk, dv);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2 * kSegs; ++j) issue_tail(src, j, dk, dv);
+    }
   };
 
   for (int d = tid; d < kD; d += kThreads) sPos[d] = sNeg[d] = 0x7fffffff;
