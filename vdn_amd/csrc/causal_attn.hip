@@ -145,6 +145,8 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   }
   const char* k_head = reinterpret_cast<const char*>(in.k + row0 * in.k_st + u * in.k_sh);
   const char* v_head = reinterpret_cast<const char*>(in.v + row0 * in.v_st + u * in.v_sh);
+  const uint32_t krow = static_cast<uint32_t>((wave * kSegRows + seg_row) * 2 * in.k_st);
+  const uint32_t vrow = static_cast<uint32_t>((wave * kSegRows + seg_row) * 2 * in.v_st);
   struct Source {
     __amdgpu_buffer_rsrc_t k, v;
     int last;   // the tile's last row with a key; rows behind it repeat that
@@ -163,12 +165,11 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   };
   auto issue_tail = [&](const Source& src, int j, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
     const bool is_v = j >= kSegs;
-    const int seg = (is_v ? j - kSegs : j) * kLoaders + wave, row = seg * kSegRows + seg_row;
-    const int r = min(row, src.last);
-    load_to_lds16(is_v ? src.v : src.k,
-                  is_v ? static_cast<uint32_t>(r * in.v_st * 2 + 16 * (phys ^ swz_v<kD>(row)))
-                       : static_cast<uint32_t>(r * in.k_st * 2 + 16 * (phys ^ swz_k<kD>(row))),
-                  0, (is_v ? dv : dk) + seg * kSegRows * kD);
+    const int js = is_v ? j - kSegs : j, seg = js * kLoaders + wave, row = seg * kSegRows + seg_row;
+    const uint32_t st = static_cast<uint32_t>(2 * (is_v ? in.v_st : in.k_st));
+    const uint32_t at = min((is_v ? vrow : krow) + js * kApart * st, src.last * st);   // min(row, last) * st
+    load_to_lds16(is_v ? src.v : src.k, at + 16 * (phys ^ (is_v ? swz_v<kD>(row) : swz_k<kD>(row))), 0,
+                  (is_v ? dv : dk) + seg * kSegRows * kD);
   };
   auto issue_all = [&](int a, uint16_t* dk, uint16_t* dv) __attribute__((always_inline)) {
     const Source src = source(a);
