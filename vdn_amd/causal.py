@@ -40,10 +40,10 @@ class CausalPlan:
 # When head dim 128 takes 256-row blocks (8 waves, one workgroup a CU) instead of 128-row ones (two
 # of 4 waves): a K/V tile then serves twice the rows, which pays where rows see many keys, and a
 # block takes the CU to itself, so that there have to be enough of them. Microseconds of 256 and
-# 128 rows, 32 heads and 8 K/V heads: 32768 tokens 7660, 8290; 8192: 506, 541; 4096: 151, 154 (the
-# mean row sees 2048 keys); 4 x 2048: 169, 163; 2048: 60, 54; 24 prompts of 77 - 1200 with 56 heads
-# 157, 126. 8 heads that share one K/V head: 16384 tokens, 512 blocks: 493, 569; 8192, 256 blocks:
-# 194, 187.
+# 128 rows, 32 heads and 8 K/V heads: 32768 tokens 7360, 8000; 8192: 491, 520; 4096: 146, 152 (the
+# mean row sees 2048 keys); 4 x 2048: 165, 161; 2048: 58, 52; 24 prompts of 77 - 1200 with 56 heads
+# 148, 120. 8 heads that share one K/V head: 16384 tokens, 512 blocks: 480, 549; 8192, 256 blocks:
+# 195, 183.
 WIDE_MEAN_KEYS = 2048
 WIDE_LEAST_BLOCKS = 512    # two for each of 256 CUs
 

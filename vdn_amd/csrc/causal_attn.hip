@@ -12,8 +12,8 @@
 // where Pᵀ is the Sᵀ accumulator itself and Vᵀ comes from the token-major V tile by transpose
 // reads. Tiles stream global -> LDS, double-buffered. MFMA bounds long prompts, with the softmax beside it
 // (59 and 51% of the time busy, the clock at 1.9 GHz by the power limit): 32768 tokens, 32 heads on 8
-// x 128, 7.6 ms, 1150 TFLOP/s, 87% of a large library product. Short ones are bound by reading Q, writing
-// O and the latency around the tiles: 24 prompts of 77 - 1200 tokens, 56 heads, 127 us.
+// x 128, 7.4 - 7.5 ms, 1180 TFLOP/s, 88% of a large library product. Short ones are bound by reading Q, writing
+// O and the latency around the tiles: 24 prompts of 77 - 1200 tokens, 56 heads, 120 us.
 //
 // A nonfinite V value of a token that a row does not see must not reach that row, and 0 inf is
 // NaN in an MFMA. Only tiles on the diagonal hold such tokens: there every wave looks its share
@@ -477,7 +477,7 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
   // 64 and 256 channels have one variant each. 64: three workgroups a CU (7% faster than two over 4 x
   // 4096 tokens of 32 heads, 18% over 64 prompts of 1 - 400; four spill). 256: Q and O alone take 192
   // registers, so one wave per SIMD with twice the registers (1.10 ms over 2 x 8192 tokens of 16
-  // heads, 1000 TFLOP/s; two waves per SIMD spill and take 2.1).
+  // heads, 1040 TFLOP/s; two waves per SIMD spill and take 2.1).
 #define VDN_CAUSAL(F16)                                                                          \
   head_dim == 64 ? launch(causal_attn_kernel<64, 4, 64, 3, true, F16>, 256)                      \
   : head_dim == 256 ? launch(causal_attn_kernel<256, 4, 64, 1, true, F16>, 256)                  \
