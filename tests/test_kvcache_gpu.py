@@ -264,7 +264,8 @@ def test_pages(device, page, dim, dtype):
 @pytest.mark.parametrize("batch,longest,heads,kv_heads,dim,dtype", [
     (1, 40000, 8, 1, 128, BF16), (3, 9000, 5, 5, 64, FP16), (300, 700, 2, 1, 64, BF16),
     (2, 5000, 36, 2, 128, BF16), (1, 20000, 2, 2, 256, BF16), (700, 30, 3, 3, 64, BF16),
-    (300, 512, 8, 2, 128, BF16), (900, 500, 3, 1, 64, FP16), (1, 512, 2, 2, 256, BF16)])
+    (300, 512, 8, 2, 128, BF16), (900, 500, 3, 1, 64, FP16), (1, 512, 2, 2, 256, BF16),
+    (1, 1500, 1, 1, 64, BF16), (5, 1100, 4, 2, 128, FP16), (70, 3000, 8, 4, 128, BF16)])
 @torch.no_grad()
 def test_split_work(device, batch, longest, heads, kv_heads, dim, dtype):
     """Sequences that many workgroups share, workgroups that go through many sequences; the same

@@ -19,9 +19,9 @@
 // taken relative to the tile's largest one, and O is kept in units of that.
 //
 // Work: a quad is 256 tokens (one tile for each of a workgroup's 4 waves) of one (sequence, row
-// block, K/V head) unit. The quads of all units in order are shared out evenly over the
-// workgroups, which find their range from the lengths on the device (with tables of up to kWholeQuads a
-// unit stays whole, for the workgroup in whose range it starts). A workgroup that holds a
+// block, K/V head) unit. The quads of all units in order, and one more for each unit, are shared
+// out evenly over the workgroups, which find their share from the lengths on the device (with tables of up to kWholeQuads a
+// unit stays whole, for the workgroup in whose share it starts). A workgroup that holds a
 // unit's every quad writes its output; else it leaves maximum, sum and O in a slot, and a second
 // kernel joins a unit's slots in order (no atomics: the same call gives the same bits).
 #include "kv_cache.h"
@@ -68,10 +68,11 @@ struct Lengths {
 };
 
 // Workspace slots: two per workgroup (its first and its last unfinished unit), each kRows rows
-// of D + 2 floats (O, m, l).
+// of D + 4 floats (O, m, l, two unused).
 struct Split {
   float* slots;   // null: units are not split
   int workgroups;
+  int unit_cost;
 };
 
 __device__ __forceinline__ int seq_tokens(const KvCache& c, const Lengths& s, int b) {
@@ -81,13 +82,25 @@ __device__ __forceinline__ int seq_tokens(const KvCache& c, const Lengths& s, in
 
 __device__ __forceinline__ int quads_of(int tokens) { return max((tokens + kQuad - 1) / kQuad, 1); }
 
-// Where quad `at` of the flattened order lies (sequence b's quads: units * quads_of(len_b)), from a
+// What a unit counts for when the work is shared out: its quads, and in front of them unit_cost for its
+// queries, its first loads' latency and the join of the waves. One quad where units are split: 64
+// sequences of 100 - 1000 tokens, 32 heads on 8: 22.4 us against 25.0 with quads alone, 16 of 100 - 4097
+// with 12 heads x 64 18.1, 19.9; even ones the same (two: 64 of 100 - 2048 tokens 30.7, 28.6). Nothing
+// where they stay whole: 128 of 100 - 300 tokens 22.0, 23.2.
+constexpr int kUnitCost = 1;
+__device__ __forceinline__ int cost_of(const Split& sp, int tokens) { return quads_of(tokens) + sp.unit_cost; }
+
+// Workgroup w of n has the positions share_from(w) .. share_from(w + 1) - 1 of `total` >= n, x is one of
+// share_of(x)'s. Rounded up: where a whole number of workgroups share a unit, they have as many quads each.
+__device__ __forceinline__ int64_t share_from(int64_t total, int n, int w) { return (total * w + n - 1) / n; }
+__device__ __forceinline__ int64_t share_of(int64_t total, int n, int64_t x) { return x * n / total; }
+
+// Where a workgroup's share of all units' costs begins (sequence b: units times its cost), from a
 // prefix over the lengths. Every wave does it for itself, 64 strips of sequences at a time: no
 // barrier, and for up to 64 sequences one load.
 struct Place {
-  int64_t total;    // quads of all units
-  int64_t per;      // quads of a workgroup
-  int64_t before;   // quads in front of sequence seq
+  int64_t from, to;   // the workgroup's share (none: from = to)
+  int64_t before;   // costs in front of sequence seq
   int seq;
 };
 
@@ -100,17 +113,19 @@ __device__ __forceinline__ int wave_prefix(int x, int lane) {   // inclusive
   return x;
 }
 
-__device__ Place find_quad(const KvCache& c, const Lengths& s, int units, int workgroups, int wg) {
+__device__ Place find_share(const KvCache& c, const Lengths& s, const Split& sp, int units, int wg) {
   const int lane = threadIdx.x & 63;
   const int strip = (s.batch + 63) / 64;
   const int b0 = min(lane * strip, s.batch), b1 = min(b0 + strip, s.batch);
   int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += quads_of(seq_tokens(c, s, b));
+  for (int b = b0; b < b1; ++b) mine += cost_of(sp, seq_tokens(c, s, b));
   const int incl = wave_prefix(mine, lane);
   Place p;
-  p.total = static_cast<int64_t>(__builtin_amdgcn_readlane(incl, 63)) * units;
-  p.per = max((p.total + workgroups - 1) / workgroups, static_cast<int64_t>(1));
-  const int64_t at = p.per * wg;
+  const int64_t total = static_cast<int64_t>(__builtin_amdgcn_readlane(incl, 63)) * units;
+  const int n_wg = static_cast<int>(min(total, static_cast<int64_t>(sp.workgroups)));
+  p.from = wg < n_wg ? share_from(total, n_wg, wg) : total;
+  p.to = wg < n_wg ? share_from(total, n_wg, wg + 1) : total;
+  const int64_t at = p.from;
   // the strip, then the sequence inside it
   const int front = __popcll(__ballot(static_cast<int64_t>(incl) * units <= at));
   const int owner = min(front, 63);
@@ -119,7 +134,7 @@ __device__ Place find_quad(const KvCache& c, const Lengths& s, int units, int wo
   if (strip > 1) {
     const int last = min(seq + strip, s.batch) - 1;
     for (; seq < last; ++seq) {
-      const int n = quads_of(seq_tokens(c, s, seq));
+      const int n = cost_of(sp, seq_tokens(c, s, seq));
       if (at < static_cast<int64_t>(before + n) * units) break;
       before += n;
     }
@@ -197,36 +212,38 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   const int page = 1 << c.log_page;
   const int units = row_blocks * c.kv_heads;
   const int wg = blockIdx.x;
-  const Place place = find_quad(c, s, units, sp.workgroups, wg);
-  int64_t at = place.per * wg;
-  const int64_t end = min(at + place.per, place.total);
+  const Place place = find_share(c, s, sp, units, wg);
+  int64_t at = place.from;
+  const int64_t end = place.to;
   if (at >= end) return;
   const int64_t range0 = at;
   int b = __builtin_amdgcn_readfirstlane(place.seq);
-  int64_t seq0 = place.before;   // first quad of sequence b
+  int64_t seq0 = place.before;   // where sequence b's units begin
   const int all_rows = io.tokens * io.group;
 
   while (at < end) {
     const int len = __builtin_amdgcn_readfirstlane(seq_tokens(c, s, b));
     const bool too_long = s.lengths[b] < 0 || s.lengths[b] > len;
-    const int nq = quads_of(len);
-    const int unit = static_cast<int>((at - seq0) / nq);
-    const int64_t unit0 = seq0 + static_cast<int64_t>(unit) * nq;
-    const int qa = static_cast<int>(at - unit0);
-    int qb = static_cast<int>(min(end - unit0, static_cast<int64_t>(nq)));
+    const int nq = quads_of(len), cost = nq + sp.unit_cost;
+    const int unit = static_cast<int>((at - seq0) / cost);
+    const int64_t unit0 = seq0 + static_cast<int64_t>(unit) * cost;
+    const int64_t here = at;
+    at = min(end, unit0 + cost);
+    int qa = max(static_cast<int>(here - unit0) - sp.unit_cost, 0);
+    int qb = static_cast<int>(at - unit0) - sp.unit_cost;
     if (sp.slots == nullptr) {
-      if (qa > 0) {   // another workgroup's
-        at = unit0 + nq;
-        if (at - seq0 >= static_cast<int64_t>(nq) * units) {
-          seq0 = at;
-          ++b;
-        }
-        continue;
-      }
-      qb = nq;
+      qb = here > unit0 ? 0 : nq;   // another workgroup's, or all of it
+      at = unit0 + cost;
     }
+    const int b_now = b;
+    const bool next_seq = unit + 1 == units && at == unit0 + cost;
+    if (next_seq) {
+      seq0 = at;
+      ++b;
+    }
+    if (qb <= qa) continue;
     const int u = unit % c.kv_heads, r_block = (unit / c.kv_heads) * kRows;
-    const int* table = s.table + b * s.t_st;
+    const int* table = s.table + b_now * s.t_st;
     const int seen0 = len - io.tokens + 1;   // keys that the first of the Q tokens sees
 
     // ---- Q: row r_block + 16 nr + row16, channels 64 j + 16 g + 8 s .. + 8 ----
@@ -237,7 +254,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
       const int r = min(r_block + 16 * nr + row16, all_rows - 1);
       const int i = r / io.group, h = u * io.group + r - i * io.group;
       limit[nr] = seen0 + i;
-      const uint16_t* src = io.q + b * io.q_sb + i * io.q_st + h * io.q_sh + 16 * g;
+      const uint16_t* src = io.q + b_now * io.q_sb + i * io.q_st + h * io.q_sh + 16 * g;
 #pragma unroll
       for (int j = 0; j < kKL; ++j) {
         qf[nr][2 * j] = *reinterpret_cast<const u32x4*>(src + 64 * j);
@@ -481,7 +498,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     }
     __syncthreads();
     const bool whole = qa == 0 && qb == nq;
-    const int64_t slot = 2 * static_cast<int64_t>(wg) + (at == range0 ? 0 : 1);
+    const int64_t slot = 2 * static_cast<int64_t>(wg) + (here == range0 ? 0 : 1);
     constexpr int kVec = kD / 4;
     for (int e = tid; e < kRows * kVec; e += kThreads) {
       const int r = e / kVec, d = (e % kVec) * 4;
@@ -510,9 +527,9 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
         u32x2 y;
         y[0] = E::pack(acc[0] * inv, acc[1] * inv);
         y[1] = E::pack(acc[2] * inv, acc[3] * inv);
-        *reinterpret_cast<u32x2*>(io.out + b * io.o_sb + i * io.o_st + h * io.o_sh + d) = y;
+        *reinterpret_cast<u32x2*>(io.out + b_now * io.o_sb + i * io.o_st + h * io.o_sh + d) = y;
         if (io.lse != nullptr && d == 0)
-          io.lse[(static_cast<int64_t>(b) * io.tokens + i) * c.kv_heads * io.group + h] =
+          io.lse[(static_cast<int64_t>(b_now) * io.tokens + i) * c.kv_heads * io.group + h] =
               sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
         float* dst = sp.slots + (slot * kRows + r) * (kD + 4);
@@ -522,11 +539,6 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
           dst[kD + 1] = sum;
         }
       }
-    }
-    at = unit0 + qb;
-    if (at - seq0 >= static_cast<int64_t>(nq) * units) {
-      seq0 = at;
-      ++b;
     }
   }
 }
@@ -547,7 +559,7 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
   const int tid = threadIdx.x, lane = tid & 63;
   int all = 0, front = 0, own = 0;
   for (int i = lane; i < s.batch; i += 64) {
-    const int n = quads_of(seq_tokens(c, s, i));
+    const int n = cost_of(sp, seq_tokens(c, s, i));
     all += n;
     if (i < b) front += n;
     if (i == b) own = n;
@@ -558,12 +570,14 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
     front += __shfl_xor(front, d);
     own += __shfl_xor(own, d);
   }
-  const int64_t per = max((static_cast<int64_t>(all) * units + sp.workgroups - 1) / sp.workgroups,
-                          static_cast<int64_t>(1));
+  const int64_t total = static_cast<int64_t>(all) * units;
   const int64_t start = static_cast<int64_t>(front) * units +
                         static_cast<int64_t>((row / kRows) * c.kv_heads + u) * own;
-  const int64_t w0 = start / per, w1 = (start + own - 1) / per;
+  const int n_wg = static_cast<int>(min(total, static_cast<int64_t>(sp.workgroups)));
+  const int64_t w0 = share_of(total, n_wg, start + sp.unit_cost);
+  const int64_t w1 = share_of(total, n_wg, start + own - 1);
   if (w0 == w1) return;   // written by its one workgroup
+  const int second = start > share_from(total, n_wg, static_cast<int>(w0)) ? 1 : 0;
   const int d = (tid % kVec) * 4, part = tid / kVec;
   float top = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -574,7 +588,7 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
 #pragma unroll
     for (int a = 0; a < kAhead; ++a) {
       const int64_t wa = min(w + a * kLanes, w1);
-      const int64_t slot = 2 * wa + (wa == w0 && start != w0 * per ? 1 : 0);
+      const int64_t slot = 2 * wa + (wa == w0 ? second : 0);
       const float* src = sp.slots + (slot * kRows + row % kRows) * (kD + 4);
       x[a] = *reinterpret_cast<const f32x4*>(src + d);
       m[a] = src[kD];
@@ -693,7 +707,7 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
   const int64_t units = static_cast<int64_t>(row_blocks) * kv_heads * batch;
   const int workgroups = static_cast<int>(workgroups_of(units * unit_quads, head_dim, block));
   const bool split = unit_quads > kWholeQuads;
-  const Split sp{split ? static_cast<float*>(workspace) : nullptr, workgroups};
+  const Split sp{split ? static_cast<float*>(workspace) : nullptr, workgroups, split ? kUnitCost : 0};
   if (split) {
     if (workspace == nullptr || !aligned16(workspace) ||
         workspace_bytes < 4ll * 2 * workgroups * block * (head_dim + 4))
@@ -702,7 +716,7 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
   const Queries io{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lse, q_sb, q_st, q_sh,
                    o_sb, o_st, o_sh, tokens, group};
   const Lengths s{table, lengths, table_st, batch, width};
-  if (batch * unit_quads > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many tokens", name);
+  if (batch * (unit_quads + kUnitCost) > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many tokens", name);
   const int64_t join_rows = rows * kv_heads * batch;
   const auto launch = [&](auto main, auto join1, auto join4) {
     const auto st = static_cast<hipStream_t>(stream);
