@@ -20,10 +20,11 @@
 //
 // Work: a quad is 256 tokens (one tile for each of a workgroup's 4 waves) of one (sequence, row
 // block, K/V head) unit. The quads of all units in order, and one more for each unit, are shared
-// out evenly over the workgroups, which find their share from the lengths on the device (with tables of up to kWholeQuads a
-// unit stays whole, for the workgroup in whose share it starts). A workgroup that holds a
-// unit's every quad writes its output; else it leaves maximum, sum and O in a slot, and a second
-// kernel joins a unit's slots in order (no atomics: the same call gives the same bits).
+// out evenly over the workgroups, which find their share from the lengths on the device (with
+// tables of up to kWholeQuads a unit stays whole, for the workgroup in whose share it starts). A
+// workgroup that holds a unit's every quad writes its output; else it leaves maximum, sum and O in
+// a slot, and a second kernel joins a unit's slots in order (no atomics: the same call gives the
+// same bits).
 #include "kv_cache.h"
 
 #include "attn_tiles.h"

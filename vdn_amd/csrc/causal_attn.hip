@@ -12,7 +12,7 @@
 // where Pᵀ is the Sᵀ accumulator itself and Vᵀ comes from the token-major V tile by transpose
 // reads. Tiles stream global -> LDS, double-buffered. MFMA bounds long prompts, with the softmax beside it
 // (59 and 51% of the time busy, the clock at 1.9 GHz by the power limit): 32768 tokens, 32 heads on 8
-// x 128, 7.4 - 7.5 ms, 1180 TFLOP/s, 88% of a large library product. Short ones are bound by reading Q, writing
+// x 128, 7.4 - 7.7 ms, 1140 - 1190 TFLOP/s, 87% of a large library product. Short ones are bound by reading Q, writing
 // O and the latency around the tiles: 24 prompts of 77 - 1200 tokens, 56 heads, 120 us.
 //
 // A nonfinite V value of a token that a row does not see must not reach that row, and 0 inf is
