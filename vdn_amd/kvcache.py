@@ -58,6 +58,7 @@ class KVCache:
                                            self.v_scales.data_ptr(), self.faults.data_ptr(),
                                            *k.shape))
         object.__setattr__(self, "_index", k.get_device())   # -1 off the GPU
+        object.__setattr__(self, "_row", (k.shape[1], k.shape[3]))
 
     @property
     def pages(self):
@@ -110,34 +111,40 @@ def _check_cache(cache, what):
 
 
 def _check_table(table, index):
-    if table.ndim != 2 or table.dtype is not torch.int32 or table.get_device() != index \
-            or table.stride(1) != 1 and table.shape[1] > 1:
+    """(batch, width, row stride) of a page table."""
+    if table.ndim != 2 or table.dtype is not torch.int32 or table.get_device() != index:
         raise ValueError("table must be int32 [batch, width] on the cache's device, unit inner stride")
+    batch, width = table.shape
+    row, inner = table.stride()
+    if inner != 1 and width > 1:
+        raise ValueError("table must be int32 [batch, width] on the cache's device, unit inner stride")
+    return batch, width, row
 
 
 def _check_vector(name, t, n, index):
-    if t.shape != (n,) or t.dtype is not torch.int32 or t.get_device() != index \
+    if t.ndim != 1 or t.shape[0] != n or t.dtype is not torch.int32 or t.get_device() != index \
             or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
 
 
-def _move(name, cache, key, value, table, starts, offsets):
-    rows, index = key.shape[0], cache._index
-    _check_table(table, index)
-    batch, width = table.shape
+def _move(name, cache, key, value, rows, dtype, table, starts, offsets):
+    index = cache._index
+    batch, width, t_st = _check_table(table, index)
     _check_vector("starts", starts, batch, index)
     if offsets is not None:
         _check_vector("offsets", offsets, batch + 1, index)
+        offsets = offsets.data_ptr()
     elif rows != batch:
         raise ValueError("without offsets there is one row for each sequence")
     if rows > 2 ** 31 - 1:
         raise ValueError("too many rows")
-    k_st, k_sh, _ = key.stride()
-    v_st, v_sh, _ = value.stride()
-    _lib.call_on(index, name, *cache._args, table.data_ptr(), table.stride(0), batch, width,
-                 starts.data_ptr(), _lib.ptr(offsets), key.data_ptr(), k_st, k_sh,
-                 value.data_ptr(), v_st, v_sh, rows, int(key.dtype is torch.float16),
-                 _lib.raw_stream(index))
+    k_st, k_sh, k_sd = key.stride()
+    v_st, v_sh, v_sd = value.stride()
+    if k_sd != 1 or v_sd != 1:
+        raise ValueError("key and value must have unit innermost stride")
+    _lib.call_on(index, name, *cache._args, table.data_ptr(), t_st, batch, width,
+                 starts.data_ptr(), offsets, key.data_ptr(), k_st, k_sh, value.data_ptr(), v_st,
+                 v_sh, rows, 1 if dtype is torch.float16 else 0, _lib.raw_stream(index))
 
 
 def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
@@ -154,15 +161,13 @@ def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
     leaves the scale alone. No page may be written twice in one call, by two sequences or by a table
     that names it twice."""
     _check_cache(cache, "write_cache")
-    _, heads, _, d = cache._args[5:]
-    if key.ndim != 3 or key.shape != (key.shape[0], heads, d) or value.shape != key.shape:
+    index, shape, dtype = cache._index, key.shape, key.dtype
+    if len(shape) != 3 or shape[1:] != cache._row or value.shape != shape:
         raise ValueError("key and value must be [rows, kv_heads, D] of the cache")
-    if key.dtype not in _DTYPES or value.dtype is not key.dtype or key.stride(2) != 1 \
-            or value.stride(2) != 1 or key.get_device() != cache._index \
-            or value.get_device() != cache._index:
-        raise ValueError("key and value must share BF16 or FP16, unit innermost stride and the "
-                         "cache's device")
-    _move("vdn_cache_write", cache, key, value, table, starts, offsets)
+    if dtype not in _DTYPES or value.dtype is not dtype or key.get_device() != index \
+            or value.get_device() != index:
+        raise ValueError("key and value must share BF16 or FP16 and the cache's device")
+    _move("vdn_cache_write", cache, key, value, shape[0], dtype, table, starts, offsets)
 
 
 def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bfloat16):
@@ -176,10 +181,9 @@ def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bflo
         raise ValueError("rows must be a non-negative integer")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be BF16 or FP16")
-    _, heads, _, d = cache._args[5:]
-    key = torch.empty((rows, heads, d), dtype=dtype, device=cache.k_codes.device)
+    key = torch.empty((rows, *cache._row), dtype=dtype, device=cache.k_codes.device)
     value = torch.empty_like(key)
-    _move("vdn_cache_read", cache, key, value, table, starts, offsets)
+    _move("vdn_cache_read", cache, key, value, rows, dtype, table, starts, offsets)
     return key, value
 
 
@@ -213,9 +217,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
         raise ValueError("query heads must be a multiple of the cache's, D the same, Q positive")
     if dtype not in _DTYPES or q_sd != 1 or query.get_device() != index:
         raise ValueError("query must be BF16 or FP16 with unit innermost stride, on the cache's device")
-    _check_table(table, index)
+    table_batch, width, t_st = _check_table(table, index)
     _check_vector("lengths", lengths, batch, index)
-    table_batch, width = table.shape
     if table_batch != batch or width <= 0:
         raise ValueError("table must name at least one page for each sequence of the query")
     if width * page > 2 ** 31 - 1024:
@@ -237,7 +240,7 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
         nbytes = _workspace_bytes(index, tokens, group, d)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
     _lib.call_on(index, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
-                 *cache._args, table.data_ptr(), table.stride(0), batch, width,
+                 *cache._args, table.data_ptr(), t_st, batch, width,
                  lengths.data_ptr(), tokens, group, int(dtype is torch.float16), scale,
                  out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), _lib.ptr(workspace), nbytes,
                  _lib.raw_stream(index))
