@@ -238,7 +238,7 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     if width * page > WHOLE_TOKENS:
         # from the allocator in stream order: calls on other streams and captured graphs have their own
         nbytes = _workspace_bytes(index, tokens, group, d)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+        workspace = query.new_empty(nbytes // 2)   # 2-byte elements
     _lib.call_on(index, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
                  *cache._args, table.data_ptr(), t_st, batch, width,
                  lengths.data_ptr(), tokens, group, int(dtype is torch.float16), scale,
