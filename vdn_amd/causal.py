@@ -32,6 +32,17 @@ class CausalPlan:
     blocks: torch.Tensor
     wide_blocks: torch.Tensor | None
 
+    def __post_init__(self):
+        def launch(blocks, block_rows):
+            return blocks.data_ptr(), blocks.shape[0], block_rows
+
+        # the entry point's arguments
+        narrow = launch(self.blocks, 128)
+        object.__setattr__(self, "_narrow", narrow)
+        object.__setattr__(self, "_wide", narrow if self.wide_blocks is None
+                           else launch(self.wide_blocks, 256))
+        object.__setattr__(self, "_index", self.blocks.get_device())   # -1 off the GPU
+
     @property
     def device(self):
         return self.blocks.device
@@ -119,31 +130,32 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
             or q_sd != 1 or k_sd != 1 or v_sd != 1:
         raise ValueError("Q/K/V must share BF16 or FP16 and have unit innermost stride")
     index = query.get_device()
-    if not query.is_cuda or key.get_device() != index or value.get_device() != index \
-            or plan.blocks.get_device() != index:
+    if index < 0 or key.get_device() != index or value.get_device() != index \
+            or plan._index != index:
         raise ValueError("Q/K/V and prepared plan must be on the same CUDA device")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        o_st, o_sh = heads * d, d
         if rows > plan.rows:
             out[plan.rows:].zero_()
     elif (out.shape != query.shape or out.dtype is not dtype or out.device != query.device
           or out.stride(2) != 1 or 0 in out.stride()):
         raise ValueError("out must be a [rows, H, D] view like the queries, unit channel stride, "
                          "no broadcast")
-    lse = None
+    else:
+        o_st, o_sh, _ = out.stride()
+    lse = lse_ptr = None
     if return_lse:
         lse = torch.empty((rows, heads), dtype=torch.float32, device=query.device)
+        lse_ptr = lse.data_ptr()
         if rows > plan.rows:
             lse[plan.rows:].fill_(-math.inf)
-    blocks, block_rows = plan.blocks, 128
-    if d == 128 and plan.wide_blocks is not None:
-        blocks, block_rows = plan.wide_blocks, 256
     _lib.call_on(index, "vdn_causal_attention", query.data_ptr(), q_st, q_sh, key.data_ptr(),
-                 k_st, k_sh, value.data_ptr(), v_st, v_sh, blocks.data_ptr(), blocks.shape[0],
-                 block_rows, kv_heads, heads // kv_heads, d,
-                 int(dtype is torch.float16), scale, out.data_ptr(), out.stride(0), out.stride(1),
-                 _lib.ptr(lse), heads, 1, _lib.raw_stream(index))
+                 k_st, k_sh, value.data_ptr(), v_st, v_sh,
+                 *(plan._wide if d == 128 else plan._narrow), kv_heads, heads // kv_heads, d,
+                 1 if dtype is torch.float16 else 0, scale, out.data_ptr(), o_st, o_sh, lse_ptr,
+                 heads, 1, _lib.raw_stream(index))
     return (out, lse) if return_lse else out
