@@ -31,7 +31,10 @@ WHOLE_TOKENS = 512   # tokens of a sequence that are never split: no workspace f
 @dataclass(frozen=True, eq=False)
 class KVCache:
     """k_codes uint8 [pages, kv_heads, page, D], k_scales uint8 [pages, kv_heads] (e + 127), v_codes
-    uint8 [pages, kv_heads, D, page], v_scales like k_scales, faults int32 [1]; all contiguous."""
+    uint8 [pages, kv_heads, D, page], v_scales like k_scales, faults int32 [1]; all contiguous.
+
+    copy.deepcopy and pickle give a pool of its own. Each call takes the tensors as they are then:
+    their storage may be exchanged (moved to the host and back) for one of the same size."""
     k_codes: torch.Tensor
     k_scales: torch.Tensor
     v_codes: torch.Tensor
@@ -53,11 +56,10 @@ class KVCache:
         if any(t.device != k.device or not t.is_contiguous()
                for t in (k, v, self.k_scales, self.v_scales, self.faults)):
             raise ValueError("the cache's tensors must be contiguous and on one device")
-        # the entry points' arguments, and what every call asks for
-        object.__setattr__(self, "_args", (k.data_ptr(), self.k_scales.data_ptr(), v.data_ptr(),
-                                           self.v_scales.data_ptr(), self.faults.data_ptr(),
-                                           *k.shape))
-        object.__setattr__(self, "_index", k.get_device())   # -1 off the GPU
+        # sizes only: a copied handle has tensors of its own, so addresses are read at each call
+        object.__setattr__(self, "_nbytes", tuple(
+            t.nbytes for t in (k, self.k_scales, v, self.v_scales)))
+        object.__setattr__(self, "_geometry", tuple(k.shape))
         object.__setattr__(self, "_row", (k.shape[1], k.shape[3]))
 
     @property
@@ -102,12 +104,29 @@ def empty_cache(pages, kv_heads, head_dim, page=64, *, device):
 
 
 def _check_cache(cache, what):
+    """(device index, the entry points' arguments) of a cache."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{what} is inference-only; use no_grad/inference_mode")
     if not isinstance(cache, KVCache):
         raise TypeError("cache must be a KVCache")
-    if cache._index < 0:
+    index, args = _cache_args(cache)
+    if index < 0:
         raise ValueError("the cache must be on a CUDA (HIP) device")
+    return index, args
+
+
+def _cache_args(cache):
+    """The device index (-1 off the GPU) and the entry points' arguments, from the tensors that the
+    handle holds now: one that was copied, unpickled or given other storage follows its own."""
+    k, ks, v, vs, faults = cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales, cache.faults
+    index = k.get_device()
+    if ks.get_device() != index or v.get_device() != index or vs.get_device() != index \
+            or faults.get_device() != index:
+        raise ValueError("the cache's tensors must be on one device")
+    if (k.nbytes, ks.nbytes, v.nbytes, vs.nbytes) != cache._nbytes:
+        raise ValueError("the cache's tensors are not of the size that the handle was made for")
+    return index, (k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), faults.data_ptr(),
+                   *cache._geometry)
 
 
 def _check_table(table, index):
@@ -127,8 +146,7 @@ def _check_vector(name, t, n, index):
         raise ValueError(f"{name} must be contiguous int32 [{n}] on the cache's device")
 
 
-def _move(name, cache, key, value, rows, dtype, table, starts, offsets):
-    index = cache._index
+def _move(name, index, args, key, value, rows, dtype, table, starts, offsets):
     batch, width, t_st = _check_table(table, index)
     _check_vector("starts", starts, batch, index)
     if offsets is not None:
@@ -142,7 +160,7 @@ def _move(name, cache, key, value, rows, dtype, table, starts, offsets):
     v_st, v_sh, v_sd = value.stride()
     if k_sd != 1 or v_sd != 1:
         raise ValueError("key and value must have unit innermost stride")
-    _lib.call_on(index, name, *cache._args, table.data_ptr(), t_st, batch, width,
+    _lib.call_on(index, name, *args, table.data_ptr(), t_st, batch, width,
                  starts.data_ptr(), offsets, key.data_ptr(), k_st, k_sh, value.data_ptr(), v_st,
                  v_sh, rows, 1 if dtype is torch.float16 else 0, _lib.raw_stream(index))
 
@@ -160,14 +178,14 @@ def write_cache(cache: KVCache, key, value, table, starts, offsets=None):
     tokens', the held codes are rounded once more. A nonfinite value becomes the NaN code and
     leaves the scale alone. No page may be written twice in one call, by two sequences or by a table
     that names it twice."""
-    _check_cache(cache, "write_cache")
-    index, shape, dtype = cache._index, key.shape, key.dtype
+    index, args = _check_cache(cache, "write_cache")
+    shape, dtype = key.shape, key.dtype
     if len(shape) != 3 or shape[1:] != cache._row or value.shape != shape:
         raise ValueError("key and value must be [rows, kv_heads, D] of the cache")
     if dtype not in _DTYPES or value.dtype is not dtype or key.get_device() != index \
             or value.get_device() != index:
         raise ValueError("key and value must share BF16 or FP16 and the cache's device")
-    _move("vdn_cache_write", cache, key, value, shape[0], dtype, table, starts, offsets)
+    _move("vdn_cache_write", index, args, key, value, shape[0], dtype, table, starts, offsets)
 
 
 def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bfloat16):
@@ -176,14 +194,14 @@ def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bflo
     (arguments as write_cache). Exact in BF16; FP16 rounds what is under its normal range and
     saturates at 65504. Rows of a page that is not there are NaN, rows from offsets[batch] on
     zero."""
-    _check_cache(cache, "read_cache")
+    index, args = _check_cache(cache, "read_cache")
     if type(rows) is not int or rows < 0:
         raise ValueError("rows must be a non-negative integer")
     if dtype not in _DTYPES:
         raise ValueError("dtype must be BF16 or FP16")
     key = torch.empty((rows, *cache._row), dtype=dtype, device=cache.k_codes.device)
     value = torch.empty_like(key)
-    _move("vdn_cache_read", cache, key, value, rows, dtype, table, starts, offsets)
+    _move("vdn_cache_read", index, args, key, value, rows, dtype, table, starts, offsets)
     return key, value
 
 
@@ -201,11 +219,11 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
 
     A sequence with a bad page id or length gets NaN (see KVCache.check). For FP16 queries
     the cached values must be within FP16's range."""
-    _check_cache(cache, "cache_attention")
+    index, args = _check_cache(cache, "cache_attention")
     if query.ndim not in (3, 4):
         raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
-    dtype, index = query.dtype, cache._index
-    _, kv_heads, page, dim = cache._args[5:]
+    dtype = query.dtype
+    _, kv_heads, page, dim = cache._geometry
     if query.ndim == 4:
         batch, tokens, heads, d = query.shape
         q_sb, q_st, q_sh, q_sd = query.stride()
@@ -240,7 +258,7 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
         nbytes = _workspace_bytes(index, tokens, group, d)
         workspace = query.new_empty(nbytes // 2)   # 2-byte elements
     _lib.call_on(index, "vdn_cache_attention", query.data_ptr(), q_sb, q_st, q_sh,
-                 *cache._args, table.data_ptr(), t_st, batch, width,
+                 *args, table.data_ptr(), t_st, batch, width,
                  lengths.data_ptr(), tokens, group, int(dtype is torch.float16), scale,
                  out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse), _lib.ptr(workspace), nbytes,
                  _lib.raw_stream(index))
