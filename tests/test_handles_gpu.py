@@ -5,6 +5,7 @@ import io
 import pytest
 import torch
 
+from vdn_amd import causal as vc
 from vdn_amd import kvcache as kv
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +66,19 @@ def test_a_cache_that_goes_to_the_host_and_back(device):
         assert torch.equal(kv.cache_attention(q, cache, table, held), want)
         del filler
     cache.check()
+
+
+@torch.no_grad()
+def test_a_forked_plan_outlives_the_first_one(device):
+    x = torch.randn(150, 6, 64, generator=torch.Generator().manual_seed(1)).bfloat16().to(device)
+    q, k, v = x[:, :4], x[:, 4:5], x[:, 5:]
+    plan = vc.prepare_causal_plan([100, 50], 4, 1, device=device)
+    want = vc.causal_attention(q, k, v, plan)
+    fork, loaded = forks(plan)
+    plan.blocks.copy_(vc.prepare_causal_plan([50, 100], 4, 1).blocks)
+    assert not torch.equal(vc.causal_attention(q, k, v, plan), want)
+    for own in (fork, loaded):
+        assert torch.equal(vc.causal_attention(q, k, v, own), want)
+    loaded.blocks.data = loaded.blocks.data.cpu()
+    with pytest.raises(ValueError, match="device"):
+        vc.causal_attention(q, k, v, loaded)

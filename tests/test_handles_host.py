@@ -5,6 +5,7 @@ import pickle
 import pytest
 import torch
 
+from vdn_amd import causal as vc
 from vdn_amd import kvcache as kv
 
 PARTS = ("k_codes", "k_scales", "v_codes", "v_scales", "faults")
@@ -45,3 +46,16 @@ def test_cache_refuses_storage_of_another_size(part):
     tensor.data = tensor[:3].clone()
     with pytest.raises(ValueError, match="size"):
         kv._cache_args(cache)
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,block_rows", [([40, 3], 4, 2, 128), ([4096], 32, 8, 256)])
+def test_plan_copies_name_their_own_blocks(lengths, heads, kv_heads, block_rows):
+    plan = vc.prepare_causal_plan(lengths, heads, kv_heads)
+    for fork in (plan, copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
+        own = fork.blocks if block_rows == 128 else fork.wide_blocks
+        assert fork is plan or own.data_ptr() not in (plan.blocks.data_ptr(), plan.blocks.data_ptr() + 16 * len(
+            plan.blocks))
+        assert vc._launch(fork, 128) == ((own.data_ptr(), own.shape[0], block_rows), -1)
+        assert vc._launch(fork, 64) == ((fork.blocks.data_ptr(), fork.blocks.shape[0], 128), -1)
+    plan.blocks.data = plan.blocks.clone()
+    assert vc._launch(plan, 256)[0][0] == plan.blocks.data_ptr()

@@ -32,20 +32,17 @@ class CausalPlan:
     blocks: torch.Tensor
     wide_blocks: torch.Tensor | None
 
-    def __post_init__(self):
-        def launch(blocks, block_rows):
-            return blocks.data_ptr(), blocks.shape[0], block_rows
-
-        # the entry point's arguments
-        narrow = launch(self.blocks, 128)
-        object.__setattr__(self, "_narrow", narrow)
-        object.__setattr__(self, "_wide", narrow if self.wide_blocks is None
-                           else launch(self.wide_blocks, 256))
-        object.__setattr__(self, "_index", self.blocks.get_device())   # -1 off the GPU
-
     @property
     def device(self):
         return self.blocks.device
+
+
+def _launch(plan, head_dim):
+    """The entry point's block arguments, from the tensors that the plan holds now (a copied or
+    unpickled plan has its own), and their device index (-1 off the GPU)."""
+    wide = head_dim == 128 and plan.wide_blocks is not None
+    blocks = plan.wide_blocks if wide else plan.blocks
+    return (blocks.data_ptr(), blocks.shape[0], 256 if wide else 128), blocks.get_device()
 
 
 # When head dim 128 takes 256-row blocks (8 waves, one workgroup a CU) instead of 128-row ones (two
@@ -130,8 +127,9 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
             or q_sd != 1 or k_sd != 1 or v_sd != 1:
         raise ValueError("Q/K/V must share BF16 or FP16 and have unit innermost stride")
     index = query.get_device()
+    launch, plan_index = _launch(plan, d)
     if index < 0 or key.get_device() != index or value.get_device() != index \
-            or plan._index != index:
+            or plan_index != index:
         raise ValueError("Q/K/V and prepared plan must be on the same CUDA device")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
@@ -155,7 +153,7 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
             lse[plan.rows:].fill_(-math.inf)
     _lib.call_on(index, "vdn_causal_attention", query.data_ptr(), q_st, q_sh, key.data_ptr(),
                  k_st, k_sh, value.data_ptr(), v_st, v_sh,
-                 *(plan._wide if d == 128 else plan._narrow), kv_heads, heads // kv_heads, d,
+                 *launch, kv_heads, heads // kv_heads, d,
                  1 if dtype is torch.float16 else 0, scale, out.data_ptr(), o_st, o_sh, lse_ptr,
                  heads, 1, _lib.raw_stream(index))
     return (out, lse) if return_lse else out
