@@ -159,6 +159,7 @@ struct Half<false> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
+  static __device__ __forceinline__ uint32_t pack_out(float a, float b) { return pack(a, b); }
 };
 
 template <>
@@ -173,6 +174,10 @@ struct Half<true> {
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     return f32_to_f16_bits(a) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16;
+  }
+  // An output: E4M3 takes values next to fp16's largest one to 65536, which would be an infinity.
+  static __device__ __forceinline__ uint32_t pack_out(float a, float b) {
+    return pack(f16_in_range(a), f16_in_range(b));
   }
 };
 
@@ -526,8 +531,8 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
         const int i = row / io.group, h = u * io.group + row - i * io.group;
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;
         u32x2 y;
-        y[0] = E::pack(acc[0] * inv, acc[1] * inv);
-        y[1] = E::pack(acc[2] * inv, acc[3] * inv);
+        y[0] = E::pack_out(acc[0] * inv, acc[1] * inv);
+        y[1] = E::pack_out(acc[2] * inv, acc[3] * inv);
         *reinterpret_cast<u32x2*>(io.out + b_now * io.o_sb + i * io.o_st + h * io.o_sh + d) = y;
         if (io.lse != nullptr && d == 0)
           io.lse[(static_cast<int64_t>(b_now) * io.tokens + i) * c.kv_heads * io.group + h] =
@@ -631,8 +636,8 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int i = row / io.group, h = u * io.group + row - i * io.group;
   u32x2 y;
-  y[0] = Half<kF16>::pack(acc[0] * inv, acc[1] * inv);
-  y[1] = Half<kF16>::pack(acc[2] * inv, acc[3] * inv);
+  y[0] = Half<kF16>::pack_out(acc[0] * inv, acc[1] * inv);
+  y[1] = Half<kF16>::pack_out(acc[2] * inv, acc[3] * inv);
   *reinterpret_cast<u32x2*>(io.out + b * io.o_sb + i * io.o_st + h * io.o_sh + d) = y;
   if (io.lse != nullptr && d == 0)
     io.lse[(static_cast<int64_t>(b) * io.tokens + i) * c.kv_heads * io.group + h] =

@@ -130,6 +130,13 @@ __device__ __forceinline__ uint16_t f32_to_f16_bits(float f) {
   return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
 }
 
+// A finite value beyond fp16's largest one becomes that: for results that the exact arithmetic
+// keeps in range. Infinities and NaN stay.
+__device__ __forceinline__ float f16_in_range(float f) {
+  const float a = fabsf(f);
+  return a > 65504.f && a < INFINITY ? copysignf(65504.f, f) : f;
+}
+
 __device__ __forceinline__ float round_f16(float f) {
   return static_cast<float>(static_cast<_Float16>(f));
 }

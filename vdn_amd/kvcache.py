@@ -218,7 +218,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     rounded to the query's dtype before the product with V, the codes' values are exact.
 
     A sequence with a bad page id or length gets NaN (see KVCache.check). For FP16 queries
-    the cached values must be within FP16's range."""
+    the cached values must be within FP16's range; an output that E4M3's rounding takes over its
+    largest value is that value."""
     index, args = _check_cache(cache, "cache_attention")
     if query.ndim not in (3, 4):
         raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
