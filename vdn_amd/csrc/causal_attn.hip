@@ -407,7 +407,11 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     for (int j = 0; j < 4; ++j) {
       typename E::x4 y;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = static_cast<typename E::type>(o[db][4 * j + i] * inv_l);
+      for (int i = 0; i < 4; ++i) {
+        // the rounded weights can take a mean of values next to fp16's largest one over it
+        const float x = o[db][4 * j + i] * inv_l;
+        y[i] = static_cast<typename E::type>(kF16 ? f16_in_range(x) : x);
+      }
       *reinterpret_cast<typename E::x4*>(sO + col * kD + ((4 * db + j) ^ swz_k<kD>(col)) * 8 + 4 * g) = y;
     }
   if (to.lse != nullptr && live && g == 0)
