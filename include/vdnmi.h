@@ -345,8 +345,9 @@ int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * kv_heads, head_dim, page] (E4M3, 16-byte aligned), k_scales and v_scales uint8 [pages, kv_heads]
  * (E8M0: exponent + 127, at least 27), contiguous; page a power of two in 16..256, head_dim 64,
  * 128 or 256. table int32 [batch, width] (row stride table_st): the pages of each sequence in
- * order. A page id outside [0, pages), a negative or too large length and offsets outside the rows
- * are not followed; *faults (device int32) becomes 1.
+ * order. A page id outside [0, pages), a negative or too large length and offsets that fall or lie
+ * outside the rows are not followed (nor, with the latter, the sequences next to them); *faults (device
+ * int32) becomes 1.
  *
  * vdn_cache_write: rows offsets[i] .. offsets[i + 1] - 1 (int32 [batch + 1]; null: one row each)
  * of key and value [rows, kv_heads, head_dim] (dtype 0 bf16, 1 fp16; (token, head) strides,

@@ -40,3 +40,54 @@ def test_fp16_outputs_next_to_the_largest_value(device, n, dim):
     assert (out[..., 2::4] == 65504).all() and torch.isfinite(lse).all()
     assert torch.isfinite(out).all()
     cache.check()
+
+
+def faulty(cache, key, table, starts, offsets):
+    """Whether a write of these rows, and a read, raise the fault word; their results may be anything."""
+    said = []
+    for call in (lambda: kv.write_cache(cache, key, key, table, starts, offsets),
+                 lambda: kv.read_cache(cache, table, starts, offsets, key.shape[0])):
+        call()
+        said.append(bool(cache.faults.item()))
+        cache.faults.zero_()
+    assert said[0] == said[1]
+    return said[0]
+
+
+@pytest.mark.parametrize("offsets", [(0, 40, 8, 60), (0, 60, 0, 60), (0, 17, 16, 60), (0, 59, 60, 59),
+                                     (0, 30, 61, 61), (0, -1, 20, 60), (1, 20, 40, 60)])
+@torch.no_grad()
+def test_offsets_that_fall_or_leave_the_rows(device, offsets):
+    """The sequence between 40 and 8 owns no page step, so the search for a page passes it over. No
+    page of these sequences changes."""
+    cache = kv.empty_cache(13, 1, 64, 16, device=device)
+    for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales):
+        t.fill_(0x38)
+    table = torch.arange(12, dtype=torch.int32, device=device).view(3, 4)
+    x = torch.randn(60, 1, 64, generator=torch.Generator().manual_seed(0)).to(BF16).cuda()
+    assert not faulty(cache, x, table, ints(0, 0, 0), ints(0, 20, 20, 60))
+    for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales):
+        t.fill_(0x38)
+    assert faulty(cache, x, table, ints(0, 0, 0), ints(*offsets))
+    for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales):
+        assert (t == 0x38).all()
+
+
+@pytest.mark.parametrize("batch", [64, 65, 200, 5000])
+@pytest.mark.parametrize("page", [16, 256])
+@torch.no_grad()
+def test_one_fall_among_many_offsets(device, batch, page):
+    """Wherever the pair lies that falls, and however far, the word is raised."""
+    rows, places = 3 * batch, {0, 1, 62, 63, 64, 127, 128, batch // 2, batch - 2, batch - 1}
+    cache = kv.empty_cache(batch, 1, 64, page, device=device)
+    table = torch.arange(batch, dtype=torch.int32, device=device)[:, None]
+    x = torch.zeros(rows, 1, 64, dtype=BF16, device=device)
+    starts = torch.zeros(batch, dtype=torch.int32, device=device)
+    good = 3 * torch.arange(batch + 1, dtype=torch.int32)
+    assert not faulty(cache, x, table, starts, good.cuda())
+    for i in sorted(p for p in places if p < batch):
+        for value in {int(good[i + 1]) + 4, 0, rows, rows + 1, -1}:
+            bad = good.clone()
+            bad[i] = value
+            ok_pairs = bool((bad.diff() >= 0).all()) and bad[0] == 0 and int(bad.max()) <= rows
+            assert faulty(cache, x, table, starts, bad.cuda()) == (not ok_pairs), (i, value)

@@ -59,6 +59,21 @@ __device__ __forceinline__ int seq_base(const Seqs& s, int i, int log_page) {
   return (s.offsets[i] >> log_page) + 2 * i;
 }
 
+// Whether sequence i, with rows off .. next - 1, is not behind the one before it or not inside the rows.
+__device__ __forceinline__ bool bad_offsets(int off, int next, int i, int rows) {
+  return off < 0 || next < off || next > rows || (i == 0 && off != 0);
+}
+
+// One workgroup looks at the offsets of more sequences than its search loads: no other may come across
+// a pair that falls.
+__device__ __forceinline__ void check_offsets(const KvCache& c, const Seqs& s, int rows) {
+  if (blockIdx.x != 0 || s.offsets == nullptr || s.batch <= 64) return;
+  bool bad = false;
+  for (int i = threadIdx.x; i < s.batch; i += blockDim.x)
+    bad |= bad_offsets(s.offsets[i], s.offsets[i + 1], i, rows);
+  if (bad) *c.faults = 1;
+}
+
 __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot) {
   const int log_page = c.log_page;
   Piece p{0, 0, 0, 0, 0};
@@ -99,6 +114,12 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
       from = s.starts[i];
       base = (off >> log_page) + 2 * i;
     }
+    // Offsets that fall would name a row twice, and the search would pass sequences over; out of range
+    // they name rows that are not there. Either way none of these sequences is followed.
+    if (__any(i < s.batch && bad_offsets(off, next, i, rows))) {
+      *c.faults = 1;
+      return p;
+    }
     const int found = __popcll(__ballot(i < s.batch && base <= slot));
     const int base_end = (behind >> log_page) + 2 * s.batch;
     int o0, o1;
@@ -119,7 +140,7 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
       *c.faults = 1;   // rows in front of the first sequence
       return p;
     }
-    if (o0 < 0 || o1 < o0 || o1 > rows || (p.seq == 0 && o0 > 0)) *c.faults = 1;
+    if (o0 < 0 || o1 < o0 || o1 > rows) *c.faults = 1;
     first = min(max(o0, 0), rows);
     end = min(max(o1, 0), rows);
     if (p.seq == s.batch) {
@@ -342,6 +363,7 @@ __device__ __forceinline__ void write_page(const KvCache& c, const Rows& rows, c
 
 template <int kD, int kTiles, bool kF16>
 __global__ void __launch_bounds__(1024) cache_write_kernel(KvCache c, Rows rows, Seqs s) {
+  check_offsets(c, s, rows.count);
   const Item item = item_of(c);
   const Piece p = find_piece(c, s, rows.count, item.slot);
   if (p.n <= 0 || p.seq >= s.batch) return;
@@ -423,6 +445,7 @@ __device__ __forceinline__ void read_page(const KvCache& c, const Rows& rows, co
 
 template <int kD, int kTiles, bool kF16>
 __global__ void __launch_bounds__(1024) cache_read_kernel(KvCache c, Rows rows, Seqs s) {
+  check_offsets(c, s, rows.count);
   const Item item = item_of(c);
   const Piece p = find_piece(c, s, rows.count, item.slot);
   if (p.n <= 0) return;

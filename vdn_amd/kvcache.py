@@ -8,8 +8,9 @@ codes [pages, kv_heads, D, page], the order in which the attention reads them.
 The caller owns the pool's bookkeeping: an int32 table [batch, width] names each sequence's pages
 in order, an int32 tensor the tokens that it holds. Both stay on the device, so that a decode step
 can be captured into a graph and replayed as they change. A page id outside the pool, a
-length that the table cannot hold, offsets that do not fit the rows: kernels follow none of
-them; they raise the cache's `faults` word, and KVCache.check() reports it.
+length that the table cannot hold, offsets that fall or do not fit the rows: kernels follow none of
+them; they raise the cache's `faults` word, and KVCache.check() reports it. (Around bad offsets
+other sequences of that call may be left out too.)
 """
 from __future__ import annotations
 
