@@ -60,18 +60,9 @@ __device__ __forceinline__ int seq_base(const Seqs& s, int i, int log_page) {
 }
 
 // Whether sequence i, with rows off .. next - 1, is not behind the one before it or not inside the rows.
-__device__ __forceinline__ bool bad_offsets(int off, int next, int i, int rows) {
-  return off < 0 || next < off || next > rows || (i == 0 && off != 0);
-}
-
-// One workgroup looks at the offsets of more sequences than its search loads: no other may come across
-// a pair that falls.
-__device__ __forceinline__ void check_offsets(const KvCache& c, const Seqs& s, int rows) {
-  if (blockIdx.x != 0 || s.offsets == nullptr || s.batch <= 64) return;
-  bool bad = false;
-  for (int i = threadIdx.x; i < s.batch; i += blockDim.x)
-    bad |= bad_offsets(s.offsets[i], s.offsets[i + 1], i, rows);
-  if (bad) *c.faults = 1;
+// (unsigned: a negative number is larger than any)
+__device__ __forceinline__ bool bad_offsets(uint32_t off, uint32_t next, int i, uint32_t rows) {
+  return off > (i == 0 ? 0u : next) || next > rows;
 }
 
 __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot) {
@@ -95,6 +86,13 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
     const int behind = s.offsets[s.batch];
     int lo = 0, step = 1;
     while (static_cast<int64_t>(step) * 64 < s.batch) step *= 64;
+    if (step > 1 && blockIdx.x == 0) {
+      // the search loads only a part of the offsets, and may pass over a pair that falls
+      bool bad = false;
+      for (int i = threadIdx.x; i < s.batch; i += blockDim.x)
+        bad |= bad_offsets(s.offsets[i], s.offsets[i + 1], i, rows);
+      if (bad) *c.faults = 1;
+    }
     for (; step > 1; step /= 64) {
       const int64_t i = lo + static_cast<int64_t>(lane) * step;
       const bool le = i < s.batch && seq_base(s, static_cast<int>(i), log_page) <= slot;
@@ -116,10 +114,7 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
     }
     // Offsets that fall would name a row twice, and the search would pass sequences over; out of range
     // they name rows that are not there. Either way none of these sequences is followed.
-    if (__any(i < s.batch && bad_offsets(off, next, i, rows))) {
-      *c.faults = 1;
-      return p;
-    }
+    const bool bad = __ballot(bad_offsets(off, next, i, rows)) != 0;   // 0, 0 behind the last one
     const int found = __popcll(__ballot(i < s.batch && base <= slot));
     const int base_end = (behind >> log_page) + 2 * s.batch;
     int o0, o1;
@@ -129,7 +124,7 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
       start = 0;
       o0 = behind;
       o1 = rows;
-    } else if (found > 0) {
+    } else if (found > 0 && !bad) {
       p.seq = lo + found - 1;
       j = slot - __builtin_amdgcn_readlane(base, found - 1);
       if (j < 0) return p;
@@ -137,7 +132,7 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
       o0 = __builtin_amdgcn_readlane(off, found - 1);
       o1 = __builtin_amdgcn_readlane(next, found - 1);
     } else {
-      *c.faults = 1;   // rows in front of the first sequence
+      *c.faults = 1;   // bad offsets, or rows in front of the first sequence
       return p;
     }
     if (o0 < 0 || o1 < o0 || o1 > rows) *c.faults = 1;
@@ -363,7 +358,6 @@ __device__ __forceinline__ void write_page(const KvCache& c, const Rows& rows, c
 
 template <int kD, int kTiles, bool kF16>
 __global__ void __launch_bounds__(1024) cache_write_kernel(KvCache c, Rows rows, Seqs s) {
-  check_offsets(c, s, rows.count);
   const Item item = item_of(c);
   const Piece p = find_piece(c, s, rows.count, item.slot);
   if (p.n <= 0 || p.seq >= s.batch) return;
@@ -445,7 +439,6 @@ __device__ __forceinline__ void read_page(const KvCache& c, const Rows& rows, co
 
 template <int kD, int kTiles, bool kF16>
 __global__ void __launch_bounds__(1024) cache_read_kernel(KvCache c, Rows rows, Seqs s) {
-  check_offsets(c, s, rows.count);
   const Item item = item_of(c);
   const Piece p = find_piece(c, s, rows.count, item.slot);
   if (p.n <= 0) return;
