@@ -45,3 +45,35 @@ def test_fp16_means_of_the_largest_value(device, dim, block_rows):
     got = vc.causal_attention(q, k, v, plan_of([n], 1, 1, block_rows, device), scale)
     assert got[n - 1, 0, 2] == math.inf and got[n - 1, 0, 3] == -math.inf
     assert torch.isfinite(got[:n - 1]).all()
+
+
+@pytest.mark.parametrize("dim,block_rows", VARIANTS)
+@pytest.mark.parametrize("heads,dtype", [(2, BF16), (2, FP16), (1, BF16), (1, FP16)])
+@torch.no_grad()
+def test_infinite_values_in_front_of_a_steep_rise(device, dim, block_rows, heads, dtype):
+    """Scores rise by 288 binary orders from one tile of a block's diagonal to the next, so that fp32
+    keeps nothing of what was summed before. An infinity of a token that a row sees, in the tile
+    before the rise or in that of the rise, is in its output all the same; rows before it are as
+    without it."""
+    n, rise = 300, 70
+    q = torch.zeros(n, heads, dim)
+    q[..., 0] = 1.0
+    k = torch.zeros(n, 1, dim)
+    k[rise:, :, 0] = 200.0
+    v = torch.randn(n, 1, dim, generator=torch.Generator().manual_seed(2))
+    q, k, v = (x.to(dtype).cuda() for x in (q, k, v))
+    plan = plan_of([n], heads, 1, block_rows, device)
+    clean = vc.causal_attention(q, k, v, plan, 1.0)
+    notes = ((5, 3, math.inf), (5, 4, -math.inf), (rise, 9, math.inf), (rise + 1, 10, -math.inf))
+    bad = v.clone()
+    for token, channel, value in notes:
+        bad[token, 0, channel] = value
+    block = block_rows // heads                    # tokens of the first block
+    for _ in range(3):
+        got = vc.causal_attention(q, k, bad, plan, 1.0)
+        for token, channel, value in notes:
+            assert torch.equal(got[:token, :, channel], clean[:token, :, channel])
+            assert (got[token:block, :, channel] == value).all()
+            assert not torch.isfinite(got[max(block, token):, :, channel]).any()
+        others = [c for c in range(dim) if c not in (3, 4, 9, 10)]
+        assert torch.equal(got[..., others], clean[..., others])

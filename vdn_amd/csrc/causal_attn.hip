@@ -19,7 +19,8 @@
 // NaN in an MFMA. Only tiles on the diagonal hold such tokens: there every wave looks its share
 // of the V tile over as it lands, replaces nonfinite values by zeros and notes, per channel, the
 // first token with a positive and with a negative one. What a row sees is a prefix, so the row
-// holds that value exactly if the token is not behind its own: it is added after the product.
+// holds that value exactly if the token is not behind its own: it is added after the last tile, when
+// no wave changes the notes any more.
 #include "attn_tiles.h"
 
 #include <float.h>
@@ -372,18 +373,6 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
       __builtin_amdgcn_sched_barrier(0x406);
     }
     if (behind && loads && t + 1 < ntiles) issue_all(a + kBN, ndk, ndv);
-    if (diagonal && sDirty != 0) {
-      keep();
-#pragma unroll
-      for (int db = 0; db < kDB; ++db)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const int d = 32 * db + (v >> 2) * 8 + g * 4 + (v & 3);
-          if (sPos[d] <= my_i) o[db][v] += INFINITY;
-          if (sNeg[d] <= my_i) o[db][v] -= INFINITY;
-        }
-      keep();
-    }
   };
   __syncthreads();  // sPos, sNeg, sDirty
   for (int t = 0; t < ntiles; t += 2) {
@@ -393,7 +382,19 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   keep();
   l = sum_halves(l);
   const float inv_l = 1.0f / l;   // l = 0 only if all scores are -inf: NaN, LSE -inf
-  __syncthreads();                // the epilogue reuses the tile buffers
+  __syncthreads();                // the notes are final; the epilogue reuses the tile buffers
+  if (sDirty != 0) {
+    keep();
+#pragma unroll
+    for (int db = 0; db < kDB; ++db)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int d = 32 * db + (v >> 2) * 8 + g * 4 + (v & 3);
+        if (sPos[d] <= my_i) o[db][v] += INFINITY;
+        if (sNeg[d] <= my_i) o[db][v] -= INFINITY;
+      }
+    keep();
+  }
 
   // ---- epilogue: O / l through LDS to rows. Each wave stages its own 32 (no further barrier), four
   // channels a write; chunk c of row r lies at c ^ swz_k(r), so that the 32 rows of a write and the
