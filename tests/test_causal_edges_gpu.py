@@ -77,3 +77,22 @@ def test_infinite_values_in_front_of_a_steep_rise(device, dim, block_rows, heads
             assert not torch.isfinite(got[max(block, token):, :, channel]).any()
         others = [c for c in range(dim) if c not in (3, 4, 9, 10)]
         assert torch.equal(got[..., others], clean[..., others])
+
+
+@pytest.mark.parametrize("dim,block_rows", VARIANTS)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@torch.no_grad()
+def test_rows_without_weight_are_nan_also_over_infinite_values(device, dim, block_rows, dtype):
+    """All scores of the first rows are -inf: no weights exist, so every channel is NaN, those with an
+    infinity among the values too."""
+    n, shut = 200, 90
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(n, 1, dim, generator=g) for _ in range(3))
+    q[..., 5] = 1.0
+    k[:shut, :, 5] = -math.inf
+    v[3, 0, 7], v[40, 0, 8] = math.inf, -math.inf
+    q, k, v = (x.to(dtype).cuda() for x in (q, k, v))
+    got, lse = vc.causal_attention(q, k, v, plan_of([n], 1, 1, block_rows, device), return_lse=True)
+    assert got[:shut].isnan().all() and torch.isneginf(lse[:shut]).all()
+    others = [c for c in range(dim) if c not in (7, 8)]
+    assert torch.isfinite(got[shut:][..., others]).all() and torch.isfinite(lse[shut:]).all()

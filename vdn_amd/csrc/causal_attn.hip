@@ -381,7 +381,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   }
   keep();
   l = sum_halves(l);
-  const float inv_l = 1.0f / l;   // l = 0 only if all scores are -inf: NaN, LSE -inf
+  const float inv_l = l == 0.f ? NAN : 1.0f / l;   // l = 0 only if all scores are -inf: NaN, LSE -inf
   __syncthreads();                // the notes are final; the epilogue reuses the tile buffers
   if (sDirty != 0) {
     keep();
