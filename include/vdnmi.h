@@ -371,7 +371,8 @@ int vdn_cache_read(const void* k_codes, const void* k_scales, const void* v_code
 /*
  * Softmax attention of the `tokens` newest tokens of each sequence, whose K/V are in the cache
  * already, over its lengths[b] cached tokens: query i sees tokens j < lengths[b] - tokens + 1
- * + i; a row that sees none is zero, its lse -inf; rows of a sequence with a fault are NaN. q, out:
+ * + i; a row that sees none is zero, one whose scores are all -inf NaN, the lse of both -inf; rows
+ * of a sequence with a fault are NaN. q, out:
  * [batch, tokens, kv_heads * group, head_dim] by (sequence, token, head) strides, multiples of 8,
  * dtype 0 bf16 or 1 fp16; lse (nullable): fp32 [batch, tokens, heads] contiguous. workspace:
  * 16-byte aligned, vdn_cache_attention_workspace's byte count, its contents need no preparation; not

@@ -91,3 +91,35 @@ def test_one_fall_among_many_offsets(device, batch, page):
             bad[i] = value
             ok_pairs = bool((bad.diff() >= 0).all()) and bad[0] == 0 and int(bad.max()) <= rows
             assert faulty(cache, x, table, starts, bad.cuda()) == (not ok_pairs), (i, value)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, BF16), (256, BF16)])
+@pytest.mark.parametrize("n", [3, 100, 500, 3000])     # fewer than the queries, whole units, a split one
+@torch.no_grad()
+def test_rows_whose_scores_are_all_minus_infinity(device, dim, dtype, n):
+    """A query whose every score is -inf has no softmax: NaN, its LSE -inf. A query that sees no key
+    is zero; the others are as without it."""
+    tokens = 5
+    cache = kv.empty_cache(-(-n // 16), 1, dim, 16, device=device)
+    table = in_order(n, 16).cuda()
+    if n > 500:
+        table = torch.cat((table, torch.zeros_like(table)), 1)
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(n, 1, dim, generator=g) for _ in range(2))
+    k[..., 0] = 1.0 + k[..., 0].abs()
+    kv.write_cache(cache, k.to(dtype).cuda(), v.to(dtype).cuda(), table, ints(0), ints(0, n))
+    q = torch.randn(1, tokens, 3, dim, generator=g).to(dtype).cuda()
+    want, wlse = kv.cache_attention(q, cache, table, ints(n), return_lse=True)
+    shut = q.clone()
+    shut[0, 0, 1, 0] = shut[0, tokens - 1, 2, 0] = -math.inf
+    got, lse = kv.cache_attention(shut, cache, table, ints(n), return_lse=True)
+    first = (0, 0, 1)
+    if n < tokens:                                     # the first query sees none
+        assert got[first].count_nonzero() == 0 and not got[first].isnan().any()
+    else:
+        assert got[first].isnan().all()
+    assert torch.isneginf(lse[first]) and got[0, -1, 2].isnan().all() and torch.isneginf(lse[0, -1, 2])
+    got[first], lse[first] = want[first], wlse[first]
+    got[0, -1, 2], lse[0, -1, 2] = want[0, -1, 2], wlse[0, -1, 2]
+    assert torch.equal(got, want) and torch.equal(lse, wlse)
+    cache.check()

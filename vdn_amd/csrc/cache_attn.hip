@@ -202,6 +202,12 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return out;
 }
 
+// Factor of a row's output from its sum of weights and the number of keys that it sees. No weights: a row
+// that sees no key is zero, one whose scores are all -inf has no softmax and is NaN.
+__device__ __forceinline__ float inverse_of(float sum, int keys) {
+  return sum == 0.f ? (keys > 0 ? NAN : 0.f) : 1.0f / sum;
+}
+
 template <int kD, int kNR, bool kF16>
 __global__ void __launch_bounds__(kThreads, workgroups_per_cu(kD, 16 * kNR))
 cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2) {
@@ -529,7 +535,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
       }
       if (whole) {
         const int i = row / io.group, h = u * io.group + row - i * io.group;
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        const float inv = inverse_of(sum, seen0 + i);
         u32x2 y;
         y[0] = E::pack_out(acc[0] * inv, acc[1] * inv);
         y[1] = E::pack_out(acc[2] * inv, acc[3] * inv);
@@ -633,8 +639,8 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
       for (int j = 0; j < 4; ++j) acc[j] += f == 0.f ? 0.f : x[j] * f;
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int i = row / io.group, h = u * io.group + row - i * io.group;
+  const float inv = inverse_of(sum, seq_tokens(c, s, b) - io.tokens + 1 + i);
   u32x2 y;
   y[0] = Half<kF16>::pack_out(acc[0] * inv, acc[1] * inv);
   y[1] = Half<kF16>::pack_out(acc[2] * inv, acc[3] * inv);

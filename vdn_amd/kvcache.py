@@ -213,7 +213,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16, H a multiple of the cache's
     kv_heads (query head h reads K/V head h // (H / kv_heads)); lengths int32 [batch] counts
     the tokens that the cache holds, the Q queries' own among them: query i sees the tokens j <
-    lengths - Q + 1 + i. A row that sees none is zero (LSE -inf). Returns a tensor like the query,
+    lengths - Q + 1 + i. A row that sees none is zero, one
+    whose scores are all -inf NaN (LSE -inf). Returns a tensor like the query,
     with return_lse also the natural-log sum of exp of the scaled scores, fp32 [batch, Q, H]
     (or [batch, H]). Scores, sums and the output are accumulated in fp32; probabilities are
     rounded to the query's dtype before the product with V, the codes' values are exact.
