@@ -123,3 +123,32 @@ def test_rows_whose_scores_are_all_minus_infinity(device, dim, dtype, n):
     got[0, -1, 2], lse[0, -1, 2] = want[0, -1, 2], wlse[0, -1, 2]
     assert torch.equal(got, want) and torch.equal(lse, wlse)
     cache.check()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, BF16), (256, BF16)])
+@pytest.mark.parametrize("at", [0, 70, 250, 600, 2900])
+@pytest.mark.parametrize("n", [300, 3000])             # a whole unit, a split one
+@torch.no_grad()
+def test_a_nan_value_outweighed(device, dim, dtype, n, at):
+    """The NaN code of a seen token reaches its channel wherever the heavy token lies, also where the
+    token's weight underflows in fp32: in the same wave, another one of the workgroup, another slot."""
+    if at >= n:
+        return
+    cache = kv.empty_cache(-(-n // 16), 1, dim, 16, device=device)
+    table = in_order(n, 16).cuda()
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(n, 1, dim, generator=g) for _ in range(2))
+    k[..., 0] = 0.0
+    v[at, 0, 5] = math.nan
+    q = torch.randn(1, 2, dim, generator=g)
+    q[..., 0] = 16.0
+    others = [c for c in range(dim) if c != 5]
+    for heavy in (10, 90, 130, 260, 700, 1500, 2990):
+        if heavy >= n or heavy // 16 == at // 16:      # (a page with one loud channel keeps its own scale)
+            continue
+        loud = k.clone()
+        loud[heavy, 0, 0] = 400.0
+        kv.write_cache(cache, loud.to(dtype).cuda(), v.to(dtype).cuda(), table, ints(0), ints(0, n))
+        out, lse = kv.cache_attention(q.to(dtype).cuda(), cache, table, ints(n), 1.0, return_lse=True)
+        assert out[..., 5].isnan().all(), heavy
+        assert torch.isfinite(out[..., others]).all() and torch.isfinite(lse).all()

@@ -526,12 +526,13 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
       f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        // a wave without a visible key: weight 0 (its sum still carries a fault's NaN)
+        // a wave without a visible key: weight 0. Its sum still carries a fault's NaN; and a NaN of V
+        // stays one however small the factor is, so that the result does not depend on the split.
         const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - top);
         sum += s_l[w][r] * f;
         const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[w][r][d]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] += f == 0.f ? 0.f : x[i] * f;
+        for (int i = 0; i < 4; ++i) acc[i] += x[i] * f;
       }
       if (whole) {
         const int i = row / io.group, h = u * io.group + row - i * io.group;
@@ -614,8 +615,7 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
       const float f1 = m[a] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[a] - m_new);
       sum = sum * f0 + l[a] * f1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        acc[i] = (f0 == 0.f ? 0.f : acc[i] * f0) + (f1 == 0.f ? 0.f : x[a][i] * f1);
+      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * f0 + x[a][i] * f1;
       top = m_new;
     }
   }
@@ -636,7 +636,7 @@ cache_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks) {
       sum += s_pl[i] * f;
       const f32x4 x = *reinterpret_cast<const f32x4*>(&s_part[i][d]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] += f == 0.f ? 0.f : x[j] * f;
+      for (int j = 0; j < 4; ++j) acc[j] += x[j] * f;
     }
   }
   const int i = row / io.group, h = u * io.group + row - i * io.group;
