@@ -96,3 +96,30 @@ def test_rows_without_weight_are_nan_also_over_infinite_values(device, dim, bloc
     assert got[:shut].isnan().all() and torch.isneginf(lse[:shut]).all()
     others = [c for c in range(dim) if c not in (7, 8)]
     assert torch.isfinite(got[shut:][..., others]).all() and torch.isfinite(lse[shut:]).all()
+
+
+@pytest.mark.parametrize("dim,block_rows", VARIANTS)
+@pytest.mark.parametrize("heavy", [0, 20000])
+@torch.no_grad()
+def test_fp16_weights_that_are_small_but_many(device, dim, block_rows, heavy):
+    """32767 tokens of weight 2^-25.3 relative to a heavy one, whose value is 0: their sum is the
+    output. A weight is rounded to within 2^-36 of the largest or to half a step of fp16 (the bound's
+    own term for small weights, 2^-25 each, would be larger than the output)."""
+    n = 32768
+    q = torch.zeros(n, 1, dim)
+    q[..., 0] = 1.0
+    k = torch.zeros(n, 1, dim)
+    k[heavy, 0, 0] = 17.53
+    v = torch.rand(n, 1, dim, generator=torch.Generator().manual_seed(3)) + 0.5
+    v[heavy] = 0.0
+    q, k, v = (x.to(FP16) for x in (q, k, v))
+    got, lse = vc.causal_attention(q.cuda(), k.cuda(), v.cuda(), plan_of([n], 1, 1, block_rows, device), 1.0,
+                                   return_lse=True)
+    for a, b in ((32752, n), (25000, 25010), (heavy + 100, heavy + 105)):
+        out, el, mass, size = oc.attention(q[a:b], k[:b], v[:b], a, 1.0)
+        tol, ltol = oc.bounds(out, mass, size, v[:b], FP16, dim, b)
+        top = float(v.abs().max())
+        tol += b * (2.0 ** -36 - 2.0 ** -25) * top
+        err = (got[a:b].cpu().double() - out).abs()
+        assert bool((err <= tol).all()), f"rows {a}: worst {float((err / tol).max())}"
+        assert bool(((lse[a:b].cpu().double() - el).abs() <= ltol).all())

@@ -221,9 +221,12 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
   const int tr_row = 4 * (G >> 1) + (L >> 2);
   const int tr_col = 16 * (G & 1) + 4 * (L & 3);
 
-  // Running maximum m in scaled (exp2) units; it may lag the true one by up to kLazy, so that
-  // most tiles need no rescale (p <= 2^kLazy).
-  constexpr float kLazy = 8.f;
+  // m is what the exponents are taken relative to (exp2 units): a row's running maximum less kAbove, which
+  // may lag the true one by up to kLazy, so that most tiles need no rescale. Any m gives the same
+  // weights; with kAbove those of fp16 reach up to 2^15, and one is rounded to within 2^-36 of the
+  // largest instead of 2^-25 (32767 tokens of weight 2^-25 beside a heavy one would lose all of theirs).
+  // bf16 has fp32's range.
+  constexpr float kLazy = kF16 ? 4.f : 8.f, kAbove = kF16 ? 11.f : 0.f;
   auto process = [&](int t, auto buf_tag) __attribute__((always_inline)) {
     constexpr int kBuf = decltype(buf_tag)::value;
     const uint16_t* tk = kBuf == 0 ? sK0 : sK1;
@@ -320,9 +323,9 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kt][v]);
     mx = max_halves(mx) * scale_log2;
-    const bool grow = mx > m + kLazy;
+    const bool grow = mx > m + (kLazy + kAbove);
     if (__any(grow)) {
-      const float m_new = grow ? mx : m;
+      const float m_new = grow ? mx - kAbove : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
       l *= corr;
       keep();
