@@ -152,3 +152,36 @@ def test_a_nan_value_outweighed(device, dim, dtype, n, at):
         out, lse = kv.cache_attention(q.to(dtype).cuda(), cache, table, ints(n), 1.0, return_lse=True)
         assert out[..., 5].isnan().all(), heavy
         assert torch.isfinite(out[..., others]).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heavy", [0, 20000])
+@pytest.mark.parametrize("n,heads", [(500, 1), (32768, 1), (32768, 24)])
+@torch.no_grad()
+def test_fp16_weights_that_are_small_but_many(device, dim, heavy, n, heads):
+    """Tokens of weight 2^-25.3 relative to a heavy one, whose value is 0: their sum is the output. A
+    weight is rounded to within 2^-39 of the largest or to half a step of fp16 (the bound's own term
+    for small weights, 2^-25 each, would be larger than the output)."""
+    heavy = min(heavy, n - 1)
+    cache = kv.empty_cache(-(-n // 64), 1, dim, 64, device=device)
+    oracle = ok.Cache(-(-n // 64), 1, 64, dim)
+    table = in_order(n, 64)
+    k = torch.zeros(n, 1, dim)
+    k[heavy, 0, 0] = 16.0
+    v = torch.rand(n, 1, dim, generator=torch.Generator().manual_seed(3)) + 0.5
+    v[heavy] = 0.0
+    k, v = k.to(FP16), v.to(FP16)
+    kv.write_cache(cache, k.cuda(), v.cuda(), table.cuda(), ints(0), ints(0, n))
+    oracle.write(k, v, table, [0], [n])
+    kk, vv = (oracle.tokens(side, table[0], 0, n) for side in range(2))
+    assert kk[heavy, 0, 0] == 16
+    q = torch.zeros(1, heads, dim)
+    q[..., 0] = 1.0957
+    q = q.to(FP16)
+    got, lse = kv.cache_attention(q.cuda(), cache, table.cuda(), ints(n), 1.0, return_lse=True)
+    out, el, mass, size = oc.attention(q, kk, vv, n - 1, 1.0)
+    tol, ltol = oc.bounds(out, mass, size, vv, FP16, dim, n)
+    tol += n * (2.0 ** -39 - 2.0 ** -25) * float(vv.abs().max())
+    err = (got.cpu().double() - out).abs()
+    assert bool((err <= tol).all()), f"worst {float((err / tol).max())}"
+    assert bool(((lse.cpu().double() - el).abs() <= ltol).all())

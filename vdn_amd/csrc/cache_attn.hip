@@ -214,6 +214,11 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   constexpr int kRows = 16 * kNR;     // query rows of a unit
   constexpr int kKL = kD / 64;        // 16-byte K loads per key row and lane
   constexpr int kDB = kD / 16;        // 16-channel blocks of O
+  // m, what the exponents are taken relative to, is the running maximum less kAbove. Any m gives the same
+  // weights; with kAbove those of fp16 reach up to 2^14, and one is rounded to within 2^-39 of the
+  // largest instead of 2^-25 (many tokens under 2^-25 beside a heavy one would lose all of theirs).
+  // bf16 has fp32's range.
+  constexpr float kAbove = kF16 ? 14.f : 0.f;
   typedef Half<kF16> E;
   __shared__ float s_o[kWaves][kRows][kD + 4];
   __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
@@ -376,7 +381,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
               sc_t[nr][t][i] = x;
               mx = fmaxf(mx, x);
             }
-          mx = max_quad_rows(mx);
+          mx = max_quad_rows(mx) - kAbove;
           if (__any(mx > m[nr])) {
             const float m_new = fmaxf(m[nr], mx);
             const float corr = m[nr] == m_new ? 1.f : __builtin_amdgcn_exp2f(m[nr] - m_new);
