@@ -185,3 +185,48 @@ def test_fp16_weights_that_are_small_but_many(device, dim, heavy, n, heads):
     err = (got.cpu().double() - out).abs()
     assert bool((err <= tol).all()), f"worst {float((err / tol).max())}"
     assert bool(((lse.cpu().double() - el).abs() <= ltol).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page,tokens", [(16, 1), (32, 3)])
+@pytest.mark.parametrize("drop", [-112.0, -20.0, 0.0])   # score of the loud page's tokens
+@pytest.mark.parametrize("apart", [4, 12, 15, 16, 20, 26, 33])
+@torch.no_grad()
+def test_fp16_pages_of_different_scales_in_one_tile(device, dim, page, tokens, drop, apart):
+    """A page of values up to fp16's largest beside pages 2^-apart of it: what those are worth in fp16
+    reaches the output. A weight w is rounded to half a step of fp16, or to within 2^-39 of the
+    largest (at most w); where it also takes a page's scale, to within 2^-25 of a value of at most 448
+    2^-15 units of 2^8, less the weights' 2^14: 2^-37. The output to half a step, 2^-25 if subnormal."""
+    n, loud = 150, 80                              # the loud page lies inside the second tile
+    pages = -(-n // page)
+    g = torch.Generator().manual_seed(apart)
+    cache = kv.empty_cache(pages, 1, dim, page, device=device)
+    kc = (torch.randn(pages, 1, page, dim, generator=g) * 100).clamp(-400, 400)
+    kc[..., 0] = 0.0
+    kc[loud // page, :, :, 0] = drop
+    vc = (torch.randn(pages, 1, dim, page, generator=g) * 100).clamp(-224, 224)
+    kc, vc = kc.to(torch.float8_e4m3fn), vc.to(torch.float8_e4m3fn)
+    ke = torch.zeros(pages, 1, dtype=torch.int64)
+    ve = torch.full((pages, 1), 8 - apart, dtype=torch.int64)
+    ve[loud // page] = 8
+    for to, x in ((cache.k_codes, kc), (cache.v_codes, vc)):
+        to.copy_(x.view(torch.uint8))
+    for to, e in ((cache.k_scales, ke), (cache.v_scales, ve)):
+        to.copy_((e + 127).to(torch.uint8))
+    k = (kc.double() * torch.exp2(ke.double())[..., None, None]).transpose(0, 1).flatten(1, 2)[0, :n, None]
+    v = (vc.double() * torch.exp2(ve.double())[..., None, None]).permute(1, 0, 3, 2).flatten(1, 2)[0, :n, None]
+    q = torch.randn(1, tokens, 2, dim, generator=g) * 0.004
+    q[..., 0] = 1.0
+    q = q.to(FP16)
+    got = kv.cache_attention(q.cuda(), cache, in_order(n, page).cuda(), ints(n), 1.0)
+    out, lse, mass, size = oc.attention(q[0], k, v, n - tokens, 1.0)
+    tol, _ = oc.bounds(out, mass, size, v, FP16, dim, n)
+    tol -= torch.finfo(FP16).tiny + n * 2.0 ** -25 * float(v.abs().max())
+    s = torch.einsum("ihd,jd->ihj", q[0].double(), k[:, 0])
+    s = s.masked_fill(torch.arange(n) > torch.arange(tokens)[:, None, None] + n - tokens, -math.inf)
+    w = torch.exp(s - lse[..., None])
+    tol += w.clamp_max(2.0 ** -39) @ v[:, 0].abs() + n * 2.0 ** -37 + 2.0 ** -25
+    err = (got[0].cpu().double() - out).abs()
+    assert bool((err <= tol).all()), f"worst {float((err / tol).max())}"
+    assert float(out.abs().max()) > 8 * 2.0 ** (8 - apart)       # the output is worth looking at
+    cache.check()

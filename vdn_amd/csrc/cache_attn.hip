@@ -366,6 +366,32 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
           vs = scale_of(c.vs, next.v);
         }
 
+        // ---- fp16: V's scales relative to the tile's largest one ----
+        // A code keeps all its bits down to 2^-15 of that (2^-9, the least, is then 2^-24); what a page is
+        // further below goes into its tokens' weights instead, which the lane holds with their V.
+        float weight = 1.f;
+        bool apart = false;
+        if (kF16) {
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+          // within what fp16 values ask for (2^-32 .. 2^16), so that no rescaling overflows
+          const float tile_scale = e8m0_scale(min(max(top, 127u - 32u), 127u + 16u));
+          if (tile_scale != unit_scale) {   // wave-uniform
+            const float f = unit_scale == 0.f ? 1.f : unit_scale / tile_scale;
+#pragma unroll
+            for (int nr = 0; nr < kNR; ++nr)
+#pragma unroll
+              for (int db = 0; db < kDB; ++db)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nr][db][i] *= f;
+            unit_scale = tile_scale;
+          }
+          const float below = v_scale / tile_scale;
+          v_scale = fmaxf(below, 0x1p-15f);
+          weight = fminf(below * 0x1p15f, 1.f);
+          apart = __any(weight < 1.f);
+        }
+
         // ---- softmax: scores times K's scale, running maximum in exp2 units ----
         const bool masked = tile0 + kTile > seen0;
         u32x4 pb[kNR][2];
@@ -402,30 +428,17 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
               sum += p[4 * t + i];
             }
           l[nr] += sum;                     // of this lane's keys; joined after the last tile
+          if (apart) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] *= weight;
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i) pb[nr][h][i] = E::pack(p[8 * h + 2 * i], p[8 * h + 2 * i + 1]);
         }
 
-        // ---- V: tail bytes to zero, scale ----
-        if (kF16) {
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-          // within what fp16 values ask for (2^-32 .. 2^16), so that no rescaling overflows
-          const float tile_scale = e8m0_scale(min(max(top, 127u - 32u), 127u + 16u));
-          if (tile_scale != unit_scale) {   // wave-uniform
-            const float f = unit_scale == 0.f ? 1.f : unit_scale / tile_scale;
-#pragma unroll
-            for (int nr = 0; nr < kNR; ++nr)
-#pragma unroll
-              for (int db = 0; db < kDB; ++db)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[nr][db][i] *= f;
-            unit_scale = tile_scale;
-          }
-          v_scale = v_scale / tile_scale;
-        }
+        // ---- V: tail bytes to zero ----
         if (tile0 + kTile > len) {
           const int n = len - (tile0 + 16 * g);
 #pragma unroll
