@@ -123,3 +123,27 @@ def test_fp16_weights_that_are_small_but_many(device, dim, block_rows, heavy):
         err = (got[a:b].cpu().double() - out).abs()
         assert bool((err <= tol).all()), f"rows {a}: worst {float((err / tol).max())}"
         assert bool(((lse[a:b].cpu().double() - el).abs() <= ltol).all())
+
+
+@pytest.mark.parametrize("dim,block_rows", VARIANTS)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@torch.no_grad()
+def test_the_output_over_its_queries(device, dim, block_rows, dtype):
+    """A workgroup has read its rows before it writes them: out = query gives what a fresh output
+    does, also as a column slice beside key and value. What others still read is refused."""
+    lengths, heads, kv_heads = [200, 1, 300], 6, 2
+    g = torch.Generator().manual_seed(6)
+    fused = torch.randn(510, heads + 2 * kv_heads, dim, generator=g).to(dtype).cuda()
+    q, k, v = fused.split((heads, kv_heads, kv_heads), 1)
+    plan = plan_of(lengths, heads, kv_heads, block_rows, device)
+    want = vc.causal_attention(q, k, v, plan)
+    rest = q[501:].clone()
+    for out in (fused[:, 1:7], fused[:, 3:9], fused[:, 4:10]):
+        with pytest.raises(ValueError, match="overlap"):
+            vc.causal_attention(q, k, v, plan, out=out)
+    with pytest.raises(ValueError, match="itself"):
+        vc.causal_attention(q, k, v, plan, out=torch.zeros(510 * heads * dim, dtype=dtype, device=device)
+                            .as_strided((510, heads, dim), (dim * (heads - 1), dim, 1)))
+    assert torch.equal(vc.causal_attention(q, k, v, plan), want)      # nothing was written
+    got = vc.causal_attention(q, k, v, plan, out=q)
+    assert got is q and torch.equal(q[:501], want[:501]) and torch.equal(q[501:], rest)

@@ -230,3 +230,27 @@ def test_fp16_pages_of_different_scales_in_one_tile(device, dim, page, tokens, d
     assert bool((err <= tol).all()), f"worst {float((err / tol).max())}"
     assert float(out.abs().max()) > 8 * 2.0 ** (8 - apart)       # the output is worth looking at
     cache.check()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, BF16), (256, BF16)])
+@pytest.mark.parametrize("n", [400, 6000])             # whole units, split ones
+@torch.no_grad()
+def test_the_output_over_its_queries(device, dim, dtype, n):
+    """out = query gives what a fresh output does; another overlap is refused."""
+    cache = kv.empty_cache(-(-n // 16), 2, dim, 16, device=device)
+    table = in_order(n, 16).cuda().repeat(3, 1)
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, 2, dim, generator=g).to(dtype).cuda()
+    kv.write_cache(cache, x, -x, table[:1], ints(0), ints(0, n))
+    q = torch.randn(3, 5, 20, dim, generator=g).to(dtype).cuda()
+    lengths = ints(n, n - 7, 3)
+    want = kv.cache_attention(q, cache, table, lengths)
+    part, pwant = q.clone()[:, :, 4:10], kv.cache_attention(q[:, :, 4:10], cache, table, lengths)
+    with pytest.raises(ValueError, match="overlap"):
+        kv.cache_attention(q[:, :4], cache, table, lengths, out=q[:, 1:])
+    with pytest.raises(ValueError, match="itself"):
+        kv.cache_attention(q, cache, table, lengths, out=q.as_strided(q.shape, (4 * 20 * dim, 20 * dim, dim, 1)))
+    assert torch.equal(kv.cache_attention(q, cache, table, lengths), want)
+    for queries, result in ((q, want), (part, pwant)):
+        got = kv.cache_attention(queries, cache, table, lengths, out=queries)
+        assert got is queries and torch.equal(queries, result)

@@ -14,6 +14,7 @@ import os
 import threading
 
 import torch
+import numpy as np
 
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libvdnmi.so")
 
@@ -194,3 +195,67 @@ def raw_stream(device_index: int) -> int:
 def require_gpu(t: torch.Tensor, what: str) -> None:
     if t.device.type != "cuda":
         raise ValueError(f"{what} must be a CUDA (HIP) tensor")
+
+
+def _reach(t: torch.Tensor, first_dim: int = 0) -> int:
+    """Elements from a view's first one up to behind its last one, of its dimensions from first_dim on."""
+    return 1 + sum((n - 1) * s for n, s in zip(t.shape[first_dim:], t.stride()[first_dim:]))
+
+
+def _starts(t: torch.Tensor, dims) -> np.ndarray:
+    """Where the runs of a view's last dimension begin, over the given dimensions."""
+    at = np.zeros(1, dtype=np.int64)
+    for i in dims:
+        at = (at[:, None] + t.stride(i) * np.arange(t.shape[i])).ravel()
+    return at
+
+
+def overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether elements of a view (unit last stride) share memory."""
+    reach = 1
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s < reach:       # its dimensions do not nest, as those of slices of a dense tensor do
+            return bool((np.diff(np.sort(_starts(t, range(t.ndim - 1)))) < t.shape[-1]).any())
+        reach += (n - 1) * s
+    return False
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two views of rows (unit last stride, as long in both) share memory. Where that would be
+    long to tell (rows of different strides in ranges that cross, rows of very many interleaved
+    runs) they are taken not to."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    if apart >= _reach(a) or -apart >= _reach(b):
+        return False
+    row = a.stride(0)
+    if b.stride(0) != row or row == 0:
+        return False
+    wide_a, wide_b, column = _reach(a, 1), _reach(b, 1), apart % row
+    if column >= wide_a and column + wide_b <= row:     # slices beside each other
+        return False
+    # runs that lie less than a run's length apart, in some row of a and the k-th one behind it in b
+    dims = range(1, a.ndim - 1)
+    if a[0].numel() * b[0].numel() > a.shape[-1] ** 2 << 20:
+        return False
+    delta = apart + _starts(b, dims)[None] - _starts(a, dims)[:, None]
+    k = -((delta + a.shape[-1] - 1) // row)             # the least k with delta + k row > -length
+    k = np.maximum(k, 1 - a.shape[0])
+    return bool(((delta + k * row < a.shape[-1]) & (k < b.shape[0])).any())
+
+
+def check_attention_out(out: torch.Tensor, query: torch.Tensor, *sources: torch.Tensor) -> None:
+    """Refuses a caller's `out` whose elements share memory, or that lies over what other workgroups
+    still read: the sources, or the query unless it is the query itself (a workgroup writes the
+    rows that it has read)."""
+    if not out.is_contiguous() and overlaps_itself(out):
+        raise ValueError("out must not overlap itself")
+    storage = out.untyped_storage().data_ptr()
+    for x in sources:
+        if x.untyped_storage().data_ptr() == storage and overlap(out, x):
+            raise ValueError("out must not overlap key or value")
+    if query.untyped_storage().data_ptr() == storage \
+            and (out.data_ptr() != query.data_ptr() or out.stride() != query.stride()) \
+            and overlap(out, query):
+        raise ValueError("out may be the query itself, but must not overlap it otherwise")

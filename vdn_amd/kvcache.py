@@ -219,6 +219,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     (or [batch, H]). Scores, sums and the output are accumulated in fp32; probabilities are
     rounded to the query's dtype before the product with V, the codes' values are exact.
 
+    `out` may be the query itself; it must not overlap it otherwise, nor itself, nor the cache.
+
     A sequence with a bad page id or length gets NaN (see KVCache.check). For FP16 queries
     the cached values must be within FP16's range; an output that E4M3's rounding takes over its
     largest value is that value."""
@@ -252,6 +254,8 @@ def cache_attention(query, cache: KVCache, table, lengths, scale=None, *, return
     elif (out.shape != query.shape or out.dtype is not dtype or out.get_device() != index
           or out.stride(-1) != 1 or 0 in out.stride()):
         raise ValueError("out must be a view like the query, unit channel stride, no broadcast")
+    else:
+        _lib.check_attention_out(out, query)
     o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
     lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=query.device) if return_lse else None
     group = heads // kv_heads
