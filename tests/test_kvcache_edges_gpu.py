@@ -8,6 +8,8 @@ from oracle import causal as oc
 from oracle import kvcache as ok
 from vdn_amd import kvcache as kv
 
+from test_kvcache_gpu import check, filled, tables
+
 pytestmark = pytest.mark.gpu
 
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -254,3 +256,62 @@ def test_the_output_over_its_queries(device, dim, dtype, n):
     for queries, result in ((q, want), (part, pwant)):
         got = kv.cache_attention(queries, cache, table, lengths, out=queries)
         assert got is queries and torch.equal(queries, result)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16), (256, BF16)])
+@torch.no_grad()
+def test_codes_behind_the_end_stay(device, page, dim, dtype):
+    """What a write leaves of a page that it fills in part, for ends at, before and behind multiples of 16
+    and 4: every code behind the end, but that a run of 16 V codes which holds earlier tokens is
+    rounded again with them when the scale grows."""
+    g = torch.Generator().manual_seed(page + dim)
+    for held, new in ((0, 1), (0, 16), (0, page - 16), (3, 1), (5, 4), (16, 16), (page // 2, 2), (7, 9),
+                      (page // 2 + 1, page // 4), (page - 3, 2)):
+        n = held + new
+        if not 0 < new or n > page:
+            continue
+        for growth in (0.01, 100.0):
+            cache = kv.empty_cache(3, 2, dim, page, device=device)
+            for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales):
+                t.copy_(torch.randint(0, 120, t.shape, generator=g))
+            table = ints(1)[None]
+            x = torch.randn(max(held, 1), 4, dim, generator=g).to(dtype).cuda()
+            if held:
+                kv.write_cache(cache, x[:, :2], x[:, 2:], table, ints(0), ints(0, held))
+            k0, v0, ks0, vs0 = (t.clone() for t in (cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales))
+            y = (torch.randn(new, 4, dim, generator=g) * growth).to(dtype).cuda()
+            kv.write_cache(cache, y[:, :2], y[:, 2:], table, ints(held), ints(0, new))
+            assert torch.equal(cache.k_codes[1, :, n:], k0[1, :, n:])
+            # the runs that begin in front of the first new token are rounded again where V's scale grew
+            again = -(-held // 16) * 16 if held else 0
+            assert torch.equal(cache.v_codes[1, :, :, max(n, again):], v0[1, :, :, max(n, again):]), (held, new)
+            for u in range(2):
+                grew = held and int(cache.v_scales[1, u]) != int(vs0[1, u])
+                assert not held or bool(grew) == (growth > 1)
+                if not grew:
+                    assert torch.equal(cache.v_codes[1, u, :, n:], v0[1, u, :, n:]), (held, new)
+                    assert torch.equal(cache.v_codes[1, u, :, :held], v0[1, u, :, :held])
+            for p in (0, 2):
+                assert torch.equal(cache.k_codes[p], k0[p]) and torch.equal(cache.v_codes[p], v0[p])
+                assert torch.equal(cache.k_scales[p], ks0[p]) and torch.equal(cache.v_scales[p], vs0[p])
+    cache.check()
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, BF16), (256, BF16)])
+@pytest.mark.parametrize("tokens,heads,kv_heads", [(33, 4, 2), (130, 5, 1), (256, 4, 4), (700, 2, 1)])
+@torch.no_grad()
+def test_many_queries(device, dim, dtype, tokens, heads, kv_heads):
+    """A piece of a prompt behind cached tokens: more queries than a row block, lengths around them (some
+    queries then see nothing), whole and split units."""
+    lengths = [tokens, tokens + 1, 700 + tokens, 0, tokens // 2, 3000]
+    table, pages = tables([-(-n // 64) for n in lengths], seed=dim)
+    cache, kval, vval = filled(pages, kv_heads, dim, 64, seed=heads)
+    q = torch.randn(len(lengths), tokens, heads, dim, generator=torch.Generator().manual_seed(tokens))
+    q = q.to(dtype).cuda()
+    out, lse = kv.cache_attention(q, cache, table.cuda(), ints(*lengths), return_lse=True)
+    check(q, cache, kval, vval, table, lengths, out, lse)
+    assert out[3].count_nonzero() == 0
+    short = kv.cache_attention(q[:1], cache, table[:1, :-(-tokens // 64)].cuda(), ints(tokens))
+    check(q[:1], cache, kval, vval, table[:1], lengths[:1], short)
+    cache.check()
