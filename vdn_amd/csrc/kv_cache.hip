@@ -86,12 +86,11 @@ __device__ Piece find_piece(const KvCache& c, const Seqs& s, int rows, int slot)
     const int behind = s.offsets[s.batch];
     int lo = 0, step = 1;
     while (static_cast<int64_t>(step) * 64 < s.batch) step *= 64;
-    if (step > 1 && blockIdx.x == 0) {
-      // the search loads only a part of the offsets, and may pass over a pair that falls
-      bool bad = false;
-      for (int i = threadIdx.x; i < s.batch; i += blockDim.x)
-        bad |= bad_offsets(s.offsets[i], s.offsets[i + 1], i, rows);
-      if (bad) *c.faults = 1;
+    if (step > 1) {
+      // The search loads only a part of the offsets and may pass over a pair that falls, so the threads
+      // of the grid look at one pair each (there are more of them than sequences).
+      const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+      if (i < s.batch && bad_offsets(s.offsets[i], s.offsets[i + 1], static_cast<int>(i), rows)) *c.faults = 1;
     }
     for (; step > 1; step /= 64) {
       const int64_t i = lo + static_cast<int64_t>(lane) * step;
