@@ -48,10 +48,10 @@ def _launch(plan, head_dim):
 # When head dim 128 takes 256-row blocks (8 waves, one workgroup a CU) instead of 128-row ones (two
 # of 4 waves): a K/V tile then serves twice the rows, which pays where rows see many keys, and a
 # block takes the CU to itself, so that there have to be enough of them. Microseconds of 256 and
-# 128 rows, 32 heads and 8 K/V heads: 32768 tokens 7360, 8000; 8192: 491, 520; 4096: 146, 152 (the
-# mean row sees 2048 keys); 4 x 2048: 165, 161; 2048: 58, 52; 24 prompts of 77 - 1200 with 56 heads
-# 148, 120. 8 heads that share one K/V head: 16384 tokens, 512 blocks: 480, 549; 8192, 256 blocks:
-# 195, 183.
+# 128 rows, 32 heads and 8 K/V heads: 32768 tokens 7285, 7630; 8192: 485, 485; 4096: 131, 138 (the
+# mean row sees 2048 keys); 4 x 2048: 151, 142; 2048: 55, 45; 24 prompts of 77 - 1200 with 56 heads
+# 140, 111. 8 heads that share one K/V head: 16384 tokens, 512 blocks: 467, 519; 8192, 256 blocks:
+# 186, 160.
 WIDE_MEAN_KEYS = 2048
 WIDE_LEAST_BLOCKS = 512    # two for each of 256 CUs
 
@@ -104,7 +104,8 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
     query [rows, H, D], key and value [rows, Hkv, D] (BF16 or FP16, D 64, 128 or 256, unit
     channel stride, rows >= plan.rows; any token and head strides that keep 16-byte alignment);
     query head h reads K/V head h // (H / Hkv). Returns [rows, H, D] of the same dtype, scores
-    and sums in fp32, probabilities rounded to the activation dtype before the product with V;
+    and sums in fp32 (within whose range |V| times 256 times the tokens has to stay), probabilities
+    rounded to the activation dtype before the product with V;
     with return_lse also the natural-log sum of exp of the scaled scores, fp32 [rows, H].
     Rows behind the plan's last sequence are zero (LSE -inf); in a caller's `out` they are left
     as they were. `out` may be the query itself; it must not overlap key, value or itself. Values of tokens that a row does not see never reach it, nonfinite ones

@@ -16,7 +16,13 @@
 //     page, and Pᵀ's operand layout, so P stays in registers too.
 // E4M3 codes widen to 16 bits exactly. K's scale multiplies the scores, in fp32 (a lane's 16 keys
 // lie in one page). V's goes into the widening: bf16 holds every code's value; for fp16 it is
-// taken relative to the tile's largest one, and O is kept in units of that.
+// taken relative to the tile's largest one, and O is kept in units of that. P is rounded to 16 bits,
+// the MFMA's operand; its sum keeps fp32.
+//
+// Each 16 or 32 rows read and widen all codes of their K/V head again. For the few rows of a decode step
+// that is one reading; many queries (a piece of a prompt behind cached tokens) pay for it in VALU work: 256
+// behind 8192 tokens, 40 heads on 8 x 128, 40 row blocks: 119 us, VALU busy 54% and MFMA 15% of the
+// time, where the products alone ask for 33.
 //
 // Work: a quad is 256 tokens (one tile for each of a workgroup's 4 waves) of one (sequence, row
 // block, K/V head) unit. The quads of all units in order, and one more for each unit, are shared

@@ -10,10 +10,13 @@
 // Per tile of kBN keys, as the frame-window kernel: Sᵀ = K Qᵀ on 32x32x16 MFMAs with Q in
 // registers, online softmax in the exp2 domain (fp32 maximum and sum per row), and Oᵀ += Vᵀ Pᵀ,
 // where Pᵀ is the Sᵀ accumulator itself and Vᵀ comes from the token-major V tile by transpose
-// reads. Tiles stream global -> LDS, double-buffered. MFMA bounds long prompts, with the softmax beside it
-// (59 and 51% of the time busy, the clock at 1.9 GHz by the power limit): 32768 tokens, 32 heads on 8
-// x 128, 7.4 - 7.7 ms, 1140 - 1190 TFLOP/s, 87% of a large library product. Short ones are bound by reading Q, writing
-// O and the latency around the tiles: 24 prompts of 77 - 1200 tokens, 56 heads, 120 us.
+// reads. P is rounded to 16 bits, the MFMA's operand, while its sum keeps fp32: errors of half a step
+// each, which the sum over the keys averages (outputs within 2.1e-3 relative of 64 bits in bf16, where the
+// output's own rounding makes 1.6e-3; 2.3e-4 and 2.0e-4 in fp16). Tiles stream global -> LDS,
+// double-buffered. MFMA bounds long prompts, with the softmax beside it
+// (63 and 49% of the time busy, the clock at 1.9 GHz by the power limit): 32768 tokens, 32 heads on 8
+// x 128, 7.3 ms, 1200 TFLOP/s, 90% of a large library product. Short ones are bound by reading Q, writing
+// O and the latency around the tiles: 24 prompts of 77 - 1200 tokens, 56 heads, 121 us.
 //
 // A nonfinite V value of a token that a row does not see must not reach that row, and 0 inf is
 // NaN in an MFMA. Only tiles on the diagonal hold such tokens: there every wave looks its share
@@ -469,10 +472,11 @@ VDN_API int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, cons
                     static_cast<const uint16_t*>(v), q_st, q_sh, k_st, k_sh, v_st, v_sh};
   const CausalOut to{static_cast<uint16_t*>(out), lse, o_st, o_sh, l_st, l_sh};
   // An XCD's heads all at once finish evenly, but their K/V no longer fits the L2: that pays as long
-  // as all K/V fits the 256 MB cache behind it. At once against one after the other, tokens x heads
-  // of their own x 128, us: 2048 x 32 55, 68; 4096 x 32 145, 190; 4096 x 56 253, 283; 8192 x 56 943,
-  // 1029; 16384 x 32 (256 MB) 2000, 2070; 4 x 4096 x 56 1200, 1055; 32768 x 32 8390, 7850. Of many
-  // short prompts 24 x 77 - 1200 x 16 47.6, 48.7, but 16 x 512 x 32 74.6, 69.5.
+  // as all K/V fits the 256 MB cache behind it (a sequence's last block is counted in full). At once
+  // against one after the other, tokens x heads of their own x 128, us: 2048 x 32 50, 59; 4096 x 32 138,
+  // 181; 4096 x 56 241, 275; 8192 x 56 892, 987; 16384 x 32 (256 MB) 1932, 2014; 4 x 4096 x 56 1156,
+  // 1016; 32768 x 32 8240, 7825. Many short prompts, which share little, do not follow the rule: 24 x 77 -
+  // 1200 x 16 43, 42; 16 x 512 x 32 70, 65.
   const int64_t kv_bytes = static_cast<int64_t>(nblocks) * block_rows / group * head_dim * 4 * kv_heads;
   const int together = kv_heads % 8 == 0 && kv_bytes <= (256ll << 20) ? kv_heads / 8 : 1;
   const int ceil_log2 = group > 1 ? 32 - __builtin_clz(static_cast<unsigned>(group - 1)) : 0;

@@ -23,8 +23,8 @@ struct KvCache {
   int pages, kv_heads, log_page;
 };
 
-// Scales start at 2^-100: 2^e and every code's value then are normal in fp32 and bf16. Values
-// under 448 * 2^-100 keep an absolute error of 2^-110.
+// Scales start at 2^-100: 2^e and every code's value then are normal in fp32 and bf16. Below that a
+// page's values are rounded as E4M3 numbers times 2^-100: by 2^-4 relative, under 2^-106 by 2^-110.
 constexpr uint32_t kLeastScaleByte = 27;
 
 // Scale byte of a block from its largest finite magnitude: the least e with amax <= 448 * 2^e.
