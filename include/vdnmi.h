@@ -332,7 +332,7 @@ int vdn_window_attention(const void* q, int64_t q_st, int64_t q_sh, const void* 
  * sequence, its tokens, first row of the block, unused). q, k, v, out addressed by (token, head)
  * strides (multiples of 8 elements, unit channel stride, 16-byte aligned); K/V token strides up
  * to 2^22. lse (nullable): fp32 natural-log sum-exp of the scaled scores. Only the rows of
- * the blocks are written.
+ * the blocks are written. out may be q, and must not overlap it otherwise, nor k or v.
  */
 int vdn_causal_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
                          int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,

@@ -133,8 +133,8 @@ __device__ __forceinline__ uint16_t f32_to_f16_bits(float f) {
 // A finite value beyond fp16's largest one becomes that: for results that the exact arithmetic
 // keeps in range. Infinities and NaN stay.
 __device__ __forceinline__ float f16_in_range(float f) {
-  const float a = fabsf(f);
-  return a > 65504.f && a < INFINITY ? copysignf(65504.f, f) : f;
+  constexpr int kNanOrInf = 0x207;   // v_cmp_class: NaN, both infinities
+  return __builtin_amdgcn_classf(f, kNanOrInf) ? f : __builtin_amdgcn_fmed3f(f, -65504.f, 65504.f);
 }
 
 __device__ __forceinline__ float round_f16(float f) {

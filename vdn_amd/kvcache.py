@@ -194,7 +194,7 @@ def read_cache(cache: KVCache, table, starts, offsets, rows, *, dtype=torch.bflo
     fresh [rows, kv_heads, D] tensors (keys, values) are the tokens starts[i], ... of sequence i
     (arguments as write_cache). Exact in BF16; FP16 rounds what is under its normal range and
     saturates at 65504. Rows of a page that is not there are NaN, rows from offsets[batch] on
-    zero."""
+    zero; rows of offsets that are not followed may hold anything."""
     index, args = _check_cache(cache, "read_cache")
     if type(rows) is not int or rows < 0:
         raise ValueError("rows must be a non-negative integer")
