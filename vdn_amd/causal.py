@@ -108,8 +108,9 @@ def causal_attention(query, key, value, plan: CausalPlan, scale=None, *, return_
     rounded to the activation dtype before the product with V;
     with return_lse also the natural-log sum of exp of the scaled scores, fp32 [rows, H].
     Rows behind the plan's last sequence are zero (LSE -inf); in a caller's `out` they are left
-    as they were. `out` may be the query itself; it must not overlap key, value or itself. Values of tokens that a row does not see never reach it, nonfinite ones
-    included; a nonfinite value that it sees makes its channel nonfinite."""
+    as they were. `out` may be the query itself; it must not overlap it otherwise, nor key, value or
+    itself. Values of tokens that a row does not see never reach it, nonfinite ones included; a
+    nonfinite value that it sees makes its channel nonfinite."""
     if torch.is_grad_enabled():
         raise RuntimeError("causal attention is inference-only; use no_grad/inference_mode")
     if not isinstance(plan, CausalPlan):

@@ -9,8 +9,9 @@ The caller owns the pool's bookkeeping: an int32 table [batch, width] names each
 in order, an int32 tensor the tokens that it holds. Both stay on the device, so that a decode step
 can be captured into a graph and replayed as they change. A page id outside the pool, a
 length that the table cannot hold, offsets that fall or do not fit the rows: kernels follow none of
-them; they raise the cache's `faults` word, and KVCache.check() reports it. (Around bad offsets
-other sequences of that call may be left out too.)
+them; they raise the cache's `faults` word, and KVCache.check() reports it. Around bad offsets
+other sequences of that call may be left out too, or, among more than 64, rows that falling offsets
+name twice moved twice.
 """
 from __future__ import annotations
 
