@@ -307,6 +307,21 @@ int vdn_qk_rmsnorm_rope(const void* q, int64_t q_st, int64_t q_sh, int64_t q_sd,
                         void* stream);
 
 /*
+ * Rotation of q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (dtype 0 bf16, 1 fp16; head_dim
+ * 64, 128 or 256; (token, head) strides, multiples of 4, 8-byte aligned) by their tokens' positions (int32, or
+ * int64 with wide_positions; any values). Pair j of the first rot channels (a multiple of 8), channels (j, j +
+ * rot / 2) or (interleaved) (2 j, 2 j + 1), turns by positions[t] * steps[j] / 2^64 turns (uint64 arithmetic,
+ * modulo 2^64) and is multiplied by amplitude. q_w, k_w (each nullable; [head_dim] of the activation
+ * dtype, or fp32 with w_f32): in front of it x * rsqrt(mean(x^2) + eps) * w over the head. fp32, one rounding.
+ * qo and ko may be q and k with the same strides, and must not overlap them otherwise.
+ */
+int vdn_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+               const void* q_w, const void* k_w, int w_f32, float eps, const void* positions,
+               int wide_positions, const void* steps, int rot, int interleaved, float amplitude,
+               int64_t tokens, int heads, int kv_heads, int head_dim, int dtype, void* qo,
+               int64_t qo_st, int64_t qo_sh, void* ko, int64_t ko_st, int64_t ko_sh, void* stream);
+
+/*
  * Exact softmax attention of query blocks over key intervals (dtype 0: bf16, 1: fp16; head_dim
  * 64, 128 or 256): blocks int32 [nblocks, 3] = (first query, end of its query range, group),
  * <= 256 queries each; grp_kv int32 [groups, 8, 2] key intervals [a, b); grp_n int32 [groups].
