@@ -402,6 +402,41 @@ int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                         void* workspace, int64_t workspace_bytes, void* stream);
 int vdn_cache_attention_workspace(int tokens, int group, int head_dim, int64_t* bytes);
 
+/*
+ * vdn_cache_attention of one token of each sequence with a table for each K/V head: tables int32 [batch,
+ * kv_heads, width] (strides table_sb, table_sh). lengths, workspace and the rest as there, with tokens = 1.
+ */
+int vdn_cache_attention_heads(const void* q, int64_t q_sb, int64_t q_sh, const void* k_codes,
+                              const void* k_scales, const void* v_codes, const void* v_scales,
+                              int* faults, int pages, int kv_heads, int page, int head_dim,
+                              const int* tables, int64_t table_sb, int64_t table_sh, int batch,
+                              int width, const int* lengths, int group, int dtype, float scale,
+                              void* out, int64_t o_sb, int64_t o_sh, float* lse, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/*
+ * vdn_cache_means: means [pages, kv_heads, head_dim] bf16 (16-byte aligned): the mean key, rounded once, of
+ * every page that holds tokens starts[b] .. lengths[b] - 1 of a sequence, over its tokens in front of
+ * lengths[b]. Other pages' means stay. Sequences with a negative start or a bad length are left out, *faults 1.
+ *
+ * vdn_cache_select: for query i of sequence b and K/V head u the `count` pages that score highest, of
+ * those with tokens in front of lengths[b] - tokens + 1 + i: the largest q . mean (in fp64) over the group's
+ * heads; the first `first` and the last `last` (>= 1) pages before all others, NaN as +inf, of equal ones
+ * the one in front. selected int32 [batch, tokens, kv_heads, count]: their ids in the table's order, -1
+ * behind them; seen int32 [batch, tokens]: the tokens in them, -1 for a bad length (*faults 1). A page id that
+ * the pool does not have is selected before scored ones. q as vdn_cache_attention. workspace: 8-byte aligned,
+ * vdn_cache_select_workspace's byte count (may be 0), its contents need no preparation.
+ */
+int vdn_cache_means(const void* k_codes, const void* k_scales, int* faults, int pages, int kv_heads,
+                    int page, int head_dim, const int* table, int64_t table_st, int batch, int width,
+                    const int* starts, const int* lengths, void* means, void* stream);
+int vdn_cache_select(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* means,
+                     int* faults, int pages, int kv_heads, int page, int head_dim, const int* table,
+                     int64_t table_st, int batch, int width, const int* lengths, int tokens, int group,
+                     int dtype, int count, int first, int last, int* selected, int* seen,
+                     void* workspace, int64_t workspace_bytes, void* stream);
+int vdn_cache_select_workspace(int batch, int tokens, int kv_heads, int width, int64_t* bytes);
+
 /* vdn_window_attention with the output quantized in the epilogue instead of stored as bf16:
  * query row q, head h -> MXFP8 codes[q, 128 (chunk0 + h) .. +128) of a [rows, kp] code
  * matrix and the four E8M0 scales of that chunk in its SWIZZLE_32_4_4 scale array; the same

@@ -78,6 +78,15 @@ SIGNATURES = {
                             _i32, _i32, _ptr, _i64, _i32, _i32, _ptr, _i32, _i32, _i32, _f32,
                             _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr],
     "vdn_cache_attention_workspace": [_i32, _i32, _i32, _ptr],
+    "vdn_cache_attention_heads": [_ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i32, _i32, _i32,
+                                  _i32, _ptr, _i64, _i64, _i32, _i32, _ptr, _i32, _i32, _f32, _ptr,
+                                  _i64, _i64, _ptr, _ptr, _i64, _ptr],
+    "vdn_cache_means": [_ptr, _ptr, _ptr, _i32, _i32, _i32, _i32, _ptr, _i64, _i32, _i32, _ptr,
+                        _ptr, _ptr, _ptr],
+    "vdn_cache_select": [_ptr, _i64, _i64, _i64, _ptr, _ptr, _i32, _i32, _i32, _i32, _ptr, _i64,
+                         _i32, _i32, _ptr, _i32, _i32, _i32, _i32, _i32, _i32, _ptr, _ptr, _ptr,
+                         _i64, _ptr],
+    "vdn_cache_select_workspace": [_i32, _i32, _i32, _i32, _ptr],
     "vdn_vda_readout_mxfp8": [_ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _i32, _f32, _ptr, _i64,
                               _i64, _i64, _ptr, _ptr, _i64, _i32, _i32, _i32, _i32, _ptr],
     "vdn_vda_readout_gated": [_ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _i32, _f32, _ptr, _i64,

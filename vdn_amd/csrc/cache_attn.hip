@@ -70,7 +70,7 @@ struct Queries {
 struct Lengths {
   const int* table;
   const int* lengths;
-  int64_t t_st;
+  int64_t t_st, t_sh;   // sequence / K/V head strides of the table (0: one row for all heads)
   int batch, width;
 };
 
@@ -266,7 +266,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
     }
     if (qb <= qa) continue;
     const int u = unit % c.kv_heads, r_block = (unit / c.kv_heads) * kRows;
-    const int* table = s.table + b_now * s.t_st;
+    const int* table = s.table + b_now * s.t_st + u * s.t_sh;
     const int seen0 = len - io.tokens + 1;   // keys that the first of the Q tokens sees
 
     // ---- Q: row r_block + 16 nr + row16, channels 64 j + 16 g + 8 s .. + 8 ----
@@ -707,14 +707,14 @@ VDN_API int vdn_cache_attention_workspace(int tokens, int group, int head_dim, i
   return kOk;
 }
 
-VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
-                                const void* k_codes, const void* k_scales, const void* v_codes,
-                                const void* v_scales, int* faults, int pages, int kv_heads, int page,
-                                int head_dim, const int* table, int64_t table_st, int batch,
-                                int width, const int* lengths, int tokens, int group, int dtype,
-                                float scale, void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
-                                float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
-  const char* name = "vdn_cache_attention";
+namespace {
+
+int cache_attention(const char* name, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                    const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                    int* faults, int pages, int kv_heads, int page, int head_dim, const int* table,
+                    int64_t table_st, int64_t table_sh, int batch, int width, const int* lengths, int tokens,
+                    int group, int dtype, float scale, void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                    float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
   const KvCache c{static_cast<uint8_t*>(const_cast<void*>(k_codes)),
                   static_cast<uint8_t*>(const_cast<void*>(k_scales)),
                   static_cast<uint8_t*>(const_cast<void*>(v_codes)),
@@ -751,7 +751,7 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
   }
   const Queries io{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lse, q_sb, q_st, q_sh,
                    o_sb, o_st, o_sh, tokens, group};
-  const Lengths s{table, lengths, table_st, batch, width};
+  const Lengths s{table, lengths, table_st, table_sh, batch, width};
   if (batch * (unit_quads + kUnitCost) > (1ll << 31) - 1) return set_error(kUnsupported, "%s: too many tokens", name);
   const int64_t join_rows = rows * kv_heads * batch;
   const auto launch = [&](auto main, auto join1, auto join4) {
@@ -779,4 +779,30 @@ VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64
 #undef VDN_CACHE_D
 #undef VDN_CACHE
   return check_launch(name);
+}
+
+}  // namespace
+
+VDN_API int vdn_cache_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                const void* k_codes, const void* k_scales, const void* v_codes,
+                                const void* v_scales, int* faults, int pages, int kv_heads, int page,
+                                int head_dim, const int* table, int64_t table_st, int batch,
+                                int width, const int* lengths, int tokens, int group, int dtype,
+                                float scale, void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                                float* lse, void* workspace, int64_t workspace_bytes, void* stream) {
+  return cache_attention("vdn_cache_attention", q, q_sb, q_st, q_sh, k_codes, k_scales, v_codes, v_scales, faults,
+                         pages, kv_heads, page, head_dim, table, table_st, 0, batch, width, lengths, tokens, group,
+                         dtype, scale, out, o_sb, o_st, o_sh, lse, workspace, workspace_bytes, stream);
+}
+
+VDN_API int vdn_cache_attention_heads(const void* q, int64_t q_sb, int64_t q_sh, const void* k_codes,
+                                      const void* k_scales, const void* v_codes, const void* v_scales,
+                                      int* faults, int pages, int kv_heads, int page, int head_dim,
+                                      const int* tables, int64_t table_sb, int64_t table_sh, int batch, int width,
+                                      const int* lengths, int group, int dtype, float scale, void* out,
+                                      int64_t o_sb, int64_t o_sh, float* lse, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  return cache_attention("vdn_cache_attention_heads", q, q_sb, 0, q_sh, k_codes, k_scales, v_codes, v_scales,
+                         faults, pages, kv_heads, page, head_dim, tables, table_sb, table_sh, batch, width, lengths,
+                         1, group, dtype, scale, out, o_sb, 0, o_sh, lse, workspace, workspace_bytes, stream);
 }

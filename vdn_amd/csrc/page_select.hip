@@ -1,0 +1,458 @@
+// Mean keys of the 8-bit cache's pages, and the pages that a query's attention is limited to by them.
+//
+// Means (vdn_cache_means): mean[p, u] = sum over the page's tokens of K, / n, rounded once to bf16.
+// E4M3 values are multiples of 2^-9 up to 448, so 64 of them add up exactly in fp32: a lane's share of any
+// page. The lanes' sums meet in fp64. Reading the codes bounds it.
+//
+// Selection (vdn_cache_select): score(b, i, u, p) = max over the G query heads h of K/V head u of
+// q[b, i, h] . mean[p, u], in fp64: the products of 16-bit values are exact there and their sum nearly,
+// so that the order of two pages does not hang on the order of a sum. On 16x16x4 MFMAs with
+// the query rows as A and 16 pages as B, the maximum over the rows is over a lane's
+// four accumulators and the four lanes of its column. A page of the first or the last ones counts as
+// the largest, NaN as +inf. Of equal scores the page in front wins. Then a workgroup per (b, i, u)
+// takes the `count` best: by each page's rank, or where they are many by radix selection on the
+// scores' bits.
+#include "kv_cache.h"
+
+#include "attn_tiles.h"
+
+#include <algorithm>
+
+namespace vdn {
+namespace {
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kTakeThreads = 1024;   // of a selection from many scored pages
+
+struct Spans {
+  const int* table;    // [batch, width], row stride t_st
+  const int* starts;   // [batch]
+  const int* lengths;  // [batch]
+  int64_t t_st;
+  int batch, width;
+};
+
+__device__ __forceinline__ int most_tokens(const KvCache& c, int width) {
+  return static_cast<int>(min(static_cast<int64_t>(width) << c.log_page, (1ll << 31) - 1));
+}
+
+// Pages first .. first + n - 1 of sequence b; a bad length or start raises the fault word, and none
+// of its pages is followed.
+struct Span {
+  int first, n, tokens;
+};
+
+__device__ __forceinline__ Span span_of(const KvCache& c, const Spans& s, int b) {
+  const int start = s.starts[b], len = s.lengths[b];
+  if (start < 0 || len < 0 || len > most_tokens(c, s.width)) {
+    *c.faults = 1;
+    return Span{0, 0, 0};
+  }
+  const int first = start >> c.log_page, end = (len + (1 << c.log_page) - 1) >> c.log_page;
+  return Span{first, start < len ? end - first : 0, len};
+}
+
+template <int kD>
+__global__ void __launch_bounds__(kThreads) page_means_kernel(KvCache c, Spans s, uint16_t* means) {
+  constexpr int kChunks = kD / 16;          // lanes of a token's row
+  constexpr int kRows = 64 / kChunks;       // tokens at a time
+  constexpr int kCh = kD / 64;              // channels that a lane finishes
+  __shared__ float s_part[kWaves][kRows][kD];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int page = 1 << c.log_page;
+
+  // Pages of all sequences in order, 64 strips of sequences at a time.
+  const int strip = (s.batch + 63) / 64;
+  const int b0 = min(lane * strip, s.batch), b1 = min(b0 + strip, s.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += span_of(c, s, b).n;
+  int64_t incl = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t other = __shfl_up(incl, d);
+    incl += lane >= d ? other : 0;
+  }
+  const int64_t total = __shfl(incl, 63) * c.kv_heads;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWaves;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWaves + wave; item < total; item += stride) {
+    const int64_t at = item / c.kv_heads;
+    const int u = static_cast<int>(item - at * c.kv_heads);
+    const int owner = __popcll(__ballot(incl <= at));
+    int64_t before = __shfl(incl - mine, owner);
+    int b = __builtin_amdgcn_readlane(b0, owner);
+    Span span = span_of(c, s, b);
+    while (at - before >= span.n) {
+      before += span.n;
+      span = span_of(c, s, ++b);
+    }
+    const int index = span.first + static_cast<int>(at - before);
+    const int id = cache_page(c, s.table + b * s.t_st, index, s.width);
+    if (id < 0) continue;
+    const int n = min(page, span.tokens - (index << c.log_page));
+    const int64_t block = static_cast<int64_t>(id) * c.kv_heads + u;
+    const uint8_t* codes = c.k + block * page * kD + lane * 16;
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+    for (int t = 0; t < n; t += 4 * kRows) {
+      u32x4 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = t + j * kRows + lane / kChunks;
+        w[j] = u32x4{0, 0, 0, 0};
+        if (row < n) w[j] = *reinterpret_cast<const u32x4*>(codes + static_cast<int64_t>(t + j * kRows) * kD);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[j][i], false);
+          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[j][i], true);
+          sum[4 * i] += lo[0];
+          sum[4 * i + 1] += lo[1];
+          sum[4 * i + 2] += hi[0];
+          sum[4 * i + 3] += hi[1];
+        }
+    }
+    const double factor = static_cast<double>(e8m0_scale(max(static_cast<uint32_t>(c.ks[block]), kLeastScaleByte)));
+    float* part = s_part[wave][lane / kChunks] + lane % kChunks * 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4*>(part + 4 * i) = f32x4{sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    double total_of[kCh];
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) total_of[i] = 0.0;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) total_of[i] += static_cast<double>(s_part[wave][r][lane * kCh + i]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    // fp64 quotients of sums under 2^26 units by at most 256 are closer to a bf16 tie than fp32 could tell
+    // only where they are that tie; fp32 in between rounds to odd, so that the result is rounded once
+    uint16_t out[kCh];
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+      const double x = total_of[i] / n * factor;
+      float f = static_cast<float>(x);
+      uint32_t bits = __float_as_uint(f);
+      if (static_cast<double>(f) != x && isfinite(f)) {
+        // toward zero, then the last bit set
+        if (fabs(static_cast<double>(f)) > fabs(x)) --bits;
+        bits |= 1;
+      }
+      out[i] = f32_to_bf16_bits(__uint_as_float(bits));
+    }
+    uint16_t* dst = means + block * kD + lane * kCh;
+    if constexpr (kCh == 1)
+      *dst = out[0];
+    else
+#pragma unroll
+      for (int i = 0; i < kCh; i += 2)
+        *reinterpret_cast<uint32_t*>(dst + i) = out[i] | static_cast<uint32_t>(out[i + 1]) << 16;
+  }
+}
+
+// ---------------------------------------------------------------------- selection ----
+
+struct Select {
+  const uint16_t* q;
+  const uint16_t* means;
+  const int* table;
+  const int* lengths;
+  int* pages;               // [batch, tokens, kv_heads, count]
+  int* seen;                // [batch, tokens]
+  unsigned long long* keys; // [units, width], or null: in LDS
+  int64_t q_sb, q_st, q_sh, t_st;
+  int batch, width, tokens, group, count, first, last;
+};
+
+// What unit (b, i, u) sees: its number of pages (-1: a fault) and tokens.
+struct Sight {
+  int have, tokens;
+};
+
+__device__ __forceinline__ Sight sight_of(const KvCache& c, const Select& s, int b, int i) {
+  const int len = s.lengths[b];
+  if (len < 0 || len > most_tokens(c, s.width)) return Sight{-1, -1};
+  const int sees = max(len - s.tokens + 1 + i, 0);
+  return Sight{(sees + (1 << c.log_page) - 1) >> c.log_page, sees};
+}
+
+// A score's bits in rising order; NaN counts as +inf.
+__device__ __forceinline__ unsigned long long key_of(double x) {
+  const long long b = __double_as_longlong(x + 0.0);   // -0 becomes 0
+  return static_cast<unsigned long long>(b) ^ (b < 0 ? ~0ull : 1ull << 63);
+}
+
+constexpr unsigned long long kAlways = ~0ull;
+
+// Keys of pages tile .. tile + 15 of a unit: lane's page is tile + lane % 16 (every quarter of the wave
+// gets them). q rows: A, lane (row = lane % 16, quarter = lane / 16) holds channels
+// quarter D / 4 + s at step s; B the same of the pages.
+template <int kD, bool kF16>
+__device__ unsigned long long tile_keys(const KvCache& c, const Select& s, const int* row, int u, int tile,
+                                        int have, const uint16_t* q, int64_t q_sh) {
+  constexpr int kRun = kD / 4;      // channels of a lane
+  const int lane = threadIdx.x & 63;
+  const int at = tile + (lane & 15);
+  const int id = at < have ? row[at] : 0;
+  const bool there = id >= 0 && id < c.pages;
+  if (!there) *c.faults = 1;
+  u32x4 w[kRun / 8];
+  const uint16_t* m = s.means + (static_cast<int64_t>(there ? id : 0) * c.kv_heads + u) * kD + (lane >> 4) * kRun;
+#pragma unroll
+  for (int j = 0; j < kRun / 8; ++j) w[j] = *reinterpret_cast<const u32x4*>(m + 8 * j);
+  double best = -INFINITY;
+  for (int r0 = 0; r0 < s.group; r0 += 16) {
+    const uint16_t* src = q + min(r0 + (lane & 15), s.group - 1) * q_sh + (lane >> 4) * kRun;
+    f64x4 acc = {0., 0., 0., 0.};
+#pragma unroll
+    for (int j = 0; j < kRun / 8; ++j) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(src + 8 * j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t a = static_cast<uint16_t>(x[i / 2] >> (16 * (i & 1)));
+        const uint16_t b = static_cast<uint16_t>(w[j][i / 2] >> (16 * (i & 1)));
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(
+            static_cast<double>(kF16 ? f16_bits_to_f32(a) : bf16_bits_to_f32(a)),
+            static_cast<double>(bf16_bits_to_f32(b)), acc, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) best = fmax(best, isnan(acc[i]) ? INFINITY : acc[i]);
+  }
+  best = fmax(best, __shfl_xor(best, 16));
+  best = fmax(best, __shfl_xor(best, 32));
+  return !there ? kAlways - 1 : at < s.first || at >= have - s.last ? kAlways : key_of(best);
+}
+
+template <int kD, bool kF16>
+__global__ void __launch_bounds__(kThreads) page_scores_kernel(KvCache c, Select s, int blocks) {
+  const int unit = blockIdx.x / blocks;
+  const int u = unit % c.kv_heads, i = unit / c.kv_heads % s.tokens, b = unit / c.kv_heads / s.tokens;
+  const Sight see = sight_of(c, s, b, i);
+  const int tile = (blockIdx.x % blocks * kWaves + static_cast<int>(threadIdx.x >> 6)) * 16;
+  if (tile >= see.have || see.have <= s.count) return;
+  const uint16_t* q = s.q + b * s.q_sb + i * s.q_st + static_cast<int64_t>(u) * s.group * s.q_sh;
+  const unsigned long long key = tile_keys<kD, kF16>(c, s, s.table + b * s.t_st, u, tile, see.have, q, s.q_sh);
+  const int lane = threadIdx.x & 63;
+  if (lane < 16 && tile + lane < see.have) s.keys[static_cast<int64_t>(unit) * s.width + tile + lane] = key;
+}
+
+// Exclusive prefix of x over the workgroup's threads, and the sum.
+__device__ __forceinline__ int block_prefix(int x, int* s_sums, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  int incl = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int other = __shfl_up(incl, d);
+    incl += lane >= d ? other : 0;
+  }
+  __syncthreads();   // the last call's sums are read
+  if (lane == 63) s_sums[wave] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < waves; ++w) {
+    before += w < wave ? s_sums[w] : 0;
+    all += s_sums[w];
+  }
+  *total = all;
+  return before + incl - x;
+}
+
+// The `count` largest of n > count keys, in the order of their index; of equal ones those in front.
+template <typename Keys>
+__device__ void take_largest(const Keys& keys, int n, int count, const int* row, int* out) {
+  __shared__ int s_bins[256], s_sums[16], s_found[2];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  // ---- the least key that is taken, byte by byte ----
+  unsigned long long prefix = 0, mask = 0;
+  int need = count;     // still to take among those that match the prefix
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    for (int j = tid; j < 256; j += threads) s_bins[j] = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += threads) {
+      const unsigned long long k = keys[j];
+      if ((k & mask) == prefix) atomicAdd(&s_bins[k >> shift & 255], 1);
+    }
+    __syncthreads();
+    int total;
+    const int mine = tid < 256 ? s_bins[255 - tid] : 0;     // from the largest byte down
+    const int before = block_prefix(mine, s_sums, &total);
+    if (tid < 256 && before < need && before + mine >= need) {
+      s_found[0] = 255 - tid;
+      s_found[1] = before;
+    }
+    __syncthreads();
+    prefix |= static_cast<unsigned long long>(s_found[0]) << shift;
+    mask |= 255ull << shift;
+    need -= s_found[1];
+    const bool whole = s_bins[s_found[0]] == need;          // all that match are taken
+    __syncthreads();
+    if (whole) break;
+  }
+  // ---- indexes: a thread has a run of them ----
+  const int run = (n + threads - 1) / threads;
+  const int j0 = min(tid * run, n), j1 = min(j0 + run, n);
+  int above = 0, equal = 0;
+  for (int j = j0; j < j1; ++j) {
+    const unsigned long long k = keys[j] & mask;
+    above += k > prefix;
+    equal += k == prefix;
+  }
+  int total;
+  const int equal_before = block_prefix(equal, s_sums, &total);
+  const int taken_equal = min(max(need - equal_before, 0), equal);
+  int at = block_prefix(above + taken_equal, s_sums, &total), left = taken_equal;
+  for (int j = j0; j < j1; ++j) {
+    const unsigned long long k = keys[j] & mask;
+    if (k > prefix || (k == prefix && left-- > 0)) out[at++] = row[j];
+  }
+}
+
+template <int kD, bool kF16, bool kScore>
+__global__ void __launch_bounds__(kScore ? kThreads : kTakeThreads) page_take_kernel(KvCache c, Select s) {
+  extern __shared__ unsigned long long s_keys[];
+  const int unit = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
+  const int u = unit % c.kv_heads, i = unit / c.kv_heads % s.tokens, b = unit / c.kv_heads / s.tokens;
+  const int* row = s.table + b * s.t_st;
+  int* out = s.pages + static_cast<int64_t>(unit) * s.count;
+  const Sight see = sight_of(c, s, b, i);
+  const int taken = min(max(see.have, 0), s.count);
+  if (tid == 0) {
+    if (see.have < 0) *c.faults = 1;
+    if (u == 0)
+      s.seen[unit / c.kv_heads] = see.have <= 0 ? see.tokens : see.tokens - ((see.have - taken) << c.log_page);
+  }
+  for (int j = taken + tid; j < s.count; j += threads) out[j] = -1;
+  if (see.have <= s.count) {
+    for (int j = tid; j < taken; j += threads) out[j] = row[j];
+    return;
+  }
+  if constexpr (kScore) {
+    const uint16_t* q = s.q + b * s.q_sb + i * s.q_st + static_cast<int64_t>(u) * s.group * s.q_sh;
+    for (int tile = (tid >> 6) * 16; tile < see.have; tile += threads / 64 * 16) {
+      const unsigned long long key = tile_keys<kD, kF16>(c, s, row, u, tile, see.have, q, s.q_sh);
+      if ((tid & 63) < 16 && tile + (tid & 15) < see.have) s_keys[tile + (tid & 15)] = key;
+    }
+    __syncthreads();
+    take_largest(s_keys, see.have, s.count, row, out);
+  } else {
+    take_largest(s.keys + static_cast<int64_t>(unit) * s.width, see.have, s.count, row, out);
+  }
+}
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Tables of up to so many pages keep their keys in LDS.
+constexpr int kMostInLds = 4096;
+// Pages that one workgroup scores by itself where there are not many units
+constexpr int kScoredAlone = 256;
+
+bool scored_alone(int64_t units, int width) {
+  return width <= kScoredAlone || (width <= kMostInLds && units >= 4ll * cu_count());
+}
+
+}  // namespace
+}  // namespace vdn
+
+using namespace vdn;
+
+VDN_API int vdn_cache_means(const void* k_codes, const void* k_scales, int* faults, int pages, int kv_heads,
+                            int page, int head_dim, const int* table, int64_t table_st, int batch, int width,
+                            const int* starts, const int* lengths, void* means, void* stream) {
+  const char* name = "vdn_cache_means";
+  const KvCache c{static_cast<uint8_t*>(const_cast<void*>(k_codes)),
+                  static_cast<uint8_t*>(const_cast<void*>(k_scales)), nullptr, nullptr, faults, pages, kv_heads,
+                  page > 0 ? 31 - __builtin_clz(static_cast<unsigned>(page)) : 0};
+  if (!cache_geometry_ok(c, page, head_dim) || batch < 0 || width <= 0)
+    return set_error(kInvalidArgument,
+                     "%s: bad geometry (page a power of two in 16..256, head_dim 64, 128 or 256)", name);
+  if (batch == 0) return kOk;
+  if (c.k == nullptr || c.ks == nullptr || faults == nullptr || table == nullptr || starts == nullptr ||
+      lengths == nullptr || means == nullptr)
+    return set_error(kInvalidArgument, "%s: null pointer", name);
+  if (!aligned(c.k, 16) || !aligned(means, 16))
+    return set_error(kInvalidArgument, "%s: codes and means need 16-byte alignment", name);
+  const Spans s{table, starts, lengths, table_st, batch, width};
+  // a wave per page and head, as many workgroups as run at once
+  const int64_t most = (static_cast<int64_t>(batch) * width * kv_heads + kWaves - 1) / kWaves;
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(most, 8ll * cu_count())));
+  const auto st = static_cast<hipStream_t>(stream);
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, c, s, static_cast<uint16_t*>(means));
+  };
+  head_dim == 64 ? launch(page_means_kernel<64>)
+                 : head_dim == 128 ? launch(page_means_kernel<128>) : launch(page_means_kernel<256>);
+  return check_launch(name);
+}
+
+VDN_API int vdn_cache_select_workspace(int batch, int tokens, int kv_heads, int width, int64_t* bytes) {
+  if (bytes == nullptr || batch < 0 || tokens <= 0 || kv_heads <= 0 || width <= 0)
+    return set_error(kInvalidArgument, "vdn_cache_select_workspace: invalid argument");
+  const int64_t units = static_cast<int64_t>(batch) * tokens * kv_heads;
+  *bytes = scored_alone(units, width) ? 0 : 8 * units * width;
+  return kOk;
+}
+
+VDN_API int vdn_cache_select(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* means,
+                             int* faults, int pages, int kv_heads, int page, int head_dim, const int* table,
+                             int64_t table_st, int batch, int width, const int* lengths, int tokens, int group,
+                             int dtype, int count, int first, int last, int* selected, int* seen, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const char* name = "vdn_cache_select";
+  const KvCache c{nullptr, nullptr, nullptr, nullptr, faults, pages, kv_heads,
+                  page > 0 ? 31 - __builtin_clz(static_cast<unsigned>(page)) : 0};
+  if (!cache_geometry_ok(c, page, head_dim) || batch < 0 || width <= 0 || tokens <= 0 || group <= 0 ||
+      (static_cast<int64_t>(width) << c.log_page) > (1ll << 31) - 1024)
+    return set_error(kInvalidArgument,
+                     "%s: bad geometry (page a power of two in 16..256, head_dim 64, 128 or 256)", name);
+  if (dtype != 0 && dtype != 1) return set_error(kInvalidArgument, "%s: dtype must be 0 (bf16) or 1 (fp16)", name);
+  if (first < 0 || last < 1 || count < 1 || first > count - last)
+    return set_error(kInvalidArgument, "%s: first >= 0, last >= 1, and count at least both", name);
+  if (batch == 0) return kOk;
+  if (q == nullptr || means == nullptr || faults == nullptr || table == nullptr || lengths == nullptr ||
+      selected == nullptr || seen == nullptr)
+    return set_error(kInvalidArgument, "%s: null pointer", name);
+  if (!aligned(q, 16) || !aligned(means, 16) || q_sb % 8 || q_st % 8 || q_sh % 8)
+    return set_error(kInvalidArgument, "%s: queries and means need 16-byte alignment", name);
+  const int64_t units = static_cast<int64_t>(batch) * tokens * kv_heads;
+  const bool alone = scored_alone(units, width);
+  const int64_t blocks = (static_cast<int64_t>(width) + 16 * kWaves - 1) / (16 * kWaves);
+  if (units * (alone ? 1 : blocks) * kThreads * 4 >= (1ll << 32))
+    return set_error(kUnsupported, "%s: too many queries and pages", name);
+  if (!alone && (workspace == nullptr || !aligned(workspace, 8) || workspace_bytes < 8 * units * width))
+    return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);
+  const Select s{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(means), table, lengths, selected,
+                 seen, alone ? nullptr : static_cast<unsigned long long*>(workspace), q_sb, q_st, q_sh, table_st,
+                 batch, width, tokens, group, count, first, last};
+  const auto st = static_cast<hipStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(units));
+  const auto launch = [&](auto scores, auto fused, auto take) {
+    if (alone) {
+      hipLaunchKernelGGL(fused, grid, dim3(kThreads), 8u * width, st, c, s);
+    } else {
+      hipLaunchKernelGGL(scores, dim3(static_cast<unsigned>(units * blocks)), dim3(kThreads), 0, st, c, s,
+                         static_cast<int>(blocks));
+      hipLaunchKernelGGL(take, grid, dim3(kTakeThreads), 0, st, c, s);
+    }
+  };
+#define VDN_SELECT(D, F16) \
+  launch(page_scores_kernel<D, F16>, page_take_kernel<D, F16, true>, page_take_kernel<D, F16, false>)
+#define VDN_SELECT_D(F16) \
+  head_dim == 64 ? VDN_SELECT(64, F16) : head_dim == 128 ? VDN_SELECT(128, F16) : VDN_SELECT(256, F16)
+  if (dtype == 0)
+    VDN_SELECT_D(false);
+  else
+    VDN_SELECT_D(true);
+#undef VDN_SELECT_D
+#undef VDN_SELECT
+  return check_launch(name);
+}
