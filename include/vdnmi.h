@@ -415,6 +415,29 @@ int vdn_cache_attention_heads(const void* q, int64_t q_sb, int64_t q_sh, const v
                               int64_t workspace_bytes, void* stream);
 
 /*
+ * vdn_cache_attention of sequences that share prefixes: every query of sequence b sees all tokens of its
+ * prefix besides those of its tail that vdn_cache_attention would show it (table, lengths: the tails').
+ * prefix_table int32 [prefixes, prefix_width] (row stride prefix_table_st). The plan, from
+ * vdn_amd.prefix.prepare_prefix_plan, int32 rows of 8, 16-byte aligned: sequences [batch] = (first
+ * sequence of its prefix, the prefix's first item, pieces, row blocks, tokens, ...); items [n_items] = (prefix,
+ * first sequence, first row, rows, first tile, end tile, tokens, ...): a piece of a prefix, in tiles of 64 tokens,
+ * for 128 of its rows (sequences x tokens x group), piece by piece, in each the row blocks in order.
+ * workspace: 16-byte aligned, vdn_prefix_attention_workspace's byte count, its contents need no preparation.
+ * out may be q.
+ */
+int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                         const void* k_codes, const void* k_scales, const void* v_codes,
+                         const void* v_scales, int* faults, int pages, int kv_heads, int page,
+                         int head_dim, const int* prefix_table, int64_t prefix_table_st,
+                         int prefix_width, const int* items, int n_items, const int* sequences,
+                         const int* table, int64_t table_st, int batch, int width,
+                         const int* lengths, int tokens, int group, int dtype, float scale,
+                         void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+int vdn_prefix_attention_workspace(int items, int batch, int width, int page, int tokens, int group,
+                                   int kv_heads, int head_dim, int64_t* bytes);
+
+/*
  * vdn_cache_means: means [pages, kv_heads, head_dim] bf16 (16-byte aligned): the mean key, rounded once, of
  * every page that holds tokens starts[b] .. lengths[b] - 1 of a sequence, over its tokens in front of
  * lengths[b]. Other pages' means stay. Sequences with a negative start or a bad length are left out, *faults 1.

@@ -31,192 +31,19 @@
 // workgroup that holds a unit's every quad writes its output; else it leaves maximum, sum and O in
 // a slot, and a second kernel joins a unit's slots in order (no atomics: the same call gives the
 // same bits).
-#include "kv_cache.h"
-
-#include "attn_tiles.h"
-
-#include <math.h>
+#include "cache_units.h"
 
 #include <algorithm>
 
 namespace vdn {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = 4;
-constexpr int kTile = 64;              // tokens of a wave's step
-constexpr int kQuad = kTile * kWaves;  // tokens of a workgroup's step
+using namespace units;
 
-// Units of tables of up to so many quads are not split: the second step costs less than the join.
-// 128 sequences of 100 - 300 tokens, 32 heads on 8: 22.5 us against 25.6; one of 500, 56 heads: 8.7,
-// 10.3. With four quads 64 of 100 - 1000 tokens take 26.9 against 25.0, one of 1000 12.4 against 10.5.
-constexpr int kWholeQuads = 2;
-
-// Workgroups that share a CU, by the registers that a tile's codes, Q and O take: one for wide heads
-// or 32 rows, three for 64 channels (128 sequences of 100 - 300 tokens, 8 K/V heads: 17.4 us
-// against 20.5 with two; long sequences the same).
-constexpr int workgroups_per_cu(int head_dim, int rows) {
-  return head_dim * rows > 128 * 16 ? 1 : head_dim * rows > 64 * 16 ? 2 : 3;
-}
-
-struct Queries {
-  const uint16_t* q;
-  uint16_t* out;
-  float* lse;
-  int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;  // sequence / token / head strides (elements)
-  int tokens, group;                           // Q, G
-};
-
-struct Lengths {
-  const int* table;
-  const int* lengths;
-  int64_t t_st, t_sh;   // sequence / K/V head strides of the table (0: one row for all heads)
-  int batch, width;
-};
-
-// Workspace slots: two per workgroup (its first and its last unfinished unit), each kRows rows
-// of D + 4 floats (O, m, l, two unused).
-struct Split {
-  float* slots;   // null: units are not split
-  int workgroups;
-  int unit_cost;
-};
-
-__device__ __forceinline__ int seq_tokens(const KvCache& c, const Lengths& s, int b) {
-  const int64_t most = static_cast<int64_t>(s.width) << c.log_page;
-  return static_cast<int>(min(static_cast<int64_t>(max(s.lengths[b], 0)), most));
-}
-
-__device__ __forceinline__ int quads_of(int tokens) { return max((tokens + kQuad - 1) / kQuad, 1); }
-
-// What a unit counts for when the work is shared out: its quads, and in front of them unit_cost for its
-// queries, its first loads' latency and the join of the waves. One quad where units are split: 64
-// sequences of 100 - 1000 tokens, 32 heads on 8: 22.4 us against 25.0 with quads alone, 16 of 100 - 4097
-// with 12 heads x 64 18.1, 19.9; even ones the same (two: 64 of 100 - 2048 tokens 30.7, 28.6). Nothing
-// where they stay whole: 128 of 100 - 300 tokens 22.0, 23.2.
-constexpr int kUnitCost = 1;
-__device__ __forceinline__ int cost_of(const Split& sp, int tokens) { return quads_of(tokens) + sp.unit_cost; }
-
-// Workgroup w of n has the positions share_from(w) .. share_from(w + 1) - 1 of `total` >= n, x is one of
-// share_of(x)'s. Rounded up: where a whole number of workgroups share a unit, they have as many quads each.
-__device__ __forceinline__ int64_t share_from(int64_t total, int n, int w) { return (total * w + n - 1) / n; }
-__device__ __forceinline__ int64_t share_of(int64_t total, int n, int64_t x) { return x * n / total; }
-
-// Where a workgroup's share of all units' costs begins (sequence b: units times its cost), from a
-// prefix over the lengths. Every wave does it for itself, 64 strips of sequences at a time: no
-// barrier, and for up to 64 sequences one load.
-struct Place {
-  int64_t from, to;   // the workgroup's share (none: from = to)
-  int64_t before;   // costs in front of sequence seq
-  int seq;
-};
-
-__device__ __forceinline__ int wave_prefix(int x, int lane) {   // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int other = __shfl_up(x, d);
-    x += lane >= d ? other : 0;
-  }
-  return x;
-}
-
-__device__ Place find_share(const KvCache& c, const Lengths& s, const Split& sp, int units, int wg) {
-  const int lane = threadIdx.x & 63;
-  const int strip = (s.batch + 63) / 64;
-  const int b0 = min(lane * strip, s.batch), b1 = min(b0 + strip, s.batch);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += cost_of(sp, seq_tokens(c, s, b));
-  const int incl = wave_prefix(mine, lane);
-  Place p;
-  const int64_t total = static_cast<int64_t>(__builtin_amdgcn_readlane(incl, 63)) * units;
-  const int n_wg = static_cast<int>(min(total, static_cast<int64_t>(sp.workgroups)));
-  p.from = wg < n_wg ? share_from(total, n_wg, wg) : total;
-  p.to = wg < n_wg ? share_from(total, n_wg, wg + 1) : total;
-  const int64_t at = p.from;
-  // the strip, then the sequence inside it
-  const int front = __popcll(__ballot(static_cast<int64_t>(incl) * units <= at));
-  const int owner = min(front, 63);
-  int before = __builtin_amdgcn_readlane(incl - mine, owner);
-  int seq = __builtin_amdgcn_readlane(b0, owner);
-  if (strip > 1) {
-    const int last = min(seq + strip, s.batch) - 1;
-    for (; seq < last; ++seq) {
-      const int n = cost_of(sp, seq_tokens(c, s, seq));
-      if (at < static_cast<int64_t>(before + n) * units) break;
-      before += n;
-    }
-  }
-  p.before = static_cast<int64_t>(before) * units;
-  p.seq = seq;
-  return p;
-}
-
-template <bool kF16>
-struct Half;
-
-template <>
-struct Half<false> {
-  typedef bf16x8 x8;
-  template <bool kHi>
-  static __device__ __forceinline__ uint32_t widen2(uint32_t w, float s) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, kHi));
-  }
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
-  static __device__ __forceinline__ uint32_t pack_out(float a, float b) { return pack(a, b); }
-};
-
-template <>
-struct Half<true> {
-  typedef f16x8 x8;
-  template <bool kHi>
-  static __device__ __forceinline__ uint32_t widen2(uint32_t w, float s) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, kHi));
-  }
-  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return f32_to_f16_bits(a) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16;
-  }
-  // An output: E4M3 takes values next to fp16's largest one to 65536, which would be an infinity.
-  static __device__ __forceinline__ uint32_t pack_out(float a, float b) {
-    return pack(f16_in_range(a), f16_in_range(b));
-  }
-};
-
-// Eight codes -> eight 16-bit values of code * s (s a power of two).
-template <bool kF16>
-__device__ __forceinline__ u32x4 widen8(uint32_t lo, uint32_t hi, float s) {
-  return u32x4{Half<kF16>::template widen2<false>(lo, s), Half<kF16>::template widen2<true>(lo, s),
-               Half<kF16>::template widen2<false>(hi, s), Half<kF16>::template widen2<true>(hi, s)};
-}
-
-// The first `n` (0 .. 4) bytes of a word.
-__device__ __forceinline__ uint32_t first_bytes(int n) {
-  return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
-}
-
-// Bytes of w that hold the NaN code, as 0x38 (1.0) in the same place and 0 elsewhere.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  uint32_t out = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (((w >> (8 * i)) & 0x7fu) == 0x7fu) out |= 0x38u << (8 * i);
-  return out;
-}
-
-// Factor of a row's output from its sum of weights and the number of keys that it sees. No weights: a row
-// that sees no key is zero, one whose scores are all -inf has no softmax and is NaN.
-__device__ __forceinline__ float inverse_of(float sum, int keys) {
-  return sum == 0.f ? (keys > 0 ? NAN : 0.f) : 1.0f / sum;
-}
-
-template <int kD, int kNR, bool kF16>
+// kPart: nothing is divided by the sums; a whole unit's rows go to `part` as a slot's do.
+template <int kD, int kNR, bool kF16, bool kPart>
 __global__ void __launch_bounds__(kThreads, workgroups_per_cu(kD, 16 * kNR))
-cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2) {
+cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2, float* part) {
   constexpr int kRows = 16 * kNR;     // query rows of a unit
   constexpr int kKL = kD / 64;        // 16-byte K loads per key row and lane
   constexpr int kDB = kD / 16;        // 16-channel blocks of O
@@ -558,7 +385,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] += x[i] * f;
       }
-      if (whole) {
+      if (whole && !kPart) {
         const int i = row / io.group, h = u * io.group + row - i * io.group;
         const float inv = inverse_of(sum, seen0 + i);
         u32x2 y;
@@ -569,7 +396,10 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
           io.lse[(static_cast<int64_t>(b_now) * io.tokens + i) * c.kv_heads * io.group + h] =
               sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
-        float* dst = sp.slots + (slot * kRows + r) * (kD + 4);
+        const int i = row / io.group, h = u * io.group + row - i * io.group;
+        float* dst = kPart && whole
+            ? part + ((static_cast<int64_t>(b_now) * io.tokens + i) * c.kv_heads * io.group + h) * (kD + 4)
+            : sp.slots + (slot * kRows + r) * (kD + 4);
         *reinterpret_cast<f32x4*>(dst + d) = acc;
         if (d == 0) {
           dst[kD] = top;
@@ -696,6 +526,41 @@ int64_t workgroups_of(int64_t most_quads, int head_dim, int block) {
 }
 
 }  // namespace
+
+namespace units {
+
+UnitPlan plan_units(int batch, int width, int log_page, int64_t rows, int kv_heads, int head_dim) {
+  UnitPlan p;
+  p.block = rows_of_block(static_cast<int>(std::min<int64_t>(rows, 32)), head_dim);
+  p.row_blocks = static_cast<int>((rows + p.block - 1) / p.block);
+  const int64_t unit_quads = ((static_cast<int64_t>(width) << log_page) + kQuad - 1) / kQuad;
+  const int64_t all = static_cast<int64_t>(p.row_blocks) * kv_heads * batch;
+  p.split = unit_quads > kWholeQuads;
+  p.sp = Split{nullptr, static_cast<int>(workgroups_of(all * unit_quads, head_dim, p.block)),
+               p.split ? kUnitCost : 0};
+  p.slot_bytes = p.split ? 4ll * 2 * p.sp.workgroups * p.block * (head_dim + 4) : 0;
+  return p;
+}
+
+int launch_partials(const KvCache& c, const Queries& io, const Lengths& s, const UnitPlan& plan, float* whole,
+                    int head_dim, int dtype, float scale_log2, hipStream_t stream) {
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.sp.workgroups)), dim3(kThreads), 0, stream, c, io, s,
+                       plan.sp, plan.row_blocks, scale_log2, whole);
+  };
+#define VDN_PART(D, NR) \
+  dtype ? launch(cache_attn_kernel<D, NR, true, true>) : launch(cache_attn_kernel<D, NR, false, true>)
+  if (head_dim == 64)
+    plan.block == 16 ? (VDN_PART(64, 1)) : (VDN_PART(64, 2));
+  else if (head_dim == 128)
+    plan.block == 16 ? (VDN_PART(128, 1)) : (VDN_PART(128, 2));
+  else
+    VDN_PART(256, 1);
+#undef VDN_PART
+  return check_launch("cache partials");
+}
+
+}  // namespace units
 }  // namespace vdn
 
 VDN_API int vdn_cache_attention_workspace(int tokens, int group, int head_dim, int64_t* bytes) {
@@ -737,18 +602,16 @@ int cache_attention(const char* name, const void* q, int64_t q_sb, int64_t q_st,
   const int64_t rows = static_cast<int64_t>(tokens) * group;
   if (rows * kv_heads * batch * kThreads >= (1ll << 32))
     return set_error(kUnsupported, "%s: too many query rows", name);
-  const int block = rows_of_block(static_cast<int>(std::min<int64_t>(rows, 32)), head_dim);
-  const int row_blocks = static_cast<int>((rows + block - 1) / block);
-  const int64_t unit_quads = ((static_cast<int64_t>(width) << c.log_page) + kQuad - 1) / kQuad;
-  const int64_t units = static_cast<int64_t>(row_blocks) * kv_heads * batch;
-  const int workgroups = static_cast<int>(workgroups_of(units * unit_quads, head_dim, block));
-  const bool split = unit_quads > kWholeQuads;
-  const Split sp{split ? static_cast<float*>(workspace) : nullptr, workgroups, split ? kUnitCost : 0};
+  UnitPlan plan = plan_units(batch, width, c.log_page, rows, kv_heads, head_dim);
+  const int block = plan.block, row_blocks = plan.row_blocks, workgroups = plan.sp.workgroups;
+  const bool split = plan.split;
   if (split) {
-    if (workspace == nullptr || !aligned16(workspace) ||
-        workspace_bytes < 4ll * 2 * workgroups * block * (head_dim + 4))
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < plan.slot_bytes)
       return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);
+    plan.sp.slots = static_cast<float*>(workspace);
   }
+  const Split& sp = plan.sp;
+  const int64_t unit_quads = ((static_cast<int64_t>(width) << c.log_page) + kQuad - 1) / kQuad;
   const Queries io{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lse, q_sb, q_st, q_sh,
                    o_sb, o_st, o_sh, tokens, group};
   const Lengths s{table, lengths, table_st, table_sh, batch, width};
@@ -757,7 +620,7 @@ int cache_attention(const char* name, const void* q, int64_t q_sb, int64_t q_st,
   const auto launch = [&](auto main, auto join1, auto join4) {
     const auto st = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(main, dim3(static_cast<unsigned>(workgroups)), dim3(kThreads), 0, st, c, io, s, sp,
-                       row_blocks, scale * kLog2e);
+                       row_blocks, scale * kLog2e, static_cast<float*>(nullptr));
     if (!split) return;
     const dim3 grid(static_cast<unsigned>(join_rows));
     if (join_rows > 4 * cu_count())
@@ -766,7 +629,7 @@ int cache_attention(const char* name, const void* q, int64_t q_sb, int64_t q_st,
       hipLaunchKernelGGL(join4, grid, dim3(256), 0, st, c, io, s, sp, row_blocks);
   };
 #define VDN_CACHE(D, NR, F16)                                               \
-  launch(cache_attn_kernel<D, NR, F16>, cache_join_kernel<D, NR, F16, 1>, \
+  launch(cache_attn_kernel<D, NR, F16, false>, cache_join_kernel<D, NR, F16, 1>, \
          cache_join_kernel<D, NR, F16, 4>)
 #define VDN_CACHE_D(F16)                                                            \
   head_dim == 64 ? (block == 16 ? VDN_CACHE(64, 1, F16) : VDN_CACHE(64, 2, F16))    \
