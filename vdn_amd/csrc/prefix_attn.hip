@@ -19,6 +19,7 @@
 #include "cache_units.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vdn {
 namespace {
@@ -117,15 +118,22 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
   const int last_group = (it.tokens - 1) & ~15;
   const int64_t head_bytes = static_cast<int64_t>(page) * kD;
 
+  // A tile's page ids come two tiles ahead, its codes and scales one. They stay as loaded until the
+  // next tile: a look at an id would wait for all loads in front of it, the codes' among them.
   struct Ids {
     int at[kIds];
   };
-  auto ids_of = [&](int t) __attribute__((always_inline)) {
+  auto load_ids = [&](int t) __attribute__((always_inline)) {
     Ids ids;
 #pragma unroll
     for (int g = 0; g < kIds; ++g)
-      ids.at[g] = __builtin_amdgcn_readfirstlane(table[min(min(t * kBN + 16 * g, last_group) >> c.log_page,
-                                                          pre.width - 1)]);
+      ids.at[g] = table[min(min(t * kBN + 16 * g, last_group) >> c.log_page, pre.width - 1)];
+    return ids;
+  };
+  auto uniform = [&](const Ids& loaded) __attribute__((always_inline)) {
+    Ids ids;
+#pragma unroll
+    for (int g = 0; g < kIds; ++g) ids.at[g] = __builtin_amdgcn_readfirstlane(loaded.at[g]);
     return ids;
   };
   auto in_pool = [&](int id) __attribute__((always_inline)) { return id >= 0 && id < c.pages; };
@@ -157,10 +165,14 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
       load_to_lds16(v, voff[j], 0, dv + (wave * kSegs + j) * 1024);
     }
   };
-  // K's and V's scale bytes of the lane's two 16-token groups (16 h of either half of the tile)
+  // K's and V's scale bytes of the lane's two 16-token groups (16 h of either half of the tile). Loaded by
+  // lane, with an offset that the compiler cannot tell to be zero for all: it would make a uniform
+  // byte a scalar at once, and wait for it there.
   struct Scales {
     uint32_t k[2], v[2];
   };
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
   auto scales_of = [&](const Ids& ids) __attribute__((always_inline)) {
     Scales s;
 #pragma unroll
@@ -171,14 +183,14 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
         s.k[1] = s.k[0];
         s.v[1] = s.v[0];
       } else {
-        s.k[kt] = c.ks[block];
-        s.v[kt] = c.vs[block];
+        s.k[kt] = c.ks[block + zero];
+        s.v[kt] = c.vs[block + zero];
       }
     }
     return s;
   };
 
-  Ids now = ids_of(it.tile), next = ids_of(it.tile + 1);
+  Ids now = uniform(load_ids(it.tile)), ahead = load_ids(it.tile + 1);
   issue(now, it.tile, sK0, sV0);
   Scales sc = scales_of(now);
 
@@ -208,41 +220,84 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
   float m = -3.402823466e38f, l = 0.f;
   float unit_scale = 0.f;                  // fp16: O in units of this power of two (0: O is 0)
   bool bad = false;
+  // With one wave a SIMD half of the registers are accumulation registers, and O stays in them if the
+  // rare branches that compute on it hand it back there (causal_attn.hip).
+  auto keep = [&]() __attribute__((always_inline)) {
+    if constexpr (per_cu(kD) == 1) {
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) asm volatile("" : "+a"(o[db]));
+    }
+  };
+  // Where the lane's operands begin in a tile: read j of a key (32 keys further the swizzle is the same),
+  // and the channels of its group in either half of the tile.
   const int key_row = 16 * (col >> 2 & 1) + 4 * (col >> 3) + (col & 3);   // key of the lane's A row
+  int k_at[kKJ], v_at[2];
+#pragma unroll
+  for (int j = 0; j < kKJ; ++j) k_at[j] = key_row * kD + 16 * ((2 * j + h) ^ swz<kD>(key_row));
+#pragma unroll
+  for (int kt = 0; kt < 2; ++kt) {
+    const int g = 2 * kt + h;
+    v_at[kt] = kBig ? col * 64 + 16 * (g ^ (col >> 2 & 3)) : (g * kD + col) * 16;
+  }
 
-  auto process = [&](int t, const uint8_t* tk, const uint8_t* tv, uint8_t* ndk, uint8_t* ndv)
-      __attribute__((always_inline)) {
+  // The last tile is apart if the prefix ends inside it: the others have no token to hide.
+  auto process = [&](int t, auto buf_tag, auto tail_tag) __attribute__((always_inline)) {
+    constexpr int kBuf = decltype(buf_tag)::value;
+    constexpr bool kTail = decltype(tail_tag)::value;
+    const uint8_t* tk = kBuf == 0 ? sK0 : sK1;
+    const uint8_t* tv = kBuf == 0 ? sV0 : sV1;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's share of the tile is there
     __syncthreads();                                   // all of it, and every wave is done with the other buffer
 #pragma unroll
     for (int g = 0; g < kIds; ++g) bad |= !in_pool(now.at[g]);
-    Scales ahead = sc;
-    Ids after = next;
-    if (t + 1 < it.end) {
-      issue(next, t + 1, ndk, ndv);
-      ahead = scales_of(next);
-      after = ids_of(t + 2);
-    }
     const Scales s_now = sc;
-    sc = ahead;
-    now = next;
-    next = after;
+    if (t + 1 < it.end) {
+      now = uniform(ahead);
+      issue(now, t + 1, kBuf == 0 ? sK1 : sK0, kBuf == 0 ? sV1 : sV0);
+      sc = scales_of(now);
+      ahead = load_ids(t + 2);
+    }
     if (!live) return;
 
-    // ---- Sᵀ ----
+    // ---- Sᵀ: kAtOnce operand reads are under way before the first is used, and an operand is widened
+    // between the MFMAs of the one before ----
+    constexpr int kReads = 2 * kKJ, kAtOnce = kD == 128 && !kF16 ? 8 : 4;
     f32x16 s[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
+    for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[kt][v] = 0.f;
-      const int key = 32 * kt + key_row;
 #pragma unroll
-      for (int j = 0; j < kKJ; ++j) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(tk + key * kD + 16 * ((2 * j + h) ^ swz<kD>(key)));
-        s[kt] = E::mfma(__builtin_bit_cast(x8, units::widen8<kF16>(w[0], w[1], 1.f)), qf[j][0], s[kt]);
-        s[kt] = E::mfma(__builtin_bit_cast(x8, units::widen8<kF16>(w[2], w[3], 1.f)), qf[j][1], s[kt]);
+    for (int r0 = 0; r0 < kReads; r0 += kAtOnce) {
+      u32x4 w[kAtOnce];
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r) {
+        const int j = (r0 + r) / 2, kt = (r0 + r) & 1;
+        w[r] = *reinterpret_cast<const u32x4*>(tk + k_at[j] + kt * 32 * kD);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 lo = units::widen8<kF16>(w[0][0], w[0][1], 1.f), hi = units::widen8<kF16>(w[0][2], w[0][3], 1.f);
+#pragma unroll
+      for (int r = 0; r < kAtOnce; ++r) {
+        const int j = (r0 + r) / 2, kt = (r0 + r) & 1, n = r + 1 < kAtOnce ? r + 1 : r;
+        __builtin_amdgcn_sched_barrier(0);
+        s[kt] = E::mfma(__builtin_bit_cast(x8, lo), qf[j][0], s[kt]);
+        if (n > r) lo = units::widen8<kF16>(w[n][0], w[n][1], 1.f);
+        __builtin_amdgcn_sched_barrier(0);
+        s[kt] = E::mfma(__builtin_bit_cast(x8, hi), qf[j][1], s[kt]);
+        if (n > r) hi = units::widen8<kF16>(w[n][2], w[n][3], 1.f);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    // V's operands, the first ones read while the softmax runs
+    constexpr int kVAhead = kD == 128 && !kF16 ? 8 : 4;
+    u32x4 vw[kVAhead];
+    auto read_v = [&](int x) __attribute__((always_inline)) {
+      vw[x % kVAhead] = *reinterpret_cast<const u32x4*>(tv + v_at[x / kDB] + x % kDB * 32 * (kBig ? 64 : 16));
+    };
+#pragma unroll
+    for (int x = 0; x < kVAhead; ++x) read_v(x);
+    __builtin_amdgcn_sched_barrier(0);
 
     // ---- V's scales; fp16: relative to the tile's largest one (cache_attn.hip) ----
     float v_scale[2], weight[2] = {1.f, 1.f};
@@ -256,10 +311,12 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
       const float tile_scale = e8m0_scale(min(max(top, 127u - 32u), 127u + 16u));
       if (__any(tile_scale != unit_scale)) {   // wave-uniform
         const float f = unit_scale == 0.f ? 1.f : unit_scale / tile_scale;
+        keep();
 #pragma unroll
         for (int db = 0; db < kDB; ++db)
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[db][v] *= f;
+        keep();
         unit_scale = tile_scale;
       }
 #pragma unroll
@@ -273,8 +330,8 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
     }
 
     // ---- softmax: the scores times K's scale, m lagging the running maximum (causal_attn.hip) ----
-    const int left = it.tokens - t * kBN;     // tokens of the tile
-    if (left < kBN) {
+    [[maybe_unused]] const int left = it.tokens - t * kBN;     // tokens of the tile
+    if constexpr (kTail) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -296,10 +353,12 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
       const float m_new = grow ? mx - kAbove : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
       l *= corr;
+      keep();
 #pragma unroll
       for (int db = 0; db < kDB; ++db)
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[db][v] *= corr;
+      keep();
       m = m_new;
     }
     u32x4 pb[2][2];
@@ -321,30 +380,46 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
     l += sum;   // of this lane's keys; the halves are joined at the end
 
     // ---- Oᵀ += Vᵀ Pᵀ ----
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const int g = 2 * kt + h;
-#pragma unroll
-      for (int db = 0; db < kDB; ++db) {
-        const int ch = 32 * db + col;
-        u32x4 w = *reinterpret_cast<const u32x4*>(
-            tv + (kBig ? ch * 64 + 16 * (g ^ (ch >> 2 & 3)) : (g * kD + ch) * 16));
-        if (left < kBN) {     // behind the last token: 0 NaN is NaN
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] &= units::first_bytes(left - 16 * g - 4 * i);
-        }
-        o[db] = E::mfma(__builtin_bit_cast(x8, units::widen8<kF16>(w[0], w[1], v_scale[kt])),
-                        __builtin_bit_cast(x8, pb[kt][0]), o[db]);
-        o[db] = E::mfma(__builtin_bit_cast(x8, units::widen8<kF16>(w[2], w[3], v_scale[kt])),
-                        __builtin_bit_cast(x8, pb[kt][1]), o[db]);
+    __builtin_amdgcn_sched_barrier(0);
+    auto widen_v = [&](int x, int half) __attribute__((always_inline)) {
+      uint32_t w0 = vw[x % kVAhead][2 * half], w1 = vw[x % kVAhead][2 * half + 1];
+      if constexpr (kTail) {     // behind the last token: 0 NaN is NaN
+        const int n = left - 16 * (2 * (x / kDB) + h) - 8 * half;
+        w0 &= units::first_bytes(n);
+        w1 &= units::first_bytes(n - 4);
       }
+      return units::widen8<kF16>(w0, w1, v_scale[x / kDB]);
+    };
+    u32x4 lo = widen_v(0, 0), hi = widen_v(0, 1);
+#pragma unroll
+    for (int x = 0; x < 2 * kDB; ++x) {
+      const int kt = x / kDB, db = x % kDB;
+      if (x + kVAhead < 2 * kDB) read_v(x + kVAhead);
+      __builtin_amdgcn_sched_barrier(0);
+      o[db] = E::mfma(__builtin_bit_cast(x8, lo), __builtin_bit_cast(x8, pb[kt][0]), o[db]);
+      if (x + 1 < 2 * kDB) lo = widen_v(x + 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      o[db] = E::mfma(__builtin_bit_cast(x8, hi), __builtin_bit_cast(x8, pb[kt][1]), o[db]);
+      if (x + 1 < 2 * kDB) hi = widen_v(x + 1, 1);
     }
+    __builtin_amdgcn_sched_barrier(0);
   };
-  for (int t = it.tile; t < it.end; t += 2) {
-    process(t, sK0, sV0, sK1, sV1);
-    if (t + 1 < it.end) process(t + 1, sK1, sV1, sK0, sV0);
+  const auto first = std::integral_constant<int, 0>{};
+  const auto second = std::integral_constant<int, 1>{};
+  const int whole = min(it.end, it.tokens / kBN);      // behind the last tile that is full
+  int t = it.tile;
+  for (; t + 1 < whole; t += 2) {
+    process(t, first, std::false_type{});
+    process(t + 1, second, std::false_type{});
+  }
+  if (t < whole) {
+    process(t, first, std::false_type{});
+    if (t + 1 < it.end) process(t + 1, second, std::true_type{});
+  } else if (t < it.end) {
+    process(t, first, std::true_type{});
   }
 
+  keep();
   l = sum_halves(l);
   if (bad) {
     if (tid == 0) *c.faults = 1;
