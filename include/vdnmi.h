@@ -421,7 +421,8 @@ int vdn_cache_attention_heads(const void* q, int64_t q_sb, int64_t q_sh, const v
  * vdn_amd.prefix.prepare_prefix_plan, int32 rows of 8, 16-byte aligned: sequences [batch] = (first
  * sequence of its prefix, the prefix's first item, pieces, row blocks, tokens, ...); items [n_items] = (prefix,
  * first sequence, first row, rows, first tile, end tile, tokens, ...): a piece of a prefix, in tiles of 64 tokens,
- * for 128 of its rows (sequences x tokens x group), piece by piece, in each the row blocks in order.
+ * for 128 of its rows (sequences x tokens x group), piece by piece, in each the row blocks in order;
+ * piece_tiles: the tiles of the longest.
  * workspace: 16-byte aligned, vdn_prefix_attention_workspace's byte count, its contents need no preparation.
  * out may be q.
  */
@@ -429,8 +430,8 @@ int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
                          const void* k_codes, const void* k_scales, const void* v_codes,
                          const void* v_scales, int* faults, int pages, int kv_heads, int page,
                          int head_dim, const int* prefix_table, int64_t prefix_table_st,
-                         int prefix_width, const int* items, int n_items, const int* sequences,
-                         const int* table, int64_t table_st, int batch, int width,
+                         int prefix_width, const int* items, int n_items, int piece_tiles,
+                         const int* sequences, const int* table, int64_t table_st, int batch, int width,
                          const int* lengths, int tokens, int group, int dtype, float scale,
                          void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse,
                          void* workspace, int64_t workspace_bytes, void* stream);

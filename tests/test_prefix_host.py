@@ -51,7 +51,7 @@ def test_every_row_and_tile_is_in_one_item():
 
 def test_pieces_fill_the_card_once():
     plan = vp.prepare_prefix_plan([65536], [128], 40, 8, 128, device="cpu")
-    assert 0.85 * 512 <= plan.items.shape[0] * 8 <= 512
+    assert 0.8 * 512 <= plan.items.shape[0] * 8 <= 448     # an eighth is left for the tails
     many = vp.prepare_prefix_plan([300] * 500, [2] * 500, 16, 16, 128, device="cpu")
     assert many.items.shape[0] == 500                    # more units than workgroups: none is cut
     assert vp.prepare_prefix_plan([], [], 2, 1, 64, device="cpu").batch == 0
@@ -87,7 +87,7 @@ def test_entry_point_validates_before_launching():
     def call(q=P, q_st=64, pages=4, page=16, dim=64, p_table=P, p_width=2, items=P, n=3, seqs=P, batch=2, width=2,
              tokens=1, group=1, dtype=0, scale=0.1, out=P, ws=P, nbytes=1 << 40):
         return lib.vdn_prefix_attention(q, 128, q_st, 64, P, P, P, P, P, pages, 2, page, dim, p_table, 2, p_width,
-                                        items, n, seqs, P, 2, batch, width, P, tokens, group, dtype, scale, out, 128,
+                                        items, n, 1, seqs, P, 2, batch, width, P, tokens, group, dtype, scale, out, 128,
                                         64, 64, None, ws, nbytes, None)
 
     for bad, said in ((dict(pages=0), b"geometry"), (dict(page=24), b"geometry"), (dict(dim=32), b"geometry"),

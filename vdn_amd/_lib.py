@@ -88,7 +88,7 @@ SIGNATURES = {
                          _i64, _ptr],
     "vdn_cache_select_workspace": [_i32, _i32, _i32, _i32, _ptr],
     "vdn_prefix_attention": [_ptr, _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i32, _i32, _i32,
-                             _i32, _ptr, _i64, _i32, _ptr, _i32, _ptr, _ptr, _i64, _i32, _i32, _ptr,
+                             _i32, _ptr, _i64, _i32, _ptr, _i32, _i32, _ptr, _ptr, _i64, _i32, _i32, _ptr,
                              _i32, _i32, _i32, _f32, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr],
     "vdn_prefix_attention_workspace": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _ptr],
     "vdn_vda_readout_mxfp8": [_ptr, _i64, _i64, _i64, _i32, _ptr, _ptr, _i32, _f32, _ptr, _i64,

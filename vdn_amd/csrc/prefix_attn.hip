@@ -79,9 +79,9 @@ __device__ __forceinline__ int swz(int key) {
 // kBig: pages of at least 64 tokens, a tile lies in one; else its four groups of 16 tokens may
 // lie in as many.
 template <int kD, bool kF16, bool kBig>
-__global__ void __launch_bounds__(kThreads, per_cu(kD))
-prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__ items, int n_items, float* slots,
-                   float scale_log2) {
+__device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& io, const Prefixes& pre,
+                                              const Item* __restrict__ items, int n_items, float* slots,
+                                              float scale_log2, int pid) {
   constexpr int kDB = kD / 32;            // 32-channel accumulators of O
   constexpr int kChunks = kD / 16;        // 16-byte chunks of a key
   constexpr int kKJ = kD / 32;            // a lane's 16-byte reads of a key
@@ -98,16 +98,13 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
 
   // With a multiple of 8 K/V heads each XCD keeps its own heads: the blocks of a piece share an L2.
   int u, at;
-  {
-    const int pid = blockIdx.x;
-    if (c.kv_heads % 8 == 0) {
-      const int local = pid >> 3;
-      at = local % n_items;
-      u = (pid & 7) + 8 * (local / n_items);
-    } else {
-      u = pid % c.kv_heads;
-      at = pid / c.kv_heads;
-    }
+  if (c.kv_heads % 8 == 0) {
+    const int local = pid >> 3;
+    at = local % n_items;
+    u = (pid & 7) + 8 * (local / n_items);
+  } else {
+    u = pid % c.kv_heads;
+    at = pid / c.kv_heads;
   }
   const Item it = items[at];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -267,6 +264,7 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[kt][v] = 0.f;
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int r0 = 0; r0 < kReads; r0 += kAtOnce) {
       u32x4 w[kAtOnce];
@@ -289,6 +287,7 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_s_setprio(0);
     // V's operands, the first ones read while the softmax runs
     constexpr int kVAhead = kD == 128 && !kF16 ? 8 : 4;
     u32x4 vw[kVAhead];
@@ -390,6 +389,7 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
       }
       return units::widen8<kF16>(w0, w1, v_scale[x / kDB]);
     };
+    __builtin_amdgcn_s_setprio(1);
     u32x4 lo = widen_v(0, 0), hi = widen_v(0, 1);
 #pragma unroll
     for (int x = 0; x < 2 * kDB; ++x) {
@@ -402,6 +402,7 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
       o[db] = E::mfma(__builtin_bit_cast(x8, hi), __builtin_bit_cast(x8, pb[kt][1]), o[db]);
       if (x + 1 < 2 * kDB) hi = widen_v(x + 1, 1);
     }
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
   };
   const auto first = std::integral_constant<int, 0>{};
@@ -440,6 +441,21 @@ prefix_attn_kernel(KvCache c, Queries io, Prefixes pre, const Item* __restrict__
   }
 }
 
+// The first n_pieces workgroups take a piece of a prefix each, the others share the tails. (The other way
+// round workgroups that find nothing to share end at once, and the pieces that follow in their
+// places are spread unevenly over the CUs: 308 us instead of 236 for 128 sequences behind 65536 tokens.)
+template <int kD, bool kF16, bool kBig>
+__global__ void __launch_bounds__(kThreads, per_cu(kD))
+prefix_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int n_pieces, int row_blocks, float* whole, Prefixes pre,
+                   const Item* __restrict__ items, int n_items, float* slots, float scale_log2) {
+  __shared__ units::UnitLds<kD, 1> lds;
+  const int pid = blockIdx.x;
+  if (pid < n_pieces)
+    attend_prefix<kD, kF16, kBig>(c, io, pre, items, n_items, slots, scale_log2, pid);
+  else
+    units::attend_units<kD, 1, kF16, true>(c, io, s, sp, row_blocks, scale_log2, whole, pid - n_pieces, lds);
+}
+
 // Joins a row's partial results: of the prefix's pieces, in order, then of the tail. A workgroup per
 // row, kD / 4 lanes for the channels, the others take partial results in turn.
 template <int kD, bool kF16, int kWaves>
@@ -476,7 +492,7 @@ prefix_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int unit_rows, in
     const int64_t n_units = static_cast<int64_t>(row_blocks) * c.kv_heads;
     const int64_t total = all * n_units;
     const int64_t start = front * n_units + static_cast<int64_t>(row / unit_rows * c.kv_heads + u) * own;
-    const int n_wg = static_cast<int>(min(total, static_cast<int64_t>(sp.workgroups)));
+    const int n_wg = units::sharers(sp, total);
     w0 = units::share_of(total, n_wg, start + sp.unit_cost);
     w1 = units::share_of(total, n_wg, start + own - 1);
     second = start > units::share_from(total, n_wg, static_cast<int>(w0)) ? 1 : 0;
@@ -554,6 +570,27 @@ prefix_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int unit_rows, in
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// How the tails' units are shared out beside n pieces of at most piece_tiles tiles. A tile of 128 rows takes
+// less than half as long as a quad of 16 (2.0 and 4.5 us with 128 channels). Where the card's other
+// places would do for the longest tails that the table can hold, only those are launched: workgroups that find
+// nothing to share wait for a place all the same (128 sequences behind 65536 tokens: 235 us, 250).
+units::UnitPlan plan_tails(int batch, int width, int log_page, int64_t rows, int kv_heads, int head_dim, int64_t n,
+                           int piece_tiles) {
+  units::UnitPlan plan = units::plan_units(batch, width, log_page, rows, kv_heads, head_dim, 16);
+  Split& sp = plan.sp;
+  const int64_t fit = static_cast<int64_t>(per_cu(head_dim)) * cu_count();
+  sp.workgroups = static_cast<int>(std::min<int64_t>(sp.workgroups, fit));
+  sp.few = n > 0 && n < fit ? static_cast<int>(fit - n) : 0;
+  sp.beside = 0.45f * piece_tiles;
+  const int64_t quads = ((static_cast<int64_t>(width) << log_page) + units::kQuad - 1) / units::kQuad;
+  const int64_t most = batch * (quads + sp.unit_cost) * plan.row_blocks * kv_heads;
+  if (units::few_suffice(sp, most)) {
+    sp.workgroups = std::min(sp.workgroups, sp.few);
+    sp.few = 0;
+  }
+  return plan;
+}
+
 struct Bytes {
   int64_t pieces, whole, tails;
 };
@@ -574,8 +611,8 @@ VDN_API int vdn_prefix_attention_workspace(int items, int batch, int width, int 
       page <= 0)
     return set_error(kInvalidArgument, "vdn_prefix_attention_workspace: invalid argument");
   const int64_t rows = static_cast<int64_t>(tokens) * group;
-  const auto plan = units::plan_units(batch, width, 31 - __builtin_clz(static_cast<unsigned>(page)), rows, kv_heads,
-                                      head_dim);
+  const auto plan = plan_tails(batch, width, 31 - __builtin_clz(static_cast<unsigned>(page)), rows, kv_heads, head_dim,
+                               0, 0);
   const Bytes b = workspace_of(items, rows * kv_heads * batch, kv_heads, head_dim, plan);
   *bytes = b.pieces + b.whole + b.tails;
   return kOk;
@@ -585,7 +622,7 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
                                  const void* k_scales, const void* v_codes, const void* v_scales, int* faults,
                                  int pages, int kv_heads, int page, int head_dim, const int* prefix_table,
                                  int64_t prefix_table_st, int prefix_width, const int* items, int n_items,
-                                 const int* sequences, const int* table, int64_t table_st, int batch, int width,
+                                 int piece_tiles, const int* sequences, const int* table, int64_t table_st, int batch, int width,
                                  const int* lengths, int tokens, int group, int dtype, float scale, void* out,
                                  int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse, void* workspace,
                                  int64_t workspace_bytes, void* stream) {
@@ -596,6 +633,7 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
                   static_cast<uint8_t*>(const_cast<void*>(v_scales)), faults, pages, kv_heads,
                   page > 0 ? 31 - __builtin_clz(static_cast<unsigned>(page)) : 0};
   if (!cache_geometry_ok(c, page, head_dim) || batch < 0 || width <= 0 || tokens <= 0 || group <= 0 || n_items < 0 ||
+      piece_tiles < 0 ||
       prefix_width < 0 || (n_items > 0 && prefix_width == 0) ||
       (static_cast<int64_t>(std::max(width, prefix_width)) << c.log_page) > (1ll << 31) - 1024)
     return set_error(kInvalidArgument,
@@ -618,7 +656,8 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
           (((static_cast<int64_t>(width) << c.log_page) + units::kQuad - 1) / units::kQuad + units::kUnitCost) >
       (1ll << 31) - 1)
     return set_error(kUnsupported, "%s: too many tokens", name);
-  units::UnitPlan plan = units::plan_units(batch, width, c.log_page, rows, kv_heads, head_dim);
+  units::UnitPlan plan = plan_tails(batch, width, c.log_page, rows, kv_heads, head_dim,
+                                    static_cast<int64_t>(n_items) * kv_heads, piece_tiles);
   const Bytes need = workspace_of(n_items, out_rows, kv_heads, head_dim, plan);
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need.pieces + need.whole + need.tails)
     return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);
@@ -631,24 +670,22 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
   const Prefixes pre{prefix_table, prefix_table_st, prefix_width};
   const auto st = static_cast<hipStream_t>(stream);
   const float scale_log2 = scale * kLog2e;
-  if (n_items > 0) {
-    const auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_items * kv_heads)), dim3(kThreads), 0, st, c, io, pre,
-                         reinterpret_cast<const Item*>(items), n_items, slots, scale_log2);
-    };
+  const int n_pieces = n_items * kv_heads;
+  const auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_pieces + plan.sp.workgroups)), dim3(kThreads), 0, st, c, io,
+                       s, plan.sp, n_pieces, plan.row_blocks, whole, pre, reinterpret_cast<const Item*>(items), n_items,
+                       slots, scale_log2);
+  };
 #define VDN_PREFIX(D)                                                                                       \
   dtype ? (page >= kBN ? launch(prefix_attn_kernel<D, true, true>) : launch(prefix_attn_kernel<D, true, false>)) \
         : (page >= kBN ? launch(prefix_attn_kernel<D, false, true>) : launch(prefix_attn_kernel<D, false, false>))
-    if (head_dim == 64)
-      VDN_PREFIX(64);
-    else if (head_dim == 128)
-      VDN_PREFIX(128);
-    else
-      VDN_PREFIX(256);
+  if (head_dim == 64)
+    VDN_PREFIX(64);
+  else if (head_dim == 128)
+    VDN_PREFIX(128);
+  else
+    VDN_PREFIX(256);
 #undef VDN_PREFIX
-    if (const int status = check_launch(name)) return status;
-  }
-  if (const int status = units::launch_partials(c, io, s, plan, whole, head_dim, dtype, scale_log2, st)) return status;
   const auto join = [&](auto one, auto four) {
     const dim3 grid(static_cast<unsigned>(out_rows));
     if (out_rows > 4 * cu_count())

@@ -37,6 +37,7 @@ class PrefixPlan:
     kv_heads: int
     head_dim: int
     tokens: int
+    piece_tiles: int
     items: torch.Tensor
     sequences: torch.Tensor
 
@@ -88,7 +89,7 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     tiles = -(-n // TILE)
     pieces = np.zeros_like(n)
     if int((blocks * tiles).sum()):
-        pieces = np.where(blocks > 0, _cut(tiles, blocks * kv_heads, cus * _WORKGROUPS_PER_CU[head_dim]), 0)
+        pieces = np.where(blocks > 0, _cut(tiles, blocks * kv_heads, cus * _WORKGROUPS_PER_CU[head_dim] * 7 // 8), 0)
     made = pieces * blocks
     base = made.cumsum() - made
     if int(made.sum()) * kv_heads >= 2 ** 24:
@@ -107,7 +108,8 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     for column, values in enumerate((first, base, pieces, blocks, n)):
         sequences[:, column] = values[owner]
     both = torch.from_numpy(np.concatenate((items, sequences))).to(device)      # one transfer
-    return PrefixPlan(lengths, counts, heads, kv_heads, head_dim, tokens, both[:p.size], both[p.size:])
+    longest = int((items[:, 5] - items[:, 4]).max()) if p.size else 0
+    return PrefixPlan(lengths, counts, heads, kv_heads, head_dim, tokens, longest, both[:p.size], both[p.size:])
 
 
 def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, table, lengths, scale=None, *,
@@ -161,7 +163,7 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
         workspace = query.new_empty(nbytes // 2)
     _lib.call_on(index, "vdn_prefix_attention", query.data_ptr(), q_sb, q_st, q_sh, *args,
                  prefix_table.data_ptr(), p_st, prefix_width, items.data_ptr(), items.shape[0],
-                 sequences.data_ptr(), table.data_ptr(), t_st, batch, width, lengths.data_ptr(), tokens, group,
+                 plan.piece_tiles, sequences.data_ptr(), table.data_ptr(), t_st, batch, width, lengths.data_ptr(), tokens, group,
                  int(query.dtype is torch.float16), scale, out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse),
                  _lib.ptr(workspace), nbytes, _lib.raw_stream(index))
     return (out, lse) if return_lse else out
