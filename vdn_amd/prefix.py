@@ -37,6 +37,7 @@ class PrefixPlan:
     kv_heads: int
     head_dim: int
     tokens: int
+    longest: int
     piece_tiles: int
     items: torch.Tensor
     sequences: torch.Tensor
@@ -47,7 +48,7 @@ class PrefixPlan:
 
     @property
     def batch(self):
-        return sum(self.counts)
+        return self.sequences.shape[0]
 
 
 def _cut(tiles, units, slots):
@@ -108,8 +109,9 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     for column, values in enumerate((first, base, pieces, blocks, n)):
         sequences[:, column] = values[owner]
     both = torch.from_numpy(np.concatenate((items, sequences))).to(device)      # one transfer
-    longest = int((items[:, 5] - items[:, 4]).max()) if p.size else 0
-    return PrefixPlan(lengths, counts, heads, kv_heads, head_dim, tokens, longest, both[:p.size], both[p.size:])
+    tiles_of_one = int((items[:, 5] - items[:, 4]).max()) if p.size else 0
+    return PrefixPlan(lengths, counts, heads, kv_heads, head_dim, tokens, max(lengths, default=0), tiles_of_one,
+                      both[:p.size], both[p.size:])
 
 
 def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, table, lengths, scale=None, *,
@@ -135,7 +137,7 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
     if items.get_device() != index or sequences.get_device() != index:
         raise ValueError("the plan must be on the cache's device")
     prefixes, prefix_width, p_st = _check_table(prefix_table, index)
-    if prefixes != len(plan.lengths) or max(plan.lengths, default=0) > prefix_width * page:
+    if prefixes != len(plan.lengths) or plan.longest > prefix_width * page:
         raise ValueError("prefix_table must name every prefix's pages")
     table_batch, width, t_st = _check_table(table, index)
     _check_vector("lengths", lengths, batch, index)
@@ -146,15 +148,19 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
+    dtype = query.dtype
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif (out.shape != query.shape or out.dtype is not query.dtype or out.get_device() != index
+        out, o_sb, o_st, o_sh = query.new_empty(query.shape), tokens * heads * d, heads * d, d
+    elif (out.shape != query.shape or out.dtype is not dtype or out.get_device() != index
           or out.stride(-1) != 1 or 0 in out.stride()):
         raise ValueError("out must be a view like the query, unit channel stride, no broadcast")
     else:
         _lib.check_attention_out(out, query)
-    o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
-    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=query.device) if return_lse else None
+        o_sb, o_sh, o_st = out.stride(0), out.stride(-2), out.stride(1) if out.ndim == 4 else 0
+    lse = lse_ptr = None
+    if return_lse:
+        lse = query.new_empty(query.shape[:-1], dtype=torch.float32)
+        lse_ptr = lse.data_ptr()
     group = heads // kv_heads
     workspace, nbytes = None, 0
     if batch:
@@ -164,7 +170,7 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
     _lib.call_on(index, "vdn_prefix_attention", query.data_ptr(), q_sb, q_st, q_sh, *args,
                  prefix_table.data_ptr(), p_st, prefix_width, items.data_ptr(), items.shape[0],
                  plan.piece_tiles, sequences.data_ptr(), table.data_ptr(), t_st, batch, width, lengths.data_ptr(), tokens, group,
-                 int(query.dtype is torch.float16), scale, out.data_ptr(), o_sb, o_st, o_sh, _lib.ptr(lse),
+                 int(dtype is torch.float16), scale, out.data_ptr(), o_sb, o_st, o_sh, lse_ptr,
                  _lib.ptr(workspace), nbytes, _lib.raw_stream(index))
     return (out, lse) if return_lse else out
 

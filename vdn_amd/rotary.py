@@ -102,14 +102,11 @@ def prepare_rotary_plan(head_dim, *, rotary_dim=None, base=10000.0, layout="half
     return RotaryPlan(head_dim, rotary_dim, layout, amplitude, steps)
 
 
-def _check_weight(name, w, plan, dtype):
-    if w is None:
-        return None
-    if w.shape != (plan.head_dim,) or w.dtype not in (dtype, torch.float32) or w.device != plan.device \
+def _check_weight(name, w, dim, dtype, index):
+    if w.ndim != 1 or w.shape[0] != dim or w.dtype not in (dtype, torch.float32) or w.get_device() != index \
             or not w.is_contiguous():
         raise ValueError(f"{name} must be contiguous [head_dim] of the activation dtype or FP32, on the "
-                         "plan's device")
-    return w
+                         "query's device")
 
 
 def _check_out(name, out, x, others):
@@ -138,42 +135,48 @@ def rotate_qk(query, key, positions, plan: RotaryPlan, q_weight=None, k_weight=N
     if not isinstance(plan, RotaryPlan):
         raise TypeError("plan must be a RotaryPlan")
     dtype, index = query.dtype, query.get_device()
-    if query.ndim != 3 or key.ndim != 3 or query.shape[2] != plan.head_dim or key.shape[2] != plan.head_dim \
-            or key.shape[0] != query.shape[0] or query.shape[1] == 0 or key.shape[1] == 0:
-        raise ValueError("query must be [tokens, H, D] and key [tokens, H_kv, D], D that of the plan")
-    if dtype not in _DTYPES or key.dtype is not dtype or query.stride(2) != 1 or key.stride(2) != 1:
+    if query.ndim != 3 or key.ndim != 3:
+        raise ValueError("query must be [tokens, H, D] and key [tokens, H_kv, D]")
+    (tokens, heads, dim), (k_tokens, kv_heads, k_dim) = query.shape, key.shape
+    (q_st, q_sh, q_sd), (k_st, k_sh, k_sd) = query.stride(), key.stride()
+    if dim != plan.head_dim or k_dim != dim or k_tokens != tokens or heads == 0 or kv_heads == 0:
+        raise ValueError("query and key must have the same tokens, at least one head and the plan's D")
+    if dtype not in _DTYPES or key.dtype is not dtype or q_sd != 1 or k_sd != 1:
         raise ValueError("query and key must share BF16 or FP16, with unit innermost stride")
     if index < 0:
         raise ValueError("query must be on a CUDA (HIP) device")
-    if key.get_device() != index or plan.steps.get_device() != index or positions.get_device() != index:
+    steps = plan.steps
+    if key.get_device() != index or steps.get_device() != index or positions.get_device() != index:
         raise ValueError("query, key, positions and the plan must be on one device")
-    tokens, heads, dim = query.shape
-    if positions.shape != (tokens,) or positions.dtype not in (torch.int32, torch.int64) \
-            or not positions.is_contiguous():
+    if positions.ndim != 1 or positions.shape[0] != tokens or not positions.is_contiguous() \
+            or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be contiguous int32 or int64 [tokens]")
-    q_weight = _check_weight("q_weight", q_weight, plan, dtype)
-    k_weight = _check_weight("k_weight", k_weight, plan, dtype)
-    wide = {w.dtype for w in (q_weight, k_weight) if w is not None}
-    if len(wide) > 1:
-        raise ValueError("q_weight and k_weight must share a dtype")
+    q_w = k_w = None
+    wide = 0
+    if q_weight is not None:
+        _check_weight("q_weight", q_weight, dim, dtype, index)
+        q_w, wide = q_weight.data_ptr(), int(q_weight.dtype is torch.float32)
+    if k_weight is not None:
+        _check_weight("k_weight", k_weight, dim, dtype, index)
+        k_w, wide = k_weight.data_ptr(), int(k_weight.dtype is torch.float32)
+        if q_weight is not None and q_weight.dtype is not k_weight.dtype:
+            raise ValueError("q_weight and k_weight must share a dtype")
     eps = float(eps)
     if not math.isfinite(eps) or eps < 0:
         raise ValueError("eps must be finite and not negative")
-    if plan.steps.shape != (plan.rotary_dim // 2,) or plan.steps.dtype is not torch.int64 \
-            or not plan.steps.is_contiguous():
+    if steps.numel() * 2 != plan.rotary_dim or steps.dtype is not torch.int64 or not steps.is_contiguous():
         raise ValueError("the plan's steps are not those that it was made with")
     if out is None:
-        q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        k_out = torch.empty_like(key, memory_format=torch.contiguous_format)
+        q_out, k_out = query.new_empty((tokens, heads, dim)), query.new_empty((tokens, kv_heads, dim))
+        qo_st, ko_st, qo_sh, ko_sh = heads * dim, kv_heads * dim, dim, dim
     else:
         q_out, k_out = out
         _check_out("query", q_out, query, (key,))
         _check_out("key", k_out, key, (query, q_out))
-    _lib.call_on(index, "vdn_rotary", query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(),
-                 key.stride(0), key.stride(1), _lib.ptr(q_weight), _lib.ptr(k_weight),
-                 int(torch.float32 in wide), eps, positions.data_ptr(), int(positions.dtype is torch.int64),
-                 plan.steps.data_ptr(), plan.rotary_dim, int(plan.layout == "interleaved"),
-                 plan.amplitude, tokens, heads, key.shape[1], dim, int(dtype is torch.float16),
-                 q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k_out.data_ptr(), k_out.stride(0),
-                 k_out.stride(1), _lib.raw_stream(index))
+        (qo_st, qo_sh, _), (ko_st, ko_sh, _) = q_out.stride(), k_out.stride()
+    _lib.call_on(index, "vdn_rotary", query.data_ptr(), q_st, q_sh, key.data_ptr(), k_st, k_sh, q_w, k_w, wide,
+                 eps, positions.data_ptr(), int(positions.dtype is torch.int64), steps.data_ptr(),
+                 plan.rotary_dim, int(plan.layout == "interleaved"), plan.amplitude, tokens, heads, kv_heads, dim,
+                 int(dtype is torch.float16), q_out.data_ptr(), qo_st, qo_sh, k_out.data_ptr(), ko_st, ko_sh,
+                 _lib.raw_stream(index))
     return q_out, k_out

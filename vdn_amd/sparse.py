@@ -31,7 +31,8 @@ def empty_means(cache: KVCache):
 
 
 def _check_means(cache, means, index):
-    if means.shape != (cache.pages, cache.kv_heads, cache.head_dim) or means.dtype is not torch.bfloat16 \
+    pages, kv_heads, _, dim = cache._geometry
+    if means.shape != (pages, kv_heads, dim) or means.dtype is not torch.bfloat16 \
             or means.get_device() != index or not means.is_contiguous():
         raise ValueError("means must be contiguous BF16 [pages, kv_heads, D] on the cache's device")
 
@@ -55,16 +56,17 @@ def write_means(cache: KVCache, means, table, starts, lengths):
 
 def _check_query(query, cache, index):
     """(batch, Q, H, D, strides of the first three)"""
-    if query.ndim not in (3, 4):
-        raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
     if query.ndim == 4:
         batch, tokens, heads, d = query.shape
         q_sb, q_st, q_sh, q_sd = query.stride()
-    else:
+    elif query.ndim == 3:
         batch, heads, d = query.shape
         q_sb, q_sh, q_sd = query.stride()
         tokens, q_st = 1, 0
-    if d != cache.head_dim or heads <= 0 or heads % cache.kv_heads or tokens <= 0:
+    else:
+        raise ValueError("query must be [batch, Q, H, D] or [batch, H, D]")
+    _, kv_heads, _, dim = cache._geometry
+    if d != dim or heads <= 0 or heads % kv_heads or tokens <= 0:
         raise ValueError("query heads must be a multiple of the cache's, D the same, Q positive")
     if query.dtype not in _DTYPES or q_sd != 1 or query.get_device() != index:
         raise ValueError("query must be BF16 or FP16 with unit innermost stride, on the cache's device")
@@ -97,8 +99,8 @@ def select_pages(query, cache: KVCache, means, table, lengths, count, *, first=1
     if any(type(n) is not int for n in (count, first, last)) or first < 0 or last < 1 or count < first + last:
         raise ValueError("count must be at least first + last, first >= 0, last >= 1")
     lead = query.shape[:-2]
-    pages = query.new_empty((*lead, kv_heads, count), dtype=torch.int32)
-    seen = query.new_empty(lead, dtype=torch.int32)
+    pages = lengths.new_empty((*lead, kv_heads, count))
+    seen = lengths.new_empty(lead)
     nbytes = _select_bytes(index, batch, tokens, kv_heads, width) if batch else 0
     workspace = query.new_empty(nbytes // 2) if nbytes else None
     faults, geometry = args[4], args[5:]
@@ -109,13 +111,16 @@ def select_pages(query, cache: KVCache, means, table, lengths, count, *, first=1
     return pages, seen
 
 
-def _merged(x, what):
-    """[batch, Q, ...] -> [batch * Q, ...] as a view."""
-    if x.ndim == 3 or x.shape[1] == 1:
-        return x if x.ndim == 3 else x[:, 0]
-    if x.shape[0] > 1 and x.stride(0) != x.shape[1] * x.stride(1):
-        raise ValueError(f"{what}'s queries must follow each other at one stride")
-    return x.flatten(0, 1)
+def _merged(x, tokens, what):
+    """Strides of [batch * Q, heads] of a [batch, Q, heads, ..] or [batch, heads, ..] tensor."""
+    if x.ndim == 3:
+        return x.stride()[:2]
+    s_b, s_t, s_h, _ = x.stride()
+    if tokens == 1:
+        return s_b, s_h
+    if x.shape[0] > 1 and s_b != tokens * s_t:
+        raise ValueError(f"{what}'s tokens must follow each other at one stride")
+    return s_t, s_h
 
 
 def selected_attention(query, cache: KVCache, pages, tokens, scale=None, *, return_lse=False, out=None):
@@ -131,9 +136,9 @@ def selected_attention(query, cache: KVCache, pages, tokens, scale=None, *, retu
     index, args = _check_cache(cache, "selected_attention")
     batch, q_tokens, heads, d, *_ = _check_query(query, cache, index)
     _, kv_heads, page, _ = cache._geometry
-    lead = query.shape[:-2]
-    if pages.ndim != query.ndim or pages.shape[:-1] != (*lead, kv_heads) or pages.dtype is not torch.int32 \
-            or pages.get_device() != index or pages.shape[-1] == 0 or pages.stride(-1) != 1:
+    shape, lead, dtype = query.shape, query.shape[:-2], query.dtype
+    if pages.shape[:-1] != (*lead, kv_heads) or pages.dtype is not torch.int32 or pages.get_device() != index \
+            or pages.shape[-1] == 0 or pages.stride(-1) != 1:
         raise ValueError("pages must be int32 [batch, Q, kv_heads, count] for the query, unit inner stride, on "
                          "the cache's device")
     if tokens.shape != lead or tokens.dtype is not torch.int32 or tokens.get_device() != index \
@@ -146,23 +151,28 @@ def selected_attention(query, cache: KVCache, pages, tokens, scale=None, *, retu
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif (out.shape != query.shape or out.dtype is not query.dtype or out.get_device() != index
+        out, o_sb, o_sh = query.new_empty(shape), heads * d, d
+    elif (out.shape != shape or out.dtype is not dtype or out.get_device() != index
           or out.stride(-1) != 1 or 0 in out.stride()):
         raise ValueError("out must be a view like the query, unit channel stride, no broadcast")
     else:
         _lib.check_attention_out(out, query)
-    q, o, p = _merged(query, "query"), _merged(out, "out"), _merged(pages, "pages")
-    lse = torch.empty(query.shape[:-1], dtype=torch.float32, device=query.device) if return_lse else None
+        o_sb, o_sh = _merged(out, q_tokens, "out")
+    q_sb, q_sh = _merged(query, q_tokens, "query")
+    p_sb, p_sh = _merged(pages, q_tokens, "pages")
+    lse = lse_ptr = None
+    if return_lse:
+        lse = query.new_empty(shape[:-1], dtype=torch.float32)
+        lse_ptr = lse.data_ptr()
     group = heads // kv_heads
     workspace, nbytes = None, 0
     if count * page > WHOLE_TOKENS:
+        # from the allocator in stream order: calls on other streams and captured graphs have their own
         nbytes = _workspace_bytes(index, 1, group, d)
-        workspace = query.new_empty(nbytes // 2)
-    _lib.call_on(index, "vdn_cache_attention_heads", q.data_ptr(), q.stride(0), q.stride(1), *args, p.data_ptr(),
-                 p.stride(0), p.stride(1), batch * q_tokens, count, tokens.data_ptr(), group,
-                 int(query.dtype is torch.float16), scale, o.data_ptr(), o.stride(0), o.stride(1),
-                 _lib.ptr(lse), _lib.ptr(workspace), nbytes, _lib.raw_stream(index))
+        workspace = query.new_empty(nbytes // 2)   # 2-byte elements
+    _lib.call_on(index, "vdn_cache_attention_heads", query.data_ptr(), q_sb, q_sh, *args, pages.data_ptr(), p_sb, p_sh,
+                 batch * q_tokens, count, tokens.data_ptr(), group, int(dtype is torch.float16), scale,
+                 out.data_ptr(), o_sb, o_sh, lse_ptr, _lib.ptr(workspace), nbytes, _lib.raw_stream(index))
     return (out, lse) if return_lse else out
 
 
