@@ -158,7 +158,7 @@ def test_selection(device, dim, dtype, heads, kv_heads, tokens):
     cache.check()
 
 
-@pytest.mark.parametrize("length,count", [(16 * 257, 3), (16 * 1500 - 3, 64), (16 * 5000, 700), (16 * 9000, 8999)])
+@pytest.mark.parametrize("length,count", [(16 * 257, 3), (16 * 1500 - 3, 64), (16 * 5000, 700), (16 * 9000, 8999), (16 * 20000, 37)])
 @torch.no_grad()
 def test_selection_of_long_sequences(device, length, count):
     """Keys in a workspace, and scores that share their upper bits."""
@@ -170,6 +170,37 @@ def test_selection_of_long_sequences(device, length, count):
     q[:, :, 1] = -1
     got = sp.select_pages(q, cache, means, table.cuda(), ints(length, 40), count)
     check_selection(q, cache, means, table, [length, 40], count, 1, 1, got)
+
+
+@pytest.mark.parametrize("spread", ["even", "alike", "two", "infinite"])
+@torch.no_grad()
+def test_selection_where_scores_crowd(device, spread):
+    """Many pages: scores spread evenly, all within a millionth but for two far off, of two values only,
+    and with infinities of both signs among them."""
+    n, dim = 6001, 64
+    g = torch.Generator().manual_seed(1)
+    table, pages = tables([n, 700])
+    cache = kv.empty_cache(pages, 1, dim, 16, device="cuda")
+    means = torch.zeros(pages, 1, dim)
+    if spread == "even":
+        means[:, 0, :4] = torch.randn(pages, 4, generator=g)
+    elif spread == "alike":
+        means[:, 0, 0] = 1000
+        means[:, 0, 1] = 2.0 ** -8 * torch.rand(pages, generator=g)
+        means[table[0, 17], 0, 0], means[table[0, 400], 0, 0] = 3e38, -3e38
+    elif spread == "two":
+        means[:, 0, 0] = torch.randint(0, 2, (pages,), generator=g).float()
+    else:
+        means[:, 0, 0] = torch.randn(pages, generator=g)
+        means[table[0, 5::100].long(), 0, 0] = math.inf
+        means[table[0, 7::50].long(), 0, 0] = -math.inf
+    means = means.to(BF16).cuda()
+    q = torch.zeros(2, 1, 2, dim, dtype=BF16, device="cuda")
+    q[..., :4] = 1
+    lengths = [16 * n - 5, 16 * 700]
+    for count in (2, 50, 300, 5000):
+        got = sp.select_pages(q, cache, means, table.cuda(), ints(*lengths), count)
+        check_selection(q, cache, means, table, lengths, count, 1, 1, got)
 
 
 @pytest.mark.parametrize("length", [16 * 40, 16 * 600])

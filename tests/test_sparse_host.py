@@ -66,9 +66,8 @@ def test_entry_points_validate_before_launching():
                       (dict(last=0), b"last"), (dict(first=-1), b"first"), (dict(first=2 ** 31 - 1), b"count"),
                       (dict(q=None), b"null"), (dict(m=None), b"null"), (dict(out=None), b"null"),
                       (dict(q_sh=60), b"alignment"), (dict(q=P + 8), b"alignment"),
-                      (dict(batch=1 << 30), b"too many"), (dict(width=1 << 20), b"workspace")):
-        if bad == dict(width=1 << 20):
-            bad = dict(bad, ws=None)
+                      (dict(batch=1 << 30), b"too many"), (dict(width=1 << 17), b"geometry"), (dict(width=1 << 16, ws=None), b"workspace"),
+                      (dict(width=1 << 16, nbytes=1000), b"workspace")):
         assert select(**bad) != 0, bad
         assert said in lib.vdn_last_error(), (bad, lib.vdn_last_error())
     assert select(batch=0, q=None) == 0

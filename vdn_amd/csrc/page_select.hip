@@ -10,8 +10,8 @@
 // the query rows as A and 16 pages as B, the maximum over the rows is over a lane's
 // four accumulators and the four lanes of its column. A page of the first or the last ones counts as
 // the largest, NaN as +inf. Of equal scores the page in front wins. Then a workgroup per (b, i, u)
-// takes the `count` best: by each page's rank, or where they are many by radix selection on the
-// scores' bits.
+// takes the `count` best: by each page's rank, or where they are many by bisection for the least
+// score that is taken.
 #include "kv_cache.h"
 
 #include "attn_tiles.h"
@@ -25,7 +25,8 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kTakeThreads = 1024;   // of a selection from many scored pages
+constexpr int kAloneThreads = 512;   // of a selection whose pages one workgroup scores
+constexpr int kTakeThreads = 1024;   // of one from scored pages
 
 struct Spans {
   const int* table;    // [batch, width], row stride t_st
@@ -246,79 +247,305 @@ __global__ void __launch_bounds__(kThreads) page_scores_kernel(KvCache c, Select
   if (lane < 16 && tile + lane < see.have) s.keys[static_cast<int64_t>(unit) * s.width + tile + lane] = key;
 }
 
-// Exclusive prefix of x over the workgroup's threads, and the sum.
-__device__ __forceinline__ int block_prefix(int x, int* s_sums, int* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  int incl = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int other = __shfl_up(incl, d);
-    incl += lane >= d ? other : 0;
-  }
-  __syncthreads();   // the last call's sums are read
-  if (lane == 63) s_sums[wave] = incl;
-  __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < waves; ++w) {
-    before += w < wave ? s_sums[w] : 0;
-    all += s_sums[w];
-  }
-  *total = all;
-  return before + incl - x;
+__device__ __forceinline__ double value_of(unsigned long long key) {
+  return __longlong_as_double(static_cast<long long>(key ^ (key >> 63 ? 1ull << 63 : ~0ull)));
 }
 
-// The `count` largest of n > count keys, in the order of their index; of equal ones those in front.
-template <typename Keys>
-__device__ void take_largest(const Keys& keys, int n, int count, const int* row, int* out) {
-  __shared__ int s_bins[256], s_sums[16], s_found[2];
-  const int tid = threadIdx.x, threads = blockDim.x;
-  // ---- the least key that is taken, byte by byte ----
-  unsigned long long prefix = 0, mask = 0;
-  int need = count;     // still to take among those that match the prefix
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int j = tid; j < 256; j += threads) s_bins[j] = 0;
+// The `count` largest of n > count keys, of equal ones those in front. Few: a key per thread and its rank
+// among all, which lie in LDS with zeros (less than any key) up to a multiple of 8.
+__device__ void take_by_rank(const unsigned long long* keys, int n, int count, const int* row, int* out) {
+  __shared__ int s_sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int at = min(tid, n - 1);
+  const int page = row[at];
+  const unsigned long long mine = keys[at];
+  int rank = 0;
+  for (int j = 0; j < n; j += 8) {
+    unsigned long long k[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) k[i] = keys[j + i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) rank += k[i] > mine || (k[i] == mine && j + i < tid);
+  }
+  const bool taken = tid < n && rank < count;
+  const unsigned long long all = __ballot(taken);
+  if (lane == 0) s_sums[wave] = __popcll(all);
+  __syncthreads();
+  int before = __popcll(all & ((1ull << lane) - 1));
+#pragma unroll
+  for (int w = 0; w < kAloneThreads / 64; ++w) before += w < wave ? s_sums[w] : 0;
+  if (taken) out[before] = page;
+}
+
+// Many. Thread t holds the keys t, t + threads, .. in registers, up to kRun of them, or, kRun = 0, reads
+// them again for every step. With registers the scores go into as many bins as there are threads,
+// evenly between the least and the largest finite one: the bin that the last taken one lies in has few
+// others in it, and those are ranked. Where it has many (scores that are alike but for a few far off), and
+// without registers, the least key that is taken is found by bisection, first between values, then
+// between bit patterns. 128 of 8192 pages, 8 units: 10 us, by bisection 17.
+constexpr int kMostRuns = 64, kMostWaves = kTakeThreads / 64;
+constexpr int kMostInBin = 256;
+
+template <int kRun>
+__device__ void take_many(const unsigned long long* keys, int n, int count, const int* row, int* out) {
+  __shared__ int s_counts[3], s_before[(kRun > 0 ? kRun : kMostRuns) * kMostWaves];
+  __shared__ unsigned long long s_low[kMostWaves], s_high[kMostWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
+  const int run = (n + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
+  unsigned long long held[kRun > 0 ? kRun : 1];
+  int ids[kRun > 0 ? kRun : 1];
+  if constexpr (kRun > 0) {
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int j = min(tid + i * static_cast<int>(blockDim.x), n - 1);
+      held[i] = keys[j];
+      ids[i] = row[j];
+    }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+      if (tid + i * static_cast<int>(blockDim.x) >= n) held[i] = 0;   // less than any key
+  }
+  // f(key, whether it is one, page, turn) of every key of the thread; all lanes take part in every call
+  auto each = [&](auto f) __attribute__((always_inline)) {
+    if constexpr (kRun > 0) {
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) f(held[i], tid + i * static_cast<int>(blockDim.x) < n, ids[i], i);
+    } else {
+      for (int i = 0; i < run; ++i) {
+        const int j = tid + i * static_cast<int>(blockDim.x);
+        f(j < n ? keys[min(j, n - 1)] : 0ull, j < n, row[min(j, n - 1)], i);
+      }
+    }
+  };
+  // Turns the counts of s_before[turn][wave] into how many there are in front of each.
+  auto scan_counts = [&]() __attribute__((always_inline)) {
     __syncthreads();
-    for (int j = tid; j < n; j += threads) {
-      const unsigned long long k = keys[j];
-      if ((k & mask) == prefix) atomicAdd(&s_bins[k >> shift & 255], 1);
+    if (wave == 0) {
+      const int all = (kRun > 0 ? kRun : run) * waves, each_lane = (all + 63) / 64;
+      int mine = 0;
+      for (int i = lane * each_lane; i < min((lane + 1) * each_lane, all); ++i) mine += s_before[i];
+      int incl = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(incl, d);
+        incl += lane >= d ? other : 0;
+      }
+      int at = incl - mine;
+      for (int i = lane * each_lane; i < min((lane + 1) * each_lane, all); ++i) {
+        const int x = s_before[i];
+        s_before[i] = at;
+        at += x;
+      }
     }
     __syncthreads();
-    int total;
-    const int mine = tid < 256 ? s_bins[255 - tid] : 0;     // from the largest byte down
-    const int before = block_prefix(mine, s_sums, &total);
-    if (tid < 256 && before < need && before + mine >= need) {
-      s_found[0] = 255 - tid;
-      s_found[1] = before;
+  };
+  const unsigned long long in_front = (1ull << lane) - 1;
+  // Writes the pages whose bits are set, in order.
+  auto write_taken = [&](unsigned long long taken) __attribute__((always_inline)) {
+    __syncthreads();
+    each([&](unsigned long long, bool, int, int i) {
+      const int some = __popcll(__ballot(taken >> i & 1));
+      if (lane == 0) s_before[i * waves + wave] = some;
+    });
+    scan_counts();
+    each([&](unsigned long long, bool, int page, int i) {
+      const bool mine = taken >> i & 1;
+      const int at = s_before[i * waves + wave] + __popcll(__ballot(mine) & in_front);
+      if (mine) out[at] = page;
+    });
+  };
+
+  if constexpr (kRun > 0) {
+    __shared__ int s_bins[kTakeThreads], s_sums[kMostWaves], s_bin[3];
+    __shared__ float s_least[kMostWaves], s_most[kMostWaves];
+    __shared__ unsigned long long s_list[kMostInBin];
+    __shared__ int s_index[kMostInBin];
+    __shared__ unsigned int s_taken[kRun * kTakeThreads / 32];
+    const int threads = blockDim.x;
+    // a key's score to fp32, which keeps the order; +inf for what always goes first
+    float x[kRun], least = INFINITY, most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      x[i] = held[i] >= kAlways - 1 ? INFINITY : static_cast<float>(value_of(held[i]));
+      const bool counts = held[i] != 0 && fabsf(x[i]) < INFINITY;
+      least = fminf(least, counts ? x[i] : INFINITY);
+      most = fmaxf(most, counts ? x[i] : -INFINITY);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      least = fminf(least, __shfl_xor(least, d));
+      most = fmaxf(most, __shfl_xor(most, d));
+    }
+    if (lane == 0) {
+      s_least[wave] = least;
+      s_most[wave] = most;
+    }
+    s_bins[tid] = 0;
+    for (int j = tid; j < kRun * kTakeThreads / 32; j += threads) s_taken[j] = 0;
+    if (tid == 0) s_bin[2] = 0;
+    __syncthreads();
+    for (int w = 0; w < waves; ++w) {
+      least = fminf(least, s_least[w]);
+      most = fmaxf(most, s_most[w]);
+    }
+    const float per_bin = static_cast<float>(threads - 2) / (most - least);
+    if (per_bin > 0.f && per_bin < INFINITY) {          // the same for all threads
+      int bin[kRun];
+#pragma unroll
+      for (int i = 0; i < kRun; ++i) {
+        bin[i] = x[i] == INFINITY ? threads - 1
+                                  : static_cast<int>(fminf(fmaxf((x[i] - least) * per_bin, 0.f), threads - 2.f));
+        if (held[i] != 0) atomicAdd(&s_bins[bin[i]], 1);
+      }
+      __syncthreads();
+      const int mine = s_bins[threads - 1 - tid];       // from the last bin down
+      int incl = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(incl, d);
+        incl += lane >= d ? other : 0;
+      }
+      if (lane == 63) s_sums[wave] = incl;
+      __syncthreads();
+      int before = incl - mine;
+      for (int w = 0; w < wave; ++w) before += s_sums[w];
+      if (before < count && before + mine >= count) {
+        s_bin[0] = threads - 1 - tid;
+        s_bin[1] = count - before;
+      }
+      __syncthreads();
+      const int last = s_bin[0], need = s_bin[1], in_bin = s_bins[last];
+      if (in_bin == need || in_bin <= kMostInBin) {
+        if (in_bin > need) {
+#pragma unroll
+          for (int i = 0; i < kRun; ++i)
+            if (held[i] != 0 && bin[i] == last) {
+              const int at = atomicAdd(&s_bin[2], 1);
+              s_list[at] = held[i];
+              s_index[at] = tid + i * threads;
+            }
+          __syncthreads();
+          if (tid < in_bin) {
+            const unsigned long long k = s_list[tid];
+            const int index = s_index[tid];
+            int rank = 0;
+            for (int j = 0; j < in_bin; ++j) rank += s_list[j] > k || (s_list[j] == k && s_index[j] < index);
+            if (rank < need) atomicOr(&s_taken[index >> 5], 1u << (index & 31));
+          }
+          __syncthreads();
+        }
+        unsigned long long taken = 0;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          const int index = tid + i * threads;
+          const bool one = held[i] != 0 && (bin[i] > last || (bin[i] == last && (in_bin == need ||
+                                                              (s_taken[index >> 5] >> (index & 31) & 1))));
+          taken |= static_cast<unsigned long long>(one) << i;
+        }
+        write_taken(taken);
+        return;
+      }
+    }
+  }
+
+  if (tid < 3) s_counts[tid] = 0;
+  __syncthreads();
+  int turn = 0;
+  // Keys that `what` says yes to, over the workgroup: a ballot each, one atomic a wave, one barrier. The
+  // three counters go round: one is summed, one may still be read, one is cleared.
+  auto count_of = [&](auto what) __attribute__((always_inline)) {
+    int mine = 0;
+    each([&](unsigned long long k, bool there, int, int) { mine += __popcll(__ballot(what(k, there))); });
+    if (lane == 0) atomicAdd(&s_counts[turn], mine);
+    const int last = turn;
+    turn = turn == 2 ? 0 : turn + 1;
+    if (tid == 0) s_counts[turn == 2 ? 0 : turn + 1] = 0;
+    __syncthreads();
+    return s_counts[last];
+  };
+  auto at_least = [&](unsigned long long bound) __attribute__((always_inline)) {
+    return count_of([&](unsigned long long k, bool) { return k >= bound; });
+  };
+
+  // ---- bounds: at least `count` keys are >= low, less are >= high ----
+  unsigned long long low, high;
+  int found;                                   // keys that are >= low
+  const int special = at_least(kAlways - 1);   // always taken, or pages that are not there
+  if (special >= count) {
+    const int always = at_least(kAlways);      // at most first + last <= count
+    low = always >= count ? kAlways : kAlways - 1;
+    found = always >= count ? always : special;
+  } else {
+    unsigned long long least = ~0ull, most = 0;
+    each([&](unsigned long long k, bool there, int, int) {
+      least = there && k < least ? k : least;
+      most = k < kAlways - 1 && k > most ? k : most;
+    });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+      const unsigned long long a = __shfl_xor(least, d), b = __shfl_xor(most, d);
+      least = a < least ? a : least;
+      most = b > most ? b : most;
+    }
+    if (lane == 0) {
+      s_low[wave] = least;
+      s_high[wave] = most;
     }
     __syncthreads();
-    prefix |= static_cast<unsigned long long>(s_found[0]) << shift;
-    mask |= 255ull << shift;
-    need -= s_found[1];
-    const bool whole = s_bins[s_found[0]] == need;          // all that match are taken
-    __syncthreads();
-    if (whole) break;
+    for (int w = 0; w < waves; ++w) {
+      least = s_low[w] < least ? s_low[w] : least;
+      most = s_high[w] > most ? s_high[w] : most;
+    }
+    low = least;
+    high = most + 1;
+    found = n;
+    for (int step = 0; found != count && high - low > 1; ++step) {
+      unsigned long long middle = low + ((high - low) >> 1);
+      if (step < 40) {
+        const double m = 0.5 * value_of(low) + 0.5 * value_of(high - 1);
+        const unsigned long long k = m == m ? key_of(m) : 0;
+        if (k > low && k < high) middle = k;
+      }
+      const int some = at_least(middle);
+      if (some >= count) {
+        low = middle;
+        found = some;
+      } else {
+        high = middle;
+      }
+    }
   }
-  // ---- indexes: a thread has a run of them ----
-  const int run = (n + threads - 1) / threads;
-  const int j0 = min(tid * run, n), j1 = min(j0 + run, n);
-  int above = 0, equal = 0;
-  for (int j = j0; j < j1; ++j) {
-    const unsigned long long k = keys[j] & mask;
-    above += k > prefix;
-    equal += k == prefix;
+  // ---- all above low, and of those that equal it (found is count: all of them) the first ones ----
+  int need = n;
+  if (found != count) {
+    need = count - count_of([&](unsigned long long k, bool) { return k > low; });
+    each([&](unsigned long long k, bool there, int, int i) {
+      const int some = __popcll(__ballot(there && k == low));
+      if (lane == 0) s_before[i * waves + wave] = some;
+    });
+    scan_counts();
   }
-  int total;
-  const int equal_before = block_prefix(equal, s_sums, &total);
-  const int taken_equal = min(max(need - equal_before, 0), equal);
-  int at = block_prefix(above + taken_equal, s_sums, &total), left = taken_equal;
-  for (int j = j0; j < j1; ++j) {
-    const unsigned long long k = keys[j] & mask;
-    if (k > prefix || (k == prefix && left-- > 0)) out[at++] = row[j];
-  }
+  unsigned long long taken = 0;      // a bit for each of the thread's keys
+  each([&](unsigned long long k, bool there, int, int i) {
+    const bool equal = there && k == low;
+    const int before = need < n ? s_before[i * waves + wave] + __popcll(__ballot(equal) & in_front) : 0;
+    taken |= static_cast<unsigned long long>(k > low || (equal && before < need)) << i;
+  });
+  write_taken(taken);
+}
+
+__device__ __forceinline__ void take_largest(const unsigned long long* keys, int n, int count, const int* row, int* out,
+                                             bool in_lds) {
+  if (in_lds && n <= kAloneThreads)
+    take_by_rank(keys, n, count, row, out);
+  else if (n <= 8 * static_cast<int>(blockDim.x))
+    take_many<8>(keys, n, count, row, out);
+  else
+    take_many<0>(keys, n, count, row, out);
 }
 
 template <int kD, bool kF16, bool kScore>
-__global__ void __launch_bounds__(kScore ? kThreads : kTakeThreads) page_take_kernel(KvCache c, Select s) {
+__global__ void __launch_bounds__(kScore ? kAloneThreads : kTakeThreads) page_take_kernel(KvCache c, Select s) {
   extern __shared__ unsigned long long s_keys[];
   const int unit = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
   const int u = unit % c.kv_heads, i = unit / c.kv_heads % s.tokens, b = unit / c.kv_heads / s.tokens;
@@ -340,17 +567,18 @@ __global__ void __launch_bounds__(kScore ? kThreads : kTakeThreads) page_take_ke
     const uint16_t* q = s.q + b * s.q_sb + i * s.q_st + static_cast<int64_t>(u) * s.group * s.q_sh;
     for (int tile = (tid >> 6) * 16; tile < see.have; tile += threads / 64 * 16) {
       const unsigned long long key = tile_keys<kD, kF16>(c, s, row, u, tile, see.have, q, s.q_sh);
-      if ((tid & 63) < 16 && tile + (tid & 15) < see.have) s_keys[tile + (tid & 15)] = key;
+      if ((tid & 63) < 16) s_keys[tile + (tid & 15)] = tile + (tid & 15) < see.have ? key : 0;
     }
     __syncthreads();
-    take_largest(s_keys, see.have, s.count, row, out);
+    take_largest(s_keys, see.have, s.count, row, out, true);
   } else {
-    take_largest(s.keys + static_cast<int64_t>(unit) * s.width, see.have, s.count, row, out);
+    take_largest(s.keys + static_cast<int64_t>(unit) * s.width, see.have, s.count, row, out, false);
   }
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+constexpr int kMostPages = kMostRuns * kTakeThreads;
 // Tables of up to so many pages keep their keys in LDS.
 constexpr int kMostInLds = 4096;
 // Pages that one workgroup scores by itself where there are not many units
@@ -411,9 +639,9 @@ VDN_API int vdn_cache_select(const void* q, int64_t q_sb, int64_t q_st, int64_t 
   const KvCache c{nullptr, nullptr, nullptr, nullptr, faults, pages, kv_heads,
                   page > 0 ? 31 - __builtin_clz(static_cast<unsigned>(page)) : 0};
   if (!cache_geometry_ok(c, page, head_dim) || batch < 0 || width <= 0 || tokens <= 0 || group <= 0 ||
-      (static_cast<int64_t>(width) << c.log_page) > (1ll << 31) - 1024)
-    return set_error(kInvalidArgument,
-                     "%s: bad geometry (page a power of two in 16..256, head_dim 64, 128 or 256)", name);
+      width > kMostPages || (static_cast<int64_t>(width) << c.log_page) > (1ll << 31) - 1024)
+    return set_error(kInvalidArgument, "%s: bad geometry (page a power of two in 16..256, head_dim 64, 128 or 256, "
+                     "tables of at most %d pages)", name, kMostPages);
   if (dtype != 0 && dtype != 1) return set_error(kInvalidArgument, "%s: dtype must be 0 (bf16) or 1 (fp16)", name);
   if (first < 0 || last < 1 || count < 1 || first > count - last)
     return set_error(kInvalidArgument, "%s: first >= 0, last >= 1, and count at least both", name);
@@ -437,7 +665,8 @@ VDN_API int vdn_cache_select(const void* q, int64_t q_sb, int64_t q_st, int64_t 
   const dim3 grid(static_cast<unsigned>(units));
   const auto launch = [&](auto scores, auto fused, auto take) {
     if (alone) {
-      hipLaunchKernelGGL(fused, grid, dim3(kThreads), 8u * width, st, c, s);
+      hipLaunchKernelGGL(fused, grid, dim3(kAloneThreads),
+                         8u * static_cast<unsigned>((width + 15) / 16 * 16), st, c, s);
     } else {
       hipLaunchKernelGGL(scores, dim3(static_cast<unsigned>(units * blocks)), dim3(kThreads), 0, st, c, s,
                          static_cast<int>(blocks));

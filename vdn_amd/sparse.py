@@ -25,6 +25,9 @@ from .kvcache import (KVCache, WHOLE_TOKENS, _DTYPES, _check_cache, _check_table
                       _workspace_bytes)
 
 
+MOST_PAGES = 65536   # of a table that pages are selected from
+
+
 def empty_means(cache: KVCache):
     """BF16 [pages, kv_heads, D] for write_means: the mean keys of the cache's pages, not yet set."""
     return torch.empty((*cache.k_scales.shape, cache.head_dim), dtype=torch.bfloat16, device=cache.device)
@@ -94,8 +97,8 @@ def select_pages(query, cache: KVCache, means, table, lengths, count, *, first=1
     _, kv_heads, page, _ = cache._geometry
     if table_batch != batch or width <= 0:
         raise ValueError("table must name at least one page for each sequence of the query")
-    if width * page > 2 ** 31 - 1024:
-        raise ValueError("the table is too wide")
+    if width > MOST_PAGES or width * page > 2 ** 31 - 1024:
+        raise ValueError(f"the table must not be wider than {MOST_PAGES} pages or 2^31 tokens")
     if any(type(n) is not int for n in (count, first, last)) or first < 0 or last < 1 or count < first + last:
         raise ValueError("count must be at least first + last, first >= 0, last >= 1")
     lead = query.shape[:-2]
