@@ -6,12 +6,10 @@
 //
 // Selection (vdn_cache_select): score(b, i, u, p) = max over the G query heads h of K/V head u of
 // q[b, i, h] . mean[p, u], in fp64: the products of 16-bit values are exact there and their sum nearly,
-// so that the order of two pages does not hang on the order of a sum. On 16x16x4 MFMAs with
-// the query rows as A and 16 pages as B, the maximum over the rows is over a lane's
-// four accumulators and the four lanes of its column. A page of the first or the last ones counts as
-// the largest, NaN as +inf. Of equal scores the page in front wins. Then a workgroup per (b, i, u)
-// takes the `count` best: by each page's rank, or where they are many by bisection for the least
-// score that is taken.
+// so that the order of two pages does not hang on the order of a sum. A page of the first or the last
+// ones counts as the largest, NaN as +inf. Of equal scores the page in front wins. Then a workgroup per
+// (b, i, u) takes the `count` best: by each page's rank, or where they are many by bins and the
+// ranks in the last one.
 #include "kv_cache.h"
 
 #include "attn_tiles.h"
@@ -20,8 +18,6 @@
 
 namespace vdn {
 namespace {
-
-typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
@@ -194,40 +190,53 @@ __device__ __forceinline__ unsigned long long key_of(double x) {
 
 constexpr unsigned long long kAlways = ~0ull;
 
-// Keys of pages tile .. tile + 15 of a unit: lane's page is tile + lane % 16 (every quarter of the wave
-// gets them). q rows: A, lane (row = lane % 16, quarter = lane / 16) holds channels
-// quarter D / 4 + s at step s; B the same of the pages.
+// Keys of pages tile .. tile + 15 of a unit: lane's page is tile + lane % 16 (every quarter of the wave gets
+// them). An MFMA has four blocks of 4 query rows (A) x 4 pages (B) x 4 channels: lane 16 k + 4 b + i holds row
+// i, or page 4 b + i, and channel k D / 4 + s at step s; the product of row i and page j of block b comes
+// to lane 16 i + 4 b + j. Four rows a time waste less of the group than an MFMA of 16 rows: 5 rows of 128
+// channels take 1024 cycles of the pipe for 16 pages instead of 2048.
 template <int kD, bool kF16>
 __device__ unsigned long long tile_keys(const KvCache& c, const Select& s, const int* row, int u, int tile,
                                         int have, const uint16_t* q, int64_t q_sh) {
   constexpr int kRun = kD / 4;      // channels of a lane
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, k = lane >> 4;
   const int at = tile + (lane & 15);
   const int id = at < have ? row[at] : 0;
   const bool there = id >= 0 && id < c.pages;
   if (!there) *c.faults = 1;
   u32x4 w[kRun / 8];
-  const uint16_t* m = s.means + (static_cast<int64_t>(there ? id : 0) * c.kv_heads + u) * kD + (lane >> 4) * kRun;
+  const uint16_t* m = s.means + (static_cast<int64_t>(there ? id : 0) * c.kv_heads + u) * kD + k * kRun;
 #pragma unroll
   for (int j = 0; j < kRun / 8; ++j) w[j] = *reinterpret_cast<const u32x4*>(m + 8 * j);
   double best = -INFINITY;
-  for (int r0 = 0; r0 < s.group; r0 += 16) {
-    const uint16_t* src = q + min(r0 + (lane & 15), s.group - 1) * q_sh + (lane >> 4) * kRun;
-    f64x4 acc = {0., 0., 0., 0.};
+  for (int r0 = 0; r0 < s.group; r0 += 8) {
+    // two row groups at a time (the second is the first again if there is none): two chains of MFMAs
+    const uint16_t* src[2];
+    u32x4 x[2][kRun / 8];
 #pragma unroll
-    for (int j = 0; j < kRun / 8; ++j) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(src + 8 * j);
+    for (int g = 0; g < 2; ++g) {
+      const int r = r0 + 4 * g < s.group ? r0 + 4 * g : r0;
+      src[g] = q + min(r + (lane & 3), s.group - 1) * q_sh + k * kRun;
+#pragma unroll
+      for (int j = 0; j < kRun / 8; ++j) x[g][j] = *reinterpret_cast<const u32x4*>(src[g] + 8 * j);
+    }
+    double acc[2] = {0., 0.};
+    const bool both = r0 + 4 < s.group;
+#pragma unroll
+    for (int j = 0; j < kRun / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint16_t a = static_cast<uint16_t>(x[i / 2] >> (16 * (i & 1)));
-        const uint16_t b = static_cast<uint16_t>(w[j][i / 2] >> (16 * (i & 1)));
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(
-            static_cast<double>(kF16 ? f16_bits_to_f32(a) : bf16_bits_to_f32(a)),
-            static_cast<double>(bf16_bits_to_f32(b)), acc, 0, 0, 0);
-      }
-    }
+        const double b = static_cast<double>(bf16_bits_to_f32(static_cast<uint16_t>(w[j][i / 2] >> (16 * (i & 1)))));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) best = fmax(best, isnan(acc[i]) ? INFINITY : acc[i]);
+        for (int g = 0; g < 2; ++g) {
+          if (g == 1 && !both) continue;
+          const uint16_t a = static_cast<uint16_t>(x[g][j][i / 2] >> (16 * (i & 1)));
+          acc[g] = __builtin_amdgcn_mfma_f64_4x4x4f64(
+              static_cast<double>(kF16 ? f16_bits_to_f32(a) : bf16_bits_to_f32(a)), b, acc[g], 0, 0, 0);
+        }
+      }
+    best = fmax(best, isnan(acc[0]) ? INFINITY : acc[0]);
+    if (both) best = fmax(best, isnan(acc[1]) ? INFINITY : acc[1]);
   }
   best = fmax(best, __shfl_xor(best, 16));
   best = fmax(best, __shfl_xor(best, 32));
