@@ -12,8 +12,10 @@
 // [-pi/4, pi/4] (x^9 and x^10: under 2^-28). A token's R/2 pairs are computed once for all its
 // heads, and shared through LDS.
 //
-// A row's lane holds channels 4 l .. + 4 and R/2 + 4 l .. + 4 (half layout) or 8 l .. + 8, so both channels
-// of a pair are in one lane: no exchange but the norm's sum.
+// A row's lane holds V = 8 (or 4) channels from V l and from R/2 + V l on (half layout) or 2 V from 2 V l on,
+// so both channels of a pair are in one lane: no exchange but the norm's sum. Moving q and k once bounds
+// it: 32768 tokens of 40 + 8 heads x 128, both norms, 805 MB in 147 us (5.5 TB/s; a large copy 5.1, a
+// negation 6.3).
 #include "common.h"
 
 #include <math.h>
@@ -41,7 +43,7 @@ struct RotaryArgs {
   int heads, all_heads;    // query heads; query and key heads
   int rot;
   int wide_positions, w_f32;
-  int block_tokens, block_heads;   // of a workgroup
+  int block_tokens;        // of a workgroup
   float amplitude, eps;
 };
 
@@ -64,46 +66,47 @@ __device__ __forceinline__ float widen(uint32_t w, int hi) {
   return kF16 ? f16_bits_to_f32(h) : bf16_bits_to_f32(h);
 }
 
-template <bool kF16>
-__device__ __forceinline__ u32x2 pack4(const float* y) {
-  u32x2 r;
+// Streams past the caches: what is written is not read again here.
+template <bool kF16, int kV>
+__device__ __forceinline__ void store(const float* y, uint16_t* dst) {
+  typedef unsigned int words __attribute__((ext_vector_type(kV / 2)));
+  words r;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < kV / 2; ++i)
     r[i] = kF16 ? f32_to_f16_bits(y[2 * i]) | static_cast<uint32_t>(f32_to_f16_bits(y[2 * i + 1])) << 16
                 : pack_bf16x2(y[2 * i], y[2 * i + 1]);
-  return r;
+  __builtin_nontemporal_store(r, reinterpret_cast<words*>(dst));
 }
 
-template <int kD, bool kHalf, bool kF16>
+template <int kD, bool kHalf, bool kF16, int kV>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
-  constexpr int kLanes = kD / 8;                // of a row
+  constexpr int kLanes = kD / (2 * kV);         // of a row
+  typedef unsigned int words __attribute__((ext_vector_type(kV / 2)));
   constexpr int kRows = kThreads / kLanes;      // rows at a time
   __shared__ float s_cos[kMostTokens][kD / 2], s_sin[kMostTokens][kD / 2];
   __shared__ float s_w[2][kD];
   const int tid = threadIdx.x, l = tid % kLanes;
   const int64_t token0 = static_cast<int64_t>(blockIdx.x) * a.block_tokens;
   const int n_tokens = static_cast<int>(min(static_cast<int64_t>(a.block_tokens), a.tokens - token0));
-  const int head0 = blockIdx.y * a.block_heads;
-  const int n_heads = min(a.block_heads, a.all_heads - head0);
-  const int rows = n_tokens * n_heads;
-  const bool turned = 8 * l < a.rot;
-  const int c0 = kHalf && turned ? 4 * l : 8 * l;
-  const int c1 = kHalf && turned ? a.rot / 2 + 4 * l : 8 * l + 4;
+  const int rows = n_tokens * a.all_heads;
+  const bool turned = 2 * kV * l < a.rot;
+  const int c0 = kHalf && turned ? kV * l : 2 * kV * l;
+  const int c1 = kHalf && turned ? a.rot / 2 + kV * l : 2 * kV * l + kV;
 
   struct Row {
-    u32x2 lo, hi;
+    words lo, hi;
     int token, head;   // head: among queries and keys
   };
   auto load = [&](int r) __attribute__((always_inline)) {
     Row x;
     r = min(r, rows - 1);
-    x.token = r / n_heads;
-    x.head = head0 + r - x.token * n_heads;
+    x.token = r / a.all_heads;
+    x.head = r - x.token * a.all_heads;
     const bool is_k = x.head >= a.heads;
     const RotaryRows& io = is_k ? a.k : a.q;
     const uint16_t* p = io.x + (token0 + x.token) * io.st + (x.head - (is_k ? a.heads : 0)) * io.sh;
-    x.lo = *reinterpret_cast<const u32x2*>(p + c0);
-    x.hi = *reinterpret_cast<const u32x2*>(p + c1);
+    x.lo = *reinterpret_cast<const words*>(p + c0);
+    x.hi = *reinterpret_cast<const words*>(p + c1);
     return x;
   };
   int r = tid / kLanes;
@@ -135,43 +138,49 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
     const Row x = next;
     next = load(r + kRows);
     const bool is_k = x.head >= a.heads;
-    float y[8];
+    float y[2 * kV];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kV; ++i) {
       y[i] = widen<kF16>(x.lo[i / 2], i & 1);
-      y[4 + i] = widen<kF16>(x.hi[i / 2], i & 1);
+      y[kV + i] = widen<kF16>(x.hi[i / 2], i & 1);
     }
     const RotaryRows& io = is_k ? a.k : a.q;
     if (io.w != nullptr) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += y[i] * y[i];
+      for (int i = 0; i < 2 * kV; ++i) sum += y[i] * y[i];
 #pragma unroll
       for (int d = 1; d < kLanes; d <<= 1) sum += __shfl_xor(sum, d);
       const float scale = rsqrtf(sum * (1.f / kD) + a.eps);
-      const f32x4 w0 = *reinterpret_cast<const f32x4*>(&s_w[is_k][c0]);
-      const f32x4 w1 = *reinterpret_cast<const f32x4*>(&s_w[is_k][c1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[i] *= scale * w0[i];
-        y[4 + i] *= scale * w1[i];
+      for (int j = 0; j < kV; j += 4) {
+        const f32x4 w0 = *reinterpret_cast<const f32x4*>(&s_w[is_k][c0 + j]);
+        const f32x4 w1 = *reinterpret_cast<const f32x4*>(&s_w[is_k][c1 + j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y[j + i] *= scale * w0[i];
+          y[kV + j + i] *= scale * w1[i];
+        }
       }
     }
     if (turned) {
-      const f32x4 c = *reinterpret_cast<const f32x4*>(&s_cos[x.token][4 * l]);
-      const f32x4 s = *reinterpret_cast<const f32x4*>(&s_sin[x.token][4 * l]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float& p = kHalf ? y[i] : y[2 * i];
-        float& q = kHalf ? y[4 + i] : y[2 * i + 1];
-        const float u = p * c[i] - q * s[i], v = q * c[i] + p * s[i];
-        p = u;
-        q = v;
+      for (int j = 0; j < kV; j += 4) {
+        const f32x4 c = *reinterpret_cast<const f32x4*>(&s_cos[x.token][kV * l + j]);
+        const f32x4 s = *reinterpret_cast<const f32x4*>(&s_sin[x.token][kV * l + j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float& p = kHalf ? y[j + i] : y[2 * (j + i)];
+          float& q = kHalf ? y[kV + j + i] : y[2 * (j + i) + 1];
+          const float u = p * c[i] - q * s[i], v = q * c[i] + p * s[i];
+          p = u;
+          q = v;
+        }
       }
     }
     uint16_t* dst = io.out + (token0 + x.token) * io.o_st + (x.head - (is_k ? a.heads : 0)) * io.o_sh;
-    *reinterpret_cast<u32x2*>(dst + c0) = pack4<kF16>(y);
-    *reinterpret_cast<u32x2*>(dst + c1) = pack4<kF16>(y + 4);
+    store<kF16, kV>(y, dst + c0);
+    store<kF16, kV>(y + kV, dst + c1);
   }
 }
 
@@ -207,35 +216,37 @@ VDN_API int vdn_rotary(const void* q, int64_t q_st, int64_t q_sh, const void* k,
   if (!aligned(positions, wide_positions ? 8 : 4) || !aligned(q_w, w_f32 ? 4 : 2) || !aligned(k_w, w_f32 ? 4 : 2))
     return set_error(kInvalidArgument, "%s: positions and weights need their type's alignment", name);
 
-  // Where rows are few, a workgroup per token and per pass over some of its heads; else a few tokens a
-  // workgroup with all their heads, enough rows for several passes.
-  const int pass = kThreads / (head_dim / 8), all = heads + kv_heads;
-  int block_tokens = 1, block_heads = all;
-  if (tokens * all >= 8ll * pass * 4 * cu_count()) {
-    block_tokens = std::min(kMostTokens, std::max(4, (4 * pass + all - 1) / all));
-  } else if (tokens < 4ll * cu_count()) {
-    block_heads = std::min(pass, all);
-  }
+  // 16-byte pieces where channels, strides and addresses allow them: 147 us against 172 with 8-byte ones
+  // (32768 tokens, 40 + 8 heads x 128, both norms).
+  bool wide = rot % 16 == 0;
+  for (const int64_t s : {q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh}) wide &= s % 8 == 0;
+  for (const void* p : {q, k, static_cast<const void*>(qo), static_cast<const void*>(ko)}) wide &= aligned(p, 16);
+  // A workgroup has a token's heads, or those of several tokens where they are few: about three rows for
+  // each place of a pass. Longer ones leave too few loads under way (4 tokens of 48 heads: 161 us against 147),
+  // parts of a token's heads compute its angles again (200 us with one pass).
+  const int all = heads + kv_heads, pass = kThreads / (head_dim / (wide ? 16 : 8));
+  const int block_tokens = std::min(kMostTokens, std::max(1, 3 * pass / all));
   const int64_t blocks = (tokens + block_tokens - 1) / block_tokens;
   if (blocks > (1ll << 31) / kThreads) return set_error(kUnsupported, "%s: too many tokens", name);
   const RotaryArgs a{
       {static_cast<const uint16_t*>(q), static_cast<uint16_t*>(qo), q_w, q_st, q_sh, qo_st, qo_sh},
       {static_cast<const uint16_t*>(k), static_cast<uint16_t*>(ko), k_w, k_st, k_sh, ko_st, ko_sh},
       positions, static_cast<const uint64_t*>(steps), tokens, heads, all, rot, wide_positions, w_f32,
-      block_tokens, block_heads, amplitude, eps};
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>((all + block_heads - 1) / block_heads));
+      block_tokens, amplitude, eps};
   const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
   };
-#define VDN_ROT(D)                                                                                \
-  interleaved ? (dtype ? launch(rotary_kernel<D, false, true>) : launch(rotary_kernel<D, false, false>)) \
-              : (dtype ? launch(rotary_kernel<D, true, true>) : launch(rotary_kernel<D, true, false>))
+#define VDN_ROT(D, V)                                                                                \
+  interleaved ? (dtype ? launch(rotary_kernel<D, false, true, V>) : launch(rotary_kernel<D, false, false, V>)) \
+              : (dtype ? launch(rotary_kernel<D, true, true, V>) : launch(rotary_kernel<D, true, false, V>))
+#define VDN_ROT_V(D) wide ? (VDN_ROT(D, 8)) : (VDN_ROT(D, 4))
   if (head_dim == 64)
-    VDN_ROT(64);
+    VDN_ROT_V(64);
   else if (head_dim == 128)
-    VDN_ROT(128);
+    VDN_ROT_V(128);
   else
-    VDN_ROT(256);
+    VDN_ROT_V(256);
+#undef VDN_ROT_V
 #undef VDN_ROT
   return check_launch(name);
 }
