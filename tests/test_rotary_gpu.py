@@ -106,6 +106,25 @@ def test_in_place_strides_and_nonfinite_rows(device):
     assert torch.equal(buffer[:, :, 2], beside)
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@torch.no_grad()
+def test_rows_at_odd_8_bytes(device, layout):
+    """Rows that are 8-byte but not 16-byte aligned take the narrower pieces."""
+    buffer = torch.randn(50, 9 * 128 + 4).to(FP16).cuda()
+    plan = vr.prepare_rotary_plan(128, rotary_dim=96, layout=layout, device="cuda")
+    positions = torch.arange(50).cuda()
+    w = torch.rand(128).to(FP16).cuda()
+    q, k = (buffer[:, 4 + a:4 + a + n * 128].unflatten(1, (n, 128)) for a, n in ((0, 7), (7 * 128, 2)))
+    assert q.data_ptr() % 16 == 8
+    want = vr.rotate_qk(q.contiguous(), k.contiguous(), positions, plan, w, w)
+    got = vr.rotate_qk(q, k, positions, plan, w, w)
+    for a, b in zip(got, want):      # the norm's sum is over 16 lanes instead of 8
+        assert ((a.float() - b.float()).abs() <= torch.finfo(FP16).eps * b.float().abs() + 2.0 ** -24).all()
+    frequencies, _ = vr.rotary_frequencies(96)
+    check(got[0], q, positions, frequencies, plan, w)
+    check(got[1], k, positions, frequencies, plan, w)
+
+
 @torch.no_grad()
 def test_rows_behind_2_31_elements(device):
     """Head rows of a strided buffer beyond 2^31 elements."""

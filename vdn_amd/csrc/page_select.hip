@@ -461,14 +461,14 @@ __device__ void take_many(const unsigned long long* keys, int n, int count, cons
   __syncthreads();
   int turn = 0;
   // Keys that `what` says yes to, over the workgroup: a ballot each, one atomic a wave, one barrier. The
-  // three counters go round: one is summed, one may still be read, one is cleared.
+  // three counters go round: one is summed, the last call's may still be read, the next call's is cleared.
   auto count_of = [&](auto what) __attribute__((always_inline)) {
     int mine = 0;
     each([&](unsigned long long k, bool there, int, int) { mine += __popcll(__ballot(what(k, there))); });
     if (lane == 0) atomicAdd(&s_counts[turn], mine);
     const int last = turn;
     turn = turn == 2 ? 0 : turn + 1;
-    if (tid == 0) s_counts[turn == 2 ? 0 : turn + 1] = 0;
+    if (tid == 0) s_counts[turn] = 0;   // the next call's: it was read in front of the last barrier
     __syncthreads();
     return s_counts[last];
   };

@@ -650,7 +650,7 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
     return set_error(kInvalidArgument, "%s: codes, rows and the plan need 16-byte alignment", name);
   const int64_t rows = static_cast<int64_t>(tokens) * group, out_rows = rows * kv_heads * batch;
   if (out_rows * kThreads >= (1ll << 32) || rows * batch > (1ll << 31) - 512 ||
-      static_cast<int64_t>(n_items) * kv_heads * kThreads >= (1ll << 32))
+      (static_cast<int64_t>(n_items) * kv_heads + (1 << 16)) * kThreads >= (1ll << 32))
     return set_error(kUnsupported, "%s: too many query rows", name);
   if (static_cast<int64_t>(batch) *
           (((static_cast<int64_t>(width) << c.log_page) + units::kQuad - 1) / units::kQuad + units::kUnitCost) >

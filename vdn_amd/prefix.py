@@ -93,7 +93,7 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
         pieces = np.where(blocks > 0, _cut(tiles, blocks * kv_heads, cus * _WORKGROUPS_PER_CU[head_dim] * 7 // 8), 0)
     made = pieces * blocks
     base = made.cumsum() - made
-    if int(made.sum()) * kv_heads >= 2 ** 24:
+    if int(made.sum()) * kv_heads >= 2 ** 24 - 2 ** 16:
         raise ValueError("too many rows for one plan")
     # a prefix's items, piece by piece; its tiles are spread evenly over the pieces
     p = np.repeat(np.arange(len(lengths)), made)
@@ -175,7 +175,7 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
     return (out, lse) if return_lse else out
 
 
-@lru_cache(maxsize=None)
+@lru_cache(maxsize=4096)
 def _workspace_bytes(device_index, items, batch, width, page, tokens, group, kv_heads, head_dim):
     nbytes = ctypes.c_int64(0)
     _lib.call_on(device_index, "vdn_prefix_attention_workspace", items, batch, width, page, tokens, group,

@@ -125,7 +125,8 @@ def rotate_qk(query, key, positions, plan: RotaryPlan, q_weight=None, k_weight=N
 
     BF16 or FP16, unit channel stride; positions int32 or int64 [tokens], any values. With q_weight (k_weight),
     [D] of the activation dtype or FP32, a query (key) head is first divided by the root of its
-    mean square plus eps and multiplied by the weight. Both in fp32, rounded once. Channels from
+    mean square plus eps and multiplied by the weight (its squares have to be within fp32's range). All in
+    fp32, rounded once. Channels from
     plan.rotary_dim on are not turned; plan.amplitude multiplies the turned ones only.
 
     Returns two fresh contiguous tensors, or `out`, a pair of views to write to: these may be query and key

@@ -44,7 +44,8 @@ def write_means(cache: KVCache, means, table, starts, lengths):
     """Sets the mean key of every page that holds tokens starts[i] .. lengths[i] - 1 of a sequence (int32
     [batch] each): over all the page's tokens in front of lengths[i], from the codes that the cache holds,
     rounded once to BF16. Call it after write_cache, with its starts and the new lengths. A NaN key
-    makes its channel's mean NaN. Other pages' means stay as they are."""
+    makes its channel's mean NaN. Other pages' means stay as they are. Sequences may share full pages, but
+    not one that is partly filled to different lengths in the same call."""
     index, args = _check_cache(cache, "write_means")
     _check_means(cache, means, index)
     batch, width, t_st = _check_table(table, index)
@@ -179,7 +180,7 @@ def selected_attention(query, cache: KVCache, pages, tokens, scale=None, *, retu
     return (out, lse) if return_lse else out
 
 
-@lru_cache(maxsize=None)
+@lru_cache(maxsize=4096)
 def _select_bytes(device_index, batch, tokens, kv_heads, width):
     nbytes = ctypes.c_int64(0)
     _lib.call_on(device_index, "vdn_cache_select_workspace", batch, tokens, kv_heads, width,
