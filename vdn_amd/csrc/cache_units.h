@@ -164,7 +164,8 @@ struct Half<true> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    return f32_to_f16_bits(a) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16;
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(a), static_cast<_Float16>(b)});
   }
   // An output: E4M3 takes values next to fp16's largest one to 65536, which would be an infinity.
   static __device__ __forceinline__ uint32_t pack_out(float a, float b) {

@@ -87,7 +87,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
   constexpr int kKJ = kD / 32;            // a lane's 16-byte reads of a key
   constexpr int kSegs = kD / 64;          // 1 KB segments of K and of V that a wave loads
   constexpr int kIds = kBig ? 1 : 4;
-  constexpr float kLazy = kF16 ? 4.f : 8.f, kAbove = kF16 ? 11.f : 0.f;
+  constexpr float kAbove = kF16 ? 11.f : 0.f;   // m: the running maximum less kAbove (cache_attn.hip)
   typedef Elem<kF16> E;
   typedef typename E::x8 x8;
   // one array per buffer: the compiler then tells a prefetch into one from reads of the other
@@ -328,7 +328,9 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
       apart = __any(apart);
     }
 
-    // ---- softmax: the scores times K's scale, m lagging the running maximum (causal_attn.hip) ----
+    // ---- softmax: the scores times K's scale. m follows the running maximum at once, so that the heaviest
+    // weight is a power of two and not rounded: outputs within 2.1e-3 relative of 64 bits in bf16, where
+    // their own rounding makes 1.7e-3; with an m that may lag by 2^8 it is 2.3e-3, and 4% faster ----
     [[maybe_unused]] const int left = it.tokens - t * kBN;     // tokens of the tile
     if constexpr (kTail) {
 #pragma unroll
@@ -347,7 +349,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
       mx = fmaxf(mx, top * k_scale[kt]);
     }
     mx = max_halves(mx);
-    const bool grow = mx > m + (kLazy + kAbove);
+    const bool grow = mx > m + kAbove;
     if (__any(grow)) {
       const float m_new = grow ? mx - kAbove : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;

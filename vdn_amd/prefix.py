@@ -23,6 +23,11 @@ from .sparse import _check_query
 BLOCK_ROWS = 128   # query rows of a prefix that a workgroup takes
 TILE = 64          # tokens of its step
 LEAST_TILES = 2    # of a piece, where the prefix has more
+# The pieces leave an eighth of the card's places to the tails, or half of them where even so the longest
+# is shorter than this: the tails then take as long as the pieces. 46 sequences behind 12 prompts of up
+# to 4097 tokens: 21.3 us against 23.7, 36 behind 8 of up to 2000, 40 heads: 23.0, 27.4; with 16, 16
+# sequences behind 4 prompts of 8000 - 16384: 39.3 against 28.5.
+SHORT_TILES = 8
 _WORKGROUPS_PER_CU = {64: 2, 128: 2, 256: 1}
 
 
@@ -90,7 +95,11 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     tiles = -(-n // TILE)
     pieces = np.zeros_like(n)
     if int((blocks * tiles).sum()):
-        pieces = np.where(blocks > 0, _cut(tiles, blocks * kv_heads, cus * _WORKGROUPS_PER_CU[head_dim] * 7 // 8), 0)
+        places = cus * _WORKGROUPS_PER_CU[head_dim]
+        for share in (7 / 8, 1 / 2):
+            pieces = np.where(blocks > 0, _cut(tiles, blocks * kv_heads, int(places * share)), 0)
+            if int((-(-tiles // np.maximum(pieces, 1)))[blocks > 0].max()) >= SHORT_TILES:
+                break
     made = pieces * blocks
     base = made.cumsum() - made
     if int(made.sum()) * kv_heads >= 2 ** 24 - 2 ** 16:
