@@ -264,17 +264,28 @@ __device__ __forceinline__ double value_of(unsigned long long key) {
 // among all, which lie in LDS with zeros (less than any key) up to a multiple of 8.
 __device__ void take_by_rank(const unsigned long long* keys, int n, int count, const int* row, int* out) {
   __shared__ int s_sums[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int at = min(tid, n - 1);
-  const int page = row[at];
-  const unsigned long long mine = keys[at];
-  int rank = 0;
-  for (int j = 0; j < n; j += 8) {
-    unsigned long long k[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int first = wave * 64;         // of the wave's keys
+  int rank = count, page = 0;          // a wave without keys takes none
+  if (first < n) {
+    const int at = min(tid, n - 1);
+    page = row[at];
+    // in front of the wave's own keys an equal one counts as larger, behind them it does not
+    const unsigned long long mine = keys[at];
+    rank = 0;
+    auto larger = [&](int j0, int j1, auto bound) __attribute__((always_inline)) {   // j0, j1 multiples of 8
+      for (int j = j0; j < j1; j += 8) {
+        unsigned long long k[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) k[i] = keys[j + i];
+        for (int i = 0; i < 8; ++i) k[i] = keys[j + i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) rank += k[i] > mine || (k[i] == mine && j + i < tid);
+        for (int i = 0; i < 8; ++i) rank += k[i] > bound(j + i);
+      }
+    };
+    const int end = (n + 7) / 8 * 8;
+    larger(0, first, [&](int) { return mine - 1; });
+    larger(first, min(first + 64, end), [&](int j) { return j < tid ? mine - 1 : mine; });
+    larger(first + 64, end, [&](int) { return mine; });
   }
   const bool taken = tid < n && rank < count;
   const unsigned long long all = __ballot(taken);
