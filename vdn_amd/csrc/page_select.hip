@@ -2,14 +2,16 @@
 //
 // Means (vdn_cache_means): mean[p, u] = sum over the page's tokens of K, / n, rounded once to bf16.
 // E4M3 values are multiples of 2^-9 up to 448, so 64 of them add up exactly in fp32: a lane's share of any
-// page. The lanes' sums meet in fp64. Reading the codes bounds it.
+// page. The lanes' sums meet in fp64. Reading the codes bounds it: 34 MB of 8 prompts of 2048 - 8192 tokens x 8 x
+// 128 in 5.2 us (in part from the cache in front of HBM). A wave has a page and head to itself: no barrier.
 //
 // Selection (vdn_cache_select): score(b, i, u, p) = max over the G query heads h of K/V head u of
 // q[b, i, h] . mean[p, u], in fp64: the products of 16-bit values are exact there and their sum nearly,
 // so that the order of two pages does not hang on the order of a sum. A page of the first or the last
 // ones counts as the largest, NaN as +inf. Of equal scores the page in front wins. Then a workgroup per
 // (b, i, u) takes the `count` best: by each page's rank, or where they are many by bins and the
-// ranks in the last one.
+// ranks in the last one. Latency and the conversions to fp64 bound it: 64 sequences of up to 128 pages, 40 heads
+// on 8 x 128: 11.7 us; 8192 pages, 56 heads on 8: 10.5 for the scores and 8.5 for the taking.
 #include "kv_cache.h"
 
 #include "attn_tiles.h"

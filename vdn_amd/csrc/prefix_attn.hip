@@ -4,9 +4,10 @@
 //                  j < len_b - Q + 1 + i) of scale q[b, i, h] . k[j, u], times v[j, u];   u = h / G
 //
 // The rows (sequence, i, g) of a prefix that share a K/V head are cut into blocks of 128; the host's plan
-// cuts the prefix's tokens into pieces, so that all blocks' pieces fill the card once. A
+// cuts the prefix's tokens into pieces, so that all blocks' pieces fill most of the card once. A
 // workgroup takes one piece for one block: four waves of 32 rows, tiles of 64 tokens whose codes
-// go global -> LDS, double-buffered, and are widened to 16 bits by each wave as it reads them.
+// go global -> LDS, double-buffered, and are widened to 16 bits by each wave as it reads them. (128 rows: one
+// reading of the codes serves many sequences, and two workgroups of 128 channels fit a CU.)
 //   Sᵀ[key][row] = K Qᵀ on 32x32x16 MFMAs; row r of the A operand is key 16 (r / 4 % 2) + 4 (r / 8)
 //     + r % 4, so that half h of the wave ends up with the scores of keys 16 h .. 16 h + 15
 //   Oᵀ += Vᵀ Pᵀ: those are the keys of one 16-byte read of a channel of the transposed V page, and
@@ -14,8 +15,15 @@
 // K's scale multiplies the scores in fp32; V's goes into the widening (bf16), or is taken relative to
 // the tile's largest one (fp16, as in cache_attn.hip). P is rounded to 16 bits, its sum keeps fp32.
 //
-// Each piece leaves maximum, sum and O of its rows in fp32, cache_attn.hip's kernel the same of the
-// tails, and a last kernel joins them in order (no atomics: the same call gives the same bits).
+// Each piece leaves maximum, sum and O of its rows in fp32, other workgroups of the launch, with the decode
+// kernel's code, the same of the tails, and a second kernel joins them in order (no atomics: the
+// same call gives the same bits).
+//
+// VALU work bounds it, with the MFMAs beside it and the clock at the power limit: of a wave's 32 rows and
+// 64 tokens x 128 channels, 128 conversions and 160 instructions of softmax go with 32 MFMAs (60 and
+// 36% of the time busy). 128 sequences behind 65536 tokens, 40 heads on 8 x 128, tails of 16 - 1000: 213 us,
+// 0.81 PFLOP/s; a large library product reaches 1.24. Short prefixes are bound by latency: 4 sequences
+// behind 500 tokens, 12 heads on 2 x 64: 6.9 us and 3.6 of the join.
 #include "cache_units.h"
 
 #include <algorithm>
