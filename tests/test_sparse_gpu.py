@@ -172,6 +172,23 @@ def test_selection_of_long_sequences(device, length, count):
     check_selection(q, cache, means, table, [length, 40], count, 1, 1, got)
 
 
+@pytest.mark.parametrize("pages_of_one", [100, 300, 1100])
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (128, FP16), (256, BF16), (256, FP16)])
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (4, 1), (5, 1), (8, 1), (9, 1), (36, 2)])
+@torch.no_grad()
+def test_selection_of_every_group(device, pages_of_one, dim, dtype, heads, kv_heads):
+    """Groups that end in the first and second four rows, scored by the workgroup that takes or by a
+    grid over all pages."""
+    g = torch.Generator().manual_seed(heads)
+    table, pages = tables([pages_of_one, pages_of_one - 7])
+    cache = kv.empty_cache(pages, kv_heads, dim, 16, device="cuda")
+    means = torch.randn(pages, kv_heads, dim, generator=g).to(BF16).cuda()
+    q = torch.randn(2, 1, heads, dim, generator=g).to(dtype).cuda()
+    lengths = [16 * pages_of_one - 3, 16 * (pages_of_one - 7)]
+    got = sp.select_pages(q, cache, means, table.cuda(), ints(*lengths), 20)
+    check_selection(q, cache, means, table, lengths, 20, 1, 1, got)
+
+
 @pytest.mark.parametrize("spread", ["even", "alike", "two", "infinite"])
 @torch.no_grad()
 def test_selection_where_scores_crowd(device, spread):

@@ -17,6 +17,7 @@
 #include "attn_tiles.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vdn {
 namespace {
@@ -211,34 +212,40 @@ __device__ unsigned long long tile_keys(const KvCache& c, const Select& s, const
 #pragma unroll
   for (int j = 0; j < kRun / 8; ++j) w[j] = *reinterpret_cast<const u32x4*>(m + 8 * j);
   double best = -INFINITY;
-  for (int r0 = 0; r0 < s.group; r0 += 8) {
-    // two row groups at a time (the second is the first again if there is none): two chains of MFMAs
-    const uint16_t* src[2];
-    u32x4 x[2][kRun / 8];
+  // Four rows, or eight in two chains of MFMAs. Each chain is one block of code with the reads of its results: a
+  // branch inside it (to leave the second out) led to reads without the wait that they need.
+  auto rows = [&](int r0, auto groups_tag) __attribute__((always_inline)) {
+    constexpr int kGroups = decltype(groups_tag)::value;
+    u32x4 x[kGroups][kRun / 8];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int r = r0 + 4 * g < s.group ? r0 + 4 * g : r0;
-      src[g] = q + min(r + (lane & 3), s.group - 1) * q_sh + k * kRun;
+    for (int g = 0; g < kGroups; ++g) {
+      const uint16_t* src = q + min(r0 + 4 * g + (lane & 3), s.group - 1) * q_sh + k * kRun;
 #pragma unroll
-      for (int j = 0; j < kRun / 8; ++j) x[g][j] = *reinterpret_cast<const u32x4*>(src[g] + 8 * j);
+      for (int j = 0; j < kRun / 8; ++j) x[g][j] = *reinterpret_cast<const u32x4*>(src + 8 * j);
     }
-    double acc[2] = {0., 0.};
-    const bool both = r0 + 4 < s.group;
+    double acc[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) acc[g] = 0.;
 #pragma unroll
     for (int j = 0; j < kRun / 8; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const double b = static_cast<double>(bf16_bits_to_f32(static_cast<uint16_t>(w[j][i / 2] >> (16 * (i & 1)))));
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          if (g == 1 && !both) continue;
+        for (int g = 0; g < kGroups; ++g) {
           const uint16_t a = static_cast<uint16_t>(x[g][j][i / 2] >> (16 * (i & 1)));
           acc[g] = __builtin_amdgcn_mfma_f64_4x4x4f64(
               static_cast<double>(kF16 ? f16_bits_to_f32(a) : bf16_bits_to_f32(a)), b, acc[g], 0, 0, 0);
         }
       }
-    best = fmax(best, isnan(acc[0]) ? INFINITY : acc[0]);
-    if (both) best = fmax(best, isnan(acc[1]) ? INFINITY : acc[1]);
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) best = fmax(best, isnan(acc[g]) ? INFINITY : acc[g]);
+  };
+  for (int r0 = 0; r0 < s.group; r0 += 8) {
+    if (r0 + 4 < s.group)
+      rows(r0, std::integral_constant<int, 2>{});
+    else
+      rows(r0, std::integral_constant<int, 1>{});
   }
   best = fmax(best, __shfl_xor(best, 16));
   best = fmax(best, __shfl_xor(best, 32));
