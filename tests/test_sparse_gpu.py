@@ -304,6 +304,28 @@ def test_attention_over_selected_pages(device, page, dim, dtype, heads, kv_heads
     cache.check()
 
 
+@pytest.mark.parametrize("batch,kv_heads,dim,count", [(70, 8, 128, 9), (130, 3, 64, 40), (40, 8, 256, 3)])
+@torch.no_grad()
+def test_many_queries_a_workgroup_each(device, batch, kv_heads, dim, count):
+    """As many units as the card has places, short and empty ones among them."""
+    g = torch.Generator().manual_seed(batch)
+    page = 16
+    lengths = torch.randint(0, 50 * page, (batch,), generator=g).tolist()
+    lengths[3], lengths[5] = 0, 1
+    table, pages = tables([-(-n // page) for n in lengths])
+    cache, *values = filled(pages, kv_heads, dim, page)
+    q = torch.randn(batch, 1, 2 * kv_heads, dim, generator=g).to(BF16).cuda()
+    means = sp.empty_means(cache)
+    sp.write_means(cache, means, table.cuda(), torch.zeros(batch, dtype=torch.int32).cuda(), ints(*lengths))
+    got = sp.select_pages(q, cache, means, table.cuda(), ints(*lengths), count)
+    out, lse = sp.selected_attention(q, cache, *got, return_lse=True)
+    some = [0, 3, 5, batch // 2, batch - 1]
+    check_attention(q[some], values, page, got[0][some], got[1][some], out[some], lse[some], dim ** -0.5)
+    again = sp.selected_attention(q[7:8], cache, got[0][7:8].contiguous(), got[1][7:8].contiguous())
+    assert (again - out[7:8]).abs().max() <= 2.0 ** -6 * out[7:8].abs().max()       # alone it may be split
+    cache.check()
+
+
 @torch.no_grad()
 def test_all_pages_are_the_dense_attention(device):
     """A selection that leaves nothing out gives cache_attention's bits, steps of a prompt and behind it."""

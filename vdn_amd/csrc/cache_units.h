@@ -61,9 +61,10 @@ __host__ __device__ __forceinline__ bool few_suffice(const Split& sp, int64_t to
   return sp.few > 0 && (few > sp.beside ? few : sp.beside) < sp.beside + cost / sp.workgroups;
 }
 
-// How many workgroups share `total` costs: all, behind the other work, or the few.
+// How many workgroups share `total` costs: all (kBeside: behind the other work, or the few).
+template <bool kBeside>
 __device__ __forceinline__ int sharers(const Split& sp, int64_t total) {
-  const int n = few_suffice(sp, total) ? min(sp.workgroups, sp.few) : sp.workgroups;
+  const int n = kBeside && few_suffice(sp, total) ? min(sp.workgroups, sp.few) : sp.workgroups;
   return static_cast<int>(min(total, static_cast<int64_t>(n)));
 }
 
@@ -105,6 +106,7 @@ __device__ __forceinline__ int wave_prefix(int x, int lane) {   // inclusive
   return x;
 }
 
+template <bool kBeside>
 __device__ inline Place find_share(const KvCache& c, const Lengths& s, const Split& sp, int units, int wg) {
   const int lane = threadIdx.x & 63;
   const int strip = (s.batch + 63) / 64;
@@ -114,7 +116,7 @@ __device__ inline Place find_share(const KvCache& c, const Lengths& s, const Spl
   const int incl = wave_prefix(mine, lane);
   Place p;
   const int64_t total = static_cast<int64_t>(__builtin_amdgcn_readlane(incl, 63)) * units;
-  const int n_wg = sharers(sp, total);
+  const int n_wg = sharers<kBeside>(sp, total);
   p.from = wg < n_wg ? share_from(total, n_wg, wg) : total;
   p.to = wg < n_wg ? share_from(total, n_wg, wg + 1) : total;
   const int64_t at = p.from;
@@ -134,6 +136,13 @@ __device__ inline Place find_share(const KvCache& c, const Lengths& s, const Spl
   p.before = static_cast<int64_t>(before) * units;
   p.seq = seq;
   return p;
+}
+
+// Unit wg, whole, as a share of its own.
+__device__ __forceinline__ Place place_of(const KvCache& c, const Lengths& s, const Split& sp, int units, int wg) {
+  const int b = wg / units;
+  const int64_t at = static_cast<int64_t>(wg - b * units) * cost_of(sp, seq_tokens(c, s, b));
+  return Place{at, at + 1, 0, b};
 }
 
 template <bool kF16>
@@ -200,18 +209,31 @@ __device__ __forceinline__ float inverse_of(float sum, int keys) {
   return sum == 0.f ? (keys > 0 ? NAN : 0.f) : 1.0f / sum;
 }
 
-// A workgroup's share of all units (workgroup wg of sp.workgroups). kPart: nothing is divided by the sums;
-// a whole unit's rows go to `part` as a slot's do.
-template <int kD, int kNR>
-struct UnitLds {
-  float o[kWaves][16 * kNR][kD + 4];
-  float m[kWaves][16 * kNR], l[kWaves][16 * kNR];
+// What a workgroup does: its share of all units (workgroup wg of sp.workgroups), with one table a sequence or one
+// a K/V head; unit wg, whole, with one a K/V head; or its share beside other work, with nothing
+// divided by the sums: a whole unit's rows go to `part` as a slot's do ([row][D + 4]).
+enum Mode { kShare, kShareHeads, kOneEach, kParts };
+
+// In front of a launch's workgroups there may be others with work of their own (kParts): Front::workgroups of them,
+// Front::run is what they do, and kPerCu of either fit a CU. (The body stands in the kernel itself: as a function
+// that two kernels call it took a hundred more scalar spills and 2 - 5% more time.)
+struct NoFront {
+  static constexpr int kPerCu = 0;
 };
 
-template <int kD, int kNR, bool kF16, bool kPart>
-__device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io, const Lengths& s, const Split& sp,
-                                             int row_blocks, float scale_log2, float* part, int wg,
-                                             UnitLds<kD, kNR>& lds) {
+template <int kD, int kNR, bool kF16, Mode kMode, class Front>
+__global__ void __launch_bounds__(kThreads, Front::kPerCu > 0 ? Front::kPerCu : workgroups_per_cu(kD, 16 * kNR))
+cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2, float* part,
+                  Front front) {
+  constexpr bool kPart = kMode == kParts;
+  int wg = blockIdx.x;
+  if constexpr (kPart) {
+    if (wg < front.workgroups) {
+      front.run(c, io, scale_log2, wg);
+      return;
+    }
+    wg -= front.workgroups;
+  }
   constexpr int kRows = 16 * kNR;     // query rows of a unit
   constexpr int kKL = kD / 64;        // 16-byte K loads per key row and lane
   constexpr int kDB = kD / 16;        // 16-channel blocks of O
@@ -221,13 +243,15 @@ __device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io
   // bf16 has fp32's range.
   constexpr float kAbove = kF16 ? 14.f : 0.f;
   typedef Half<kF16> E;
+  __shared__ float s_o[kWaves][kRows][kD + 4];
+  __shared__ float s_m[kWaves][kRows], s_l[kWaves][kRows];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row16 = lane & 15, g = lane >> 4;
   const int page = 1 << c.log_page;
   const int units = row_blocks * c.kv_heads;
-  const Place place = find_share(c, s, sp, units, wg);
+  const Place place = kMode == kOneEach ? place_of(c, s, sp, units, wg) : find_share<kPart>(c, s, sp, units, wg);
   int64_t at = place.from;
   const int64_t end = place.to;
   if (at >= end) return;
@@ -258,7 +282,8 @@ __device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io
     }
     if (qb <= qa) continue;
     const int u = unit % c.kv_heads, r_block = (unit / c.kv_heads) * kRows;
-    const int* table = s.table + b_now * s.t_st + u * s.t_sh;
+    const int* table = s.table + b_now * s.t_st;
+    if constexpr (kMode == kShareHeads || kMode == kOneEach) table += u * s.t_sh;
     const int seen0 = len - io.tokens + 1;   // keys that the first of the Q tokens sees
 
     // ---- Q: row r_block + 16 nr + row16, channels 64 j + 16 g + 8 s .. + 8 ----
@@ -511,8 +536,8 @@ __device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io
     for (int nr = 0; nr < kNR; ++nr) {
       const float sum = sum_quad_rows(l[nr]);
       if (g == 0) {
-        lds.m[wave][16 * nr + row16] = m[nr];
-        lds.l[wave][16 * nr + row16] = sum;
+        s_m[wave][16 * nr + row16] = m[nr];
+        s_l[wave][16 * nr + row16] = sum;
       }
       const float f = kF16 ? unit_scale : 1.f;
 #pragma unroll
@@ -521,7 +546,7 @@ __device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io
         if (kF16)
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[i] *= f;
-        *reinterpret_cast<f32x4*>(&lds.o[wave][16 * nr + row16][16 * db + 4 * g]) = x;
+        *reinterpret_cast<f32x4*>(&s_o[wave][16 * nr + row16][16 * db + 4 * g]) = x;
       }
     }
     __syncthreads();
@@ -535,7 +560,7 @@ __device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io
       float mw[kWaves], top = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        mw[w] = lds.m[w][r];
+        mw[w] = s_m[w][r];
         top = fmaxf(top, mw[w]);
       }
       float sum = 0.f;
@@ -545,8 +570,8 @@ __device__ __forceinline__ void attend_units(const KvCache& c, const Queries& io
         // a wave without a visible key: weight 0. Its sum still carries a fault's NaN; and a NaN of V
         // stays one however small the factor is, so that the result does not depend on the split.
         const float f = mw[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw[w] - top);
-        sum += lds.l[w][r] * f;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(&lds.o[w][r][d]);
+        sum += s_l[w][r] * f;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&s_o[w][r][d]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] += x[i] * f;
       }

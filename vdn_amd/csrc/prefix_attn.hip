@@ -451,20 +451,20 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
   }
 }
 
-// The first n_pieces workgroups take a piece of a prefix each, the others share the tails. (The other way
-// round workgroups that find nothing to share end at once, and the pieces that follow in their
+// The first workgroups of the decode kernel's launch take a piece of a prefix each, the others share the tails. (The
+// other way round workgroups that find nothing to share end at once, and the pieces that follow in their
 // places are spread unevenly over the CUs: 308 us instead of 236 for 128 sequences behind 65536 tokens.)
 template <int kD, bool kF16, bool kBig>
-__global__ void __launch_bounds__(kThreads, per_cu(kD))
-prefix_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int n_pieces, int row_blocks, float* whole, Prefixes pre,
-                   const Item* __restrict__ items, int n_items, float* slots, float scale_log2) {
-  __shared__ units::UnitLds<kD, 1> lds;
-  const int pid = blockIdx.x;
-  if (pid < n_pieces)
+struct PrefixFront {
+  static constexpr int kPerCu = per_cu(kD);
+  Prefixes pre;
+  const Item* items;
+  float* slots;
+  int n_items, workgroups;
+  __device__ __forceinline__ void run(const KvCache& c, const Queries& io, float scale_log2, int pid) const {
     attend_prefix<kD, kF16, kBig>(c, io, pre, items, n_items, slots, scale_log2, pid);
-  else
-    units::attend_units<kD, 1, kF16, true>(c, io, s, sp, row_blocks, scale_log2, whole, pid - n_pieces, lds);
-}
+  }
+};
 
 // Joins a row's partial results: of the prefix's pieces, in order, then of the tail. A workgroup per
 // row, kD / 4 lanes for the channels, the others take partial results in turn.
@@ -502,7 +502,7 @@ prefix_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int unit_rows, in
     const int64_t n_units = static_cast<int64_t>(row_blocks) * c.kv_heads;
     const int64_t total = all * n_units;
     const int64_t start = front * n_units + static_cast<int64_t>(row / unit_rows * c.kv_heads + u) * own;
-    const int n_wg = units::sharers(sp, total);
+    const int n_wg = units::sharers<true>(sp, total);
     w0 = units::share_of(total, n_wg, start + sp.unit_cost);
     w1 = units::share_of(total, n_wg, start + own - 1);
     second = start > units::share_from(total, n_wg, static_cast<int>(w0)) ? 1 : 0;
@@ -681,20 +681,23 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
   const auto st = static_cast<hipStream_t>(stream);
   const float scale_log2 = scale * kLog2e;
   const int n_pieces = n_items * kv_heads;
-  const auto launch = [&](auto kernel) {
+  const auto launch = [&](auto kernel, auto front) {
+    front = {pre, reinterpret_cast<const Item*>(items), slots, n_items, n_pieces};
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_pieces + plan.sp.workgroups)), dim3(kThreads), 0, st, c, io,
-                       s, plan.sp, n_pieces, plan.row_blocks, whole, pre, reinterpret_cast<const Item*>(items), n_items,
-                       slots, scale_log2);
+                       s, plan.sp, plan.row_blocks, scale_log2, whole, front);
   };
-#define VDN_PREFIX(D)                                                                                       \
-  dtype ? (page >= kBN ? launch(prefix_attn_kernel<D, true, true>) : launch(prefix_attn_kernel<D, true, false>)) \
-        : (page >= kBN ? launch(prefix_attn_kernel<D, false, true>) : launch(prefix_attn_kernel<D, false, false>))
+#define VDN_PREFIX(D, F16, BIG) \
+  launch(units::cache_attn_kernel<D, 1, F16, units::kParts, PrefixFront<D, F16, BIG>>, PrefixFront<D, F16, BIG>{})
+#define VDN_PREFIX_D(D)                                                            \
+  dtype ? (page >= kBN ? VDN_PREFIX(D, true, true) : VDN_PREFIX(D, true, false))   \
+        : (page >= kBN ? VDN_PREFIX(D, false, true) : VDN_PREFIX(D, false, false))
   if (head_dim == 64)
-    VDN_PREFIX(64);
+    VDN_PREFIX_D(64);
   else if (head_dim == 128)
-    VDN_PREFIX(128);
+    VDN_PREFIX_D(128);
   else
-    VDN_PREFIX(256);
+    VDN_PREFIX_D(256);
+#undef VDN_PREFIX_D
 #undef VDN_PREFIX
   const auto join = [&](auto one, auto four) {
     const dim3 grid(static_cast<unsigned>(out_rows));
