@@ -2,7 +2,8 @@
 
 Host code mirrors the reference's operator API (MXFP8 producers and linears, VDA
 linear-attention ops, frame-window softmax attention, QK RMSNorm + 3D RoPE), adds causal
-attention over packed prompts and an 8-bit key/value cache, and calls hand-written HIP kernels
-in libvdnmi.so through a C ABI (include/vdnmi.h).
+attention over packed prompts, an 8-bit key/value cache, rotation by position and attention
+over selected pages and shared prefixes of that cache, and calls hand-written HIP kernels in
+libvdnmi.so through a C ABI (include/vdnmi.h).
 """
 __all__ = ["mxfp8"]
