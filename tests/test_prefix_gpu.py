@@ -128,6 +128,28 @@ def test_blocks_and_pieces(device, prefix, count, heads, kv_heads, dim, dtype, p
     assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
 
 
+@pytest.mark.parametrize("longest", [40, 500])              # a wave's tile, and tables of two steps
+@pytest.mark.parametrize("dim,dtype,page", [(64, FP16, 16), (128, BF16, 64), (128, FP16, 128), (256, BF16, 32)])
+@torch.no_grad()
+def test_many_short_tails(device, longest, dim, dtype, page):
+    """More tails than the card takes at once, empty ones between them, more query rows than a row block."""
+    count, heads, kv_heads, tokens = 75, 48, 16, 6
+    tails = [(53 * i) % (longest + 1) if i % 7 else 0 for i in range(count - 1)] + [longest]
+    case = Batch([70, 0], [count - 1, 1], tails, kv_heads, dim, page)
+    q = queries(count, tokens, heads, dim, dtype)
+    plan = case.plan(heads, tokens)
+    out, lse = case.run(q, plan, return_lse=True)
+    case.check(q, out, lse, rows={0, 1, 2, 7, 30, 51, count - 2, count - 1})
+    again = case.run(q, plan, return_lse=True)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    case.cache.check()
+    case.table[5, 0] = case.cache.pages                      # a page outside the pool
+    bad = case.run(q, plan)
+    assert bad[5].isnan().all() and torch.equal(bad[[4, 6, count - 1]], out[[4, 6, count - 1]])
+    with pytest.raises(RuntimeError):
+        case.cache.check()
+
+
 @torch.no_grad()
 def test_as_cache_attention_over_both_parts(device):
     """The same pages through tables that repeat the prefix: both within the bound of the definition."""

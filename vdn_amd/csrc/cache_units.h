@@ -211,8 +211,9 @@ __device__ __forceinline__ float inverse_of(float sum, int keys) {
 
 // What a workgroup does: its share of all units (workgroup wg of sp.workgroups), with one table a sequence or one
 // a K/V head; unit wg, whole, with one a K/V head; or its share beside other work, with nothing
-// divided by the sums: a whole unit's rows go to `part` as a slot's do ([row][D + 4]).
-enum Mode { kShare, kShareHeads, kOneEach, kParts };
+// divided by the sums: a whole unit's rows go to `part` as a slot's do ([row][D + 4]); or the same with a unit for
+// each wave, whole (short tables: the waves have nothing to join, and four units are under way at a time).
+enum Mode { kShare, kShareHeads, kOneEach, kParts, kPartsByWave };
 
 // In front of a launch's workgroups there may be others with work of their own (kParts): Front::workgroups of them,
 // Front::run is what they do, and kPerCu of either fit a CU. (The body stands in the kernel itself: as a function
@@ -225,7 +226,8 @@ template <int kD, int kNR, bool kF16, Mode kMode, class Front>
 __global__ void __launch_bounds__(kThreads, Front::kPerCu > 0 ? Front::kPerCu : workgroups_per_cu(kD, 16 * kNR))
 cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2, float* part,
                   Front front) {
-  constexpr bool kPart = kMode == kParts;
+  constexpr bool kByWave = kMode == kPartsByWave, kPart = kMode == kParts || kByWave;
+  constexpr int kStep = kByWave ? kTile : kQuad;   // tokens between two tiles of a wave
   int wg = blockIdx.x;
   if constexpr (kPart) {
     if (wg < front.workgroups) {
@@ -251,7 +253,9 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   const int row16 = lane & 15, g = lane >> 4;
   const int page = 1 << c.log_page;
   const int units = row_blocks * c.kv_heads;
-  const Place place = kMode == kOneEach ? place_of(c, s, sp, units, wg) : find_share<kPart>(c, s, sp, units, wg);
+  const Place place = kMode == kOneEach ? place_of(c, s, sp, units, wg)
+                      : kByWave ? Place{wg * kWaves + wave, static_cast<int64_t>(s.batch) * units, 0, 0}
+                                : find_share<kPart>(c, s, sp, units, wg);
   int64_t at = place.from;
   const int64_t end = place.to;
   if (at >= end) return;
@@ -261,21 +265,23 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   const int all_rows = io.tokens * io.group;
 
   while (at < end) {
+    if constexpr (kByWave) b = static_cast<int>(at / units);
     const int len = __builtin_amdgcn_readfirstlane(seq_tokens(c, s, b));
     const bool too_long = s.lengths[b] < 0 || s.lengths[b] > len;
     const int nq = quads_of(len), cost = nq + sp.unit_cost;
-    const int unit = static_cast<int>((at - seq0) / cost);
+    if constexpr (kByWave) seq0 = static_cast<int64_t>(b) * units;
+    const int unit = static_cast<int>(kByWave ? at - seq0 : (at - seq0) / cost);
     const int64_t unit0 = seq0 + static_cast<int64_t>(unit) * cost;
     const int64_t here = at;
-    at = min(end, unit0 + cost);
-    int qa = max(static_cast<int>(here - unit0) - sp.unit_cost, 0);
-    int qb = static_cast<int>(at - unit0) - sp.unit_cost;
-    if (sp.slots == nullptr) {
+    at = kByWave ? at + static_cast<int64_t>(sp.workgroups) * kWaves : min(end, unit0 + cost);
+    int qa = kByWave ? 0 : max(static_cast<int>(here - unit0) - sp.unit_cost, 0);
+    int qb = kByWave ? nq : static_cast<int>(at - unit0) - sp.unit_cost;
+    if (!kByWave && sp.slots == nullptr) {
       qb = here > unit0 ? 0 : nq;   // another workgroup's, or all of it
       at = unit0 + cost;
     }
     const int b_now = b;
-    const bool next_seq = unit + 1 == units && at == unit0 + cost;
+    const bool next_seq = !kByWave && unit + 1 == units && at == unit0 + cost;
     if (next_seq) {
       seq0 = at;
       ++b;
@@ -351,18 +357,18 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
 
     // The codes of a tile are loaded one step ahead, K's as soon as the scores have used the
     // last ones and V's after the product; their page ids one step before that, the scales with K.
-    int tile0 = (qa * kWaves + wave) * kTile;
+    int tile0 = kByWave ? 0 : (qa * kWaves + wave) * kTile;
     const int tile_end = min(qb * kQuad, len);
     if (tile0 < tile_end) {
-      Ids now = ids_of(tile0), next = ids_of(tile0 + kQuad);
+      Ids now = ids_of(tile0), next = ids_of(tile0 + kStep);
       load_k(now.k, tile0);
       uint32_t ks = scale_of(c.ks, now.v), vs = scale_of(c.vs, now.v);
       load_v(now.v, tile0);
-      for (; tile0 < tile_end; tile0 += kQuad) {
+      for (; tile0 < tile_end; tile0 += kStep) {
         bad |= !in_pool(now.v);                          // the g groups are all of the tile's
-        const int next0 = tile0 + kQuad;
+        const int next0 = tile0 + kStep;
         const bool more = next0 < tile_end;
-        const Ids after = ids_of(next0 + kQuad);
+        const Ids after = ids_of(next0 + kStep);
         // ---- Sᵀ ----
         f32x4 sc_t[kNR][4];
 #pragma unroll
@@ -530,6 +536,30 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
       if (lane == 0) *c.faults = 1;
 #pragma unroll
       for (int nr = 0; nr < kNR; ++nr) l[nr] = __uint_as_float(0x7fc00000u);
+    }
+    if constexpr (kByWave) {     // nothing to join: the wave's values are the unit's
+      const float f = kF16 ? unit_scale : 1.f;
+#pragma unroll
+      for (int nr = 0; nr < kNR; ++nr) {
+        const float sum = sum_quad_rows(l[nr]);
+        const int row = r_block + 16 * nr + row16;
+        if (row >= all_rows) continue;
+        const int i = row / io.group, h = u * io.group + row - i * io.group;
+        float* dst = part + ((static_cast<int64_t>(b_now) * io.tokens + i) * c.kv_heads * io.group + h) * (kD + 4);
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) {
+          f32x4 x = o[nr][db];
+          if (kF16)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] *= f;
+          *reinterpret_cast<f32x4*>(dst + 16 * db + 4 * g) = x;
+        }
+        if (g == 0) {
+          dst[kD] = m[nr];
+          dst[kD + 1] = sum;
+        }
+      }
+      continue;
     }
     __syncthreads();   // the previous unit's values are read
 #pragma unroll

@@ -584,11 +584,26 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 // less than half as long as a quad of 16 (2.0 and 4.5 us with 128 channels). Where the card's other
 // places would do for the longest tails that the table can hold, only those are launched: workgroups that find
 // nothing to share wait for a place all the same (128 sequences behind 65536 tokens: 235 us, 250).
-units::UnitPlan plan_tails(int batch, int width, int log_page, int64_t rows, int kv_heads, int head_dim, int64_t n,
-                           int piece_tiles) {
-  units::UnitPlan plan = units::plan_units(batch, width, log_page, rows, kv_heads, head_dim, 16);
+//
+// Short tables leave a workgroup's waves little to share: one quad of 60 tokens keeps one of the four busy, and
+// the workgroup's units run one after another. Where units are not split, each wave takes its own when the
+// table holds no more than one wave's tile, or when the units outnumber the places. 40 query heads on 8 of 128
+// channels: 256 tails of 1 - 60 tokens 34.1 us against 53.2, of 200 - 500 69.3 against 91.2; but 16 of
+// 200 - 500 22.8 against 17.2. Tables of four quads and more gain nothing by it (96 tails of 100 - 1000: 46.2, 43.2).
+struct TailPlan : units::UnitPlan {
+  bool by_wave;
+};
+TailPlan plan_tails(int batch, int width, int log_page, int64_t rows, int kv_heads, int head_dim, int64_t n,
+                    int piece_tiles) {
+  TailPlan plan{units::plan_units(batch, width, log_page, rows, kv_heads, head_dim, 16), false};
   Split& sp = plan.sp;
   const int64_t fit = static_cast<int64_t>(per_cu(head_dim)) * cu_count();
+  const int64_t n_units = static_cast<int64_t>(batch) * plan.row_blocks * kv_heads;
+  plan.by_wave = !plan.split && ((static_cast<int64_t>(width) << log_page) <= units::kTile || n_units > fit);
+  if (plan.by_wave) {
+    sp.workgroups = static_cast<int>(std::min((n_units + units::kWaves - 1) / units::kWaves, fit));
+    return plan;
+  }
   sp.workgroups = static_cast<int>(std::min<int64_t>(sp.workgroups, fit));
   sp.few = n > 0 && n < fit ? static_cast<int>(fit - n) : 0;
   sp.beside = 0.45f * piece_tiles;
@@ -666,8 +681,8 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
           (((static_cast<int64_t>(width) << c.log_page) + units::kQuad - 1) / units::kQuad + units::kUnitCost) >
       (1ll << 31) - 1)
     return set_error(kUnsupported, "%s: too many tokens", name);
-  units::UnitPlan plan = plan_tails(batch, width, c.log_page, rows, kv_heads, head_dim,
-                                    static_cast<int64_t>(n_items) * kv_heads, piece_tiles);
+  TailPlan plan = plan_tails(batch, width, c.log_page, rows, kv_heads, head_dim,
+                             static_cast<int64_t>(n_items) * kv_heads, piece_tiles);
   const Bytes need = workspace_of(n_items, out_rows, kv_heads, head_dim, plan);
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need.pieces + need.whole + need.tails)
     return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);
@@ -686,8 +701,11 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(n_pieces + plan.sp.workgroups)), dim3(kThreads), 0, st, c, io,
                        s, plan.sp, plan.row_blocks, scale_log2, whole, front);
   };
-#define VDN_PREFIX(D, F16, BIG) \
-  launch(units::cache_attn_kernel<D, 1, F16, units::kParts, PrefixFront<D, F16, BIG>>, PrefixFront<D, F16, BIG>{})
+#define VDN_PREFIX(D, F16, BIG)                                                                      \
+  (plan.by_wave ? launch(units::cache_attn_kernel<D, 1, F16, units::kPartsByWave, PrefixFront<D, F16, BIG>>, \
+                         PrefixFront<D, F16, BIG>{})                                                 \
+                : launch(units::cache_attn_kernel<D, 1, F16, units::kParts, PrefixFront<D, F16, BIG>>,       \
+                         PrefixFront<D, F16, BIG>{}))
 #define VDN_PREFIX_D(D)                                                            \
   dtype ? (page >= kBN ? VDN_PREFIX(D, true, true) : VDN_PREFIX(D, true, false))   \
         : (page >= kBN ? VDN_PREFIX(D, false, true) : VDN_PREFIX(D, false, false))
