@@ -226,11 +226,19 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
   float unit_scale = 0.f;                  // fp16: O in units of this power of two (0: O is 0)
   bool bad = false;
   // With one wave a SIMD half of the registers are accumulation registers, and O stays in them if the
-  // rare branches that compute on it hand it back there (causal_attn.hip).
-  auto keep = [&]() __attribute__((always_inline)) {
-    if constexpr (per_cu(kD) == 1) {
+  // rare branches that compute on it hand it back there (causal_attn.hip). An accumulator at a time: all at once
+  // pass through 128 registers, and what those spilled was reloaded behind the next tile's codes (8 prefixes
+  // of 32768 tokens, two sequences each: 451 us, 337).
+  auto keep = [&](int db) __attribute__((always_inline)) {
+    if constexpr (per_cu(kD) == 1) asm volatile("" : "+a"(o[db]));
+  };
+  auto rescale = [&](float f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int db = 0; db < kDB; ++db) asm volatile("" : "+a"(o[db]));
+    for (int db = 0; db < kDB; ++db) {
+      keep(db);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[db][v] *= f;
+      keep(db);
     }
   };
   // Where the lane's operands begin in a tile: read j of a key (32 keys further the swizzle is the same),
@@ -265,8 +273,8 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
     if (!live) return;
 
     // ---- Sᵀ: kAtOnce operand reads are under way before the first is used, and an operand is widened
-    // between the MFMAs of the one before ----
-    constexpr int kReads = 2 * kKJ, kAtOnce = kD == 128 && !kF16 ? 8 : 4;
+    // between the MFMAs of the one before. With 256 channels all of them (323 us; four at once 337) ----
+    constexpr int kReads = 2 * kKJ, kAtOnce = kD == 256 ? 16 : kD == 128 && !kF16 ? 8 : 4;
     f32x16 s[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -297,7 +305,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
     }
     __builtin_amdgcn_s_setprio(0);
     // V's operands, the first ones read while the softmax runs
-    constexpr int kVAhead = kD == 128 && !kF16 ? 8 : 4;
+    constexpr int kVAhead = kD == 256 || (kD == 128 && !kF16) ? 8 : 4;
     u32x4 vw[kVAhead];
     auto read_v = [&](int x) __attribute__((always_inline)) {
       vw[x % kVAhead] = *reinterpret_cast<const u32x4*>(tv + v_at[x / kDB] + x % kDB * 32 * (kBig ? 64 : 16));
@@ -318,12 +326,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
       const float tile_scale = e8m0_scale(min(max(top, 127u - 32u), 127u + 16u));
       if (__any(tile_scale != unit_scale)) {   // wave-uniform
         const float f = unit_scale == 0.f ? 1.f : unit_scale / tile_scale;
-        keep();
-#pragma unroll
-        for (int db = 0; db < kDB; ++db)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) o[db][v] *= f;
-        keep();
+        rescale(f);
         unit_scale = tile_scale;
       }
 #pragma unroll
@@ -362,12 +365,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
       const float m_new = grow ? mx - kAbove : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
       l *= corr;
-      keep();
-#pragma unroll
-      for (int db = 0; db < kDB; ++db)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[db][v] *= corr;
-      keep();
+      rescale(corr);
       m = m_new;
     }
     u32x4 pb[2][2];
@@ -430,7 +428,8 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
     process(t, first, std::true_type{});
   }
 
-  keep();
+#pragma unroll
+  for (int db = 0; db < kDB; ++db) keep(db);
   l = sum_halves(l);
   if (bad) {
     if (tid == 0) *c.faults = 1;
