@@ -327,6 +327,104 @@ def test_pages_behind_two_to_the_31_bytes(device):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dim,dtype,page", [(64, FP16, 16), (64, BF16, 128), (128, BF16, 64), (128, FP16, 32),
+                                            (256, BF16, 16), (256, FP16, 64)])
+@pytest.mark.parametrize("count,group,tokens", [(4, 4, 1), (1, 17, 1), (5, 13, 2), (3, 7, 6)])
+@torch.no_grad()
+def test_few_rows(device, dim, dtype, page, count, group, tokens):
+    """16 rows, 17, 130 (a block and two) and 126: few rows are taken by tiles, more by rows."""
+    tails = [(41 * i + 7) % 90 for i in range(count + 1)]
+    case = Batch([1100, 64 * 4 + 1], [count, 1], tails, 2, dim, page)
+    q = queries(count + 1, tokens, 2 * group, dim, dtype)
+    plan = case.plan(2 * group, tokens)
+    out, lse = case.run(q, plan, return_lse=True)
+    case.check(q, out, lse)
+    again = case.run(q, plan, return_lse=True)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+    case.cache.check()
+
+
+@pytest.mark.parametrize("dim,dtype,page", [(64, FP16, 16), (128, BF16, 64), (128, FP16, 256), (256, BF16, 32)])
+@pytest.mark.parametrize("heads", [4, 68])                      # few rows of a prefix, and a block of them
+@torch.no_grad()
+def test_odd_values_in_prefixes(device, dim, dtype, page, heads):
+    """NaN codes behind the last token and inside, bad pages, infinite scores."""
+    case = Batch([page + 5, 3 * page - 7, 40], [2, 1, 2], [3, 2, 20, 1, 5], 2, dim, page)
+    c = case.cache
+    for p, n in enumerate(case.prefixes):
+        last = int(case.shared[p, (n - 1) // page])
+        c.k_codes[last, :, (n - 1) % page + 1:] = 0x7f
+        c.v_codes[last, :, :, (n - 1) % page + 1:] = 0xff
+    q = queries(5, 1, heads, dim, dtype)
+    plan, half = case.plan(heads), heads // 2
+    clean = case.run(q, plan)
+    assert torch.isfinite(clean).all()
+    good = int(case.shared[1, 1])
+    for bad in (-1, c.pages, 2 ** 31 - 1):
+        case.shared[1, 1] = bad
+        out = case.run(q, plan)
+        with pytest.raises(RuntimeError):
+            c.check()
+        assert out[2].isnan().all() and torch.equal(out[[0, 1, 3, 4]], clean[[0, 1, 3, 4]])
+    case.shared[1, 1] = good
+    c.v_codes[good, 1, 9, 3] = 0x7f
+    out = case.run(q, plan)
+    assert out.isnan().nonzero().tolist() == [[2, 0, h, 9] for h in range(half, heads)]
+    assert torch.equal(torch.nan_to_num(out)[[0, 1, 3, 4]], clean[[0, 1, 3, 4]])
+    c.k_codes[int(case.shared[0, 0]), 0, 2, 7] = 0xff
+    out = case.run(q, plan)
+    assert out[:2, :, :half].isnan().all() and torch.isfinite(out[:2, :, half:]).all()
+    assert torch.equal(out[3:], clean[3:])
+    c.check()
+    c.k_codes.fill_(0xb8)                                       # -1
+    q[3:] = math.inf                                            # scores -inf: no softmax
+    out, lse = case.run(q, plan, return_lse=True)
+    assert out[3:].isnan().all() and (lse[3:] == -math.inf).all()
+
+
+@torch.no_grad()
+def test_fp16_scales_far_apart_in_a_block(device):
+    page, dim, heads = 16, 64, 40
+    case = Batch([128], [2], [4, 20], 1, dim, page)
+    c = case.cache
+    low = case.shared[0, ::2].long().cuda()
+    c.v_scales[low] = 127 - 24
+    c.v_scales[case.shared[0, 1::2].long().cuda()] = 127 - 2
+    c.v_scales[case.table[1, :2].long().cuda()] = 127 - 30
+    q = queries(2, 1, heads, dim, FP16)
+    out, lse = case.run(q, case.plan(heads), return_lse=True)
+    case.check(q, out, lse)
+    c.k_codes.zero_()
+    c.k_codes[int(low[1]), 0, 5] = 0x7e
+    c.k_scales.fill_(127)
+    q = torch.ones(2, 1, heads, dim, dtype=FP16, device="cuda")
+    out = case.run(q, case.plan(heads), scale=1.0)
+    _, v = values_of(c)
+    want = v[int(low[1]), 0, 5]
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -10 * want.abs() + 2.0 ** -24).all()
+
+
+@torch.no_grad()
+def test_a_block_behind_two_to_the_31_bytes(device):
+    page, dim = 256, 256
+    pages = 2 ** 31 // (page * dim) + 40
+    cache = kv.empty_cache(pages, 1, dim, page, device="cuda")
+    small = Batch([700], [2], [300, 5], 1, dim, page)
+    n = small.cache.pages
+    for a, b in ((cache.k_codes, small.cache.k_codes), (cache.v_codes, small.cache.v_codes),
+                 (cache.k_scales, small.cache.k_scales), (cache.v_scales, small.cache.v_scales)):
+        a[-n:] = b
+    q = queries(2, 1, 40, dim, BF16)
+    plan = small.plan(40)
+    want = small.run(q, plan)
+
+    def moved(t):
+        return torch.where(t >= 0, t + pages - n, t).int().cuda()
+
+    got = vp.prefix_attention(q, cache, moved(small.shared), plan, moved(small.table), ints(*small.tails))
+    assert torch.equal(got, want)
+
+
 @torch.no_grad()
 def test_refusals_and_nothing_to_do(device):
     case = Batch([40, 20], [2, 1], [3, 2, 5], 2, 64, 16)

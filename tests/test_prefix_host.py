@@ -57,6 +57,21 @@ def test_pieces_fill_the_card_once():
     assert vp.prepare_prefix_plan([], [], 2, 1, 64, device="cpu").batch == 0
 
 
+def test_pieces_of_few_rows_are_whole_steps():
+    """16 rows and fewer: four tiles at a time, of which only a prefix's last may be missing."""
+    for lengths, counts in (([5000, 64, 1, 700, 65], [2, 1, 4, 2, 3]), ([100000], [4]), ([9000, 9000], [4, 30])):
+        plan = vp.prepare_prefix_plan(lengths, counts, 32, 8, 128, device="cpu")
+        seen = [0] * len(lengths)
+        for p, first, row, rows, tile, end, tokens, _ in plan.items.tolist():
+            assert rows == counts[p] * 4 and tokens == lengths[p] and tile < end
+            if rows <= vp.FEW_ROWS:
+                last = -(-tokens // vp.TILE)
+                assert row == 0 and tile == seen[p] and tile % vp.FEW_STEP == 0
+                assert end == last or end % vp.FEW_STEP == 0
+                seen[p] = end
+        assert all(n == -(-length // vp.TILE) for n, length, c in zip(seen, lengths, counts) if c * 4 <= vp.FEW_ROWS)
+
+
 @pytest.mark.parametrize("args", [
     ([1], [1, 2], 2, 1, 64), ([-1], [1], 2, 1, 64), ([1.0], [1], 2, 1, 64), ([1], [-1], 2, 1, 64),
     ([1], [1], 3, 2, 64), ([1], [1], 0, 1, 64), ([1], [1], 2, 0, 64), ([1], [1], 2, 1, 96),

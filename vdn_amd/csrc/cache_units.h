@@ -215,6 +215,14 @@ __device__ __forceinline__ float inverse_of(float sum, int keys) {
 // each wave, whole (short tables: the waves have nothing to join, and four units are under way at a time).
 enum Mode { kShare, kShareHeads, kOneEach, kParts, kPartsByWave };
 
+// Few query rows of a prefix (prefix_attn.hip), which a workgroup takes like a unit, its waves the tiles
+// in turn: rows row .. + rows of the sequences behind it, tiles from .. to of `tokens`, which all rows see.
+struct FewRows {
+  const int* table;
+  float* slot;
+  int first, row, rows, head, from, to, tokens;
+};
+
 // In front of a launch's workgroups there may be others with work of their own (kParts): Front::workgroups of them,
 // Front::run is what they do, and kPerCu of either fit a CU. (The body stands in the kernel itself: as a function
 // that two kernels call it took a hundred more scalar spills and 2 - 5% more time.)
@@ -227,12 +235,13 @@ __global__ void __launch_bounds__(kThreads, Front::kPerCu > 0 ? Front::kPerCu : 
 cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, float scale_log2, float* part,
                   Front front) {
   constexpr bool kByWave = kMode == kPartsByWave, kPart = kMode == kParts || kByWave;
-  constexpr int kStep = kByWave ? kTile : kQuad;   // tokens between two tiles of a wave
   int wg = blockIdx.x;
+  [[maybe_unused]] FewRows few{};
+  bool is_few = false;
   if constexpr (kPart) {
     if (wg < front.workgroups) {
-      front.run(c, io, scale_log2, wg);
-      return;
+      is_few = front.run(c, io, scale_log2, wg, few);
+      if (!is_few) return;
     }
     wg -= front.workgroups;
   }
@@ -254,6 +263,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   const int page = 1 << c.log_page;
   const int units = row_blocks * c.kv_heads;
   const Place place = kMode == kOneEach ? place_of(c, s, sp, units, wg)
+                      : is_few ? Place{0, 1, 0, 0}
                       : kByWave ? Place{wg * kWaves + wave, static_cast<int64_t>(s.batch) * units, 0, 0}
                                 : find_share<kPart>(c, s, sp, units, wg);
   int64_t at = place.from;
@@ -262,12 +272,13 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
   const int64_t range0 = at;
   int b = __builtin_amdgcn_readfirstlane(place.seq);
   int64_t seq0 = place.before;   // where sequence b's units begin
-  const int all_rows = io.tokens * io.group;
+  const int all_rows = is_few ? few.rows : io.tokens * io.group;
+  const int step = kByWave && !is_few ? kTile : kQuad;   // tokens between two tiles of a wave
 
   while (at < end) {
     if constexpr (kByWave) b = static_cast<int>(at / units);
-    const int len = __builtin_amdgcn_readfirstlane(seq_tokens(c, s, b));
-    const bool too_long = s.lengths[b] < 0 || s.lengths[b] > len;
+    const int len = is_few ? few.tokens : __builtin_amdgcn_readfirstlane(seq_tokens(c, s, b));
+    const bool too_long = !is_few && (s.lengths[b] < 0 || s.lengths[b] > len);
     const int nq = quads_of(len), cost = nq + sp.unit_cost;
     if constexpr (kByWave) seq0 = static_cast<int64_t>(b) * units;
     const int unit = static_cast<int>(kByWave ? at - seq0 : (at - seq0) / cost);
@@ -286,11 +297,16 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
       seq0 = at;
       ++b;
     }
+    if (is_few) {
+      qa = 0;
+      qb = 1;
+      at = end;
+    }
     if (qb <= qa) continue;
-    const int u = unit % c.kv_heads, r_block = (unit / c.kv_heads) * kRows;
-    const int* table = s.table + b_now * s.t_st;
+    const int u = is_few ? few.head : unit % c.kv_heads, r_block = is_few ? 0 : (unit / c.kv_heads) * kRows;
+    const int* table = is_few ? few.table : s.table + b_now * s.t_st;
     if constexpr (kMode == kShareHeads || kMode == kOneEach) table += u * s.t_sh;
-    const int seen0 = len - io.tokens + 1;   // keys that the first of the Q tokens sees
+    const int seen0 = is_few ? len : len - io.tokens + 1;   // keys that the first of the Q tokens sees
 
     // ---- Q: row r_block + 16 nr + row16, channels 64 j + 16 g + 8 s .. + 8 ----
     u32x4 qf[kNR][2 * kKL];
@@ -298,9 +314,18 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
 #pragma unroll
     for (int nr = 0; nr < kNR; ++nr) {
       const int r = min(r_block + 16 * nr + row16, all_rows - 1);
-      const int i = r / io.group, h = u * io.group + r - i * io.group;
-      limit[nr] = seen0 + i;
-      const uint16_t* src = io.q + b_now * io.q_sb + i * io.q_st + h * io.q_sh + 16 * g;
+      int64_t from = b_now;
+      int i = r / io.group, h = u * io.group + r - i * io.group;
+      if constexpr (kPart)
+        if (is_few) {
+          const int row = few.row + r;
+          i = row / io.group;
+          h = u * io.group + row - i * io.group;
+          from = few.first + i / io.tokens;
+          i %= io.tokens;
+        }
+      limit[nr] = is_few ? len : seen0 + i;
+      const uint16_t* src = io.q + from * io.q_sb + i * io.q_st + h * io.q_sh + 16 * g;
 #pragma unroll
       for (int j = 0; j < kKL; ++j) {
         qf[nr][2 * j] = *reinterpret_cast<const u32x4*>(src + 64 * j);
@@ -357,18 +382,18 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
 
     // The codes of a tile are loaded one step ahead, K's as soon as the scores have used the
     // last ones and V's after the product; their page ids one step before that, the scales with K.
-    int tile0 = kByWave ? 0 : (qa * kWaves + wave) * kTile;
-    const int tile_end = min(qb * kQuad, len);
+    int tile0 = is_few ? (few.from + wave) * kTile : kByWave ? 0 : (qa * kWaves + wave) * kTile;
+    const int tile_end = min(is_few ? few.to * kTile : qb * kQuad, len);
     if (tile0 < tile_end) {
-      Ids now = ids_of(tile0), next = ids_of(tile0 + kStep);
+      Ids now = ids_of(tile0), next = ids_of(tile0 + step);
       load_k(now.k, tile0);
       uint32_t ks = scale_of(c.ks, now.v), vs = scale_of(c.vs, now.v);
       load_v(now.v, tile0);
-      for (; tile0 < tile_end; tile0 += kStep) {
+      for (; tile0 < tile_end; tile0 += step) {
         bad |= !in_pool(now.v);                          // the g groups are all of the tile's
-        const int next0 = tile0 + kStep;
+        const int next0 = tile0 + step;
         const bool more = next0 < tile_end;
-        const Ids after = ids_of(next0 + kStep);
+        const Ids after = ids_of(next0 + step);
         // ---- Sᵀ ----
         f32x4 sc_t[kNR][4];
 #pragma unroll
@@ -537,7 +562,7 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
 #pragma unroll
       for (int nr = 0; nr < kNR; ++nr) l[nr] = __uint_as_float(0x7fc00000u);
     }
-    if constexpr (kByWave) {     // nothing to join: the wave's values are the unit's
+    if (kByWave && !is_few) {    // nothing to join: the wave's values are the unit's
       const float f = kF16 ? unit_scale : 1.f;
 #pragma unroll
       for (int nr = 0; nr < kNR; ++nr) {
@@ -617,7 +642,8 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
               sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
         const int i = row / io.group, h = u * io.group + row - i * io.group;
-        float* dst = kPart && whole
+        float* dst = is_few ? few.slot + static_cast<int64_t>(r) * (kD + 4)
+            : kPart && whole
             ? part + ((static_cast<int64_t>(b_now) * io.tokens + i) * c.kv_heads * io.group + h) * (kD + 4)
             : sp.slots + (slot * kRows + r) * (kD + 4);
         *reinterpret_cast<f32x4*>(dst + d) = acc;

@@ -15,6 +15,11 @@
 // K's scale multiplies the scores in fp32; V's goes into the widening (bf16), or is taken relative to
 // the tile's largest one (fp16, as in cache_attn.hip). P is rounded to 16 bits, its sum keeps fp32.
 //
+// 16 rows or fewer would leave three of the four waves without work: the workgroup takes such a piece with
+// the decode kernel's code instead, the waves dividing its tiles. 8 prefixes of 32768 tokens, two sequences
+// each, 16 heads on 8: 50 us against 79 with 64 channels, 109 against 113 with 128, 198 against 323 with 256
+// (the bytes alone are 45, 90 and 179; decode over repeated tables takes 68, 135 and 258).
+//
 // Each piece leaves maximum, sum and O of its rows in fp32, other workgroups of the launch, with the decode
 // kernel's code, the same of the tails, and a second kernel joins them in order (no atomics: the
 // same call gives the same bits).
@@ -35,6 +40,7 @@ namespace {
 constexpr int kRowsOfBlock = 128;
 constexpr int kBN = 64;         // tokens of a tile
 constexpr int kThreads = 256;
+constexpr int kFewRows = 16;    // the plan's pieces of so few rows are whole steps of four tiles
 
 using units::Half;
 using units::Lengths;
@@ -84,12 +90,23 @@ __device__ __forceinline__ int swz(int key) {
   return kD == 64 ? (key >> 2 & 1) | far << 1 : kD == 128 ? (key >> 1 & 3) | far << 2 : (key & 7) | far << 3;
 }
 
+// The item and the K/V head of a workgroup. With a multiple of 8 K/V heads each XCD keeps its own heads: the
+// blocks of a piece share an L2.
+struct Piece {
+  int item, head;
+};
+__device__ __forceinline__ Piece piece_of(int pid, int n_items, int kv_heads) {
+  if (kv_heads % 8) return {pid / kv_heads, pid % kv_heads};
+  const int local = pid >> 3;
+  return {local % n_items, (pid & 7) + 8 * (local / n_items)};
+}
+
 // kBig: pages of at least 64 tokens, a tile lies in one; else its four groups of 16 tokens may
 // lie in as many.
 template <int kD, bool kF16, bool kBig>
 __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& io, const Prefixes& pre,
                                               const Item* __restrict__ items, int n_items, float* slots,
-                                              float scale_log2, int pid) {
+                                              float scale_log2, const Piece& piece) {
   constexpr int kDB = kD / 32;            // 32-channel accumulators of O
   constexpr int kChunks = kD / 16;        // 16-byte chunks of a key
   constexpr int kKJ = kD / 32;            // a lane's 16-byte reads of a key
@@ -104,16 +121,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
   __shared__ __attribute__((aligned(1024))) uint8_t sV0[kBN * kD];
   __shared__ __attribute__((aligned(1024))) uint8_t sV1[kBN * kD];
 
-  // With a multiple of 8 K/V heads each XCD keeps its own heads: the blocks of a piece share an L2.
-  int u, at;
-  if (c.kv_heads % 8 == 0) {
-    const int local = pid >> 3;
-    at = local % n_items;
-    u = (pid & 7) + 8 * (local / n_items);
-  } else {
-    u = pid % c.kv_heads;
-    at = pid / c.kv_heads;
-  }
+  const int at = piece.item, u = piece.head;
   const Item it = items[at];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -460,8 +468,19 @@ struct PrefixFront {
   const Item* items;
   float* slots;
   int n_items, workgroups;
-  __device__ __forceinline__ void run(const KvCache& c, const Queries& io, float scale_log2, int pid) const {
-    attend_prefix<kD, kF16, kBig>(c, io, pre, items, n_items, slots, scale_log2, pid);
+  // true: the workgroup is to take `few` as a unit.
+  __device__ __forceinline__ bool run(const KvCache& c, const Queries& io, float scale_log2, int pid,
+                                      units::FewRows& few) const {
+    const Piece piece = piece_of(pid, n_items, c.kv_heads);
+    const Item it = items[piece.item];
+    if (it.rows - it.row <= kFewRows) {
+      few = {pre.table + it.prefix * pre.t_st,
+             slots + (static_cast<int64_t>(piece.item) * c.kv_heads + piece.head) * kRowsOfBlock * (kD + 4), it.first,
+             it.row, it.rows - it.row, piece.head, it.tile, it.end, min(it.tokens, pre.width << c.log_page)};
+      return true;
+    }
+    attend_prefix<kD, kF16, kBig>(c, io, pre, items, n_items, slots, scale_log2, piece);
+    return false;
   }
 };
 

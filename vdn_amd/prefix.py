@@ -23,6 +23,9 @@ from .sparse import _check_query
 BLOCK_ROWS = 128   # query rows of a prefix that a workgroup takes
 TILE = 64          # tokens of its step
 LEAST_TILES = 2    # of a piece, where the prefix has more
+FEW_ROWS = 16      # so many rows are taken otherwise: the workgroup's waves divide the tiles, not the rows
+FEW_STEP = 4       # its tiles at once
+FEW_COST = 0.55    # time of a tile, of that of a block of rows (4.5 us for four with 128 channels, and 2.0 for one)
 # The pieces leave an eighth of the card's places to the tails, or half of them where even so the longest
 # is shorter than this: the tails then take as long as the pieces. 46 sequences behind 12 prompts of up
 # to 4097 tokens: 21.3 us against 23.7, 36 behind 8 of up to 2000, 40 heads: 23.0, 27.4; with 16, 16
@@ -56,10 +59,11 @@ class PrefixPlan:
         return self.sequences.shape[0]
 
 
-def _cut(tiles, units, slots):
-    """Pieces of each prefix (tiles of tokens, units that walk them): as long ones as fill the slots once."""
+def _cut(tiles, step, units, slots):
+    """Pieces of each prefix (tiles of tokens, of which a workgroup takes `step` at once, and units that walk
+    them): as long ones as fill the slots once."""
     def pieces(most):
-        return -(-tiles // most)
+        return -(-tiles // (-(-most // step) * step))
     lo, hi = min(LEAST_TILES, int(tiles.max())), int(tiles.max())
     while lo < hi:                                      # the least length whose pieces fit
         mid = (lo + hi) // 2
@@ -93,11 +97,12 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     rows = count * tokens * (heads // kv_heads)
     blocks = np.where(n > 0, -(-rows // BLOCK_ROWS), 0)
     tiles = -(-n // TILE)
+    step = np.where(rows <= FEW_ROWS, FEW_STEP, 1)
     pieces = np.zeros_like(n)
     if int((blocks * tiles).sum()):
         places = cus * _WORKGROUPS_PER_CU[head_dim]
         for share in (7 / 8, 1 / 2):
-            pieces = np.where(blocks > 0, _cut(tiles, blocks * kv_heads, int(places * share)), 0)
+            pieces = np.where(blocks > 0, _cut(tiles, step, blocks * kv_heads, int(places * share)), 0)
             if int((-(-tiles // np.maximum(pieces, 1)))[blocks > 0].max()) >= SHORT_TILES:
                 break
     made = pieces * blocks
@@ -110,15 +115,17 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     items = np.zeros((p.size, 8), dtype=np.int32)
     if p.size:
         piece, block = at // blocks[p], at % blocks[p]
-        for column, values in enumerate((p, first[p], block * BLOCK_ROWS, rows[p], tiles[p] * piece // pieces[p],
-                                         tiles[p] * (piece + 1) // pieces[p], n[p])):
+        steps = -(-tiles // step)
+        cuts = [np.minimum(steps[p] * at // pieces[p] * step[p], tiles[p]) for at in (piece, piece + 1)]
+        for column, values in enumerate((p, first[p], block * BLOCK_ROWS, rows[p], *cuts, n[p])):
             items[:, column] = values
     owner = np.repeat(np.arange(len(lengths)), count)
     sequences = np.zeros((owner.size, 8), dtype=np.int32)
     for column, values in enumerate((first, base, pieces, blocks, n)):
         sequences[:, column] = values[owner]
     both = torch.from_numpy(np.concatenate((items, sequences))).to(device)      # one transfer
-    tiles_of_one = int((items[:, 5] - items[:, 4]).max()) if p.size else 0
+    # the longest piece's time, in tiles of a block of rows
+    tiles_of_one = int(np.ceil((items[:, 5] - items[:, 4]) * np.where(step[p] > 1, FEW_COST, 1)).max()) if p.size else 0
     return PrefixPlan(lengths, counts, heads, kv_heads, head_dim, tokens, max(lengths, default=0), tiles_of_one,
                       both[:p.size], both[p.size:])
 
@@ -178,7 +185,8 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
         workspace = query.new_empty(nbytes // 2)
     _lib.call_on(index, "vdn_prefix_attention", query.data_ptr(), q_sb, q_st, q_sh, *args,
                  prefix_table.data_ptr(), p_st, prefix_width, items.data_ptr(), items.shape[0],
-                 plan.piece_tiles, sequences.data_ptr(), table.data_ptr(), t_st, batch, width, lengths.data_ptr(), tokens, group,
+                 plan.piece_tiles, sequences.data_ptr(), table.data_ptr(), t_st, batch, width, lengths.data_ptr(),
+                 tokens, group,
                  int(dtype is torch.float16), scale, out.data_ptr(), o_sb, o_st, o_sh, lse_ptr,
                  _lib.ptr(workspace), nbytes, _lib.raw_stream(index))
     return (out, lse) if return_lse else out
