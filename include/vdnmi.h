@@ -422,7 +422,7 @@ int vdn_cache_attention_heads(const void* q, int64_t q_sb, int64_t q_sh, const v
  * sequence of its prefix, the prefix's first item, pieces, row blocks, tokens, ...); items [n_items] = (prefix,
  * first sequence, first row, rows, first tile, end tile, tokens, ...): a piece of a prefix, in tiles of 64 tokens,
  * for 128 of its rows (sequences x tokens x group), piece by piece, in each the row blocks in order;
- * piece_tiles: the tiles of the longest.
+ * piece_tiles: about how many tiles of a full block take as long as the longest piece.
  * workspace: 16-byte aligned, vdn_prefix_attention_workspace's byte count, its contents need no preparation.
  * out may be q.
  */
