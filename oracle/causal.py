@@ -4,6 +4,8 @@ TEST INFRASTRUCTURE ONLY (see oracle/__init__.py). torch-CPU.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 
@@ -50,3 +52,28 @@ def bounds(out, mass, size, v, dtype, head_dim, keys):
     tiny = keys * 2.0 ** -25 * v.double().abs().max() if dtype == torch.float16 and v.numel() else 0.0
     o = half * (mass + out.abs()) * 1.01 + (2 * score[..., None] + extra) * mass + tiny
     return o + torch.finfo(dtype).tiny, score + extra + 2.0 ** -23 * size + 2.0 ** -23
+
+
+def decided(q, k, v, first, scale):
+    """attention() of scores that are far apart: each row's heaviest value [m, H, D], how far an output may be
+    from it, the log-sum-exp and how far that may be; and which rows [m, H] that holds for.
+
+    A kernel's score is off by at most (head_dim + 4) half steps of fp32 of `size`, the sum of its products'
+    magnitudes times scale (the products' sum, the scaling, log2 e and what the exponents are taken relative to). Where
+    the second score is further away than that error of both, and 40 doublings, the other weights together are under
+    n 2^-40. The heaviest one may be rounded to 16 bits while the sum is not, the output is: a half step each."""
+    group, dim, n = q.shape[1] // k.shape[1], q.shape[2], k.shape[0]
+    size = attention(q, k, v, first, scale)[3]
+    kd = k.double().repeat_interleave(group, 1).transpose(0, 1)
+    vd = v.double().repeat_interleave(group, 1).transpose(0, 1)
+    s = q.double().transpose(0, 1) @ kd.transpose(1, 2) * scale
+    i, j = torch.arange(q.shape[0])[:, None], torch.arange(n)[None]
+    s = s.masked_fill(j > i + first, -float("inf"))
+    top, at = s.max(-1)
+    second = s.scatter(-1, at[..., None], -float("inf")).amax(-1)
+    off = (dim + 4) * 2.0 ** -24 * size.T
+    sure = (top - second > 2 * off + 40 * math.log(2)).T
+    want = vd.gather(1, at[..., None].expand(-1, -1, v.shape[2])).transpose(0, 1)
+    half = torch.finfo(q.dtype).eps / 2
+    near = 2.02 * half * want.abs() + n * 2.0 ** -39 * v.double().abs().max() + torch.finfo(q.dtype).tiny
+    return want, near, top.T, (off + 2.0 ** -22 * top.abs() + 2.0 ** -20).T, sure

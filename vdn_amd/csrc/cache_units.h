@@ -203,6 +203,14 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return out;
 }
 
+// mx - above, which a row's exponents are taken relative to. Where the steps of fp32 are wider than that it may come
+// out lower, and weights of 2^16 are infinite in fp16: mx itself does then.
+template <bool kF16>
+__device__ __forceinline__ float below(float mx, float above) {
+  const float m = mx - above;
+  return kF16 && mx - m > 15.f ? mx : m;
+}
+
 // Factor of a row's output from its sum of weights and the number of keys that it sees. No weights: a row
 // that sees no key is zero, one whose scores are all -inf has no softmax and is NaN.
 __device__ __forceinline__ float inverse_of(float sum, int keys) {
@@ -461,9 +469,10 @@ cache_attn_kernel(KvCache c, Queries io, Lengths s, Split sp, int row_blocks, fl
               sc_t[nr][t][i] = x;
               mx = fmaxf(mx, x);
             }
-          mx = max_quad_rows(mx) - kAbove;
-          if (__any(mx > m[nr])) {
-            const float m_new = fmaxf(m[nr], mx);
+          mx = max_quad_rows(mx);
+          const bool grow = mx - m[nr] > kAbove;
+          if (__any(grow)) {
+            const float m_new = grow ? below<kF16>(mx, kAbove) : m[nr];
             const float corr = m[nr] == m_new ? 1.f : __builtin_amdgcn_exp2f(m[nr] - m_new);
             m[nr] = m_new;
             l[nr] *= corr;
