@@ -73,3 +73,28 @@ def test_few_rows_and_tails(device, dim, dtype, page):
             sure += check_decided(q[b].cpu(), *own, m, scale, tail[b], tail_lse[b])
         assert scale < 2 ** 10 or sure > 25, (scale, sure)            # of 36
     case.cache.check()
+
+
+# ---------------------------------------------------------------------- prefixes ----
+
+@pytest.mark.parametrize("dim,dtype,page", [(64, BF16, 16), (64, FP16, 64), (128, BF16, 64), (128, FP16, 32), (256, BF16, 32),
+                                            (256, FP16, 128)])
+@torch.no_grad()
+def test_prefix_blocks(device, dim, dtype, page):
+    """Blocks of rows: 34 of each K/V head behind the first prefix, 68 behind the second."""
+    case = Batch([300, 65], [1, 2], [5, 0, 70], 2, dim, page)
+    q = queries(3, 2, 34, dim, dtype)
+    plan = case.plan(34, 2)
+    k_all, v_all = values_of(case.cache)
+    for scale in FAR:
+        scale *= 2.0 ** 5 / dim
+        out, lse = case.run(q, plan, scale=scale, return_lse=True)
+        sure = 0
+        for b, p in enumerate(case.owner):
+            n, m = case.prefixes[p], case.tails[b]
+            k, v = (torch.cat((case.keys(case.shared[p], n, s), case.keys(case.table[b], m, s))) for s in (k_all, v_all))
+            for i in range(2):
+                sees = n + max(0, m - 1 + i)
+                sure += check_decided(q[b, i:i + 1].cpu(), k[:sees], v[:sees], sees, scale, out[b, i:i + 1], lse[b, i:i + 1])
+        assert scale < 2 ** 10 or sure > 150, (scale, sure)        # of 204
+    case.cache.check()

@@ -72,6 +72,18 @@ struct Elem<true> {
   static __device__ __forceinline__ uint16_t bits(float f) { return f32_to_f16_bits(f); }
 };
 
+// Exponents that are one fused product and difference, score x scale - m, have the rounding of m in them, up to
+// |m| 2^-24: 2^-4 here. Beyond it that would grow until the heaviest weight overflows, or vanishes.
+constexpr float kFarScore = 0x1p20f;
+
+// mx - above, which a row's exponents are taken relative to. Where the steps of fp32 are wider than that it may come
+// out lower, and weights of 2^16 are infinite in fp16: mx itself does then.
+template <bool kF16>
+__device__ __forceinline__ float below(float mx, float above) {
+  const float m = mx - above;
+  return kF16 && mx - m > 15.f ? mx : m;
+}
+
 // 16-byte chunk c of tile row r is stored at c ^ swz(r). K rows are read 16 rows per LDS cycle
 // (one chunk each), V rows by the transpose reads 4 rows x 4 chunks per 32 lanes; a 256-byte
 // bank window holds 256 / (2 D) rows, and the XOR spreads each read set over all of its 16

@@ -203,14 +203,6 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return out;
 }
 
-// mx - above, which a row's exponents are taken relative to. Where the steps of fp32 are wider than that it may come
-// out lower, and weights of 2^16 are infinite in fp16: mx itself does then.
-template <bool kF16>
-__device__ __forceinline__ float below(float mx, float above) {
-  const float m = mx - above;
-  return kF16 && mx - m > 15.f ? mx : m;
-}
-
 // Factor of a row's output from its sum of weights and the number of keys that it sees. No weights: a row
 // that sees no key is zero, one whose scores are all -inf has no softmax and is NaN.
 __device__ __forceinline__ float inverse_of(float sum, int keys) {

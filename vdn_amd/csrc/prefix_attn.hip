@@ -230,7 +230,9 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   // m starts finite: a tile whose scores are all -inf then adds nothing instead of inf - inf
-  float m = -3.402823466e38f, l = 0.f;
+  constexpr float kLeast = -3.402823466e38f;
+  float m = kLeast, l = 0.f;
+  bool far = false;                        // some row's m is beyond kFarScore
   float unit_scale = 0.f;                  // fp16: O in units of this power of two (0: O is 0)
   bool bad = false;
   // With one wave a SIMD half of the registers are accumulation registers, and O stays in them if the
@@ -368,13 +370,24 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
       mx = fmaxf(mx, top * k_scale[kt]);
     }
     mx = max_halves(mx);
-    const bool grow = mx > m + kAbove;
+    const bool grow = mx - m > kAbove;
     if (__any(grow)) {
-      const float m_new = grow ? mx - kAbove : m;
+      const float m_new = grow ? below<kF16>(mx, kAbove) : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
       l *= corr;
       rescale(corr);
       m = m_new;
+      far = __any(fabsf(m) > kFarScore && m != kLeast);
+    }
+    if (__builtin_expect(far, 0)) {
+      // m is the rounded product of a score and its scale: a score's own product has to be rounded like it.
+      // (Following that costs 1%: 128 sequences behind 65536 tokens, 40 heads on 8 x 128, 199.4 us against 197.7.)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kt][v] *= k_scale[kt];
+        k_scale[kt] = 1.f;
+      }
     }
     u32x4 pb[2][2];
     float sum = 0.f;
