@@ -98,3 +98,16 @@ def test_prefix_blocks(device, dim, dtype, page):
                 sure += check_decided(q[b, i:i + 1].cpu(), k[:sees], v[:sees], sees, scale, out[b, i:i + 1], lse[b, i:i + 1])
         assert scale < 2 ** 10 or sure > 150, (scale, sure)        # of 204
     case.cache.check()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@torch.no_grad()
+def test_prefix_keys_behind_the_last_where_scales_vanish(device, page):
+    """A page's scale times a small softmax scale may be zero in fp32: a key that is not there stays hidden."""
+    case = Batch([70], [20], [0] * 20, 1, 64, page)
+    c = case.cache
+    c.k_codes.zero_()
+    c.k_scales.fill_(27)                                              # 2^-100, the scale of a page of zeros
+    q = queries(20, 1, 1, 64, BF16)
+    out, lse = case.run(q, case.plan(1), scale=2.0 ** -60, return_lse=True)
+    case.check(q, out, lse, 2.0 ** -60)

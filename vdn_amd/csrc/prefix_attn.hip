@@ -396,6 +396,8 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         s[kt][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][v], k_scale[kt], -m));
+        if constexpr (kTail)     // K's scale times the softmax's may be 0 in fp32, and 0 inf is NaN
+          if (32 * kt + 16 * h + v >= left) s[kt][v] = 0.f;
         sum += s[kt][v];
       }
       if (apart) {
