@@ -6,6 +6,7 @@ import torch
 
 from oracle import causal as oc
 from test_prefix_gpu import Batch, ints, queries, values_of
+from vdn_amd import causal as vc
 from vdn_amd import kvcache as kv
 from vdn_amd import sparse as sp
 
@@ -111,3 +112,31 @@ def test_prefix_keys_behind_the_last_where_scales_vanish(device, page):
     q = queries(20, 1, 1, 64, BF16)
     out, lse = case.run(q, case.plan(1), scale=2.0 ** -60, return_lse=True)
     case.check(q, out, lse, 2.0 ** -60)
+
+
+# ------------------------------------------------------------------------- prompts ----
+
+@pytest.mark.parametrize("dim,dtype,wide", [(64, BF16, False), (64, FP16, False), (128, BF16, False), (128, FP16, False),
+                                            (128, BF16, True), (128, FP16, True), (256, BF16, False), (256, FP16, False)])
+@torch.no_grad()
+def test_causal_attention(device, dim, dtype, wide):
+    """Blocks of 128 rows, and of 256."""
+    lengths, heads, kv_heads = [130, 1, 0, 400], 6, 2
+    g = torch.Generator().manual_seed(dim)
+    qkv = torch.randn(sum(lengths), heads + 2 * kv_heads, dim, generator=g).to(dtype)
+    q, k, v = qkv.split([heads, kv_heads, kv_heads], 1)
+    plan = vc.prepare_causal_plan(lengths, heads, kv_heads, device=device)
+    if wide:
+        blocks = vc._blocks(tuple(lengths), heads // kv_heads, 256).to(device)
+        plan = vc.CausalPlan(tuple(lengths), heads, kv_heads, sum(lengths), blocks, blocks)
+    rows = qkv.cuda()
+    for scale in FAR:
+        scale *= 2.0 ** 6 / dim
+        out, lse = vc.causal_attention(*rows.split([heads, kv_heads, kv_heads], 1), plan, scale, return_lse=True)
+        sure, at = 0, 0
+        for n in lengths:
+            here = slice(at, at + n)
+            at += n
+            if n:
+                sure += check_decided(q[here], k[here], v[here], 0, scale, out[here], lse[here])
+        assert scale < 2 ** 10 or sure > 0.7 * lse.numel(), (scale, sure)

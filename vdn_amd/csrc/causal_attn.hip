@@ -209,6 +209,7 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   // m starts finite: a tile whose scores are all -inf then adds nothing instead of inf - inf
   float m = -FLT_MAX, l = 0.f;
+  bool far = false;   // some row's m is beyond kFarScore
   // With one wave per SIMD half of the registers are accumulation registers, and O stays in them
   // if the rare branches that compute on it hand it back there; otherwise the compiler moves all
   // of O to the other half and back in every tile.
@@ -326,9 +327,9 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kt][v]);
     mx = max_halves(mx) * scale_log2;
-    const bool grow = mx > m + (kLazy + kAbove);
+    const bool grow = mx - m > kLazy + kAbove;
     if (__any(grow)) {
-      const float m_new = grow ? mx - kAbove : m;
+      const float m_new = grow ? below<kF16>(mx, kAbove) : m;
       const float corr = grow ? __builtin_amdgcn_exp2f(m - m_new) : 1.f;
       l *= corr;
       keep();
@@ -338,13 +339,24 @@ causal_attn_kernel(CausalIn in, CausalOut to, const int* __restrict__ blocks, in
         for (int v = 0; v < 16; ++v) o[db][v] *= corr;
       keep();
       m = m_new;
+      far = __any(fabsf(m) > kFarScore && m != -FLT_MAX);
+    }
+    float factor = scale_log2;
+    if (__builtin_expect(far, 0)) {
+      // m is the rounded product of a score and the scale: a score's own product has to be rounded like it.
+      // (Following that costs up to 1%: two prompts of 4097 tokens, 16 heads on 1 x 256, 157.9 us against 156.1.)
+#pragma unroll
+      for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kt][v] *= scale_log2;
+      factor = 1.f;
     }
     float rs = 0.f;
 #pragma unroll
     for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][v], scale_log2, -m));
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][v], factor, -m));
         s[kt][v] = p;
         rs += p;
       }
