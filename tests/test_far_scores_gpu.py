@@ -9,6 +9,7 @@ from test_prefix_gpu import Batch, ints, queries, values_of
 from vdn_amd import causal as vc
 from vdn_amd import kvcache as kv
 from vdn_amd import sparse as sp
+from vdn_amd import window as vw
 
 pytestmark = pytest.mark.gpu
 
@@ -139,4 +140,21 @@ def test_causal_attention(device, dim, dtype, wide):
             at += n
             if n:
                 sure += check_decided(q[here], k[here], v[here], 0, scale, out[here], lse[here])
+        assert scale < 2 ** 10 or sure > 0.7 * lse.numel(), (scale, sure)
+
+
+# ------------------------------------------------------------------------- windows ----
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (64, FP16), (128, BF16), (128, FP16), (256, BF16), (256, FP16)])
+@torch.no_grad()
+def test_window_attention(device, dim, dtype):
+    """One frame and text in front of it: every row sees all."""
+    layout = vw.SequenceLayout(203, 3, 1, 200)
+    plan = vw.prepare_paper_window_plan(layout, vw.window_bounds(1, 0), device=device)
+    g = torch.Generator().manual_seed(dim)
+    q, k, v = torch.randn(3, 203, 4, dim, generator=g).to(dtype)
+    for scale in FAR:
+        scale *= 2.0 ** 6 / dim
+        out, lse = vw.paper_window_attention(q.cuda(), k.cuda(), v.cuda(), plan, scale, enabled=True, return_lse=True)
+        sure = check_decided(q, k, v, 203, scale, out, lse)
         assert scale < 2 ** 10 or sure > 0.7 * lse.numel(), (scale, sure)

@@ -219,6 +219,7 @@ window_attn_kernel(Layout in, const int* __restrict__ blocks, const int* __restr
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[db][v] = 0.f;
   float m = -INFINITY, l = 0.f;
+  bool far = false;             // some row's m is beyond kFarScore
 
   // transpose-read coordinates (16-lane group G = lane/16)
   const int G = lane >> 4, L = lane & 15;
@@ -302,7 +303,7 @@ window_attn_kernel(Layout in, const int* __restrict__ blocks, const int* __restr
 #pragma unroll
       for (int v = 0; v < 16; ++v) mx = fmaxf(mx, s[kt][v]);
     mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale_log2;
-    const bool grow = mx > m + kLazy;
+    const bool grow = mx - m > kLazy;
     if (__any(grow)) {
       const float m_new = grow ? mx : m;
       const float corr = __builtin_amdgcn_exp2f(m - m_new);
@@ -312,13 +313,23 @@ window_attn_kernel(Layout in, const int* __restrict__ blocks, const int* __restr
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[db][v] *= corr;
       m = m_new;
+      far = __any(fabsf(m) > kFarScore && m != -INFINITY);
+    }
+    float factor = scale_log2;
+    if (far) {
+      // m is the rounded product of a score and the scale: a score's own product has to be rounded like it
+#pragma unroll
+      for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kt][v] *= scale_log2;
+      factor = 1.f;
     }
     float rs = 0.f;
 #pragma unroll
     for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][v], scale_log2, -m));
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][v], factor, -m));
         s[kt][v] = p;
         rs += p;
       }
