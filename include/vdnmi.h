@@ -419,12 +419,13 @@ int vdn_cache_attention_heads(const void* q, int64_t q_sb, int64_t q_sh, const v
  * prefix besides those of its tail that vdn_cache_attention would show it (table, lengths: the tails').
  * prefix_table int32 [prefixes, prefix_width] (row stride prefix_table_st). The plan, from
  * vdn_amd.prefix.prepare_prefix_plan, int32 rows of 8, 16-byte aligned: sequences [batch] = (first
- * sequence of its prefix, the prefix's first item, pieces, row blocks, tokens, ...); items [n_items] = (prefix,
- * first sequence, first row, rows, first tile, end tile, tokens, ...): a piece of a prefix, in tiles of 64 tokens,
- * for 128 of its rows (sequences x tokens x group), piece by piece, in each the row blocks in order;
- * piece_tiles: about how many tiles of a full block take as long as the longest piece.
- * workspace: 16-byte aligned, vdn_prefix_attention_workspace's byte count, its contents need no preparation.
- * out may be q.
+ * sequence of its prefix, the prefix's first item, pieces, row blocks, tokens, slot, rows, unused); items
+ * [n_items] = (prefix, first sequence, first row, rows, first tile, end tile, tokens, slot): a piece of a prefix, in
+ * tiles of 64 tokens, for 128 of its rows (sequences x tokens x group), piece by piece, in each the row blocks in
+ * order; slot: how many rows the pieces in front of it have, of the prefixes in order (a sequence's: of its
+ * prefix's first piece). piece_tiles: about how many tiles of a full block take as long as the longest piece.
+ * workspace: 16-byte aligned, vdn_prefix_attention_workspace's byte count for as many blocks of 128 rows as the pieces
+ * have rows (n_items of them always hold those), its contents need no preparation. The plan is trusted. out may be q.
  */
 int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
                          const void* k_codes, const void* k_scales, const void* v_codes,
@@ -435,7 +436,7 @@ int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh
                          const int* lengths, int tokens, int group, int dtype, float scale,
                          void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, float* lse,
                          void* workspace, int64_t workspace_bytes, void* stream);
-int vdn_prefix_attention_workspace(int items, int batch, int width, int page, int tokens, int group,
+int vdn_prefix_attention_workspace(int blocks, int batch, int width, int page, int tokens, int group,
                                    int kv_heads, int head_dim, int64_t* bytes);
 
 /*

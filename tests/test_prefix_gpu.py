@@ -453,3 +453,24 @@ def test_refusals_and_nothing_to_do(device):
     none = vp.prepare_prefix_plan([40], [0], 4, 2, 64, device="cuda")
     assert vp.prefix_attention(q[:0], c, s[:1], none, t[:0], n[:0]).shape == (0, 1, 4, 64)
     c.check()
+
+
+@pytest.mark.parametrize("dim,dtype,page", [(64, FP16, 16), (128, BF16, 64), (256, BF16, 32)])
+@torch.no_grad()
+def test_many_small_prefixes(device, dim, dtype, page):
+    """Prefixes of one to forty rows a K/V head in one call, whose partial results lie behind each other: the
+    workspace is what their rows need."""
+    n, heads, kv_heads = 300, 8, 4
+    counts = [1 + (7 * i) % 20 if i % 3 == 0 else 1 for i in range(n)]
+    case = Batch([1 + (37 * i) % 150 for i in range(n)], counts, [(11 * i) % 40 for i in range(sum(counts))], kv_heads, dim, page)
+    q = queries(sum(counts), 1, heads, dim, dtype)
+    plan = case.plan(heads)
+    case.run(q, plan, return_lse=True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out, lse = case.run(q, plan, return_lse=True)
+    rows = 4 * (dim + 4) * (plan.slot_rows * kv_heads + sum(counts) * heads)
+    assert torch.cuda.max_memory_allocated() - before < rows + 2 ** 23       # output, LSE, tables; blocks of the allocator
+    case.check(q, out, lse, rows={0, 1, 5, 13, 14, 20, 100, 333, sum(counts) - 1})
+    case.cache.check()

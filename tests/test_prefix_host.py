@@ -121,3 +121,43 @@ def test_entry_point_validates_before_launching():
     assert n.value == 4 * 68 * (3 * 2 * 128 + 4)
     assert lib.vdn_prefix_attention_workspace(3, 2, 0, 16, 1, 1, 2, 64, ctypes.addressof(n)) != 0
     assert lib.vdn_prefix_attention_workspace(3, 2, 2, 16, 1, 1, 2, 64, None) != 0
+
+
+def test_items_and_slots_of_a_plan_are_its_own():
+    """Items: as many as pieces x blocks of the prefixes in order, none between them. Partial results: each row of each
+    piece has a place, once, and nothing more is asked for."""
+    r = random.Random(4)
+    for _ in range(100):
+        n = r.randint(1, 6)
+        lengths = [r.choice((0, 1, 64, 65, r.randint(1, 70000))) for _ in range(n)]
+        counts = [r.choice((0, 1, 2, r.randint(1, 200))) for _ in range(n)]
+        heads, kv_heads = r.choice(((1, 1), (40, 8), (12, 2), (16, 16), (24, 1)))
+        plan = vp.prepare_prefix_plan(lengths, counts, heads, kv_heads, r.choice((64, 128, 256)),
+                                      tokens=r.choice((1, 1, 4)), device="cpu")
+        items, seqs = plan.items.tolist(), plan.sequences.tolist()
+        at_item = at_row = b = 0
+        for length, count in zip(lengths, counts):
+            if not count:
+                continue
+            first, base, pieces, blocks, _, slot, rows, _ = seqs[b]
+            assert all(s == seqs[b] for s in seqs[b:b + count]) and first == b and rows == count * plan.tokens * heads // kv_heads
+            b += count
+            assert base == at_item and slot == at_row
+            for piece in range(pieces):
+                for it in items[base + piece * blocks:base + (piece + 1) * blocks]:
+                    assert it[7] == at_row and it[3] == rows
+                at_row += rows
+            at_item += pieces * blocks
+        assert len(items) == at_item and plan.slot_rows == at_row and b == len(seqs)
+
+
+@pytest.mark.parametrize("prefixes,count,heads,kv_heads,dim", [(500, 2, 16, 16, 128), (2000, 1, 40, 8, 128),
+                                                               (2000, 4, 32, 8, 256)])
+def test_workspace_of_many_small_prefixes(prefixes, count, heads, kv_heads, dim):
+    """What the rows need, not a block of 128 of them for each prefix."""
+    plan = vp.prepare_prefix_plan([300] * prefixes, [count] * prefixes, heads, kv_heads, dim, device="cpu")
+    rows = prefixes * count * heads                        # a piece each, and the tails' own
+    n = ctypes.c_int64(0)
+    assert _lib.load().vdn_prefix_attention_workspace(-(-plan.slot_rows // vp.BLOCK_ROWS), plan.batch, 2, 16, 1,
+                                                      heads // kv_heads, kv_heads, dim, ctypes.addressof(n)) == 0
+    assert 2 * rows <= n.value / (4 * (dim + 4)) < 2 * rows + vp.BLOCK_ROWS * kv_heads

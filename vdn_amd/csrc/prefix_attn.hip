@@ -54,15 +54,23 @@ struct Item {      // a piece of a prefix for a block of rows
   int row, rows;   // first row of the block, rows of the prefix (sequences x Q x G)
   int tile, end;   // tiles of 64 tokens
   int tokens;      // of the prefix
-  int unused;
+  int slot;        // where the piece's partial results begin: rows in front of them
 };
 struct Sequence {
   int first;       // first sequence of its prefix
   int item;        // first item of the prefix
   int pieces, blocks;
   int tokens;      // of the prefix
-  int unused[3];
+  int slot, rows;  // its first piece's slot, and the rows that every piece has
+  int unused;
 };
+
+// Partial result of row r of a piece of n rows, K/V head u: [D + 4] floats (O, m, l, two unused). A piece's rows lie
+// behind each other for each K/V head in turn, `slot` rows of the pieces in front of it before them.
+template <int kD>
+__device__ __forceinline__ float* slot_row(float* slots, int64_t slot, int64_t n, int kv_heads, int u, int64_t r) {
+  return slots + (slot * kv_heads + n * u + r) * (kD + 4);
+}
 
 struct Prefixes {
   const int* table;
@@ -121,8 +129,8 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
   __shared__ __attribute__((aligned(1024))) uint8_t sV0[kBN * kD];
   __shared__ __attribute__((aligned(1024))) uint8_t sV1[kBN * kD];
 
-  const int at = piece.item, u = piece.head;
-  const Item it = items[at];
+  const int u = piece.head;
+  const Item it = items[piece.item];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, col = lane & 31;
@@ -459,7 +467,7 @@ __device__ __forceinline__ void attend_prefix(const KvCache& c, const Queries& i
     l = __uint_as_float(0x7fc00000u);
   }
   if (!live || w0 + col >= it.rows) return;
-  float* dst = slots + ((static_cast<int64_t>(at) * c.kv_heads + u) * kRowsOfBlock + 32 * wave + col) * (kD + 4);
+  float* dst = slot_row<kD>(slots, it.slot, it.rows, c.kv_heads, u, w0 + col);
   const float f = kF16 ? unit_scale : 1.f;
 #pragma unroll
   for (int db = 0; db < kDB; ++db)
@@ -489,9 +497,8 @@ struct PrefixFront {
     const Piece piece = piece_of(pid, n_items, c.kv_heads);
     const Item it = items[piece.item];
     if (it.rows - it.row <= kFewRows) {
-      few = {pre.table + it.prefix * pre.t_st,
-             slots + (static_cast<int64_t>(piece.item) * c.kv_heads + piece.head) * kRowsOfBlock * (kD + 4), it.first,
-             it.row, it.rows - it.row, piece.head, it.tile, it.end, min(it.tokens, pre.width << c.log_page)};
+      few = {pre.table + it.prefix * pre.t_st, slot_row<kD>(slots, it.slot, it.rows, c.kv_heads, piece.head, it.row),
+             it.first, it.row, it.rows - it.row, piece.head, it.tile, it.end, min(it.tokens, pre.width << c.log_page)};
       return true;
     }
     attend_prefix<kD, kF16, kBig>(c, io, pre, items, n_items, slots, scale_log2, piece);
@@ -504,8 +511,7 @@ struct PrefixFront {
 template <int kD, bool kF16, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves)
 prefix_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int unit_rows, int row_blocks,
-                   const Sequence* __restrict__ seqs, const float* __restrict__ slots,
-                   const float* __restrict__ whole) {
+                   const Sequence* __restrict__ seqs, float* __restrict__ slots, const float* __restrict__ whole) {
   constexpr int kVec = kD / 4, kLanes = 64 * kWaves / kVec;
   __shared__ float s_part[kLanes][kD], s_pm[kLanes], s_pl[kLanes];
   const int rows = io.tokens * io.group;
@@ -541,12 +547,12 @@ prefix_join_kernel(KvCache c, Queries io, Lengths s, Split sp, int unit_rows, in
     second = start > units::share_from(total, n_wg, static_cast<int>(w0)) ? 1 : 0;
   }
   const int64_t r = static_cast<int64_t>(b - q.first) * rows + row;     // row of the prefix
-  const int64_t block = r / kRowsOfBlock, inside = r % kRowsOfBlock;
   const int n = q.pieces + static_cast<int>(w1 - w0) + 1;
+  const float* first = slot_row<kD>(slots, q.slot, q.rows, c.kv_heads, u, r);
+  const int64_t apart = static_cast<int64_t>(q.rows) * c.kv_heads * (kD + 4);
   auto partial = [&](int x) __attribute__((always_inline)) {
     if (x < q.pieces)
-      return slots + (((q.item + x * static_cast<int64_t>(q.blocks) + block) * c.kv_heads + u) * kRowsOfBlock + inside) *
-                         (kD + 4);
+      return first + x * apart;
     if (w0 == w1)
       return whole + ((static_cast<int64_t>(b) * io.tokens + i) * c.kv_heads * io.group + head) * (kD + 4);
     const int64_t w = w0 + x - q.pieces;
@@ -649,13 +655,14 @@ TailPlan plan_tails(int batch, int width, int log_page, int64_t rows, int kv_hea
   return plan;
 }
 
+// The workspace: the tails' rows, the tails' slots, the pieces' rows.
 struct Bytes {
-  int64_t pieces, whole, tails;
+  int64_t row, whole, tails;
 };
 
-Bytes workspace_of(int64_t items, int64_t out_rows, int kv_heads, int head_dim, const units::UnitPlan& plan) {
+Bytes workspace_of(int64_t out_rows, int head_dim, const units::UnitPlan& plan) {
   const int64_t row = 4ll * (head_dim + 4);
-  return Bytes{items * kv_heads * kRowsOfBlock * row, out_rows * row, plan.slot_bytes};
+  return Bytes{row, out_rows * row, plan.slot_bytes};
 }
 
 }  // namespace
@@ -663,16 +670,16 @@ Bytes workspace_of(int64_t items, int64_t out_rows, int kv_heads, int head_dim, 
 
 using namespace vdn;
 
-VDN_API int vdn_prefix_attention_workspace(int items, int batch, int width, int page, int tokens, int group,
+VDN_API int vdn_prefix_attention_workspace(int blocks, int batch, int width, int page, int tokens, int group,
                                            int kv_heads, int head_dim, int64_t* bytes) {
-  if (bytes == nullptr || items < 0 || batch < 0 || width <= 0 || tokens <= 0 || group <= 0 || kv_heads <= 0 ||
+  if (bytes == nullptr || blocks < 0 || batch < 0 || width <= 0 || tokens <= 0 || group <= 0 || kv_heads <= 0 ||
       page <= 0)
     return set_error(kInvalidArgument, "vdn_prefix_attention_workspace: invalid argument");
   const int64_t rows = static_cast<int64_t>(tokens) * group;
   const auto plan = plan_tails(batch, width, 31 - __builtin_clz(static_cast<unsigned>(page)), rows, kv_heads, head_dim,
                                0, 0);
-  const Bytes b = workspace_of(items, rows * kv_heads * batch, kv_heads, head_dim, plan);
-  *bytes = b.pieces + b.whole + b.tails;
+  const Bytes b = workspace_of(rows * kv_heads * batch, head_dim, plan);
+  *bytes = b.whole + b.tails + b.row * blocks * kRowsOfBlock * kv_heads;
   return kOk;
 }
 
@@ -716,12 +723,13 @@ VDN_API int vdn_prefix_attention(const void* q, int64_t q_sb, int64_t q_st, int6
     return set_error(kUnsupported, "%s: too many tokens", name);
   TailPlan plan = plan_tails(batch, width, c.log_page, rows, kv_heads, head_dim,
                              static_cast<int64_t>(n_items) * kv_heads, piece_tiles);
-  const Bytes need = workspace_of(n_items, out_rows, kv_heads, head_dim, plan);
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need.pieces + need.whole + need.tails)
+  const Bytes need = workspace_of(out_rows, head_dim, plan);
+  const int64_t left = workspace_bytes - need.whole - need.tails;      // every item has a row at least
+  if (workspace == nullptr || !aligned16(workspace) || left < need.row * n_items * kv_heads)
     return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);
-  float* slots = static_cast<float*>(workspace);
-  float* whole = slots + need.pieces / 4;
+  float* whole = static_cast<float*>(workspace);
   if (plan.split) plan.sp.slots = whole + need.whole / 4;
+  float* slots = whole + (need.whole + need.tails) / 4;
   const Queries io{static_cast<const uint16_t*>(q), static_cast<uint16_t*>(out), lse, q_sb, q_st, q_sh, o_sb, o_st,
                    o_sh, tokens, group};
   const Lengths s{table, lengths, table_st, 0, batch, width};

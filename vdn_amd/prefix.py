@@ -38,7 +38,8 @@ _WORKGROUPS_PER_CU = {64: 2, 128: 2, 256: 1}
 class PrefixPlan:
     """Prefixes of `lengths` tokens with `counts` sequences each, and how their attention is cut up:
     `items` int32 [n, 8] on the device, a piece of a prefix for a block of query rows each, and
-    `sequences` int32 [batch, 8], where each sequence finds its own (the rows of the C entry point)."""
+    `sequences` int32 [batch, 8], where each sequence finds its own (the rows of the C entry point);
+    `slot_rows`: query rows of all pieces, each of which leaves a partial result for every K/V head."""
     lengths: tuple
     counts: tuple
     heads: int
@@ -47,6 +48,7 @@ class PrefixPlan:
     tokens: int
     longest: int
     piece_tiles: int
+    slot_rows: int
     items: torch.Tensor
     sequences: torch.Tensor
 
@@ -109,6 +111,8 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
     base = made.cumsum() - made
     if int(made.sum()) * kv_heads >= 2 ** 24 - 2 ** 16:
         raise ValueError("too many rows for one plan")
+    in_slots = pieces * rows                            # partial results of a prefix's rows
+    slot = in_slots.cumsum() - in_slots
     # a prefix's items, piece by piece; its tiles are spread evenly over the pieces
     p = np.repeat(np.arange(len(lengths)), made)
     at = np.arange(p.size) - base[p]
@@ -117,17 +121,18 @@ def prepare_prefix_plan(lengths, counts, heads, kv_heads, head_dim, *, tokens=1,
         piece, block = at // blocks[p], at % blocks[p]
         steps = -(-tiles // step)
         cuts = [np.minimum(steps[p] * at // pieces[p] * step[p], tiles[p]) for at in (piece, piece + 1)]
-        for column, values in enumerate((p, first[p], block * BLOCK_ROWS, rows[p], *cuts, n[p])):
+        for column, values in enumerate((p, first[p], block * BLOCK_ROWS, rows[p], *cuts, n[p],
+                                         slot[p] + piece * rows[p])):
             items[:, column] = values
     owner = np.repeat(np.arange(len(lengths)), count)
     sequences = np.zeros((owner.size, 8), dtype=np.int32)
-    for column, values in enumerate((first, base, pieces, blocks, n)):
+    for column, values in enumerate((first, base, pieces, blocks, n, slot, rows)):
         sequences[:, column] = values[owner]
     both = torch.from_numpy(np.concatenate((items, sequences))).to(device)      # one transfer
     # the longest piece's time, in tiles of a block of rows
     tiles_of_one = int(np.ceil((items[:, 5] - items[:, 4]) * np.where(step[p] > 1, FEW_COST, 1)).max()) if p.size else 0
     return PrefixPlan(lengths, counts, heads, kv_heads, head_dim, tokens, max(lengths, default=0), tiles_of_one,
-                      both[:p.size], both[p.size:])
+                      int(in_slots.sum()), both[:p.size], both[p.size:])
 
 
 def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, table, lengths, scale=None, *,
@@ -181,7 +186,7 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
     workspace, nbytes = None, 0
     if batch:
         # from the allocator in stream order: calls on other streams and captured graphs have their own
-        nbytes = _workspace_bytes(index, items.shape[0], batch, width, page, tokens, group, kv_heads, d)
+        nbytes = _workspace_bytes(index, -(-plan.slot_rows // BLOCK_ROWS), batch, width, page, tokens, group, kv_heads, d)
         workspace = query.new_empty(nbytes // 2)
     _lib.call_on(index, "vdn_prefix_attention", query.data_ptr(), q_sb, q_st, q_sh, *args,
                  prefix_table.data_ptr(), p_st, prefix_width, items.data_ptr(), items.shape[0],
@@ -193,8 +198,8 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
 
 
 @lru_cache(maxsize=4096)
-def _workspace_bytes(device_index, items, batch, width, page, tokens, group, kv_heads, head_dim):
+def _workspace_bytes(device_index, blocks, batch, width, page, tokens, group, kv_heads, head_dim):
     nbytes = ctypes.c_int64(0)
-    _lib.call_on(device_index, "vdn_prefix_attention_workspace", items, batch, width, page, tokens, group,
+    _lib.call_on(device_index, "vdn_prefix_attention_workspace", blocks, batch, width, page, tokens, group,
                  kv_heads, head_dim, ctypes.addressof(nbytes))
     return nbytes.value
