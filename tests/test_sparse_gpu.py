@@ -220,6 +220,40 @@ def test_selection_where_scores_crowd(device, spread):
         check_selection(q, cache, means, table, lengths, count, 1, 1, got)
 
 
+@pytest.mark.parametrize("width", [256, 257, 511, 512, 513, 4096])
+@pytest.mark.parametrize("dim,dtype,tokens,crowded", [(64, BF16, 1, False), (128, FP16, 1, True), (256, BF16, 2, False)])
+@torch.no_grad()
+def test_selection_of_many_units(device, width, dim, dtype, tokens, crowded):
+    """Four units a CU and more: one workgroup scores and takes a unit's pages, up to 4096. A few sequences against the
+    oracle, all against themselves in small batches, which go through a workspace."""
+    g = torch.Generator().manual_seed(width)
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    kv_heads, heads, page = 8, 16, 16
+    batch = 4 * cus // (kv_heads * tokens) + 2
+    pool = 5000
+    cache = kv.empty_cache(pool, kv_heads, dim, page, device="cuda")
+    if crowded:                                              # few values, ties everywhere
+        means = torch.randint(-1, 2, (pool, kv_heads, dim), generator=g).to(BF16)
+        q = torch.zeros(batch, tokens, heads, dim)
+        q[..., :2] = 1
+        q = q.to(dtype).cuda()
+    else:
+        means = torch.randn(pool, kv_heads, dim, generator=g).to(BF16)
+        q = torch.randn(batch, tokens, heads, dim, generator=g).to(dtype).cuda()
+    table = torch.stack([torch.randperm(pool, generator=g)[:width] for _ in range(batch)]).int()
+    lengths = torch.randint(1, width * page + 1, (batch,), generator=g).tolist()
+    lengths[:6] = [width * page, width * page - 15, 1, 20 * page, 21 * page + 1, 0]
+    count, ids = 20, ints(*lengths)
+    got = sp.select_pages(q, cache, means.cuda(), table.cuda(), ids, count, first=2, last=2)
+    for b in (0, 1, 2, 3, 4, 5, batch - 1):
+        check_selection(q[b:b + 1], cache, means, table[b:b + 1], lengths[b:b + 1], count, 2, 2, [t[b:b + 1] for t in got])
+    for b in range(0, batch, 10):
+        part = slice(b, b + 10)
+        alone = sp.select_pages(q[part], cache, means.cuda(), table[part].cuda(), ids[part], count, first=2, last=2)
+        assert torch.equal(alone[0], got[0][part]) and torch.equal(alone[1], got[1][part])
+    cache.check()
+
+
 @pytest.mark.parametrize("length", [16 * 40, 16 * 600])
 @torch.no_grad()
 def test_equal_scores_go_to_the_front_and_nan_first(device, length):
