@@ -142,11 +142,6 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 using namespace vdn;
 
 namespace vdn {
-namespace {
-
-
-}  // namespace
-
 namespace units {
 
 // Row blocks of 32 for more than 16 rows: every code is loaded and widened once for both halves.

@@ -270,8 +270,9 @@ __device__ __forceinline__ double value_of(unsigned long long key) {
 }
 
 // The `count` largest of n > count keys, of equal ones those in front. Few: a key per thread and its rank
-// among all, which lie in LDS with zeros (less than any key) up to a multiple of 8.
-__device__ void take_by_rank(const unsigned long long* keys, int n, int count, const int* row, int* out) {
+// among all, which lie in LDS with zeros (less than any key) up to a multiple of 8. (Inlined, as the next one: as
+// functions that kernels call they took 21.4 us instead of 20.4 for 128 of 8192 pages, scores included.)
+__device__ __forceinline__ void take_by_rank(const unsigned long long* keys, int n, int count, const int* row, int* out) {
   __shared__ int s_sums[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int first = wave * 64;         // of the wave's keys
@@ -316,7 +317,7 @@ constexpr int kMostRuns = 64, kMostWaves = kTakeThreads / 64;
 constexpr int kMostInBin = 256;
 
 template <int kRun>
-__device__ void take_many(const unsigned long long* keys, int n, int count, const int* row, int* out) {
+__device__ __forceinline__ void take_many(const unsigned long long* keys, int n, int count, const int* row, int* out) {
   __shared__ int s_counts[3], s_before[(kRun > 0 ? kRun : kMostRuns) * kMostWaves];
   __shared__ unsigned long long s_low[kMostWaves], s_high[kMostWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
@@ -563,53 +564,65 @@ __device__ void take_many(const unsigned long long* keys, int n, int count, cons
   write_taken(taken);
 }
 
-__device__ __forceinline__ void take_largest(const unsigned long long* keys, int n, int count, const int* row, int* out,
-                                             bool in_lds) {
-  if (in_lds && n <= kAloneThreads)
-    take_by_rank(keys, n, count, row, out);
-  else if (n <= 8 * static_cast<int>(blockDim.x))
-    take_many<8>(keys, n, count, row, out);
-  else
-    take_many<0>(keys, n, count, row, out);
-}
-
-template <int kD, bool kF16, bool kScore>
-__global__ void __launch_bounds__(kScore ? kAloneThreads : kTakeThreads) page_take_kernel(KvCache c, Select s) {
-  extern __shared__ unsigned long long s_keys[];
+// What does not depend on scores: the tokens, and the pages where all are taken (true: nothing is left to do).
+struct Unit {
+  int b, i, u;
+  const int* row;
+  int* out;
+  Sight see;
+};
+__device__ __forceinline__ bool take_all(const KvCache& c, const Select& s, Unit& at) {
   const int unit = blockIdx.x, tid = threadIdx.x, threads = blockDim.x;
   const int u = unit % c.kv_heads, i = unit / c.kv_heads % s.tokens, b = unit / c.kv_heads / s.tokens;
-  const int* row = s.table + b * s.t_st;
-  int* out = s.pages + static_cast<int64_t>(unit) * s.count;
-  const Sight see = sight_of(c, s, b, i);
+  at = {b, i, u, s.table + b * s.t_st, s.pages + static_cast<int64_t>(unit) * s.count, sight_of(c, s, b, i)};
+  const Sight see = at.see;
   const int taken = min(max(see.have, 0), s.count);
   if (tid == 0) {
     if (see.have < 0) *c.faults = 1;
     if (u == 0)
       s.seen[unit / c.kv_heads] = see.have <= 0 ? see.tokens : see.tokens - ((see.have - taken) << c.log_page);
   }
-  for (int j = taken + tid; j < s.count; j += threads) out[j] = -1;
-  if (see.have <= s.count) {
-    for (int j = tid; j < taken; j += threads) out[j] = row[j];
-    return;
+  for (int j = taken + tid; j < s.count; j += threads) at.out[j] = -1;
+  if (see.have > s.count) return false;
+  for (int j = tid; j < taken; j += threads) at.out[j] = at.row[j];
+  return true;
+}
+
+// Tables of up to so many pages keep their keys in LDS.
+constexpr int kMostInLds = 8 * kAloneThreads;
+
+template <int kD, bool kF16>
+__global__ void __launch_bounds__(kAloneThreads) page_score_take_kernel(KvCache c, Select s) {
+  extern __shared__ unsigned long long s_keys[];
+  const int tid = threadIdx.x;
+  Unit at;
+  if (take_all(c, s, at)) return;
+  const int have = at.see.have;
+  const uint16_t* q = s.q + at.b * s.q_sb + at.i * s.q_st + static_cast<int64_t>(at.u) * s.group * s.q_sh;
+  for (int tile = (tid >> 6) * 16; tile < have; tile += kAloneThreads / 64 * 16) {
+    const unsigned long long key = tile_keys<kD, kF16>(c, s, at.row, at.u, tile, have, q, s.q_sh);
+    if ((tid & 63) < 16) s_keys[tile + (tid & 15)] = tile + (tid & 15) < have ? key : 0;
   }
-  if constexpr (kScore) {
-    const uint16_t* q = s.q + b * s.q_sb + i * s.q_st + static_cast<int64_t>(u) * s.group * s.q_sh;
-    for (int tile = (tid >> 6) * 16; tile < see.have; tile += threads / 64 * 16) {
-      const unsigned long long key = tile_keys<kD, kF16>(c, s, row, u, tile, see.have, q, s.q_sh);
-      if ((tid & 63) < 16) s_keys[tile + (tid & 15)] = tile + (tid & 15) < see.have ? key : 0;
-    }
-    __syncthreads();
-    take_largest(s_keys, see.have, s.count, row, out, true);
-  } else {
-    take_largest(s.keys + static_cast<int64_t>(unit) * s.width, see.have, s.count, row, out, false);
-  }
+  __syncthreads();
+  if (have <= kAloneThreads)
+    take_by_rank(s_keys, have, s.count, at.row, at.out);
+  else
+    take_many<8>(s_keys, have, s.count, at.row, at.out);
+}
+
+__global__ void __launch_bounds__(kTakeThreads) page_take_kernel(KvCache c, Select s) {
+  Unit at;
+  if (take_all(c, s, at)) return;
+  const unsigned long long* keys = s.keys + static_cast<int64_t>(blockIdx.x) * s.width;
+  if (at.see.have <= 8 * kTakeThreads)
+    take_many<8>(keys, at.see.have, s.count, at.row, at.out);
+  else
+    take_many<0>(keys, at.see.have, s.count, at.row, at.out);
 }
 
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 constexpr int kMostPages = kMostRuns * kTakeThreads;
-// Tables of up to so many pages keep their keys in LDS.
-constexpr int kMostInLds = 4096;
 // Pages that one workgroup scores by itself where there are not many units
 constexpr int kScoredAlone = 256;
 
@@ -692,18 +705,17 @@ VDN_API int vdn_cache_select(const void* q, int64_t q_sb, int64_t q_st, int64_t 
                  batch, width, tokens, group, count, first, last};
   const auto st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(units));
-  const auto launch = [&](auto scores, auto fused, auto take) {
+  const auto launch = [&](auto scores, auto fused) {
     if (alone) {
       hipLaunchKernelGGL(fused, grid, dim3(kAloneThreads),
                          8u * static_cast<unsigned>((width + 15) / 16 * 16), st, c, s);
     } else {
       hipLaunchKernelGGL(scores, dim3(static_cast<unsigned>(units * blocks)), dim3(kThreads), 0, st, c, s,
                          static_cast<int>(blocks));
-      hipLaunchKernelGGL(take, grid, dim3(kTakeThreads), 0, st, c, s);
+      hipLaunchKernelGGL(page_take_kernel, grid, dim3(kTakeThreads), 0, st, c, s);
     }
   };
-#define VDN_SELECT(D, F16) \
-  launch(page_scores_kernel<D, F16>, page_take_kernel<D, F16, true>, page_take_kernel<D, F16, false>)
+#define VDN_SELECT(D, F16) launch(page_scores_kernel<D, F16>, page_score_take_kernel<D, F16>)
 #define VDN_SELECT_D(F16) \
   head_dim == 64 ? VDN_SELECT(64, F16) : head_dim == 128 ? VDN_SELECT(128, F16) : VDN_SELECT(256, F16)
   if (dtype == 0)
