@@ -449,8 +449,9 @@ int vdn_prefix_attention_workspace(int blocks, int batch, int width, int page, i
  * heads; the first `first` and the last `last` (>= 1) pages before all others, NaN as +inf, of equal ones
  * the one in front. selected int32 [batch, tokens, kv_heads, count]: their ids in the table's order, -1
  * behind them; seen int32 [batch, tokens]: the tokens in them, -1 for a bad length (*faults 1). A page id that
- * the pool does not have is selected before scored ones. q as vdn_cache_attention; width at most 65536. workspace: 8-byte aligned,
- * vdn_cache_select_workspace's byte count (may be 0), its contents need no preparation.
+ * the pool does not have is selected before scored ones. q as vdn_cache_attention; width at most 65536,
+ * batch x tokens x kv_heads below 2^22 and, with width > 4096, that times ceil(width / 64) below 2^24. workspace:
+ * 8-byte aligned, vdn_cache_select_workspace's byte count (may be 0), its contents need no preparation.
  */
 int vdn_cache_means(const void* k_codes, const void* k_scales, int* faults, int pages, int kv_heads,
                     int page, int head_dim, const int* table, int64_t table_st, int batch, int width,

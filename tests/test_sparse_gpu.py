@@ -254,6 +254,31 @@ def test_selection_of_many_units(device, width, dim, dtype, tokens, crowded):
     cache.check()
 
 
+@torch.no_grad()
+def test_selection_from_the_widest_tables(device):
+    """512 sequences with tables of 65536 pages: 2 GiB of keys. The long ones, at both ends, against themselves
+    alone; and one sequence too many is refused."""
+    pool, heads, dim, batch, width, count = 3000, 8, 64, 512, 65536, 40
+    g = torch.Generator().manual_seed(2)
+    cache = kv.empty_cache(pool, heads, dim, 16, device="cuda")
+    means = torch.randn(pool, heads, dim, generator=g).to(BF16).cuda()
+    q = torch.randn(batch, heads, dim, generator=g).to(BF16).cuda()
+    table = torch.randint(0, pool, (batch, width), generator=g, dtype=torch.int32).cuda()
+    lengths = torch.randint(1, 2000, (batch,), generator=g, dtype=torch.int32)
+    long = [0, 1, batch - 2, batch - 1]
+    lengths[long] = torch.tensor([16 * width, 16 * 9000, 16 * 5000 - 3, 16 * width - 20], dtype=torch.int32)
+    lengths = lengths.cuda()
+    got = sp.select_pages(q, cache, means, table, lengths, count)
+    for b in [*long, 7, 300]:
+        rows = slice(b, b + 1)
+        alone = sp.select_pages(q[rows], cache, means, table[rows], lengths[rows], count)
+        assert torch.equal(got[0][rows], alone[0]) and torch.equal(got[1][rows], alone[1])
+    cache.check()
+    many = 2 ** 14 // heads
+    with pytest.raises(ValueError, match="too many"):
+        sp.select_pages(q[:1].expand(many, -1, -1), cache, means, table[:1].expand(many, -1), lengths[:1].repeat(many), count)
+
+
 @pytest.mark.parametrize("length", [16 * 40, 16 * 600])
 @torch.no_grad()
 def test_equal_scores_go_to_the_front_and_nan_first(device, length):

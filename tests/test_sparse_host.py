@@ -84,3 +84,18 @@ def test_entry_points_validate_before_launching():
         assert heads(**bad) != 0, bad
     assert b"vdn_cache_attention_heads" in lib.vdn_last_error()
     assert heads(batch=0) == 0
+
+
+def test_limits_of_a_selection():
+    """A grid has fewer than 2^32 threads: 1024 for a unit, and 256 for 64 of its pages where a workspace holds them."""
+    lib = _lib.load()
+
+    def select(batch, tokens, heads, width):
+        return lib.vdn_cache_select(P, 128, 128, 64, P, P, 4, heads, 16, 64, P, 2, batch, width, P, tokens, 1, 0, 2, 1, 1,
+                                    P, P, None, 0, None)
+
+    # (no workspace: what is within the limits is refused for that)
+    for sizes, said in (((511, 1, 32, 65536), b"workspace"), ((512, 1, 32, 65536), b"too many"),
+                        ((512, 1, 8, 65536), b"workspace"), ((513, 4, 8, 65472), b"too many"),
+                        ((2 ** 19, 1, 8, 16), b"too many"), ((1000, 4, 8, 4097), b"workspace")):
+        assert select(*sizes) != 0 and said in lib.vdn_last_error(), (sizes, lib.vdn_last_error())

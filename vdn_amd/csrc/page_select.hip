@@ -696,7 +696,8 @@ VDN_API int vdn_cache_select(const void* q, int64_t q_sb, int64_t q_st, int64_t 
   const int64_t units = static_cast<int64_t>(batch) * tokens * kv_heads;
   const bool alone = scored_alone(units, width);
   const int64_t blocks = (static_cast<int64_t>(width) + 16 * kWaves - 1) / (16 * kWaves);
-  if (units * (alone ? 1 : blocks) * kThreads * 4 >= (1ll << 32))
+  // a grid has fewer than 2^32 threads: of kTakeThreads for a unit, of kThreads for 64 of its pages
+  if (units * kTakeThreads >= (1ll << 32) || (!alone && units * blocks * kThreads >= (1ll << 32)))
     return set_error(kUnsupported, "%s: too many queries and pages", name);
   if (!alone && (workspace == nullptr || !aligned(workspace, 8) || workspace_bytes < 8 * units * width))
     return set_error(kInvalidArgument, "%s: workspace missing, unaligned or too small", name);

@@ -82,7 +82,8 @@ def select_pages(query, cache: KVCache, means, table, lengths, count, *, first=1
 
     query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16: the newest tokens of each sequence, as
     in cache_attention; means as write_means left them. Query i sees the pages with tokens in front of
-    lengths - Q + 1 + i; a page's score is the largest q . mean over the query heads of the K/V head, in 64 bits.
+    lengths - Q + 1 + i (tables of up to 65536 pages; batch x Q x kv_heads below 2^22, and where the table is wider than
+    4096 pages, that times its width in whole 64 pages below 2^30); a page's score is the largest q . mean over the query heads of the K/V head, in 64 bits.
     The first `first` pages and the last `last` (at least 1) that the query sees are always taken; of equal
     scores the page in front. A NaN score counts as +inf.
 
@@ -100,6 +101,9 @@ def select_pages(query, cache: KVCache, means, table, lengths, count, *, first=1
         raise ValueError("table must name at least one page for each sequence of the query")
     if width > MOST_PAGES or width * page > 2 ** 31 - 1024:
         raise ValueError(f"the table must not be wider than {MOST_PAGES} pages or 2^31 tokens")
+    units = batch * tokens * kv_heads
+    if units >= 2 ** 22 or (width > 4096 and units * -(-width // 64) >= 2 ** 24):
+        raise ValueError("too many queries and pages for one call")
     if any(type(n) is not int for n in (count, first, last)) or first < 0 or last < 1 or count < first + last:
         raise ValueError("count must be at least first + last, first >= 0, last >= 1")
     lead = query.shape[:-2]
