@@ -11,7 +11,7 @@
 // ones counts as the largest, NaN as +inf. Of equal scores the page in front wins. Then a workgroup per
 // (b, i, u) takes the `count` best: by each page's rank, or where they are many by bins and the
 // ranks in the last one. Latency and the conversions to fp64 bound it: 64 sequences of up to 128 pages, 40 heads
-// on 8 x 128: 11.7 us; 8192 pages, 56 heads on 8: 10.5 for the scores and 8.5 for the taking.
+// on 8 x 128: 12.0 us; 8192 pages, 56 heads on 8: 10.3 for the scores and 8.8 for the taking.
 #include "kv_cache.h"
 
 #include "attn_tiles.h"

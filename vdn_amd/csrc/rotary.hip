@@ -14,8 +14,8 @@
 //
 // A row's lane holds V = 8 (or 4) channels from V l and from R/2 + V l on (half layout) or 2 V from 2 V l on,
 // so both channels of a pair are in one lane: no exchange but the norm's sum. Moving q and k once bounds
-// it: 32768 tokens of 40 + 8 heads x 128, both norms, 805 MB in 147 us (5.5 TB/s; a large copy 5.1, a
-// negation 6.3).
+// it: 32768 tokens of 40 + 8 heads x 128, both norms, 805 MB in 139 - 147 us by card (5.8 - 5.5 TB/s; a large copy
+// 5.1, a negation 6.3).
 #include "common.h"
 
 #include <math.h>

@@ -139,8 +139,8 @@ def prefix_attention(query, cache: KVCache, prefix_table, plan: PrefixPlan, tabl
                      return_lse=False, out=None):
     """Softmax attention of each sequence's newest tokens over its prefix and its own tail.
 
-    query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16, batch = plan.batch and Q = plan.tokens, the
-    sequences of the first prefix in front; prefix_table int32 [prefixes, width] names the pages of each
+    query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16, rows and `out`'s 16-byte aligned, batch =
+    plan.batch and Q = plan.tokens, the sequences of the first prefix in front; prefix_table int32 [prefixes, width] names the pages of each
     prefix in order (unit inner stride), table and lengths the tails' pages and tokens, as
     cache_attention's do: the Q queries' own tokens are the tail's newest. Query i of sequence b sees all
     tokens of its prefix, and the tail's tokens j < lengths[b] - Q + 1 + i: a tail may be empty.

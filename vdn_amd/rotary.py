@@ -123,7 +123,7 @@ def _check_out(name, out, x, others):
 def rotate_qk(query, key, positions, plan: RotaryPlan, q_weight=None, k_weight=None, eps=1e-6, *, out=None):
     """Turns each head of query [tokens, H, D] and key [tokens, H_kv, D] by its token's position.
 
-    BF16 or FP16, unit channel stride; positions int32 or int64 [tokens], any values. With q_weight (k_weight),
+    BF16 or FP16, unit channel stride, rows and `out`'s 8-byte aligned; positions int32 or int64 [tokens], any values. With q_weight (k_weight),
     [D] of the activation dtype or FP32, a query (key) head is first divided by the root of its
     mean square plus eps and multiplied by the weight (its squares have to be within fp32's range). All in
     fp32, rounded once. Channels from

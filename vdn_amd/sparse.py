@@ -80,7 +80,7 @@ def _check_query(query, cache, index):
 def select_pages(query, cache: KVCache, means, table, lengths, count, *, first=1, last=1):
     """The `count` pages of its sequence that each query and K/V head attends over.
 
-    query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16: the newest tokens of each sequence, as
+    query [batch, Q, H, D] or [batch, H, D] (Q = 1), BF16 or FP16, rows 16-byte aligned: the newest tokens of each sequence, as
     in cache_attention; means as write_means left them. Query i sees the pages with tokens in front of
     lengths - Q + 1 + i (tables of up to 65536 pages; batch x Q x kv_heads below 2^22, and where the table is wider than
     4096 pages, that times its width in whole 64 pages below 2^30); a page's score is the largest q . mean over the query heads of the K/V head, in 64 bits.
