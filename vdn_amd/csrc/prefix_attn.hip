@@ -26,8 +26,8 @@
 //
 // VALU work bounds it, with the MFMAs beside it and the clock at the power limit: of a wave's 32 rows and
 // 64 tokens x 128 channels, 128 conversions and 160 instructions of softmax go with 32 MFMAs (60 and
-// 36% of the time busy). 128 sequences behind 65536 tokens, 40 heads on 8 x 128, tails of 16 - 1000: 217 - 231 us by
-// card, 0.75 - 0.79 PFLOP/s; a large library product reaches 1.24. Short prefixes are bound by latency: 4 sequences
+// 36% of the time busy). 128 sequences behind 65536 tokens, 40 heads on 8 x 128, tails of 16 - 1000: 214 - 231 us by
+// card, 0.75 - 0.81 PFLOP/s; a large library product reaches 1.24. Short prefixes are bound by latency: 4 sequences
 // behind 500 tokens, 12 heads on 2 x 64: 5.8 us and 3.6 of the join.
 #include "cache_units.h"
 
